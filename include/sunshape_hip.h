@@ -1018,6 +1018,101 @@ int ss_kmeans_blocks(const float *data, int n_blocks, int64_t n_points, int bloc
                      int n_centroids, int iters, float *centroids, uint8_t *assign,
                      void *stream);
 
+/*
+ * A paged cache of 4-bit keys and values for many requests (no reference
+ * counterpart: its caches hold one batch of equal lengths, cache.py:59-998).
+ * A page holds page_size tokens of every KV head:
+ *   k_codes  u32 [n_pages][n_kv_heads][page_size][head_dim/8]: dims 8w .. 8w+7
+ *            of a token in word w
+ *   v_codes  u32 [n_pages][n_kv_heads][page_size/8][head_dim]: tokens 8w ..
+ *            8w+7 of the page at dim d in word [w][d]
+ *   k_meta, v_meta  dtype [n_pages][n_kv_heads][head_dim/group_size][page_size][2]:
+ *            scale and zero of a token's group of dims
+ * element j of a word at bit 4*(j/2) + 16*(j%2); the stored value is zero +
+ * code * scale.  Slot s is token s % page_size of page s / page_size.
+ * head_dim 64 or 128, group_size 32, 64 or 128 (at most head_dim), page_size
+ * a power of two from 16 to 1024, dtype SS_F16 or SS_BF16; the four tensors
+ * 16-byte aligned, at most 2^31 - 1 slots.
+ */
+typedef struct {
+    void *k_codes, *v_codes, *k_meta, *v_meta;
+    int64_t n_pages;
+    int n_kv_heads, head_dim, group_size, page_size, dtype;
+} ss_paged_store;
+
+/*
+ * One scheduling step of a paged cache: block tables, slots and positions
+ * from the requests' lengths.  Request r holds lengths[r] tokens in the pages
+ * block_table[r][0 .. ceil(lengths[r]/page_size)) and adds new_lengths[r]
+ * tokens (negative: gives its last ones back; minus its length: ends).
+ *   - Pages that are no longer needed go onto the stack free_pages[0 ..
+ *     n_free[0]) (requests in order, a request's pages in order), then new
+ *     ones are taken from its top in the same order and entered in
+ *     block_table.  Other entries of the table and the stack stay as they are.
+ *   - token_starts[n_requests + 1]: where each request's new tokens start in
+ *     the packed order (request after request).
+ *   - slots[n_tokens], positions[n_tokens] (may be NULL): each packed token's
+ *     slot and its position in its request, -1 behind the last one.
+ *   - lengths_out, n_free_out: the counts after the step; they may be the
+ *     arrays lengths and n_free themselves.
+ * status[0] is 0, or the sum of what makes the step impossible; then nothing
+ * of the table, the stack and the counts changes and no token has a slot:
+ * 1 a negative length, 2 more tokens than a table row holds, 4 too few free
+ * pages, 8 more new tokens than n_tokens, 16 a stack count out of range.
+ * pool: entries of free_pages.  At most 4096 requests.
+ */
+int ss_block_tables(const int32_t *lengths, const int32_t *new_lengths, int64_t n_requests,
+                    int32_t *block_table, int64_t table_width, int32_t *free_pages, int64_t pool,
+                    const int32_t *n_free, int page_size, int64_t n_tokens, int32_t *lengths_out,
+                    int32_t *n_free_out, int32_t *token_starts, int32_t *slots, int32_t *positions,
+                    int32_t *status, void *stream);
+
+/*
+ * Quantise tokens' keys and values into their slots.  Element d of token t
+ * and head h is at keys[t*k_st + h*k_sh + d] (values: v_st, v_sh; in_dtype
+ * elements, rounded to the store's dtype first).  Per group: zero = the
+ * smallest value, scale = (largest - smallest)/15 rounded to the store's
+ * dtype, code = the nearest of 0 .. 15 to (x - zero)/scale, ties to even (0
+ * where the scale is 0).  A group with an infinity or NaN is stored as NaN.
+ * Tokens whose slot is negative or outside the pool are not stored.  Slots
+ * must be distinct: the content of one that is given twice is undefined.
+ */
+int ss_append_paged(const ss_paged_store *store, const void *keys, const void *values,
+                    int in_dtype, int64_t n_tokens, int64_t k_st, int64_t k_sh, int64_t v_st,
+                    int64_t v_sh, const int32_t *slots, void *stream);
+
+/*
+ * What the slots hold: keys and values [n_tokens][n_kv_heads][head_dim] in
+ * the store's dtype (zeros for a slot outside the pool).
+ */
+int ss_read_paged(const ss_paged_store *store, const int32_t *slots, int64_t n_tokens, void *keys,
+                  void *values, void *stream);
+
+/*
+ * Attention of packed queries over a paged cache.  Request r's queries are
+ * rows token_starts[r] .. token_starts[r+1] of q (element d of row t and head
+ * hq at q[t*q_st + hq*q_sh + d], SS_F16 or SS_BF16), the last of its
+ * lengths[r] tokens; query i of n sees the tokens up to position
+ * lengths[r] - n + i (causal) or all of them.  Query head hq reads KV head
+ * hq / (n_q_heads / n_kv_heads).
+ *   out  [n_tokens][n_q_heads][head_dim], q's dtype; rows without a token to
+ *        see are zero; rows of no request are zeroed if zero_rest, else left.
+ * Softmax statistics and sums are float32; probabilities times scales enter
+ * the matrix cores in 16 bits.  Table entries outside the pool hold no
+ * tokens.  max_new and max_length (the most new tokens and the longest
+ * length) size the launch: results do not depend on them.  workspace:
+ * ss_paged_attn_workspace_bytes of the same arguments, uninitialised, not
+ * shared with a call that may run at the same time.
+ */
+size_t ss_paged_attn_workspace_bytes(const ss_paged_store *store, int64_t n_requests,
+                                     int n_q_heads, int64_t max_new, int64_t max_length);
+int ss_paged_attn(const ss_paged_store *store, const void *q, int q_dtype, int64_t n_tokens,
+                  int64_t q_st, int64_t q_sh, int n_q_heads, const int32_t *block_table,
+                  int64_t table_width, const int32_t *lengths, const int32_t *token_starts,
+                  int64_t n_requests, float scale, int causal, int64_t max_new,
+                  int64_t max_length, void *out, int zero_rest, void *workspace,
+                  size_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

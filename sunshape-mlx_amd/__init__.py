@@ -56,6 +56,15 @@ from . import attention, cache, patch, value_codecs  # noqa: E402
 from .attention import sunshape_sdpa  # noqa: E402
 from .cache import HybridSunShapeKVCache, SunShapeKVCache, create_kv_cache  # noqa: E402
 from .value_codecs import GroupedValueCodec, TurboQuantValueCodec, build_value_codec  # noqa: E402
+from .paged import (  # noqa: E402
+    BlockPlan,
+    PagedKVStore,
+    append_paged,
+    build_block_tables,
+    check_plan,
+    paged_attention,
+    read_paged,
+)
 from .serialize import load_cache, load_codec, save_cache, save_codec  # noqa: E402
 
 __all__ = [
@@ -67,4 +76,6 @@ __all__ = [
     "pack_indices", "unpack_indices", "quantize_values", "dequantize_values", "get_kernel_stats",
     "reset_kernel_stats", "apply_permutation", "invert_permutation", "generate_rotation_matrix",
     "covariance_block_permutation", "save_codec", "load_codec", "save_cache", "load_cache",
+    "PagedKVStore", "BlockPlan", "build_block_tables", "check_plan", "append_paged", "read_paged",
+    "paged_attention",
 ]

@@ -1,0 +1,43 @@
+// The paged 4-bit cache's layout and 16-bit floats (paged.hip, paged_attn.hip).
+#pragma once
+
+#include "ss_common.hpp"
+
+namespace ss {
+
+struct PagedStore {
+    uint32_t *k_codes;  // [n_pages][heads][P][D/8]
+    uint32_t *v_codes;  // [n_pages][heads][P/8][D]
+    uint32_t *k_meta;   // [n_pages][heads][G][P] (scale low, zero high)
+    uint32_t *v_meta;
+    int n_pages, heads, log_page;
+};
+
+// Checks a caller's store; its shape in *out.
+int check_paged_store(const ss_paged_store *s, PagedStore *out, int *log_page);
+
+// Bit of element j of a word of eight codes.
+__host__ __device__ constexpr int nibble_bit(int j) { return 4 * (j >> 1) + 16 * (j & 1); }
+
+template <bool BF>
+constexpr uint32_t kNan16 = BF ? 0x7fc0u : 0x7e00u;
+
+template <bool BF>
+__device__ __forceinline__ float from_bits16(uint32_t u) {
+    if (BF) return __uint_as_float(u << 16);
+    return __half2float(__ushort_as_half((unsigned short)u));
+}
+
+// Nearest 16-bit float, ties to even.
+template <bool BF>
+__device__ __forceinline__ uint32_t to_bits16(float x) {
+    if (BF) return __bfloat16_as_ushort(__float2bfloat16(x));
+    return __half_as_ushort(__float2half(x));
+}
+
+template <bool BF>
+__device__ __forceinline__ float round16(float x) {
+    return from_bits16<BF>(to_bits16<BF>(x));
+}
+
+}  // namespace ss
