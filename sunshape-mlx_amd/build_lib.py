@@ -36,10 +36,11 @@ COMMON_FLAGS = [
 ]
 
 
-# per-source flags: the encoder's distance filter consumes every matrix-core
-# result on the vector ALUs, so its results are kept in VGPRs (no
-# v_accvgpr_read per element)
-FILE_FLAGS = {"encode.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
+# per-source flags: the encoder's distance filter and the paged attention's
+# softmax consume every matrix-core result on the vector ALUs, so these are
+# kept in VGPRs (no v_accvgpr_read per element)
+FILE_FLAGS = {"encode.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+              "paged_attn.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
 
 
 def hipcc() -> str:

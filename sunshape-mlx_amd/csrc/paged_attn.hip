@@ -36,6 +36,8 @@ constexpr int kTile = 32;          // tokens a wave takes at a time
 constexpr int kWaves = 4;          // waves of a workgroup
 constexpr int kUnit = kTile * kWaves;
 constexpr int kMaxSplits = 64;
+constexpr int kStages = 4;         // tiles of a wave in LDS, one computed while the others arrive
+constexpr int kNt = 2;             // cache policy of the stream: non-temporal
 // How far, in log2, a score may pass the running maximum before the maximum
 // moves: probabilities stay below 2^4, so p * scale stays within fp16 with
 // scales normalised to 2^10.
@@ -56,6 +58,20 @@ struct PagedAttn {
     float *ml;          // [n_req][heads][row_cap][splits][2]
 };
 
+// Tables do not change while the kernel runs: through the constant address
+// space their uniform reads are scalar loads, which do not queue behind the
+// stream of codes.
+__device__ __forceinline__ int table_read(const int32_t *p, int64_t i) {
+    return reinterpret_cast<const __attribute__((address_space(4))) int32_t *>(reinterpret_cast<uintptr_t>(p))[i];
+}
+
+// Eight 16-bit query elements from p (16-byte aligned if vec).
+__device__ __forceinline__ uint4 load_query8(const uint16_t *p, int vec) {
+    if (vec) return *reinterpret_cast<const uint4 *>(p);
+    return make_uint4(p[0] | ((uint32_t)p[1] << 16), p[2] | ((uint32_t)p[3] << 16),
+                      p[4] | ((uint32_t)p[5] << 16), p[6] | ((uint32_t)p[7] << 16));
+}
+
 // A request's rows, length and splits, from the tables on the device.
 struct Request {
     int t0, n, n_all, len, rows, splits, chunk;
@@ -63,10 +79,10 @@ struct Request {
 
 __device__ __forceinline__ Request request(const PagedAttn &a, int r) {
     Request q;
-    q.t0 = a.starts[r];
-    q.n_all = a.starts[r + 1] - q.t0;
+    q.t0 = table_read(a.starts, r);
+    q.n_all = table_read(a.starts, r + 1) - q.t0;
     q.n = q.t0 < 0 ? 0 : (int)max((int64_t)0, min((int64_t)q.n_all, a.n_tokens - q.t0));
-    q.len = (int)max((int64_t)0, min((int64_t)a.lengths[r], a.width << a.st.log_page));
+    q.len = (int)max((int64_t)0, min((int64_t)table_read(a.lengths, r), a.width << a.st.log_page));
     q.rows = q.n * a.rep;
     // more tokens than the launch was sized for: longer splits; more rows than
     // the workspace holds: one split, which writes the rows itself
@@ -80,28 +96,66 @@ __device__ __forceinline__ Request request(const PagedAttn &a, int r) {
     return q;
 }
 
-// 32 tokens of one KV head in a wave's registers.
-template <int D>
-struct Tile {
-    uint32_t k[2][D / 32];  // of token tile a, row lane%16: words lane/16 * D/32 ..
-    uint32_t v[D / 16];     // of tokens 8*(lane/16) ..: dims lane%16 * D/16 ..
-    uint32_t km[8], vm[8];  // (scale, zero) of tokens 8*(lane/16) .. in the column's group
-    int ok;                 // the tokens' page is in the pool
-};
-
+// s_waitcnt vmcnt(N), the other counters unconstrained.
 template <int N>
-__device__ __forceinline__ void load_words(const uint32_t *p, uint32_t (&w)[N]) {
-    if (N == 2) {
-        const uint2 u = *reinterpret_cast<const uint2 *>(p);
-        w[0] = u.x, w[1] = u.y;
-    } else {
+__device__ __forceinline__ void wait_loads() {
+    static_assert(N >= 0 && N < 64, "vmcnt range");
+    __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | (7 << 4) | (15 << 8));
+}
+
+template <typename T>
+using lds_ptr = __attribute__((address_space(3))) T *;
+
+template <typename T>
+__device__ __forceinline__ lds_ptr<T> as_lds(void *p) {
+    return reinterpret_cast<lds_ptr<T>>(static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p)));
+}
+
+// 32 tokens of one KV head as they lie in LDS: key rows, value blocks, the
+// keys' and the values' (scale, zero) pairs [G][32].  16-byte pieces move
+// within their row or block so that the reads below touch every bank once:
+// piece c of key row t sits at place c ^ (t / 8) % (pieces a row), piece c of
+// a value block at c ^ (c / 16) % 2.
+template <int D, int G>
+struct TileLds {
+    static constexpr int kCodes = 16 * D;       // bytes of the keys' codes, and of the values'
+    static constexpr int kMeta = G * kTile * 4; // bytes of the keys' pairs, and of the values'
+    static constexpr int kBytes = 2 * (kCodes + kMeta);
+    static constexpr int kKP = D / 32;          // 16-byte pieces of a key row
+    static constexpr int kVP = D / 4;           // of a value block
+    static constexpr int kLoads = 2 * (kCodes / 1024) + 1;
+    static constexpr int kMetaLanes = 2 * kMeta / 16;
+
+    // Starts copying the tile of tokens tb .. tb + 31 (pages p0 and p1) into a slot.
+    __device__ static void fetch(const PagedStore &st, int h, int lane, char *slot, int tb, int p0, int p1) {
+        const int heads = st.heads, log_page = st.log_page, in_page = (1 << log_page) - 1;
+        const int64_t row0 = (int64_t)max(p0, 0) * heads + h, row1 = (int64_t)max(p1, 0) * heads + h;
+        const int off0 = tb & in_page, off1 = (tb + 16) & in_page;
 #pragma unroll
-        for (int i = 0; i < N / 4; ++i) {
-            const uint4 u = reinterpret_cast<const uint4 *>(p)[i];
-            w[4 * i] = u.x, w[4 * i + 1] = u.y, w[4 * i + 2] = u.z, w[4 * i + 3] = u.w;
+        for (int i = 0; i < kCodes / 1024; ++i) {
+            // place -> (row or block, piece) -> address
+            const int place = i * 64 + lane;
+            const int kt = place / kKP, kc = (place % kKP) ^ ((kt >> 3) % kKP);
+            const bool second = D == 128 ? i == 1 : lane >= 32;
+            const int64_t row = second ? row1 : row0;
+            const int off = second ? off1 : off0;
+            const uint32_t *k = st.k_codes + ((row << log_page) + off) * (D / 8);
+            __builtin_amdgcn_global_load_lds(k + (kt % 16) * (D / 8) + kc * 4, as_lds<void>(slot + i * 1024), 16, 0, kNt);
+            const int vb = place / kVP, vc = (place % kVP) ^ (((place % kVP) >> 4) & 1);
+            const uint32_t *v = st.v_codes + (((row << log_page) + off) >> 3) * D;
+            __builtin_amdgcn_global_load_lds(v + (vb % 2) * D + vc * 4, as_lds<void>(slot + kCodes + i * 1024), 16,
+                                             0, kNt);
+        }
+        if (kMetaLanes == 64 || lane < kMetaLanes) {
+            const int e = lane % (kMetaLanes / 2), mg = e / 8, t = e % 8 * 4;
+            const int64_t row = t >= 16 ? row1 : row0;
+            const int off = (t >= 16 ? off1 : off0) + t % 16;
+            const uint32_t *m = lane < kMetaLanes / 2 ? st.k_meta : st.v_meta;
+            __builtin_amdgcn_global_load_lds(m + ((row * G + mg) << log_page) + off,
+                                             as_lds<void>(slot + 2 * kCodes), 16, 0, kNt);
         }
     }
-}
+};
 
 // A word's eight codes as the four registers of an operand: pairs (0,1) and
 // (4,5) times 2^-24, (2,3) and (6,7) times 2^-20.
@@ -116,6 +170,20 @@ __device__ __forceinline__ half8_t codes_operand(uint32_t w) {
     x.u[2] = hi & 0x000f000fu;
     x.u[3] = hi & 0x00f000f0u;
     return x.h;
+}
+
+template <int N>
+__device__ __forceinline__ void read_words(const char *p, uint32_t (&w)[N]) {
+    if constexpr (N == 2) {
+        const uint2 u = *reinterpret_cast<const uint2 *>(p);
+        w[0] = u.x, w[1] = u.y;
+    } else {
+#pragma unroll
+        for (int i = 0; i < N / 4; ++i) {
+            const uint4 u = reinterpret_cast<const uint4 *>(p)[i];
+            w[4 * i] = u.x, w[4 * i + 1] = u.y, w[4 * i + 2] = u.z, w[4 * i + 3] = u.w;
+        }
+    }
 }
 
 template <int N>
@@ -149,15 +217,19 @@ __device__ __forceinline__ float groups_sum(float v) {
 // waves take 32-token tiles in turn, the next tile's loads in flight while
 // one is computed, and their results are joined through LDS at the end.
 template <int D, int G, bool BF, int NS>
-__global__ void __launch_bounds__(256) paged_attn_kernel(const PagedAttn a) {
+__global__ void __launch_bounds__(256, 2) paged_attn_kernel(const PagedAttn a) {
     constexpr int RS = 16 / G;       // rows of a column set
     constexpr int ROWS = RS * NS;    // rows of a workgroup
     constexpr int KS = D / 32;       // matrix steps over a head's dims
     constexpr int VT = D / 16;       // 16-dim tiles of the values
-    constexpr int PAD = 4;
-    __shared__ float part[kWaves][ROWS][D + PAD];
-    __shared__ float stats[kWaves][ROWS][2];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    constexpr int OP = D + 4;        // a row of the waves' results in LDS
+    using TL = TileLds<D, G>;
+    constexpr int kRing = kWaves * kStages * TL::kBytes, kJoin = kWaves * ROWS * (OP + 2) * 4;
+    // the waves' tiles, then their results
+    __shared__ __attribute__((aligned(16))) char lds[kRing > kJoin ? kRing : kJoin];
+    float(*part)[ROWS][OP] = reinterpret_cast<float(*)[ROWS][OP]>(lds);
+    float(*stats)[ROWS][2] = reinterpret_cast<float(*)[ROWS][2]>(lds + kWaves * ROWS * OP * 4);
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 15, quad = lane >> 4;
     const int g = col % G;
     const bool in_group = quad * G / 4 == g;  // the lane's dims, and its rows of O, are in the column's group
@@ -166,7 +238,7 @@ __global__ void __launch_bounds__(256) paged_attn_kernel(const PagedAttn a) {
     const int blocks = gridDim.y / heads;
 
     if (a.zero_rest && r == a.n_req - 1 && split == 0 && (int)blockIdx.y < heads) {
-        const int64_t from = max(0, a.starts[a.n_req]);
+        const int64_t from = max(0, table_read(a.starts, a.n_req));
         const int64_t per = (int64_t)a.rep * D;  // outputs of this KV head in a row, contiguous
         for (int64_t e = threadIdx.x; e < (a.n_tokens - from) * per; e += 256) {
             const int64_t t = e / per;
@@ -179,46 +251,50 @@ __global__ void __launch_bounds__(256) paged_attn_kernel(const PagedAttn a) {
     const int end = (int)min((int64_t)begin + rq.chunk, (int64_t)rq.len);
     const int32_t *row_table = a.table + (int64_t)r * a.width;
 
+    char *ring = lds + wave * kStages * TL::kBytes;
+    // Page of the 16 tokens from `token`; -1 if the table names none of the pool.
     auto page_at = [&](int token) {
-        return row_table[min((int64_t)(token >> log_page), a.width - 1)];
+        const int p = table_read(row_table, min((int64_t)(token >> log_page), a.width - 1));
+        return (uint32_t)p < (uint32_t)a.st.n_pages ? p : -1;
     };
-    Tile<D> tiles[2];
-    auto load = [&](Tile<D> &t, int tb, int page_k, int page_v) {
-        t.ok = (uint32_t)page_v < (uint32_t)a.st.n_pages;
-        const int pk = (uint32_t)page_k < (uint32_t)a.st.n_pages ? page_k : 0, pv = t.ok ? page_v : 0;
-        // key tile x, row m: token 8*(m/4) + 4x + m%4
-        const int64_t kt = ((int64_t)(pk * heads + h) << log_page) + ((tb + 8 * (col >> 2) + (col & 3)) & in_page);
-        load_words(a.st.k_codes + kt * (D / 8) + quad * KS, t.k[0]);
-        load_words(a.st.k_codes + (kt + 4) * (D / 8) + quad * KS, t.k[1]);
-        const int64_t row = (int64_t)(pv * heads + h);
-        const int off = (tb + 8 * quad) & in_page;
-        load_words(a.st.v_codes + (((row << log_page) + off) >> 3) * D + col * VT, t.v);
-        const int64_t m = ((row * G + g) << log_page) + off;
-        load_words(a.st.k_meta + m, t.km);
-        load_words(a.st.v_meta + m, t.vm);
-    };
-
     for (int rb = blockIdx.y / heads; rb * ROWS < rq.rows; rb += blocks) {
-        int tb = begin + kTile * wave;
-        int page_k = page_at(tb + 8 * (col >> 2)), page_v = page_at(tb + 8 * quad);
+        // queries first: what is loaded later would hold them back
         int limit[NS];  // tokens that the column's row sees
+        uint4 raw[NS][KS];
+        bool live[NS];
+#pragma unroll
+        for (int s = 0; s < NS; ++s) {
+            const int row = rb * ROWS + s * RS + col / G;
+            live[s] = row < rq.rows;
+            const int i = live[s] ? row / a.rep : 0, hd = live[s] ? row % a.rep : 0;
+            limit[s] = live[s] && a.causal ? max(0, min(rq.len, rq.len - rq.n_all + i + 1)) : rq.len;
+            const uint16_t *q =
+                static_cast<const uint16_t *>(a.q) + (rq.t0 + i) * a.q_st + (h * a.rep + hd) * a.q_sh + quad * (D / 4);
+#pragma unroll
+            for (int k = 0; k < KS; ++k) raw[s][k] = load_query8(q + 8 * k, a.vec);
+        }
+        int ahead = begin + kTile * wave;  // next tile to fetch
+        int pages[kStages][2];             // of the tiles in flight, the oldest first
+#pragma unroll
+        for (int i = 0; i < kStages; ++i) {
+            pages[i][0] = page_at(ahead), pages[i][1] = page_at(ahead + 16);
+            if (i < kStages - 1 && ahead < end) TL::fetch(a.st, h, lane, ring + i * TL::kBytes, ahead, pages[i][0], pages[i][1]);
+            ahead += kUnit;
+        }
         int all_see = rq.len;
         half8_t qf[NS][KS];
         float qz[NS], factor[NS];
 #pragma unroll
         for (int s = 0; s < NS; ++s) {
-            const int row = rb * ROWS + s * RS + col / G;
-            const bool live = row < rq.rows;
-            const int i = live ? row / a.rep : 0, hd = live ? row % a.rep : 0;
-            limit[s] = live && a.causal ? max(0, min(rq.len, rq.len - rq.n_all + i + 1)) : rq.len;
-            const int64_t at = (rq.t0 + i) * a.q_st + (h * a.rep + hd) * a.q_sh + quad * (D / 4);
             float x[KS][8], top = 0.f, sum = 0.f;
 #pragma unroll
             for (int k = 0; k < KS; ++k) {
-                load8_f32(a.q, a.q_dtype, a.vec, at + 8 * k, x[k]);
+                float xh[8], xb[8];
+                unpack16<__half>(raw[s][k], xh);
+                unpack16<__hip_bfloat16>(raw[s][k], xb);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    x[k][e] = live ? x[k][e] : 0.f;
+                    x[k][e] = live[s] ? (a.q_dtype == SS_F16 ? xh[e] : xb[e]) : 0.f;
                     top = fmaxf(top, fabsf(x[k][e]));
                 }
             }
@@ -252,21 +328,42 @@ __global__ void __launch_bounds__(256) paged_attn_kernel(const PagedAttn a) {
         float vlim = 0.f;  // power of two, above every value scale seen in the column's group
 
         // masked: some row does not see some token of the tile
-        auto compute = [&](const Tile<D> &t, int tb, auto masked) {
+        auto compute = [&](const char *slot, int tb, bool ok, auto masked) {
             constexpr bool mask = decltype(masked)::value;
+            uint32_t kw[2][KS], vw[VT], km[8], vm[8];
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+                // key tile y, row col: token 8*(col/4) + 4y + col%4
+                const int t = 8 * (col >> 2) + 4 * y + (col & 3);
+                if constexpr (KS == 4) {
+                    read_words(slot + (t * TL::kKP + (quad ^ ((t >> 3) % TL::kKP))) * 16, kw[y]);
+                } else {
+                    read_words(slot + (t * TL::kKP + ((quad >> 1) ^ ((t >> 3) % TL::kKP))) * 16 + (quad & 1) * 8, kw[y]);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < VT / 4; ++i) {
+                const int c = col * (VT / 4) + i;
+                uint32_t w4[4];
+                read_words(slot + TL::kCodes + (quad * TL::kVP + (c ^ ((c >> 4) & 1))) * 16, w4);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) vw[4 * i + k] = w4[k];
+            }
+            read_words(slot + 2 * TL::kCodes + (g * kTile + 8 * quad) * 4, km);
+            read_words(slot + 2 * TL::kCodes + TL::kMeta + (g * kTile + 8 * quad) * 4, vm);
             float ks[8], kz[8], vs[8], vz[8];
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                ks[j] = from_bits16<BF>(t.km[j] & 0xffffu);
-                kz[j] = from_bits16<BF>(t.km[j] >> 16);
-                vs[j] = from_bits16<BF>(t.vm[j] & 0xffffu);
-                vz[j] = from_bits16<BF>(t.vm[j] >> 16);
+                ks[j] = from_bits16<BF>(km[j] & 0xffffu);
+                kz[j] = from_bits16<BF>(km[j] >> 16);
+                vs[j] = from_bits16<BF>(vm[j] & 0xffffu);
+                vz[j] = from_bits16<BF>(vm[j] >> 16);
             }
             const int first = tb + 8 * quad;  // the lane's first token
             if (mask) {  // (behind the request's tokens a page may hold anything, NaN too)
 #pragma unroll
                 for (int j = 0; j < 8; ++j)
-                    if (!t.ok || first + j >= rq.len) vs[j] = 0.f;
+                    if (!ok || first + j >= rq.len) vs[j] = 0.f;
             }
             // value scales enter the product times 2^10 / vlim
             const float vtop = column_max(vs);
@@ -293,7 +390,7 @@ __global__ void __launch_bounds__(256) paged_attn_kernel(const PagedAttn a) {
                     float4_t d = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                     for (int k = 0; k < KS; ++k)
-                        d = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes_operand(t.k[y][k]), qf[s][k], d, 0, 0, 0);
+                        d = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes_operand(kw[y][k]), qf[s][k], d, 0, 0, 0);
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const int j = 4 * y + i;
@@ -301,7 +398,7 @@ __global__ void __launch_bounds__(256) paged_attn_kernel(const PagedAttn a) {
                     }
                 }
                 if (mask) {
-                    const int see = t.ok ? limit[s] : 0;
+                    const int see = ok ? limit[s] : 0;
 #pragma unroll
                     for (int j = 0; j < 8; ++j)
                         if (first + j >= see) x[j] = -INFINITY;
@@ -322,7 +419,7 @@ __global__ void __launch_bounds__(256) paged_attn_kernel(const PagedAttn a) {
                 for (int j = 0; j < 8; ++j) {
                     const float p = fast_exp2(x[j] - ((j & 2) ? odd : even));
                     // (a token that the row does not see adds nothing, whatever its value holds)
-                    const bool off = mask && (!t.ok || first + j >= limit[s]);
+                    const bool off = mask && (!ok || first + j >= limit[s]);
                     const float z = off ? 0.f : vz[j];
                     if (j & 2) {
                         l_odd[s] += p;
@@ -342,35 +439,40 @@ __global__ void __launch_bounds__(256) paged_attn_kernel(const PagedAttn a) {
             }
 #pragma unroll
             for (int j = 0; j < VT; ++j) {
-                const half8_t v = codes_operand(t.v[j]);
+                const half8_t v = codes_operand(vw[j]);
 #pragma unroll
                 for (int s = 0; s < NS; ++s)
                     o[s][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, p16[s], o[s][j], 0, 0, 0);
             }
         };
 
-        auto step = [&](const Tile<D> &t, int tb) {
-            if (tb + kTile > all_see || __any(!t.ok))
-                compute(t, tb, std::true_type{});
-            else
-                compute(t, tb, std::false_type{});
-        };
-        if (tb < end) {
-            load(tiles[0], tb, page_k, page_v);
-            page_k = page_at(tb + kUnit + 8 * (col >> 2)), page_v = page_at(tb + kUnit + 8 * quad);
-            while (true) {
-                if (tb + kUnit < end) load(tiles[1], tb + kUnit, page_k, page_v);
-                page_k = page_at(tb + 2 * kUnit + 8 * (col >> 2)), page_v = page_at(tb + 2 * kUnit + 8 * quad);
-                step(tiles[0], tb);
-                tb += kUnit;
-                if (tb >= end) break;
-                if (tb + kUnit < end) load(tiles[0], tb + kUnit, page_k, page_v);
-                page_k = page_at(tb + 2 * kUnit + 8 * (col >> 2)), page_v = page_at(tb + 2 * kUnit + 8 * quad);
-                step(tiles[1], tb);
-                tb += kUnit;
-                if (tb >= end) break;
+        // one tile: the next to fetch goes into `into`, the oldest is at `slot`
+        auto step = [&](char *__restrict into, const char *__restrict slot, int tb, int p0, int p1, int next0,
+                        int next1) {
+            if (tb + (kStages - 1) * kUnit < end) {
+                TL::fetch(a.st, h, lane, into, tb + (kStages - 1) * kUnit, next0, next1);
+                wait_loads<(kStages - 1) * TL::kLoads>();
+            } else {
+                wait_loads<0>();
             }
+            const bool ok = (quad < 2 ? p0 : p1) >= 0;
+            if (tb + kTile > all_see || p0 < 0 || p1 < 0)
+                compute(slot, tb, ok, std::true_type{});
+            else
+                compute(slot, tb, ok, std::false_type{});
+        };
+        int slot = 0;
+        for (int tb = begin + kTile * wave; tb < end; tb += kUnit) {
+            constexpr int last = kStages - 1;
+            step(ring + (slot + last) % kStages * TL::kBytes, ring + slot * TL::kBytes, tb, pages[0][0], pages[0][1],
+                 pages[last][0], pages[last][1]);
+            slot = (slot + 1) % kStages;
+#pragma unroll
+            for (int i = 0; i < last; ++i) pages[i][0] = pages[i + 1][0], pages[i][1] = pages[i + 1][1];
+            pages[last][0] = page_at(ahead), pages[last][1] = page_at(ahead + 16);
+            ahead += kUnit;
         }
+        __syncthreads();  // (the ring's memory takes the results)
 
         // the waves' results, joined
 #pragma unroll
