@@ -35,13 +35,14 @@ typedef float float2_t __attribute__((ext_vector_type(2)));
 constexpr int kTile = 32;          // tokens a wave takes at a time
 constexpr int kWaves = 4;          // waves of a workgroup
 constexpr int kUnit = kTile * kWaves;
-constexpr int kMaxSplits = 64;
 constexpr int kStages = 4;         // tiles of a wave in LDS, one computed while the others arrive
 constexpr int kNt = 2;             // cache policy of the stream: non-temporal
 // How far, in log2, a score may pass the running maximum before the maximum
 // moves: probabilities stay below 2^4, so p * scale stays within fp16 with
 // scales normalised to 2^10.
 constexpr float kLag = 4.f;
+// Columns of at most kWhole units are not cut; parts have at least kMinShare.
+constexpr int kWhole = 4, kMinShare = 2;
 
 struct PagedAttn {
     PagedStore st;
@@ -52,10 +53,10 @@ struct PagedAttn {
     int64_t width, n_tokens;
     int n_req, hq, rep, q_dtype, causal, zero_rest, vec;
     float scale;
-    int splits, chunk;  // grid's splits; tokens of a split (a multiple of kUnit)
-    int row_cap;        // rows a KV head that the workspace holds
-    float *acc;         // [n_req][heads][row_cap][splits][D]
-    float *ml;          // [n_req][heads][row_cap][splits][2]
+    int most_rows;      // requests with more query rows a KV head are not this kernel's
+    int4 *cut;          // [workgroups]: the column that a workgroup leaves to be joined
+    float *acc;         // [workgroups][2][rows of a workgroup][D]
+    float *ml;          // [workgroups][2][rows of a workgroup][2]
 };
 
 // Tables do not change while the kernel runs: through the constant address
@@ -72,28 +73,45 @@ __device__ __forceinline__ uint4 load_query8(const uint16_t *p, int vec) {
                       p[4] | ((uint32_t)p[5] << 16), p[6] | ((uint32_t)p[7] << 16));
 }
 
-// A request's rows, length and splits, from the tables on the device.
+// A request, from the tables on the device: its query rows a KV head, in
+// blocks of `rows_per_block`, and the units of its tokens.
 struct Request {
-    int t0, n, n_all, len, rows, splits, chunk;
+    int t0, n, n_all, len, rows, blocks, units;
 };
 
-__device__ __forceinline__ Request request(const PagedAttn &a, int r) {
+__device__ __forceinline__ Request request(const PagedAttn &a, int r, int rows_per_block) {
     Request q;
     q.t0 = table_read(a.starts, r);
     q.n_all = table_read(a.starts, r + 1) - q.t0;
     q.n = q.t0 < 0 ? 0 : (int)max((int64_t)0, min((int64_t)q.n_all, a.n_tokens - q.t0));
     q.len = (int)max((int64_t)0, min((int64_t)table_read(a.lengths, r), a.width << a.st.log_page));
     q.rows = q.n * a.rep;
-    // more tokens than the launch was sized for: longer splits; more rows than
-    // the workspace holds: one split, which writes the rows itself
-    const int need = (q.len + a.splits - 1) / a.splits;
-    q.chunk = max(a.chunk, (need + kUnit - 1) / kUnit * kUnit);
-    q.splits = max(1, (q.len + q.chunk - 1) / q.chunk);
-    if (q.rows > a.row_cap) {
-        q.splits = 1;
-        q.chunk = INT32_MAX;
-    }
+    q.blocks = q.rows > a.most_rows ? 0 : (q.rows + rows_per_block - 1) / rows_per_block;
+    q.units = max(1, (q.len + kUnit - 1) / kUnit);
     return q;
+}
+
+// Columns of a request (0 if it adds no rows), each of `units` units.
+__device__ __forceinline__ int columns_of(const Request &q, int heads) { return q.blocks * heads; }
+
+// Inclusive sum over the lanes before (lane moves, no LDS).
+__device__ __forceinline__ int wave_scan(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);  // row_shr:1
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // row_bcast:15 -> rows 1, 3
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // row_bcast:31 -> rows 2, 3
+    return v;
+}
+
+__device__ __forceinline__ int uniform_div(int a, int b) {
+    return __builtin_amdgcn_readfirstlane((int)((uint32_t)a / (uint32_t)b));
+}
+
+// Parts of a column of `units` units at `share` units a part.
+__device__ __forceinline__ int parts_of(int units, int share) {
+    return units <= kWhole ? 1 : (int)(((uint32_t)units + (uint32_t)share - 1) / (uint32_t)share);
 }
 
 // s_waitcnt vmcnt(N), the other counters unconstrained.
@@ -186,6 +204,18 @@ __device__ __forceinline__ void read_words(const char *p, uint32_t (&w)[N]) {
     }
 }
 
+// Halves of a (scale, zero) pair.
+template <bool BF>
+__device__ __forceinline__ float low16(uint32_t u) {
+    if (BF) return __uint_as_float(u << 16);
+    return (float)__builtin_bit_cast(half2_t, u)[0];
+}
+template <bool BF>
+__device__ __forceinline__ float high16(uint32_t u) {
+    if (BF) return __uint_as_float(u & 0xffff0000u);
+    return (float)__builtin_bit_cast(half2_t, u)[1];
+}
+
 template <int N>
 __device__ __forceinline__ float column_max(const float (&x)[N]) {
     float m = x[0];
@@ -212,10 +242,17 @@ __device__ __forceinline__ float groups_sum(float v) {
     return v;
 }
 
-// One workgroup: split blockIdx.x of the tokens of (request blockIdx.z, KV
-// head), for NS column sets of 16/G query rows that share the stream.  Its
-// waves take 32-token tiles in turn, the next tile's loads in flight while
-// one is computed, and their results are joined through LDS at the end.
+// A column is (request, KV head, block of query rows); its tokens are units of
+// 128.  A workgroup takes a run of units: a part of one column, or, where
+// there are many columns, an even share of all their units, which may hold
+// several columns and end inside one.  Parts are joined by
+// paged_merge_kernel.  So uneven requests load the device evenly, and the host
+// need not know their lengths.
+//
+// In a part of a column the waves take 32-token tiles in turn, each
+// through a ring of its own in LDS that HBM streams into while older tiles
+// are computed; their results are joined through LDS at the end.  NS sets of
+// 16/G query rows share the stream.
 template <int D, int G, bool BF, int NS>
 __global__ void __launch_bounds__(256, 2) paged_attn_kernel(const PagedAttn a) {
     constexpr int RS = 16 / G;       // rows of a column set
@@ -233,31 +270,108 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(const PagedAttn a) {
     const int col = lane & 15, quad = lane >> 4;
     const int g = col % G;
     const bool in_group = quad * G / 4 == g;  // the lane's dims, and its rows of O, are in the column's group
-    const int heads = a.st.heads, log_page = a.st.log_page, in_page = (1 << log_page) - 1;
-    const int h = blockIdx.y % heads, r = blockIdx.z, split = blockIdx.x;
-    const int blocks = gridDim.y / heads;
-
-    if (a.zero_rest && r == a.n_req - 1 && split == 0 && (int)blockIdx.y < heads) {
+    const int heads = a.st.heads, log_page = a.st.log_page;
+    if (a.zero_rest) {
         const int64_t from = max(0, table_read(a.starts, a.n_req));
-        const int64_t per = (int64_t)a.rep * D;  // outputs of this KV head in a row, contiguous
-        for (int64_t e = threadIdx.x; e < (a.n_tokens - from) * per; e += 256) {
-            const int64_t t = e / per;
-            store_from_f32(a.out, a.q_dtype, ((from + t) * a.hq + h * a.rep) * D + (e - t * per), 0.f);
-        }
+        const int64_t row = (int64_t)a.hq * D;
+        for (int64_t e = from * row + blockIdx.x * 256 + threadIdx.x; e < a.n_tokens * row; e += gridDim.x * 256)
+            store_from_f32(a.out, a.q_dtype, e, 0.f);
     }
-    const Request rq = request(a, r);
-    if (rq.rows == 0 || split >= rq.splits) return;
-    const int begin = split * rq.chunk;
-    const int end = (int)min((int64_t)begin + rq.chunk, (int64_t)rq.len);
-    const int32_t *row_table = a.table + (int64_t)r * a.width;
 
-    char *ring = lds + wave * kStages * TL::kBytes;
-    // Page of the 16 tokens from `token`; -1 if the table names none of the pool.
-    auto page_at = [&](int token) {
-        const int p = table_read(row_table, min((int64_t)(token >> log_page), a.width - 1));
-        return (uint32_t)p < (uint32_t)a.st.n_pages ? p : -1;
-    };
-    for (int rb = blockIdx.y / heads; rb * ROWS < rq.rows; rb += blocks) {
+    // This workgroup's run of units [u, stop), and the request r it starts in,
+    // whose units start at `base`: every wave works it out by itself, a few
+    // requests a lane.
+    const int groups = gridDim.x, per = (a.n_req + 63) / 64;
+    const int r0 = min(lane * per, a.n_req), r1 = min(r0 + per, a.n_req);
+    int units = 0, columns = 0;  // of the lane's requests
+    for (int i = r0; i < r1; ++i) {
+        const Request q = request(a, i, ROWS);
+        const int n = columns_of(q, heads);
+        units += q.units * n, columns += n;
+    }
+    const int units_scan = wave_scan(units);
+    const int total = __builtin_amdgcn_readlane(units_scan, 63);
+    const int all_columns = __builtin_amdgcn_readlane(wave_scan(columns), 63);
+    int u, stop, base, r, share, parts = 0;
+    if (all_columns <= groups / 2) {
+        // Few columns: each is cut into parts of its own, of at most `share`
+        // units, so that no workgroup has more than one.  Sum of ceil(n/share)
+        // is at most total/share + columns, and about total/share + columns/2.
+        auto items = [&](int share) {
+            int n = 0;
+            for (int i = r0; i < r1; ++i) {
+                const Request q = request(a, i, ROWS);
+                n += columns_of(q, heads) * parts_of(q.units, share);
+            }
+            return n;
+        };
+        share = max(uniform_div(total + groups - all_columns / 2 - 1, groups - all_columns / 2), kMinShare);
+        int scan = wave_scan(items(share));
+        if (__builtin_amdgcn_readlane(scan, 63) > groups) {
+            share = max(uniform_div(total + groups - all_columns - 1, groups - all_columns), kMinShare);
+            scan = wave_scan(items(share));
+        }
+        const int item = blockIdx.x;
+        if (item >= __builtin_amdgcn_readlane(scan, 63)) {
+            u = stop = base = r = 0;
+        } else {
+            const int holder = __ffsll((unsigned long long)__ballot(item < scan)) - 1;
+            int left = item - (holder ? __builtin_amdgcn_readlane(scan, holder - 1) : 0);
+            base = holder ? __builtin_amdgcn_readlane(units_scan, holder - 1) : 0;
+            for (r = holder * per;; ++r) {
+                const Request q = request(a, r, ROWS);
+                const int n = columns_of(q, heads);
+                parts = __builtin_amdgcn_readfirstlane(parts_of(q.units, share));
+                if (left < n * parts) {
+                    const int column = uniform_div(left, parts), part = left - column * parts;
+                    u = base + column * q.units;
+                    stop = u + uniform_div((part + 1) * q.units, parts);
+                    u += uniform_div(part * q.units, parts);
+                    break;
+                }
+                left -= n * parts, base += n * q.units;
+            }
+        }
+    } else {
+        // Many: the units of all columns in one row, shared out evenly; a run
+        // may end inside a column and may hold several.
+        share = max(uniform_div(total + groups - 1, groups), kWhole);
+        u = min((int64_t)blockIdx.x * share, (int64_t)total);
+        stop = min((int64_t)u + share, (int64_t)total);
+        const uint64_t holds = __ballot(u < units_scan);
+        const int holder = holds ? __ffsll((unsigned long long)holds) - 1 : 0;
+        base = holder ? __builtin_amdgcn_readlane(units_scan, holder - 1) : 0;
+        r = holder * per;
+    }
+    const int first_unit = u;
+    int4 cut = make_int4(0, 0, 0, 0);
+
+    while (u < stop) {
+        const Request rq = request(a, r, ROWS);
+        const int in_request = columns_of(rq, heads) * rq.units;
+        if (u >= base + in_request) {
+            base += in_request, ++r;
+            continue;
+        }
+        const int column = uniform_div(u - base, rq.units);
+        const int c0 = base + column * rq.units, c1 = c0 + rq.units;
+        const int h = uniform_div(column, rq.blocks), rb = column - h * rq.blocks;
+        const int begin = (u - c0) * kUnit;
+        const int part_end = min(stop, c1);
+        const int end = min((part_end - c0) * kUnit, rq.len);
+        const bool whole = c0 >= first_unit && c1 <= stop;
+        const int place = c0 < first_unit ? 0 : 1;  // of this part, if it is one
+        if (!whole && place == 1)
+            cut = make_int4(parts ? parts : uniform_div(c1 - 1, share) - (int)blockIdx.x + 1, r, h, rb);
+        u = part_end;
+        const int32_t *row_table = a.table + (int64_t)r * a.width;
+
+        char *ring = lds + wave * kStages * TL::kBytes;
+        // Page of the 16 tokens from `token`; -1 if the table names none of the pool.
+        auto page_at = [&](int token) {
+            const int p = table_read(row_table, min((int64_t)(token >> log_page), a.width - 1));
+            return (uint32_t)p < (uint32_t)a.st.n_pages ? p : -1;
+        };
         // queries first: what is loaded later would hold them back
         int limit[NS];  // tokens that the column's row sees
         uint4 raw[NS][KS];
@@ -278,12 +392,19 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(const PagedAttn a) {
 #pragma unroll
         for (int i = 0; i < kStages; ++i) {
             pages[i][0] = page_at(ahead), pages[i][1] = page_at(ahead + 16);
-            if (i < kStages - 1 && ahead < end) TL::fetch(a.st, h, lane, ring + i * TL::kBytes, ahead, pages[i][0], pages[i][1]);
             ahead += kUnit;
+        }
+        // The queries, here and not where they are used: by then they would wait
+        // for the tiles too.
+        wait_loads<0>();
+#pragma unroll
+        for (int i = 0; i < kStages - 1; ++i) {
+            const int t = begin + kTile * wave + i * kUnit;
+            if (t < end) TL::fetch(a.st, h, lane, ring + i * TL::kBytes, t, pages[i][0], pages[i][1]);
         }
         int all_see = rq.len;
         half8_t qf[NS][KS];
-        float qz[NS], factor[NS];
+        float qz[NS], factor[NS], lag[NS];
 #pragma unroll
         for (int s = 0; s < NS; ++s) {
             float x[KS][8], top = 0.f, sum = 0.f;
@@ -301,31 +422,42 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(const PagedAttn a) {
             // a power of two brings the row into fp16's range: 16-bit
             // queries stay exact
             const int shift = row_exp_shift(lanes4_max(top));
-            const float down = exp2i(-shift);
+            const float down = a.scale < 0.f ? -exp2i(-shift) : exp2i(-shift);
 #pragma unroll
             for (int k = 0; k < KS; ++k)
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    const float y = in_group ? x[k][e] * down : 0.f;
+                    const float y = in_group ? x[k][e] * down : 0.f;  // (down: its sign is the scale's)
                     sum += y;
                     qf[s][k][e] = (_Float16)((e & 2) ? y * 0x1p-4f : y);
                 }
             qz[s] = lanes4_sum(sum) * 0x1p-24f;
-            factor[s] = a.scale * kLog2e * 0x1p24f * exp2i(shift);
+            factor[s] = fmaxf(fabsf(a.scale) * kLog2e * 0x1p24f * exp2i(shift), 1e-30f);
+            lag[s] = kLag / factor[s];
         }
         // (limits grow with the row: the first row's is the smallest)
         if (a.causal) all_see = max(0, min(rq.len, rq.len - rq.n_all + rb * ROWS / a.rep + 1));
 
+        // The sums are kept times 2^(10 - vexp): vexp is above every value scale
+        // (as a power of two) that the column's group has met, so p * scale
+        // stays within fp16 whatever the scales.  top is in units of S.
         float top[NS], l_even[NS], l_odd[NS], z_even[NS], z_odd[NS];
-        float4_t o[NS][VT];
+        float4_t o[NS][VT], ones[NS];
 #pragma unroll
         for (int s = 0; s < NS; ++s) {
             top[s] = -INFINITY;
             l_even[s] = l_odd[s] = z_even[s] = z_odd[s] = 0.f;
+            ones[s] = float4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int j = 0; j < VT; ++j) o[s][j] = float4_t{0.f, 0.f, 0.f, 0.f};
         }
-        float vlim = 0.f;  // power of two, above every value scale seen in the column's group
+        int vexp = -60;
+        auto rescale = [&](int s, float f) {
+            l_even[s] *= f, l_odd[s] *= f, z_even[s] *= f, z_odd[s] *= f;
+            ones[s] *= f;
+#pragma unroll
+            for (int j = 0; j < VT; ++j) o[s][j] *= f;
+        };
 
         // masked: some row does not see some token of the tile
         auto compute = [&](const char *slot, int tb, bool ok, auto masked) {
@@ -351,36 +483,23 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(const PagedAttn a) {
             }
             read_words(slot + 2 * TL::kCodes + (g * kTile + 8 * quad) * 4, km);
             read_words(slot + 2 * TL::kCodes + TL::kMeta + (g * kTile + 8 * quad) * 4, vm);
-            float ks[8], kz[8], vs[8], vz[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                ks[j] = from_bits16<BF>(km[j] & 0xffffu);
-                kz[j] = from_bits16<BF>(km[j] >> 16);
-                vs[j] = from_bits16<BF>(vm[j] & 0xffffu);
-                vz[j] = from_bits16<BF>(vm[j] >> 16);
-            }
             const int first = tb + 8 * quad;  // the lane's first token
             if (mask) {  // (behind the request's tokens a page may hold anything, NaN too)
 #pragma unroll
                 for (int j = 0; j < 8; ++j)
-                    if (!ok || first + j >= rq.len) vs[j] = 0.f;
+                    if (!ok || first + j >= rq.len) vm[j] = 0;
             }
-            // value scales enter the product times 2^10 / vlim
-            const float vtop = column_max(vs);
-            float vlim_was = vlim;
-            if (__any(vtop > vlim)) {
+            float vtop = low16<BF>(vm[0]);
+#pragma unroll
+            for (int j = 1; j < 8; ++j) vtop = fmaxf(vtop, low16<BF>(vm[j]));
+            if (__any(vtop > exp2i(vexp))) {
                 const float c = lanes4_max(vtop);
-                if (c > vlim) {
-                    const int e = (int)((__float_as_uint(c) >> 23) & 0xffu) - 126;  // c < 2^e
-                    vlim = exp2i(max(-100, min(126, e)));
-                }
-                const float f = vlim_was > 0.f ? vlim_was / vlim : 1.f;
+                const int e = (int)((__float_as_uint(c) >> 23) & 0xffu) - 126;  // c < 2^e
+                const int now = max(vexp, min(e, 126));
 #pragma unroll
-                for (int s = 0; s < NS; ++s)
-#pragma unroll
-                    for (int j = 0; j < VT; ++j) o[s][j] *= f;
+                for (int s = 0; s < NS; ++s) rescale(s, ldexpf(1.f, vexp - now));
+                vexp = now;
             }
-            const float vn = vlim > 0.f ? 0x1p10f / vlim : 0.f;
             half8_t p16[NS];
 #pragma unroll
             for (int s = 0; s < NS; ++s) {
@@ -393,8 +512,8 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(const PagedAttn a) {
                         d = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes_operand(kw[y][k]), qf[s][k], d, 0, 0, 0);
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        const int j = 4 * y + i;
-                        x[j] = groups_sum<G>(fmaf(d[i], ks[j], kz[j] * qz[s])) * factor[s];
+                        const uint32_t m = km[4 * y + i];
+                        x[4 * y + i] = groups_sum<G>(fmaf(low16<BF>(m), d[i], high16<BF>(m) * qz[s]));
                     }
                 }
                 if (mask) {
@@ -404,38 +523,38 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(const PagedAttn a) {
                         if (first + j >= see) x[j] = -INFINITY;
                 }
                 const float m = column_max(x);
-                if (__any(m > top[s] + kLag)) {
+                if (__any(m > top[s] + lag[s])) {
                     const float now = fmaxf(top[s], lanes4_max(m));
-                    const float f = now == top[s] ? 1.f : fast_exp2(top[s] - now);
+                    rescale(s, now == top[s] ? 1.f : fast_exp2((top[s] - now) * factor[s]));
                     top[s] = now;
-                    l_even[s] *= f, l_odd[s] *= f, z_even[s] *= f, z_odd[s] *= f;
-#pragma unroll
-                    for (int j = 0; j < VT; ++j) o[s][j] *= f;
                 }
                 // pairs (2,3) and (6,7), whose codes count 16 times, at 2^-4
-                const float even = top[s] == -INFINITY ? 0.f : top[s], odd = even + 4.f;
+                const float even = (float)(10 - vexp) - (top[s] == -INFINITY ? 0.f : top[s] * factor[s]);
                 float w[8];
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
-                    const float p = fast_exp2(x[j] - ((j & 2) ? odd : even));
-                    // (a token that the row does not see adds nothing, whatever its value holds)
-                    const bool off = mask && (!ok || first + j >= limit[s]);
-                    const float z = off ? 0.f : vz[j];
+                    const float p = fast_exp2(fmaf(x[j], factor[s], (j & 2) ? even - 4.f : even));
+                    // the value's middle, zero + 7.5 scale, in float32: what is
+                    // left for the product, (code - 7.5) scale, is small
+                    float mid = fmaf(low16<BF>(vm[j]), 7.5f, high16<BF>(vm[j]));
+                    w[j] = p * low16<BF>(vm[j]);
+                    if (mask && (!ok || first + j >= limit[s])) mid = w[j] = 0.f;  // (even of NaN)
                     if (j & 2) {
                         l_odd[s] += p;
-                        z_odd[s] = fmaf(p, z, z_odd[s]);
+                        z_odd[s] = fmaf(p, mid, z_odd[s]);
                     } else {
                         l_even[s] += p;
-                        z_even[s] = fmaf(p, z, z_even[s]);
+                        z_even[s] = fmaf(p, mid, z_even[s]);
                     }
-                    w[j] = off ? 0.f : p * (vs[j] * vn);
                 }
-                // one rounding to fp16 (2^-11 of the term): the sums stay float32
+                // one rounding to fp16, 2^-11 of w (code - 7.5): 7.5 times the
+                // sum of the rounded w is taken off again at the end
 #pragma unroll
                 for (int j = 0; j < 8; j += 2) {
                     const half2_t hh = __builtin_convertvector(float2_t{w[j], w[j + 1]}, half2_t);
                     p16[s][j] = hh[0], p16[s][j + 1] = hh[1];
                 }
+                ones[s] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes_operand(0x11111111u), p16[s], ones[s], 0, 0, 0);
             }
 #pragma unroll
             for (int j = 0; j < VT; ++j) {
@@ -472,22 +591,22 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(const PagedAttn a) {
             pages[last][0] = page_at(ahead), pages[last][1] = page_at(ahead + 16);
             ahead += kUnit;
         }
-        __syncthreads();  // (the ring's memory takes the results)
+        __syncthreads();  // the ring's memory takes the results
 
         // the waves' results, joined
 #pragma unroll
         for (int s = 0; s < NS; ++s) {
-            const float l = lanes4_sum(l_even[s] + 16.f * l_odd[s]);
-            const float z = lanes4_sum(z_even[s] + 16.f * z_odd[s]);
+            const float l = ldexpf(lanes4_sum(l_even[s] + 16.f * l_odd[s]), vexp - 10);
+            const float z = ldexpf(lanes4_sum(z_even[s] + 16.f * z_odd[s]), vexp - 10);
             const int row = s * RS + col / G;
-            if (g == 0 && quad == 0) stats[wave][row][0] = top[s], stats[wave][row][1] = l;
+            if (g == 0 && quad == 0) stats[wave][row][0] = top[s] * factor[s], stats[wave][row][1] = l;
             if (in_group) {
                 // tile j, element i: dim (4 * quad + i) * D/16 + j
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
 #pragma unroll
                     for (int j = 0; j < VT; ++j)
-                        part[wave][row][(4 * quad + i) * VT + j] = o[s][j][i] * 0x1p14f * vlim + z;
+                        part[wave][row][(4 * quad + i) * VT + j] = ldexpf(o[s][j][i] - 7.5f * ones[s][i], vexp + 14) + z;
             }
         }
         __syncthreads();
@@ -505,100 +624,103 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(const PagedAttn a) {
 #pragma unroll
                 for (int k = 0; k < 4; ++k) x[k] += f * part[w][row][c + k];
             }
-            if (rq.splits == 1) {
+            if (whole) {
                 const float inv = l == 0.f ? 0.f : 1.f / l;
                 const int64_t at = ((int64_t)(rq.t0 + n / a.rep) * a.hq + h * a.rep + n % a.rep) * D + c;
                 store4_from_f32(a.out, a.q_dtype, at, x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
             } else {
-                const int64_t at = (((int64_t)r * heads + h) * a.row_cap + n) * a.splits + split;
+                const int64_t at = ((int64_t)blockIdx.x * 2 + place) * ROWS + row;
                 *reinterpret_cast<float4 *>(a.acc + at * D + c) = make_float4(x[0], x[1], x[2], x[3]);
                 if (c == 0) *reinterpret_cast<float2 *>(a.ml + at * 2) = make_float2(m, l);
             }
         }
         __syncthreads();
     }
+    if (threadIdx.x == 0) a.cut[blockIdx.x] = cut;
 }
 
-// The rows of requests that were split, one workgroup a row: every thread
-// loads four dims of its splits at once, 8 (D 128) or 16 threads a dim.
+// Joins the parts of the column that workgroup blockIdx.y of the kernel above
+// began and did not end (its second place, then the first place of those that
+// follow), one row (blockIdx.x) a workgroup: every thread loads four dims of
+// its parts at once, 8 (D 128) or 16 threads a dim.
 template <int D>
-__global__ void __launch_bounds__(256) paged_merge_kernel(const PagedAttn a) {
-    constexpr int CH = D / 4, PARTS = 256 / CH, PER = kMaxSplits / PARTS;
+__global__ void __launch_bounds__(256) paged_merge_kernel(const PagedAttn a, int rows_per_block) {
+    constexpr int CH = D / 4, PARTS = 256 / CH, PER = 8, STEP = PARTS * PER;
     __shared__ float red[PARTS][D + 4];
-    __shared__ float weight[kMaxSplits];
-    __shared__ float total;
-    const int r = blockIdx.y, heads = a.st.heads;
-    const Request rq = request(a, r);
-    if (rq.splits == 1) return;
-    const int c = threadIdx.x % CH * 4, p = threadIdx.x / CH;
-    for (int e = blockIdx.x; e < rq.rows * heads; e += gridDim.x) {
-        const int h = e % heads, n = e / heads;
-        const int64_t at = (((int64_t)r * heads + h) * a.row_cap + n) * a.splits;
-        float4 v[PER];
+    __shared__ float total[PARTS], tops[kWaves];
+    const int4 cut = a.cut[blockIdx.y];
+    const int parts = cut.x, r = cut.y, h = cut.z, row = blockIdx.x, n = cut.w * rows_per_block + row;
+    if (parts == 0) return;
+    const Request rq = request(a, r, rows_per_block);
+    if (n >= rq.rows) return;
+    auto at = [&](int i) {
+        return (((int64_t)blockIdx.y + i) * 2 + (i == 0 ? 1 : 0)) * rows_per_block + row;
+    };
+    const int c = threadIdx.x % CH * 4, p = threadIdx.x / CH, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    float4 v[PER];
 #pragma unroll
-        for (int i = 0; i < PER; ++i)
-            v[i] = *reinterpret_cast<const float4 *>(a.acc + (at + min(p + i * PARTS, rq.splits - 1)) * D + c);
-        if (threadIdx.x < 64) {
-            const bool in = (int)threadIdx.x < rq.splits;
-            const float2 s = *reinterpret_cast<const float2 *>(a.ml + (at + min((int)threadIdx.x, rq.splits - 1)) * 2);
-            const float m = wave_max(in ? s.x : -INFINITY);
-            const float f = in ? (s.x == m ? 1.f : fast_exp2(s.x - m)) : 0.f;
-            weight[threadIdx.x] = f;
-            const float l = wave_sum(in ? f * s.y : 0.f);
-            if (threadIdx.x == 0) total = l;
-        }
-        __syncthreads();
-        float x[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < PER; ++i)
+        v[i] = *reinterpret_cast<const float4 *>(a.acc + at(min(p + i * PARTS, parts - 1)) * D + c);
+    float m = -INFINITY;
+    for (int i = threadIdx.x; i < parts; i += 256) m = fmaxf(m, a.ml[at(i) * 2]);
+    m = wave_max(m);
+    if (lane == 0) tops[wave] = m;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) m = fmaxf(m, tops[w]);
+    float x[4] = {0.f, 0.f, 0.f, 0.f}, l = 0.f;
+    for (int from = 0; from < parts; from += STEP) {
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
-            const int s = p + i * PARTS;
-            if (s >= rq.splits) break;
-            const float f = weight[s];
+            const int s = from + p + i * PARTS;
+            if (s >= parts) break;
+            const float2 e = *reinterpret_cast<const float2 *>(a.ml + at(s) * 2);
+            const float f = e.x == m ? 1.f : fast_exp2(e.x - m);
+            l += f * e.y;
             x[0] += f * v[i].x, x[1] += f * v[i].y, x[2] += f * v[i].z, x[3] += f * v[i].w;
         }
+        if (from + STEP < parts)
 #pragma unroll
-        for (int k = 0; k < 4; ++k) red[p][c + k] = x[k];
-        __syncthreads();
-        if (threadIdx.x < CH) {
-            float y[4] = {0.f, 0.f, 0.f, 0.f};
+            for (int i = 0; i < PER; ++i)
+                v[i] = *reinterpret_cast<const float4 *>(a.acc + at(min(from + STEP + p + i * PARTS, parts - 1)) * D + c);
+    }
 #pragma unroll
-            for (int i = 0; i < PARTS; ++i)
+    for (int k = 0; k < 4; ++k) red[p][c + k] = x[k];
+    if (c == 0) total[p] = l;
+    __syncthreads();
+    if (threadIdx.x < CH) {
+        float y[4] = {0.f, 0.f, 0.f, 0.f}, t = 0.f;
 #pragma unroll
-                for (int k = 0; k < 4; ++k) y[k] += red[i][c + k];
-            const float inv = total == 0.f ? 0.f : 1.f / total;
-            const int64_t o = ((int64_t)(rq.t0 + n / a.rep) * a.hq + h * a.rep + n % a.rep) * D + c;
-            store4_from_f32(a.out, a.q_dtype, o, y[0] * inv, y[1] * inv, y[2] * inv, y[3] * inv);
+        for (int i = 0; i < PARTS; ++i) {
+            t += total[i];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) y[k] += red[i][c + k];
         }
-        __syncthreads();
+        const float inv = t == 0.f ? 0.f : 1.f / t;
+        const int64_t o = ((int64_t)(rq.t0 + n / a.rep) * a.hq + h * a.rep + n % a.rep) * D + c;
+        store4_from_f32(a.out, a.q_dtype, o, y[0] * inv, y[1] * inv, y[2] * inv, y[3] * inv);
     }
 }
 
 // -------------------------------------------------------------------- host
 
 struct PagedPlan {
-    int sets, blocks, splits, chunk, row_cap;
+    int sets, rows, groups;  // column sets, query rows a workgroup takes; workgroups
     size_t bytes;
 };
 
-// Launch shape from the hints.  Workgroups are cheap to leave, so the splits
-// aim at enough of them to fill the device when every request is as long as
-// the longest.
+// Launch shape: as many workgroups as the device holds at once (two a compute
+// unit), or as the hints' units need.
 static PagedPlan paged_plan(const ss_paged_store *s, int64_t n_requests, int n_q_heads, int64_t max_new,
                             int64_t max_length) {
     PagedPlan p;
     const int rep = n_q_heads / s->n_kv_heads, rs = 16 / (s->head_dim / s->group_size);
-    const int64_t rows = max_new * rep;
-    p.sets = rows > rs ? 2 : 1;
-    p.blocks = (int)max((int64_t)1, min((rows + p.sets * rs - 1) / (p.sets * rs), (int64_t)64));
-    p.row_cap = p.blocks * p.sets * rs;
-    const int64_t groups = n_requests * s->n_kv_heads * p.blocks;
-    const int64_t want = (4 * device_cu_count() + groups - 1) / groups;
-    const int64_t most = max((int64_t)1, min((int64_t)kMaxSplits, max_length / (2 * kUnit)));
-    const int64_t n = max((int64_t)1, min(want, most));
-    p.chunk = (int)(((max_length + n - 1) / n + kUnit - 1) / kUnit * kUnit);
-    p.chunk = max(p.chunk, kUnit);
-    p.splits = (int)n;
-    p.bytes = p.splits > 1 ? (size_t)n_requests * s->n_kv_heads * p.row_cap * p.splits * (s->head_dim + 2) * 4 : 0;
+    p.sets = max_new * rep > rs ? 2 : 1;
+    p.rows = p.sets * rs;
+    const double units = (double)n_requests * s->n_kv_heads * ((max_new * rep + p.rows - 1) / p.rows) *
+                         ((max_length + kUnit - 1) / kUnit);
+    p.groups = (int)min((double)(2 * device_cu_count()), units / kMinShare + 1);
+    p.bytes = (size_t)p.groups * (16 + 2 * p.rows * (s->head_dim + 2) * 4);
     return p;
 }
 
@@ -615,13 +737,12 @@ static int check_hints(const ss_paged_store *s, int64_t n_requests, int n_q_head
 
 template <int D, int G, bool BF>
 static void launch_paged(const PagedAttn &a, const PagedPlan &p, hipStream_t st) {
-    const dim3 grid(p.splits, a.st.heads * p.blocks, a.n_req);
     if (p.sets == 1)
-        hipLaunchKernelGGL((paged_attn_kernel<D, G, BF, 1>), grid, dim3(256), 0, st, a);
+        hipLaunchKernelGGL((paged_attn_kernel<D, G, BF, 1>), dim3(p.groups), dim3(256), 0, st, a);
     else
-        hipLaunchKernelGGL((paged_attn_kernel<D, G, BF, 2>), grid, dim3(256), 0, st, a);
-    if (p.splits > 1)
-        hipLaunchKernelGGL(paged_merge_kernel<D>, dim3(p.row_cap * a.st.heads, a.n_req), dim3(256), 0, st, a);
+        hipLaunchKernelGGL((paged_attn_kernel<D, G, BF, 2>), dim3(p.groups), dim3(256), 0, st, a);
+    if (p.groups > 1)
+        hipLaunchKernelGGL(paged_merge_kernel<D>, dim3(p.rows, p.groups), dim3(256), 0, st, a, p.rows);
 }
 
 }  // namespace ss
@@ -653,6 +774,11 @@ extern "C" int ss_paged_attn(const ss_paged_store *store, const void *q, int q_d
     SS_REQUIRE(q && out && block_table && lengths && token_starts, "null pointer argument");
     SS_REQUIRE(table_width >= 1, "bad block table width");
     SS_UNSUPPORTED(table_width <= (1 << 30) / store->page_size, "a table row of more than 2^30 tokens");
+    // every unit of every column is counted in 32 bits
+    SS_UNSUPPORTED(((double)n_requests + (double)n_tokens * (n_q_heads / store->n_kv_heads)) * store->n_kv_heads *
+                           ((double)table_width * store->page_size / kUnit + 1) <
+                       2147483648.0,
+                   "too many requests and tokens for one launch");
     const PagedPlan p = paged_plan(store, n_requests, n_q_heads, max_new, max_length);
     if (p.bytes > workspace_bytes || (p.bytes && !workspace)) {
         set_error("workspace of %zu bytes, %zu needed", workspace_bytes, p.bytes);
@@ -665,9 +791,10 @@ extern "C" int ss_paged_attn(const ss_paged_store *store, const void *q, int q_d
     a.hq = n_q_heads, a.rep = n_q_heads / store->n_kv_heads;
     a.q_dtype = q_dtype, a.causal = causal, a.zero_rest = zero_rest, a.scale = scale;
     a.vec = ((uintptr_t)q & 15) == 0 && q_st % 8 == 0 && q_sh % 8 == 0;
-    a.splits = p.splits, a.chunk = p.chunk, a.row_cap = p.row_cap;
-    a.acc = static_cast<float *>(workspace);
-    a.ml = a.acc + (size_t)n_requests * store->n_kv_heads * p.row_cap * p.splits * store->head_dim;
+    a.most_rows = INT32_MAX;
+    a.cut = static_cast<int4 *>(workspace);
+    a.acc = reinterpret_cast<float *>(a.cut + p.groups);
+    a.ml = a.acc + (size_t)p.groups * 2 * p.rows * store->head_dim;
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
     const bool bf = store->dtype == SS_BF16;
     const int key = store->head_dim * 1000 + store->group_size;
