@@ -40,7 +40,8 @@ COMMON_FLAGS = [
 # softmax consume every matrix-core result on the vector ALUs, so these are
 # kept in VGPRs (no v_accvgpr_read per element)
 FILE_FLAGS = {"encode.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
-              "paged_attn.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
+              "paged_attn.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+              "paged_prompt.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
 
 
 def hipcc() -> str:

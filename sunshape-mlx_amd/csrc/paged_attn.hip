@@ -1,132 +1,40 @@
 // Attention over a paged cache of 4-bit keys and values: the few query rows
-// of decode steps and speculative verification (paged_prompt.hip takes the
-// many rows of prompts).
+// of decode steps and speculative verification (paged_attn.hpp has the
+// formulas, paged_prompt.hip the many rows of prompts).
 //
-//   S[r][t] = sum_g s_tg (q_rg . c_tg) + z_tg sum(q_rg)
-//   O[r][d] = sum_t (p_rt s'_tg) c'_td + sum_t p_rt z'_tg,   g = d's group
-//
-// with c the keys' codes, s and z their scales and zeros (primed: the
-// values').  Codes enter the matrix cores as they are: a 4-bit code in the
-// low bits of a 16-bit half is the fp16 subnormal c * 2^-24, one place
-// further left c * 2^-20, and v_mfma_f32_16x16x32_f16 takes subnormals
-// exactly, so two masks and half a shift turn eight codes into the four
-// registers of an operand and no code is ever converted.  The factor 16
-// between the places is taken from the other operand (queries, respectively
-// probabilities, of odd pairs times 2^-4); 2^24 goes into the factors that
-// the sums are multiplied by in any case.
-//
-// Scales stay out of the operands: the 16 columns of both products are
-// (row r, group g), a query entering column (r, g) with the dims of group g
-// alone.  Keys are the A operand (16 tokens), so a lane holds, of one column,
-// 4 tokens of each key tile; two key tiles whose token order is chosen so
-// make exactly the lane's 8 tokens of the second product's B operand: the
-// probabilities never leave the lane's registers.
+// Value codes enter the second product unconverted too, so scales stay out of
+// the operands: the 16 columns of both products are (row r, group g), a query
+// entering column (r, g) with the dims of group g alone, a probability times
+// the value's scale in g.  Keys are the A operand (16 tokens), so a lane
+// holds, of one column, 4 tokens of each key tile; two key tiles whose token
+// order is chosen so make exactly the lane's 8 tokens of the second product's
+// B operand: the probabilities never leave the lane's registers.
 #include <type_traits>
 
-#include "paged_common.hpp"
+#include "paged_attn.hpp"
 
 namespace ss {
-
-typedef _Float16 half8_t __attribute__((ext_vector_type(8)));
-typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
-typedef float float4_t __attribute__((ext_vector_type(4)));
-typedef float float2_t __attribute__((ext_vector_type(2)));
 
 constexpr int kTile = 32;          // tokens a wave takes at a time
 constexpr int kWaves = 4;          // waves of a workgroup
 constexpr int kUnit = kTile * kWaves;
 constexpr int kStages = 4;         // tiles of a wave in LDS, one computed while the others arrive
 constexpr int kNt = 2;             // cache policy of the stream: non-temporal
-// How far, in log2, a score may pass the running maximum before the maximum
-// moves: probabilities stay below 2^4, so p * scale stays within fp16 with
-// scales normalised to 2^10.
-constexpr float kLag = 4.f;
+// Query rows a KV head up to which a request is this kernel's.
+constexpr int kPromptRows = 64;
 // Columns of at most kWhole units are not cut; parts have at least kMinShare.
 constexpr int kWhole = 4, kMinShare = 2;
 
-struct PagedAttn {
-    PagedStore st;
-    const void *q;
-    int64_t q_st, q_sh;
-    void *out;
-    const int32_t *table, *lengths, *starts;
-    int64_t width, n_tokens;
-    int n_req, hq, rep, q_dtype, causal, zero_rest, vec;
-    float scale;
-    int most_rows;      // requests with more query rows a KV head are not this kernel's
-    int4 *cut;          // [workgroups]: the column that a workgroup leaves to be joined
-    float *acc;         // [workgroups][2][rows of a workgroup][D]
-    float *ml;          // [workgroups][2][rows of a workgroup][2]
-};
-
-// Tables do not change while the kernel runs: through the constant address
-// space their uniform reads are scalar loads, which do not queue behind the
-// stream of codes.
-__device__ __forceinline__ int table_read(const int32_t *p, int64_t i) {
-    return reinterpret_cast<const __attribute__((address_space(4))) int32_t *>(reinterpret_cast<uintptr_t>(p))[i];
+// Blocks of `rows` query rows a KV head of a request that are this kernel's,
+// and units of its tokens.
+__device__ __forceinline__ int blocks_of(const PagedAttn &a, const Request &q, int rows) {
+    return q.rows > a.most_rows ? 0 : (q.rows + rows - 1) / rows;
 }
-
-// Eight 16-bit query elements from p (16-byte aligned if vec).
-__device__ __forceinline__ uint4 load_query8(const uint16_t *p, int vec) {
-    if (vec) return *reinterpret_cast<const uint4 *>(p);
-    return make_uint4(p[0] | ((uint32_t)p[1] << 16), p[2] | ((uint32_t)p[3] << 16),
-                      p[4] | ((uint32_t)p[5] << 16), p[6] | ((uint32_t)p[7] << 16));
-}
-
-// A request, from the tables on the device: its query rows a KV head, in
-// blocks of `rows_per_block`, and the units of its tokens.
-struct Request {
-    int t0, n, n_all, len, rows, blocks, units;
-};
-
-__device__ __forceinline__ Request request(const PagedAttn &a, int r, int rows_per_block) {
-    Request q;
-    q.t0 = table_read(a.starts, r);
-    q.n_all = table_read(a.starts, r + 1) - q.t0;
-    q.n = q.t0 < 0 ? 0 : (int)max((int64_t)0, min((int64_t)q.n_all, a.n_tokens - q.t0));
-    q.len = (int)max((int64_t)0, min((int64_t)table_read(a.lengths, r), a.width << a.st.log_page));
-    q.rows = q.n * a.rep;
-    q.blocks = q.rows > a.most_rows ? 0 : (q.rows + rows_per_block - 1) / rows_per_block;
-    q.units = max(1, (q.len + kUnit - 1) / kUnit);
-    return q;
-}
-
-// Columns of a request (0 if it adds no rows), each of `units` units.
-__device__ __forceinline__ int columns_of(const Request &q, int heads) { return q.blocks * heads; }
-
-// Inclusive sum over the lanes before (lane moves, no LDS).
-__device__ __forceinline__ int wave_scan(int v) {
-    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);  // row_shr:1
-    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // row_bcast:15 -> rows 1, 3
-    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // row_bcast:31 -> rows 2, 3
-    return v;
-}
-
-__device__ __forceinline__ int uniform_div(int a, int b) {
-    return __builtin_amdgcn_readfirstlane((int)((uint32_t)a / (uint32_t)b));
-}
+__device__ __forceinline__ int units_of(const Request &q) { return max(1, (q.len + kUnit - 1) / kUnit); }
 
 // Parts of a column of `units` units at `share` units a part.
 __device__ __forceinline__ int parts_of(int units, int share) {
     return units <= kWhole ? 1 : (int)(((uint32_t)units + (uint32_t)share - 1) / (uint32_t)share);
-}
-
-// s_waitcnt vmcnt(N), the other counters unconstrained.
-template <int N>
-__device__ __forceinline__ void wait_loads() {
-    static_assert(N >= 0 && N < 64, "vmcnt range");
-    __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | (7 << 4) | (15 << 8));
-}
-
-template <typename T>
-using lds_ptr = __attribute__((address_space(3))) T *;
-
-template <typename T>
-__device__ __forceinline__ lds_ptr<T> as_lds(void *p) {
-    return reinterpret_cast<lds_ptr<T>>(static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p)));
 }
 
 // 32 tokens of one KV head as they lie in LDS: key rows, value blocks, the
@@ -174,55 +82,6 @@ struct TileLds {
         }
     }
 };
-
-// A word's eight codes as the four registers of an operand: pairs (0,1) and
-// (4,5) times 2^-24, (2,3) and (6,7) times 2^-20.
-__device__ __forceinline__ half8_t codes_operand(uint32_t w) {
-    union {
-        uint32_t u[4];
-        half8_t h;
-    } x;
-    const uint32_t hi = w >> 8;
-    x.u[0] = w & 0x000f000fu;
-    x.u[1] = w & 0x00f000f0u;
-    x.u[2] = hi & 0x000f000fu;
-    x.u[3] = hi & 0x00f000f0u;
-    return x.h;
-}
-
-template <int N>
-__device__ __forceinline__ void read_words(const char *p, uint32_t (&w)[N]) {
-    if constexpr (N == 2) {
-        const uint2 u = *reinterpret_cast<const uint2 *>(p);
-        w[0] = u.x, w[1] = u.y;
-    } else {
-#pragma unroll
-        for (int i = 0; i < N / 4; ++i) {
-            const uint4 u = reinterpret_cast<const uint4 *>(p)[i];
-            w[4 * i] = u.x, w[4 * i + 1] = u.y, w[4 * i + 2] = u.z, w[4 * i + 3] = u.w;
-        }
-    }
-}
-
-// Halves of a (scale, zero) pair.
-template <bool BF>
-__device__ __forceinline__ float low16(uint32_t u) {
-    if (BF) return __uint_as_float(u << 16);
-    return (float)__builtin_bit_cast(half2_t, u)[0];
-}
-template <bool BF>
-__device__ __forceinline__ float high16(uint32_t u) {
-    if (BF) return __uint_as_float(u & 0xffff0000u);
-    return (float)__builtin_bit_cast(half2_t, u)[1];
-}
-
-template <int N>
-__device__ __forceinline__ float column_max(const float (&x)[N]) {
-    float m = x[0];
-#pragma unroll
-    for (int i = 1; i < N; ++i) m = fmaxf(m, x[i]);
-    return m;
-}
 
 // Over the four lanes of a column (lane%16 equal).
 __device__ __forceinline__ float lanes4_max(float v) {
@@ -285,9 +144,9 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(const PagedAttn a) {
     const int r0 = min(lane * per, a.n_req), r1 = min(r0 + per, a.n_req);
     int units = 0, columns = 0;  // of the lane's requests
     for (int i = r0; i < r1; ++i) {
-        const Request q = request(a, i, ROWS);
-        const int n = columns_of(q, heads);
-        units += q.units * n, columns += n;
+        const Request q = request(a, i);
+        const int n = blocks_of(a, q, ROWS) * heads;
+        units += units_of(q) * n, columns += n;
     }
     const int units_scan = wave_scan(units);
     const int total = __builtin_amdgcn_readlane(units_scan, 63);
@@ -300,8 +159,8 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(const PagedAttn a) {
         auto items = [&](int share) {
             int n = 0;
             for (int i = r0; i < r1; ++i) {
-                const Request q = request(a, i, ROWS);
-                n += columns_of(q, heads) * parts_of(q.units, share);
+                const Request q = request(a, i);
+                n += blocks_of(a, q, ROWS) * heads * parts_of(units_of(q), share);
             }
             return n;
         };
@@ -319,17 +178,17 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(const PagedAttn a) {
             int left = item - (holder ? __builtin_amdgcn_readlane(scan, holder - 1) : 0);
             base = holder ? __builtin_amdgcn_readlane(units_scan, holder - 1) : 0;
             for (r = holder * per;; ++r) {
-                const Request q = request(a, r, ROWS);
-                const int n = columns_of(q, heads);
-                parts = __builtin_amdgcn_readfirstlane(parts_of(q.units, share));
+                const Request q = request(a, r);
+                const int n = blocks_of(a, q, ROWS) * heads, n_units = units_of(q);
+                parts = __builtin_amdgcn_readfirstlane(parts_of(n_units, share));
                 if (left < n * parts) {
                     const int column = uniform_div(left, parts), part = left - column * parts;
-                    u = base + column * q.units;
-                    stop = u + uniform_div((part + 1) * q.units, parts);
-                    u += uniform_div(part * q.units, parts);
+                    u = base + column * n_units;
+                    stop = u + uniform_div((part + 1) * n_units, parts);
+                    u += uniform_div(part * n_units, parts);
                     break;
                 }
-                left -= n * parts, base += n * q.units;
+                left -= n * parts, base += n * n_units;
             }
         }
     } else {
@@ -347,15 +206,15 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(const PagedAttn a) {
     int4 cut = make_int4(0, 0, 0, 0);
 
     while (u < stop) {
-        const Request rq = request(a, r, ROWS);
-        const int in_request = columns_of(rq, heads) * rq.units;
+        const Request rq = request(a, r);
+        const int row_blocks = blocks_of(a, rq, ROWS), n_units = units_of(rq), in_request = row_blocks * heads * n_units;
         if (u >= base + in_request) {
             base += in_request, ++r;
             continue;
         }
-        const int column = uniform_div(u - base, rq.units);
-        const int c0 = base + column * rq.units, c1 = c0 + rq.units;
-        const int h = uniform_div(column, rq.blocks), rb = column - h * rq.blocks;
+        const int column = uniform_div(u - base, n_units);
+        const int c0 = base + column * n_units, c1 = c0 + n_units;
+        const int h = uniform_div(column, row_blocks), rb = column - h * row_blocks;
         const int begin = (u - c0) * kUnit;
         const int part_end = min(stop, c1);
         const int end = min((part_end - c0) * kUnit, rq.len);
@@ -651,7 +510,7 @@ __global__ void __launch_bounds__(256) paged_merge_kernel(const PagedAttn a, int
     const int4 cut = a.cut[blockIdx.y];
     const int parts = cut.x, r = cut.y, h = cut.z, row = blockIdx.x, n = cut.w * rows_per_block + row;
     if (parts == 0) return;
-    const Request rq = request(a, r, rows_per_block);
+    const Request rq = request(a, r);
     if (n >= rq.rows) return;
     auto at = [&](int i) {
         return (((int64_t)blockIdx.y + i) * 2 + (i == 0 ? 1 : 0)) * rows_per_block + row;
@@ -715,9 +574,10 @@ static PagedPlan paged_plan(const ss_paged_store *s, int64_t n_requests, int n_q
                             int64_t max_length) {
     PagedPlan p;
     const int rep = n_q_heads / s->n_kv_heads, rs = 16 / (s->head_dim / s->group_size);
-    p.sets = max_new * rep > rs ? 2 : 1;
+    const int64_t rows = min(max_new * rep, (int64_t)kPromptRows);
+    p.sets = rows > rs ? 2 : 1;
     p.rows = p.sets * rs;
-    const double units = (double)n_requests * s->n_kv_heads * ((max_new * rep + p.rows - 1) / p.rows) *
+    const double units = (double)n_requests * s->n_kv_heads * ((rows + p.rows - 1) / p.rows) *
                          ((max_length + kUnit - 1) / kUnit);
     p.groups = (int)min((double)(2 * device_cu_count()), units / kMinShare + 1);
     p.bytes = (size_t)p.groups * (16 + 2 * p.rows * (s->head_dim + 2) * 4);
@@ -791,7 +651,8 @@ extern "C" int ss_paged_attn(const ss_paged_store *store, const void *q, int q_d
     a.hq = n_q_heads, a.rep = n_q_heads / store->n_kv_heads;
     a.q_dtype = q_dtype, a.causal = causal, a.zero_rest = zero_rest, a.scale = scale;
     a.vec = ((uintptr_t)q & 15) == 0 && q_st % 8 == 0 && q_sh % 8 == 0;
-    a.most_rows = INT32_MAX;
+    const bool prompts = max_new * a.rep > kPromptRows;
+    a.most_rows = prompts ? kPromptRows : INT32_MAX;
     a.cut = static_cast<int4 *>(workspace);
     a.acc = reinterpret_cast<float *>(a.cut + p.groups);
     a.ml = a.acc + (size_t)p.groups * 2 * p.rows * store->head_dim;
@@ -804,5 +665,5 @@ extern "C" int ss_paged_attn(const ss_paged_store *store, const void *q, int q_d
     else if (key == 64032) bf ? launch_paged<64, 2, true>(a, p, st) : launch_paged<64, 2, false>(a, p, st);
     else bf ? launch_paged<64, 1, true>(a, p, st) : launch_paged<64, 1, false>(a, p, st);
     SS_LAUNCH_CHECK("paged_attn_kernel launch");
-    return SS_OK;
+    return prompts ? launch_paged_prompt(a, store, st) : SS_OK;
 }

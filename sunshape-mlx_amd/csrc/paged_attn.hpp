@@ -1,0 +1,159 @@
+// What the kernels of attention over the paged cache share (paged_attn.hip:
+// the few query rows of decode steps, paged_prompt.hip: the many of prompts).
+//
+//   S[r][t] = sum_g s_tg (q_rg . c_tg) + z_tg sum(q_rg)
+//   O[r][d] = sum_t p_rt (s'_tg c'_td + z'_tg),   g = d's group
+//
+// with c the keys' codes, s and z their scales and zeros (primed: the
+// values').  Key codes enter the matrix cores as they are: a 4-bit code in the
+// low bits of a 16-bit half is the fp16 subnormal c * 2^-24, one place
+// further left c * 2^-20, and the fp16 matrix products take subnormals
+// exactly, so two masks and half a shift turn eight codes into the four
+// registers of an operand and no code is ever converted.  The factor 16
+// between the places is taken from the other operand (queries, respectively
+// probabilities, of odd pairs times 2^-4); 2^24 goes into the factors that
+// the sums are multiplied by in any case.
+#pragma once
+
+#include "paged_common.hpp"
+
+namespace ss {
+
+typedef _Float16 half8_t __attribute__((ext_vector_type(8)));
+typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
+typedef float float4_t __attribute__((ext_vector_type(4)));
+typedef float float2_t __attribute__((ext_vector_type(2)));
+
+// How far, in log2, a score may pass the running maximum before the maximum
+// moves: probabilities stay below 2^4, so p * scale stays within fp16 with
+// scales normalised to 2^10.
+constexpr float kLag = 4.f;
+struct PagedAttn {
+    PagedStore st;
+    const void *q;
+    int64_t q_st, q_sh;
+    void *out;
+    const int32_t *table, *lengths, *starts;
+    int64_t width, n_tokens;
+    int n_req, hq, rep, q_dtype, causal, zero_rest, vec;
+    float scale;
+    int most_rows;      // requests with more query rows a KV head are the prompt kernel's
+    int4 *cut;          // [workgroups]: the column that a workgroup leaves to be joined
+    float *acc;         // [workgroups][2][rows of a workgroup][D]
+    float *ml;          // [workgroups][2][rows of a workgroup][2]
+};
+
+// Tables do not change while the kernel runs: through the constant address
+// space their uniform reads are scalar loads, which do not queue behind the
+// stream of codes.
+__device__ __forceinline__ int table_read(const int32_t *p, int64_t i) {
+    return reinterpret_cast<const __attribute__((address_space(4))) int32_t *>(reinterpret_cast<uintptr_t>(p))[i];
+}
+
+// Eight 16-bit query elements from p (16-byte aligned if vec).
+__device__ __forceinline__ uint4 load_query8(const uint16_t *p, int vec) {
+    if (vec) return *reinterpret_cast<const uint4 *>(p);
+    return make_uint4(p[0] | ((uint32_t)p[1] << 16), p[2] | ((uint32_t)p[3] << 16),
+                      p[4] | ((uint32_t)p[5] << 16), p[6] | ((uint32_t)p[7] << 16));
+}
+
+// A request, from the tables on the device: its new tokens' first row, their
+// number (n_all, of which n rows exist), its length, its query rows a KV head.
+struct Request {
+    int t0, n, n_all, len, rows;
+};
+
+__device__ __forceinline__ Request request(const PagedAttn &a, int r) {
+    Request q;
+    q.t0 = table_read(a.starts, r);
+    q.n_all = table_read(a.starts, r + 1) - q.t0;
+    q.n = q.t0 < 0 ? 0 : (int)max((int64_t)0, min((int64_t)q.n_all, a.n_tokens - q.t0));
+    q.len = (int)max((int64_t)0, min((int64_t)table_read(a.lengths, r), a.width << a.st.log_page));
+    q.rows = q.n * a.rep;
+    return q;
+}
+
+// Inclusive sum over the lanes before (lane moves, no LDS).
+__device__ __forceinline__ int wave_scan(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);  // row_shr:1
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // row_bcast:15 -> rows 1, 3
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // row_bcast:31 -> rows 2, 3
+    return v;
+}
+
+__device__ __forceinline__ int uniform_div(int a, int b) {
+    return __builtin_amdgcn_readfirstlane((int)((uint32_t)a / (uint32_t)b));
+}
+
+// s_waitcnt vmcnt(N), the other counters unconstrained.
+template <int N>
+__device__ __forceinline__ void wait_loads() {
+    static_assert(N >= 0 && N < 64, "vmcnt range");
+    __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | (7 << 4) | (15 << 8));
+}
+
+template <typename T>
+using lds_ptr = __attribute__((address_space(3))) T *;
+
+template <typename T>
+__device__ __forceinline__ lds_ptr<T> as_lds(void *p) {
+    return reinterpret_cast<lds_ptr<T>>(static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p)));
+}
+
+// A word's eight codes as the four registers of an operand: pairs (0,1) and
+// (4,5) times 2^-24, (2,3) and (6,7) times 2^-20.
+__device__ __forceinline__ half8_t codes_operand(uint32_t w) {
+    union {
+        uint32_t u[4];
+        half8_t h;
+    } x;
+    const uint32_t hi = w >> 8;
+    x.u[0] = w & 0x000f000fu;
+    x.u[1] = w & 0x00f000f0u;
+    x.u[2] = hi & 0x000f000fu;
+    x.u[3] = hi & 0x00f000f0u;
+    return x.h;
+}
+
+template <int N>
+__device__ __forceinline__ void read_words(const char *p, uint32_t (&w)[N]) {
+    if constexpr (N == 2) {
+        const uint2 u = *reinterpret_cast<const uint2 *>(p);
+        w[0] = u.x, w[1] = u.y;
+    } else {
+#pragma unroll
+        for (int i = 0; i < N / 4; ++i) {
+            const uint4 u = reinterpret_cast<const uint4 *>(p)[i];
+            w[4 * i] = u.x, w[4 * i + 1] = u.y, w[4 * i + 2] = u.z, w[4 * i + 3] = u.w;
+        }
+    }
+}
+
+// Halves of a (scale, zero) pair.
+template <bool BF>
+__device__ __forceinline__ float low16(uint32_t u) {
+    if (BF) return __uint_as_float(u << 16);
+    return (float)__builtin_bit_cast(half2_t, u)[0];
+}
+template <bool BF>
+__device__ __forceinline__ float high16(uint32_t u) {
+    if (BF) return __uint_as_float(u & 0xffff0000u);
+    return (float)__builtin_bit_cast(half2_t, u)[1];
+}
+
+template <int N>
+__device__ __forceinline__ float column_max(const float (&x)[N]) {
+    float m = x[0];
+#pragma unroll
+    for (int i = 1; i < N; ++i) m = fmaxf(m, x[i]);
+    return m;
+}
+
+// Requests with more than most_rows query rows a KV head; the sizes of
+// paged_attn.hip's workspace are set by the caller.
+int launch_paged_prompt(const PagedAttn &a, const ss_paged_store *s, hipStream_t st);
+
+}  // namespace ss

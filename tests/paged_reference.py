@@ -60,16 +60,18 @@ def slots_of(table_row, length, page):
 
 
 def attend(q, store, table, lengths, starts, scale, causal=True, n_pages=None):
-    """(out, tol): the attention in 64 bits and how far a 32-bit kernel that
-    rounds each probability times scale to fp16 once may be from it.
+    """(out, tol): the attention in 64 bits and how far the kernels' roundings
+    may take them from it.
 
     Per row: a score is a sum of D products of a 16-bit and a 4-bit number, in
     float32, times a scale, plus a zero times a sum of D numbers: off by at
     most (D + 8) 2^-24 of the sum B of its terms' magnitudes (first order).
     exp2 and the running maximum add 2^-21; the sums over tokens at most one
     rounding a 32-token tile and 64 more.  A relative change e of every
-    probability moves an output by 2 e max|v|.  The rounding to fp16 is 2^-11
-    of each term p s c; the output's own is half a step of its type."""
+    probability moves an output by 2 e max|v|.  The output's own rounding is
+    half a step of its type.  Up to 64 rows a KV head, p s is rounded to fp16
+    (2^-11) and multiplied by code - 7.5; more rows round p and the value
+    itself, the value to at least 2^-18 of the largest of the request.""" 
     k_c, v_c, k_m, v_m = unpack(store)
     page = store[0].shape[2]
     k_all, v_all = values_of(k_c, k_m), values_of(v_c, v_m)
@@ -94,7 +96,8 @@ def attend(q, store, table, lengths, starts, scale, causal=True, n_pages=None):
             kt = k_m[at, h].double().repeat_interleave(d // k_m.shape[2], 1)
             kmag = kt[..., 0] * k_c[at, h] + kt[..., 1].abs()
             vt = v_m[at, h].double().repeat_interleave(d // v_m.shape[2], 1)
-            vcode = vt[..., 0] * v_c[at, h]
+            middle = vt[..., 0] * (v_c[at, h] - 7.5).abs()
+            largest = v.abs().nan_to_num(0.0).amax(0)
             for i in range(n):
                 row = starts[r] + i
                 see = real & (pos <= length - n + i) if causal else real
@@ -107,9 +110,13 @@ def attend(q, store, table, lengths, starts, scale, causal=True, n_pages=None):
                 out[row, h * rep:(h + 1) * rep] = o
                 b = ((qr.abs() @ kmag[see].t()) * scale).amax(-1, keepdim=True)
                 e = (d + 8) * 2.0 ** -24 * b + 2.0 ** -21 + (length / 32 + 64) * 2.0 ** -24
-                vmax = (vcode + vt[..., 1].abs())[see].amax(0)
-                tol[row, h * rep:(h + 1) * rep] = u * o.abs() + 2.0 ** -11 * (p @ vcode[see]) + \
-                    2 * e * vmax + 2.0 ** -24 * (1 if q.dtype == torch.float16 else 2.0 ** -100)
+                vmax = (vt[..., 0] * v_c[at, h] + vt[..., 1].abs())[see].amax(0)
+                if n * rep <= 64:
+                    half = 2.0 ** -11 * (p @ middle[see])
+                else:
+                    half = 2.001 * 2.0 ** -11 * (p @ v[see].abs()) + 2.0 ** -18 * largest
+                tol[row, h * rep:(h + 1) * rep] = u * o.abs() + half + 2 * e * vmax + \
+                    2.0 ** -24 * (1 if q.dtype == torch.float16 else 2.0 ** -100)
     return out, tol
 
 

@@ -296,6 +296,9 @@ CASES = [  # lengths, new tokens, query / KV heads, page
     ([300, 0, 5, 129], [1, 0, 1, 1], 16, 16, 32), ([700, 64], [4, 4], 16, 4, 32),
     ([40, 3], [7, 3], 28, 4, 128), ([9], [9], 16, 2, 16), ([2100, 100], [1, 2], 8, 1, 16),
     ([90, 200], [33, 70], 8, 2, 64), ([5], [0], 4, 4, 16),
+    # prompts, chunks, and decode steps beside them
+    ([129], [129], 8, 2, 16), ([65, 300, 1, 200], [65, 100, 1, 2], 16, 4, 32), ([333], [90], 7, 1, 128),
+    ([150, 0, 66], [150, 0, 66], 4, 4, 16),
 ]
 
 
@@ -319,7 +322,7 @@ def test_attention(lengths, new, hq, hkv, page, d, group, dtype):
     check_attention(given, q, store, table, le, starts, scale)
 
 
-@pytest.mark.parametrize("new", [1, 5])
+@pytest.mark.parametrize("new", [1, 5, 70])
 def test_attention_without_a_causal_limit(new):
     store, table, le, starts = world(3, [77, 400], [new, new], 2, 128, 64, 16, torch.float16)
     q = rows(9, 2 * new, 8, 128, torch.float16, False)
@@ -341,8 +344,9 @@ def test_attention_over_many_splits(length):
         check_attention(out, q, store, table, le, starts, 0.09)
 
 
+@pytest.mark.parametrize("new", [1, 80])
 @pytest.mark.parametrize("step", [40.0, 600.0])
-def test_attention_with_scores_that_rise_along_the_cache(step):
+def test_attention_with_scores_that_rise_along_the_cache(step, new):
     """Scores that climb by `step` log2 units: the running maximum moves all
     the way, and the last tokens alone count."""
     d, n, page = 64, 600, 16
@@ -353,15 +357,16 @@ def test_attention_with_scores_that_rise_along_the_cache(step):
     slots = torch.arange(n, dtype=torch.int32, device=DEV)
     S.append_paged(store, k, v, slots)
     table = torch.arange(38, dtype=torch.int32, device=DEV)[None]
-    q = torch.zeros((1, 4, d), dtype=torch.bfloat16, device=DEV)
+    q = torch.zeros((new, 4, d), dtype=torch.bfloat16, device=DEV)
     q[..., 0] = 8.0
     scale = step / 8 * math.log(2)
     for sign in (1, -1):
-        args = (sign * q, store, table, ints([n]), ints([0, 1]), scale)
+        args = (sign * q, store, table, ints([n]), ints([0, new]), scale)
         check_attention(S.paged_attention(*args), *args)
 
 
-def test_attention_with_value_scales_of_all_sizes():
+@pytest.mark.parametrize("new", [1, 40])
+def test_attention_with_value_scales_of_all_sizes(new):
     """Value groups from 1e-30 to 1e30 (bfloat16): what is added to what is
     far smaller swallows it, and nothing overflows on the way."""
     d, n, page = 128, 256, 16
@@ -374,47 +379,55 @@ def test_attention_with_value_scales_of_all_sizes():
         v2[:, 0, :64] *= f
         S.append_paged(store, k, v2, torch.arange(n, dtype=torch.int32, device=DEV))
         table = torch.arange(16, dtype=torch.int32, device=DEV)[None]
-        args = (rows(3, 1, 4, d, torch.bfloat16, False), store, table, ints([n]), ints([0, 1]), 0.05)
+        q = rows(3, new, 4, d, torch.bfloat16, False)
+        args = (q, store, table, ints([n]), ints([0, new]), 0.05)
         check_attention(S.paged_attention(*args), *args)
 
 
-def test_attention_with_queries_of_all_sizes():
+@pytest.mark.parametrize("new", [1, 33])
+def test_attention_with_queries_of_all_sizes(new):
     for dtype, sizes in ((torch.float16, (6e-8, 1e-4, 1.0, 6e4)), (torch.bfloat16, (1e-30, 1e-3, 1e4, 1e20))):
-        store, table, le, starts = world(6, [200], [1], 1, 64, 32, 16, dtype)
+        store, table, le, starts = world(6, [200], [new], 1, 64, 32, 16, dtype)
         for size in sizes:
-            q = (rows(3, 1, 4, 64, torch.float32, False).clamp(-1, 1) * size).to(dtype)
+            q = (rows(3, new, 4, 64, torch.float32, False).clamp(-1, 1) * size).to(dtype)
             scale = 0.125 / max(1.0, size)
             out = S.paged_attention(q, store, table, le, starts, scale)
             check_attention(out, q, store, table, le, starts, scale)
 
 
+@pytest.mark.parametrize("new", [4, 50])
 @pytest.mark.parametrize("dtype", HALF)
-def test_what_a_row_does_not_see_does_not_reach_it(dtype):
+def test_what_a_row_does_not_see_does_not_reach_it(dtype, new):
     """A NaN key or value of a later token, or behind the request's end,
-    stays out of the rows before it and makes the others NaN."""
-    n, new, d = 60, 4, 64
+    stays out of the rows before it and makes the others NaN: all dims for a
+    key, its group's for a value."""
+    n, d, group = 90, 128, 64
+    ok = new - 2
     for where in ("k", "v"):
-        store, table, le, starts = world(8, [n], [new], 2, d, 64, 16, dtype)
+        store, table, le, starts = world(8, [n], [new], 2, d, group, 16, dtype)
         x = rows(1, 1, 2, d, dtype)
-        bad = torch.full_like(x, math.inf)
+        bad = x.clone()
+        bad[0, :, group + 3] = math.inf
         at = R.slots_of(table[0], n, 16)[n - 2:n - 1].to(torch.int32).to(DEV)
         S.append_paged(store, bad if where == "k" else x, bad if where == "v" else x, at)
         q = rows(3, new, 4, d, dtype, False)
         out = S.paged_attention(q, store, table, le, starts, 0.1)
-        assert torch.isfinite(out[:2]).all() and out[2:].isnan().all()
-        good = S.paged_attention(q[:2].contiguous(), store, table, le - 2, ints([0, 2]), 0.1)
-        want, tol = R.attend(q[:2], store, table, le - 2, ints([0, 2]), 0.1)
-        for o in (out[:2], good):
+        assert torch.isfinite(out[:ok]).all() and out[ok:, :, group:].isnan().all()
+        assert out[ok:, :, :group].isnan().all() if where == "k" else out[ok:, :, :group].isfinite().all()
+        good = S.paged_attention(q[:ok].contiguous(), store, table, le - 2, ints([0, ok]), 0.1)
+        want, tol = R.attend(q[:ok], store, table, le - 2, ints([0, ok]), 0.1)
+        for o in (out[:ok], good):
             assert ((o.cpu().double() - want).abs() <= tol).all()
 
 
-def test_pages_outside_the_pool_hold_no_tokens():
-    store, table, le, starts = world(11, [100, 40], [1, 2], 2, 128, 64, 16, torch.float16)
+@pytest.mark.parametrize("new", [(1, 2), (80, 40)])
+def test_pages_outside_the_pool_hold_no_tokens(new):
+    store, table, le, starts = world(11, [100, 40], new, 2, 128, 64, 16, torch.float16)
     table[0, 2], table[0, 5], table[1, 0], table[1, 1], table[1, 2] = -1, 10 ** 6, -5, 99, 2 ** 31 - 1
-    q = rows(3, 3, 4, 128, torch.float16, False)
+    q = rows(3, sum(new), 4, 128, torch.float16, False)
     out = S.paged_attention(q, store, table, le, starts, 0.1)
     check_attention(out, q, store, table, le, starts, 0.1)
-    assert (out[1:] == 0).all()
+    assert (out[new[0]:] == 0).all()
 
 
 def test_counts_that_do_not_fit_are_cut_to_the_memory_there_is():
