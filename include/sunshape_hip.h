@@ -1104,8 +1104,9 @@ int ss_read_paged(const ss_paged_store *store, const int32_t *slots, int64_t n_t
  * ss_paged_attn_workspace_bytes of the same arguments, uninitialised, not
  * shared with a call that may run at the same time.
  */
-size_t ss_paged_attn_workspace_bytes(const ss_paged_store *store, int64_t n_requests,
-                                     int n_q_heads, int64_t max_new, int64_t max_length);
+size_t ss_paged_attn_workspace_bytes(const ss_paged_store *store, int64_t n_tokens,
+                                     int64_t n_requests, int n_q_heads, int64_t max_new,
+                                     int64_t max_length);
 int ss_paged_attn(const ss_paged_store *store, const void *q, int q_dtype, int64_t n_tokens,
                   int64_t q_st, int64_t q_sh, int n_q_heads, const int32_t *block_table,
                   int64_t table_width, const int32_t *lengths, const int32_t *token_starts,

@@ -221,7 +221,7 @@ _SIGNATURES = {
     "ss_append_paged": (_int, [_c_void_p, _c_void_p, _c_void_p, _int, _i64, _i64, _i64, _i64,
                                _i64, _c_void_p, _c_void_p]),
     "ss_read_paged": (_int, [_c_void_p, _c_void_p, _i64, _c_void_p, _c_void_p, _c_void_p]),
-    "ss_paged_attn_workspace_bytes": (_size, [_c_void_p, _i64, _int, _i64, _i64]),
+    "ss_paged_attn_workspace_bytes": (_size, [_c_void_p, _i64, _i64, _int, _i64, _i64]),
     "ss_paged_attn": (_int, [_c_void_p, _c_void_p, _int, _i64, _i64, _i64, _int, _c_void_p, _i64,
                              _c_void_p, _c_void_p, _i64, _f32, _int, _i64, _i64, _c_void_p, _int,
                              _c_void_p, _size, _c_void_p]),

@@ -486,7 +486,7 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(const PagedAttn a) {
             if (whole) {
                 const float inv = l == 0.f ? 0.f : 1.f / l;
                 const int64_t at = ((int64_t)(rq.t0 + n / a.rep) * a.hq + h * a.rep + n % a.rep) * D + c;
-                store4_from_f32(a.out, a.q_dtype, at, x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
+                store_out4(a, at, x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
             } else {
                 const int64_t at = ((int64_t)blockIdx.x * 2 + place) * ROWS + row;
                 *reinterpret_cast<float4 *>(a.acc + at * D + c) = make_float4(x[0], x[1], x[2], x[3]);
@@ -512,9 +512,7 @@ __global__ void __launch_bounds__(256) paged_merge_kernel(const PagedAttn a, int
     if (parts == 0) return;
     const Request rq = request(a, r);
     if (n >= rq.rows) return;
-    auto at = [&](int i) {
-        return (((int64_t)blockIdx.y + i) * 2 + (i == 0 ? 1 : 0)) * rows_per_block + row;
-    };
+    auto at = [&](int i) { return (((int64_t)blockIdx.y + i) * 2 + (i == 0 ? 1 : 0)) * rows_per_block + row; };
     const int c = threadIdx.x % CH * 4, p = threadIdx.x / CH, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     float4 v[PER];
 #pragma unroll
@@ -557,7 +555,7 @@ __global__ void __launch_bounds__(256) paged_merge_kernel(const PagedAttn a, int
         }
         const float inv = t == 0.f ? 0.f : 1.f / t;
         const int64_t o = ((int64_t)(rq.t0 + n / a.rep) * a.hq + h * a.rep + n % a.rep) * D + c;
-        store4_from_f32(a.out, a.q_dtype, o, y[0] * inv, y[1] * inv, y[2] * inv, y[3] * inv);
+        store_out4(a, o, y[0] * inv, y[1] * inv, y[2] * inv, y[3] * inv);
     }
 }
 
@@ -570,8 +568,8 @@ struct PagedPlan {
 
 // Launch shape: as many workgroups as the device holds at once (two a compute
 // unit), or as the hints' units need.
-static PagedPlan paged_plan(const ss_paged_store *s, int64_t n_requests, int n_q_heads, int64_t max_new,
-                            int64_t max_length) {
+static PagedPlan paged_plan(const ss_paged_store *s, int64_t n_tokens, int64_t n_requests, int n_q_heads,
+                            int64_t max_new, int64_t max_length) {
     PagedPlan p;
     const int rep = n_q_heads / s->n_kv_heads, rs = 16 / (s->head_dim / s->group_size);
     const int64_t rows = min(max_new * rep, (int64_t)kPromptRows);
@@ -581,6 +579,8 @@ static PagedPlan paged_plan(const ss_paged_store *s, int64_t n_requests, int n_q
                          ((max_length + kUnit - 1) / kUnit);
     p.groups = (int)min((double)(2 * device_cu_count()), units / kMinShare + 1);
     p.bytes = (size_t)p.groups * (16 + 2 * p.rows * (s->head_dim + 2) * 4);
+    if (max_new * rep > kPromptRows)  // (one after the other: they share it)
+        p.bytes = max(p.bytes, paged_prompt_bytes(s, n_requests, n_tokens * rep, kPromptRows));
     return p;
 }
 
@@ -609,13 +609,13 @@ static void launch_paged(const PagedAttn &a, const PagedPlan &p, hipStream_t st)
 
 using namespace ss;
 
-extern "C" size_t ss_paged_attn_workspace_bytes(const ss_paged_store *store, int64_t n_requests, int n_q_heads,
-                                                int64_t max_new, int64_t max_length) {
+extern "C" size_t ss_paged_attn_workspace_bytes(const ss_paged_store *store, int64_t n_tokens, int64_t n_requests,
+                                                int n_q_heads, int64_t max_new, int64_t max_length) {
     PagedStore ps;
     int log_page;
     if (check_paged_store(store, &ps, &log_page) || check_hints(store, n_requests, n_q_heads, max_new, max_length))
         return 0;
-    return paged_plan(store, n_requests, n_q_heads, max_new, max_length).bytes;
+    return paged_plan(store, n_tokens, n_requests, n_q_heads, max_new, max_length).bytes;
 }
 
 extern "C" int ss_paged_attn(const ss_paged_store *store, const void *q, int q_dtype, int64_t n_tokens,
@@ -632,6 +632,7 @@ extern "C" int ss_paged_attn(const ss_paged_store *store, const void *q, int q_d
     if (n_tokens == 0) return SS_OK;
     SS_UNSUPPORTED(n_tokens <= INT32_MAX / n_q_heads, "too many query rows for one launch");
     SS_REQUIRE(q && out && block_table && lengths && token_starts, "null pointer argument");
+    SS_REQUIRE(((uintptr_t)out & 7) == 0, "out must be 8-byte aligned");
     SS_REQUIRE(table_width >= 1, "bad block table width");
     SS_UNSUPPORTED(table_width <= (1 << 30) / store->page_size, "a table row of more than 2^30 tokens");
     // every unit of every column is counted in 32 bits
@@ -639,7 +640,7 @@ extern "C" int ss_paged_attn(const ss_paged_store *store, const void *q, int q_d
                            ((double)table_width * store->page_size / kUnit + 1) <
                        2147483648.0,
                    "too many requests and tokens for one launch");
-    const PagedPlan p = paged_plan(store, n_requests, n_q_heads, max_new, max_length);
+    const PagedPlan p = paged_plan(store, n_tokens, n_requests, n_q_heads, max_new, max_length);
     if (p.bytes > workspace_bytes || (p.bytes && !workspace)) {
         set_error("workspace of %zu bytes, %zu needed", workspace_bytes, p.bytes);
         return SS_ERR_WORKSPACE;
@@ -665,5 +666,5 @@ extern "C" int ss_paged_attn(const ss_paged_store *store, const void *q, int q_d
     else if (key == 64032) bf ? launch_paged<64, 2, true>(a, p, st) : launch_paged<64, 2, false>(a, p, st);
     else bf ? launch_paged<64, 1, true>(a, p, st) : launch_paged<64, 1, false>(a, p, st);
     SS_LAUNCH_CHECK("paged_attn_kernel launch");
-    return prompts ? launch_paged_prompt(a, store, st) : SS_OK;
+    return prompts ? launch_paged_prompt(a, store, workspace, st) : SS_OK;
 }

@@ -38,7 +38,8 @@ struct PagedAttn {
     int n_req, hq, rep, q_dtype, causal, zero_rest, vec;
     float scale;
     int most_rows;      // requests with more query rows a KV head are the prompt kernel's
-    int4 *cut;          // [workgroups]: the column that a workgroup leaves to be joined
+    int target;         // of the prompt kernel: workgroups that its parts fill
+    int4 *cut;          // [workgroups]: (parts, request, head, row block) of a column to be joined
     float *acc;         // [workgroups][2][rows of a workgroup][D]
     float *ml;          // [workgroups][2][rows of a workgroup][2]
 };
@@ -71,6 +72,17 @@ __device__ __forceinline__ Request request(const PagedAttn &a, int r) {
     q.len = (int)max((int64_t)0, min((int64_t)table_read(a.lengths, r), a.width << a.st.log_page));
     q.rows = q.n * a.rep;
     return q;
+}
+
+// Elements i .. i+3 of the output (i a multiple of 4), of q's 16-bit type.
+__device__ __forceinline__ void store_out4(const PagedAttn &a, int64_t i, float x0, float x1, float x2, float x3) {
+    const half2_t h0 = __builtin_convertvector(float2_t{x0, x1}, half2_t);
+    const half2_t h1 = __builtin_convertvector(float2_t{x2, x3}, half2_t);
+    const uint32_t b0 = to_bits16<true>(x0) | (to_bits16<true>(x1) << 16);
+    const uint32_t b1 = to_bits16<true>(x2) | (to_bits16<true>(x3) << 16);
+    const bool f16 = a.q_dtype == SS_F16;
+    *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(a.out) + i) =
+        make_uint2(f16 ? __builtin_bit_cast(uint32_t, h0) : b0, f16 ? __builtin_bit_cast(uint32_t, h1) : b1);
 }
 
 // Inclusive sum over the lanes before (lane moves, no LDS).
@@ -152,8 +164,9 @@ __device__ __forceinline__ float column_max(const float (&x)[N]) {
     return m;
 }
 
-// Requests with more than most_rows query rows a KV head; the sizes of
-// paged_attn.hip's workspace are set by the caller.
-int launch_paged_prompt(const PagedAttn &a, const ss_paged_store *s, hipStream_t st);
+// The requests with more than most_rows query rows a KV head (paged_prompt.hip),
+// with `workspace` of paged_prompt_bytes for n_tokens * rep rows in all.
+size_t paged_prompt_bytes(const ss_paged_store *s, int64_t n_requests, int64_t rows, int most_rows);
+int launch_paged_prompt(PagedAttn a, const ss_paged_store *s, void *workspace, hipStream_t st);
 
 }  // namespace ss

@@ -1,17 +1,24 @@
 // Attention over a paged cache of 4-bit keys and values: prompts, and chunks of
 // long ones (paged_attn.hpp has the formulas).
 //
-// A workgroup takes 128 query rows of one KV head (its group's heads at
-// consecutive positions), 32 a wave, over 64-token tiles.  Scores are exact:
-// key codes enter v_mfma_f32_32x32x16_f16 unconverted, group by group, and
-// every product sum is multiplied by its token's scale in float32; the zeros'
-// part is one more product, of the zeros and the queries' sums, both split
-// into bf16 parts.  Values are shared by all rows, so the workgroup
-// dequantises each tile once, to fp16 in LDS, while the tile before it is
-// computed; times a power of two a group that keeps the largest value met
-// below 2^-6 (a code's factor then stays within fp16: code * 2^-24 times
-// scale * 2^18).  Rounding them costs 2^-11 of a value, as the probabilities'
-// rounding does; statistics and sums are float32.
+// A workgroup of eight waves takes 256 query rows of one KV head (its group's
+// heads at consecutive positions), 32 a wave, over 64-token tiles.  While a
+// tile is computed the next one is prepared, once for all rows: its key codes
+// are spread to 16-bit halves (not converted: see paged_attn.hpp) and its
+// values dequantised to fp16, both in the operand order of
+// v_mfma_f32_32x32x16_f16, and the one after that is copied from HBM.
+//
+// Scores are exact: code products are summed group by group and each sum is
+// multiplied by its token's scale in float32; the zeros' part is one more
+// product, of the zeros and the queries' sums, both split into bf16 parts.
+// Values are rounded to fp16 times a power of two a group that keeps the
+// largest value met below 2^-6 (a code's factor then stays within fp16: code *
+// 2^-24 times scale * 2^18): 2^-11 of a value, as the probabilities' rounding
+// costs; statistics and sums are float32.
+//
+// The vector ALUs bound it (per 32 rows and 64 tokens: 2 x 32 products of
+// scale and sum, 32 exponentials), so what does not depend on the row is done
+// once a workgroup.
 #include "paged_attn.hpp"
 
 namespace ss {
@@ -19,38 +26,49 @@ namespace ss {
 typedef float float16_t __attribute__((ext_vector_type(16)));
 typedef __bf16 bf8_t __attribute__((ext_vector_type(8)));
 
-constexpr int kRows = 128;    // query rows of a workgroup
-constexpr int kTokens = 64;   // of a tile
+constexpr int kPWaves = 8;
+constexpr int kRows = 32 * kPWaves;  // query rows of a workgroup
+constexpr int kTokens = 64;          // of a tile
+constexpr int kSlots = 3;            // tiles in LDS as they come: one being prepared, two on their way
+// Fewest tiles of a part, where a workgroup's column is cut.
+constexpr int kMinTiles = 8;
 
 template <int D, int G>
 struct PromptTile {
-    // a tile's 16-token segments in LDS: key rows, value blocks, the keys' and
-    // the values' (scale, zero) pairs [G][16].  16-byte piece c of key row t
-    // sits at place c ^ (t / 4) % (pieces a row).
+    // A tile in LDS as it comes: 16-token segments of key rows, value blocks,
+    // the keys' and the values' (scale, zero) pairs [G][16].  16-byte piece c of
+    // key row t sits at place c ^ (t / 4) % (pieces a row).
     static constexpr int kKeys = 8 * D, kMeta = 2 * G * 64;
     static constexpr int kSeg = 2 * kKeys + kMeta;
     static constexpr int kBytes = 4 * kSeg;
     static constexpr int kKP = D / 32;  // 16-byte pieces of a key row
+    // Prepared, 16 bytes each: keys [2 halves of 32 tokens][D/16 steps][2][32 rows],
+    // values [8 blocks of tokens][D places], zeros [2 halves][group pairs][2][32 rows];
+    // and the keys' scales, 16 bits each, [G][64].
+    static constexpr int kOperands = kTokens * D * 2;
+    static constexpr int kPairs = (G + 1) / 2;
+    static constexpr int kZeros = 2 * kPairs * 1024, kScales = G * kTokens * 2;
+    static constexpr int kPrepared = 2 * kOperands + kZeros + kScales;
 
-    // Starts copying the segment of 16 tokens in page p (clamped by the
-    // caller) from its token `off`.
-    __device__ static void fetch(const PagedStore &st, int h, int lane, char *seg, int page, int off) {
-        const int64_t row = (int64_t)page * st.heads + h;
-        const uint32_t *k = st.k_codes + ((row << st.log_page) + off) * (D / 8);
-        const uint32_t *v = st.v_codes + (((row << st.log_page) + off) >> 3) * D;
-        const int place = lane % (kKeys / 16), t = place / kKP, c = (place % kKP) ^ ((t >> 2) % kKP);
-        const uint32_t *from_k = k + t * (D / 8) + c * 4, *from_v = v + place * 4;
-        if constexpr (D == 128) {
-            __builtin_amdgcn_global_load_lds(from_k, as_lds<void>(seg), 16, 0, 0);
-            __builtin_amdgcn_global_load_lds(from_v, as_lds<void>(seg + kKeys), 16, 0, 0);
-        } else {
-            __builtin_amdgcn_global_load_lds(lane < 32 ? from_k : from_v, as_lds<void>(seg), 16, 0, 0);
-        }
-        if (lane < kMeta / 16) {
-            const int e = lane % (4 * G);
-            const uint32_t *m = lane < 4 * G ? st.k_meta : st.v_meta;
-            __builtin_amdgcn_global_load_lds(m + ((row * G + e / 4) << st.log_page) + off + e % 4 * 4,
-                                             as_lds<void>(seg + 2 * kKeys), 16, 0, 0);
+    // Starts copying, of the segment of 16 tokens in page p from its token
+    // `off`, the keys and the pairs (part 0) or the values (part 1).
+    __device__ static void fetch(const PagedStore &st, int h, int lane, char *seg, int page, int off, int part) {
+        const int64_t slot = (((int64_t)page * st.heads + h) << st.log_page) + off;
+        if (part == 0) {
+            const int t = lane % (kKeys / 16) / kKP, c = (lane % kKP) ^ ((t >> 2) % kKP);
+            const char *k = reinterpret_cast<const char *>(st.k_codes) + slot * (D / 2);
+            if (kKeys == 1024 || lane < kKeys / 16)
+                __builtin_amdgcn_global_load_lds(k + (uint32_t)(t * (D / 2) + c * 16), as_lds<void>(seg), 16, 0, 0);
+            if (lane < kMeta / 16) {
+                const int e = lane % (4 * G);
+                const uint32_t *m = lane < 4 * G ? st.k_meta : st.v_meta;
+                m += (slot - off) * G + off;
+                __builtin_amdgcn_global_load_lds(m + (uint32_t)(((e / 4) << st.log_page) + e % 4 * 4),
+                                                 as_lds<void>(seg + 2 * kKeys), 16, 0, 0);
+            }
+        } else if (kKeys == 1024 || lane < kKeys / 16) {
+            const char *v = reinterpret_cast<const char *>(st.v_codes) + slot * (D / 2);
+            __builtin_amdgcn_global_load_lds(v + (uint32_t)(lane * 16), as_lds<void>(seg + kKeys), 16, 0, 0);
         }
     }
 };
@@ -60,44 +78,111 @@ __device__ __forceinline__ int tiles_of(const PagedAttn &a, const Request &q) {
     return q.rows > a.most_rows ? (q.rows + kRows - 1) / kRows : 0;
 }
 
+// Parts of a request's columns at `share` tiles a part.
+__device__ __forceinline__ int parts_of_tiles(const Request &q, int share) {
+    return max(1, (int)(((int64_t)(q.len + kTokens - 1) / kTokens + share - 1) / share));
+}
+
+// Largest low and largest high half of the lanes' pairs, N sets side by side.
+template <int N>
+__device__ __forceinline__ void pair_max(uint32_t (&v)[N]) {
+    typedef unsigned short us2 __attribute__((ext_vector_type(2)));
+    auto most = [](uint32_t a, int b) {
+        return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(us2, a), __builtin_bit_cast(us2, b)));
+    };
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = most(v[i], dpp_mov_i<0xB1>(v[i]));  // quad_perm [1,0,3,2]
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = most(v[i], dpp_mov_i<0x4E>(v[i]));  // quad_perm [2,3,0,1]
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = most(v[i], dpp_mov_i<0x141>(v[i]));  // row_half_mirror
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = most(v[i], dpp_mov_i<0x140>(v[i]));  // row_mirror
+#pragma unroll
+    for (int i = 0; i < N; ++i)  // row_bcast:15 -> rows 1, 3
+        v[i] = most(v[i], __builtin_amdgcn_update_dpp(v[i], v[i], 0x142, 0xa, 0xf, false));
+#pragma unroll
+    for (int i = 0; i < N; ++i)  // row_bcast:31 -> rows 2, 3
+        v[i] = most(v[i], __builtin_amdgcn_update_dpp(v[i], v[i], 0x143, 0xc, 0xf, false));
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = __builtin_amdgcn_readlane(v[i], 63);
+}
+
+// A barrier for what lies in LDS: unlike __syncthreads it leaves copies to LDS
+// on their way (each wave waits for those it needs).
+__device__ __forceinline__ void lds_barrier() {
+    __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
+    __builtin_amdgcn_s_waitcnt(15 | (3 << 14) | (7 << 4));  // lgkmcnt(0)
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
+}
+
 __device__ __forceinline__ float half_max(float v) { return fmaxf(v, __shfl_xor(v, 32)); }
 
 template <int D, int G, bool BF>
-__global__ void __launch_bounds__(256, 2) paged_prompt_kernel(const PagedAttn a) {
+__global__ void __launch_bounds__(64 * kPWaves, 2) paged_prompt_kernel(const PagedAttn a) {
     using PT = PromptTile<D, G>;
     constexpr int GW = D / 8 / G, HW = GW / 2;  // words of a group, and of a lane's half of it
     constexpr int NT = D / 32;                  // 32-dim tiles of the values
-    constexpr int kValues = kTokens * D * 2;    // bytes of a tile's values as fp16
-    __shared__ __attribute__((aligned(16))) char lds[3 * PT::kBytes + 2 * kValues];
-    char *const raw = lds, *const vals = lds + 3 * PT::kBytes;
+    __shared__ __attribute__((aligned(16))) char lds[kSlots * PT::kBytes + 2 * PT::kPrepared];
+    char *const raw = lds, *const prepared = lds + kSlots * PT::kBytes;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 31, half = lane >> 5;
     const int heads = a.st.heads, log_page = a.st.log_page, in_page = (1 << log_page) - 1;
 
+    // Columns are (request, row tile, KV head).  Where there are fewer than half
+    // as many as workgroups, each is cut along its tokens into parts of at most
+    // `share` tiles of the request's length.
     const int per = (a.n_req + 63) / 64, r0 = min(lane * per, a.n_req), r1 = min(r0 + per, a.n_req);
-    int mine = 0;
-    for (int i = r0; i < r1; ++i) mine += tiles_of(a, request(a, i));
-    const int scan = wave_scan(mine);
-    const int total = __builtin_amdgcn_readlane(scan, 63) * heads;
+    int columns = 0, all_tiles = 0;
+    for (int i = r0; i < r1; ++i) {
+        const Request q = request(a, i);
+        const int n = tiles_of(a, q) * heads;
+        columns += n, all_tiles += n * ((q.len + kTokens - 1) / kTokens);
+    }
+    int scan = wave_scan(columns);
+    const int n_columns = __builtin_amdgcn_readlane(scan, 63);
+    int share = INT32_MAX;
+    if (a.cut && 2 * n_columns <= a.target) {
+        // sum of ceil(n / share) is at most total / share + columns, and about
+        // total / share + columns / 2
+        const int total = __builtin_amdgcn_readlane(wave_scan(all_tiles), 63);
+        for (int spare = n_columns / 2;; spare = n_columns) {
+            const int free_groups = a.target - spare;
+            share = max(uniform_div(total + free_groups - 1, free_groups), kMinTiles);
+            columns = 0;
+            for (int i = r0; i < r1; ++i) {
+                const Request q = request(a, i);
+                columns += tiles_of(a, q) * heads * parts_of_tiles(q, share);
+            }
+            scan = wave_scan(columns);
+            if (spare == n_columns || __builtin_amdgcn_readlane(scan, 63) <= a.target) break;
+        }
+    }
+    const int n_items = __builtin_amdgcn_readlane(scan, 63);
+    int4 cut = make_int4(0, 0, 0, 0);
 
-    for (int item = blockIdx.x; item < total; item += gridDim.x) {
-        // (heads side by side: a head's tiles tend to meet in one L2)
-        const int h = item % heads;
-        int left = uniform_div(item, heads);
-        const int holder = __ffsll((unsigned long long)__ballot(left < scan)) - 1;
-        left -= holder ? __builtin_amdgcn_readlane(scan, holder - 1) : 0;
-        int r = holder * per;
+    for (int item = blockIdx.x; item < n_items; item += gridDim.x) {
+        const int holder = __ffsll((unsigned long long)__ballot(item < scan)) - 1;
+        int left = item - (holder ? __builtin_amdgcn_readlane(scan, holder - 1) : 0);
+        int r = holder * per, parts, row_tile;
         Request rq;
         for (;; ++r) {
             rq = request(a, r);
             const int n = tiles_of(a, rq);
-            if (left < n) {
-                left = n - 1 - left;  // the longest first
+            parts = __builtin_amdgcn_readfirstlane(parts_of_tiles(rq, share));
+            if (left < n * heads * parts) {
+                // the longest row tiles first; heads side by side, so that a head's
+                // tiles tend to meet in one L2
+                const int t = uniform_div(left, heads * parts);
+                left -= t * heads * parts;
+                row_tile = n - 1 - t;
                 break;
             }
-            left -= n;
+            left -= n * heads * parts;
         }
-        const int row0 = left * kRows + wave * 32;  // the wave's first row
+        const int part = uniform_div(left, heads), h = left - part * heads;
+        const int row0 = row_tile * kRows + wave * 32;  // the wave's first row
         const int32_t *row_table = a.table + (int64_t)r * a.width;
         auto page_at = [&](int token) {
             const int p = table_read(row_table, min((int64_t)(token >> log_page), a.width - 1));
@@ -106,15 +191,17 @@ __global__ void __launch_bounds__(256, 2) paged_prompt_kernel(const PagedAttn a)
         auto sees = [&](int row) {  // tokens that a row sees
             return a.causal ? max(0, min(rq.len, rq.len - rq.n_all + row / a.rep + 1)) : rq.len;
         };
-        const int last_row = min(left * kRows + kRows, rq.rows) - 1;
-        const int end = __builtin_amdgcn_readfirstlane(sees(last_row));          // of the workgroup
+        const int last_row = min(row_tile * kRows + kRows, rq.rows) - 1;
+        const int seen_tiles =
+            (__builtin_amdgcn_readfirstlane(sees(last_row)) + kTokens - 1) / kTokens;  // by the workgroup
+        const int first_tile = uniform_div(part * seen_tiles, parts);
+        const int n_tiles = uniform_div((part + 1) * seen_tiles, parts);
         const int wave_last = min(row0 + 31, rq.rows - 1);
         const int wave_end = row0 < rq.rows ? __builtin_amdgcn_readfirstlane(sees(wave_last)) : 0;
         const int all_see = row0 < rq.rows ? __builtin_amdgcn_readfirstlane(sees(row0)) : 0;
         const int row = row0 + col;
         const bool live = row < rq.rows;
         const int limit = live ? sees(row) : rq.len;
-        const int n_tiles = (end + kTokens - 1) / kTokens;
 
         // queries: B operand of step s of group g: dims of word g*GW + half*HW + s
         uint4 rawq[G][HW];
@@ -126,20 +213,31 @@ __global__ void __launch_bounds__(256, 2) paged_prompt_kernel(const PagedAttn a)
 #pragma unroll
                 for (int s = 0; s < HW; ++s) rawq[g][s] = load_query8(q + (g * GW + half * HW + s) * 8, a.vec);
         }
-        // pages of tile i: the wave copies the segment of tokens 16 * wave ..
-        auto fetch = [&](char *slot, int tile) {
-            const int tb = tile * kTokens + 16 * wave;
-            PT::fetch(a.st, h, lane, slot + wave * PT::kSeg, max(page_at(tb), 0), tb & in_page);
-        };
-        auto pages_ok = [&](int tile) {  // bit w: the page of tokens 16 w .. is in the pool
-            int ok = 0;
+        // A tile's four pages, of 16 tokens each; bit w of the mask: it is in the pool.
+        auto pages_of = [&](int tile, int (&p)[4]) {
 #pragma unroll
-            for (int w = 0; w < 4; ++w) ok |= (page_at(tile * kTokens + 16 * w) >= 0 ? 1 : 0) << w;
-            return ok;
+            for (int w = 0; w < 4; ++w) p[w] = page_at(tile * kTokens + 16 * w);
         };
+        auto mask_of = [](const int (&p)[4]) {
+            return (p[0] >= 0 ? 1 : 0) | (p[1] >= 0 ? 2 : 0) | (p[2] >= 0 ? 4 : 0) | (p[3] >= 0 ? 8 : 0);
+        };
+        // The wave copies a part of segment wave % 4 of a tile.
+        const int seg = wave & 3;
+        auto own = [&](const int (&p)[4]) {
+            return max(seg == 0 ? p[0] : seg == 1 ? p[1] : seg == 2 ? p[2] : p[3], 0);
+        };
+        auto offset = [&](int tile) { return (tile * kTokens + 16 * seg) & in_page; };
+        int pages[4], ok[kSlots + 1];  // ok: of the tile computed and those behind it
         wait_loads<0>();  // the queries, before tiles are waited for with them
-        if (n_tiles > 0) fetch(raw, 0);
-        if (n_tiles > 1) fetch(raw + PT::kBytes, 1);
+#pragma unroll
+        for (int i = 0; i < kSlots; ++i) {
+            pages_of(first_tile + i, pages);
+            ok[i] = mask_of(pages);
+            if (first_tile + i < n_tiles)
+                PT::fetch(a.st, h, lane, raw + i * PT::kBytes + seg * PT::kSeg, own(pages), offset(first_tile + i),
+                          wave >> 2);
+        }
+        pages_of(first_tile + kSlots, pages);
 
         half8_t qf[G][HW];
         bf8_t qz[(G + 1) / 2];
@@ -198,181 +296,210 @@ __global__ void __launch_bounds__(256, 2) paged_prompt_kernel(const PagedAttn a)
 #pragma unroll
         for (int j = 0; j < NT; ++j) o[j] = float16_t{};
         float top = -INFINITY, l = 0.f;
-        int vexp[G];  // the values met in group g are below 2^vexp
+        // The values met in group g are below 2^vexp; the tile prepared last has
+        // vnext, which the sums move to when they come to it.
+        int vexp[G], vnext[G];
 #pragma unroll
-        for (int g = 0; g < G; ++g) vexp[g] = -60;
+        for (int g = 0; g < G; ++g) vexp[g] = vnext[g] = -60;
 
         // Element i of a product's 16: its value's group, as NT dims a row of
         // the A operand make neighbours (row m of tile j is dim NT*m + j).
         auto group_of = [](int i) { return i / 4 * G / 4; };
-        // Moves the sums to powers of two that hold the tile's values; bit t of
-        // bad[g]: token t's group g is NaN.
-        auto meet = [&](const char *slot, int tb, int ok, uint64_t (&bad)[G]) {
+        // The tile's prepared form, its values times a power of two that holds
+        // them (a lane looks at one token's pairs); bit t of bad_next[g]: token
+        // t's group g is not finite.
+        uint64_t bad_next[G];
+        auto prepare = [&](const char *__restrict slot, char *__restrict out, int tb, int ok) {
+            constexpr uint32_t kInf = BF ? 0x7f80u : 0x7c00u;
+            constexpr int KW = D / 64, VW = NT / 2;  // words of keys and values that a lane takes
+            // everything that is read first
+            const char *mine = slot + (lane >> 4) * PT::kSeg;  // of token `lane`
+            const uint32_t *m = reinterpret_cast<const uint32_t *>(mine + 2 * PT::kKeys + G * 64) + (lane & 15);
+            uint32_t pair[G], kw[2], vw[2], vm[8], km = 0;
+#pragma unroll
+            for (int g = 0; g < G; ++g) pair[g] = m[16 * g];
+            if (wave < G) km = m[16 * (wave - G)];  // the keys' pairs lie before the values'
+            // key words KW * wave .. of token `lane`
+            const int w0 = wave * KW;
+            const char *kfrom = mine + ((lane & 15) * PT::kKP + ((w0 / 4) ^ ((lane >> 2) % PT::kKP))) * 16 + w0 % 4 * 4;
+            // value block `wave`, dims NT * col + j of the lane's half
+            const int j0 = half * VW, vg = col * NT * G / D;
+            const char *vseg = slot + (wave >> 1) * PT::kSeg;
+            const char *vfrom = vseg + PT::kKeys + ((wave & 1) * D + col * NT + j0) * 4;
+            if constexpr (KW == 2)
+                read_words(kfrom, kw), read_words(vfrom, vw);
+            else
+                kw[0] = *reinterpret_cast<const uint32_t *>(kfrom), vw[0] = *reinterpret_cast<const uint32_t *>(vfrom);
+            read_words(vseg + 2 * PT::kKeys + (G + vg) * 64 + (wave & 1) * 32, vm);
+
+            // keys: the A operand's row of a token, so chosen that a lane's 16
+            // results are two whole blocks of 8 tokens
+            const int t = lane & 31, row = (t & 16) | (t >> 3 & 1) << 2 | (t >> 2 & 1) << 3 | (t & 3);
+#pragma unroll
+            for (int k = 0; k < KW; ++k) {
+                const int g = (w0 + k) / GW, in = (w0 + k) % GW;
+                const int place = (((lane >> 5) * (D / 16) + g * HW + in % HW) * 2 + in / HW) * 32 + row;
+                *reinterpret_cast<half8_t *>(out + place * 16) = codes_operand(kw[k]);
+            }
+            if (wave < 2 * PT::kPairs) {  // zeros and scales of the keys' group `wave` (one past an odd number: 0)
+                const float zf = high16<BF>(km);
+                const uint32_t zh = __float_as_uint(zf) >> 16;
+                const uint32_t zl = __float_as_uint(zf - __uint_as_float(zh << 16)) >> 16;
+                const int place = (((lane >> 5) * PT::kPairs + (wave >> 1)) * 2 + (wave & 1)) * 32 + row;
+                *reinterpret_cast<uint4 *>(out + 2 * PT::kOperands + place * 16) =
+                    make_uint4(zh | (zh << 16), zh | (zl << 16), zl, 0);
+                if (wave < G)
+                    reinterpret_cast<uint16_t *>(out + 2 * PT::kOperands + PT::kZeros)[wave * kTokens + lane] = (uint16_t)km;
+            }
+
             const bool real = tb + lane < rq.len && (ok >> (lane >> 4) & 1);
-            const uint32_t *m = reinterpret_cast<const uint32_t *>(slot + (lane >> 4) * PT::kSeg + 2 * PT::kKeys + G * 64) + (lane & 15);
+            bool odd_ones = tb + kTokens > rq.len || ok != 15;
+            uint32_t most[G];
 #pragma unroll
             for (int g = 0; g < G; ++g) {
-                const uint32_t u = m[16 * g];
-                const float s = low16<BF>(u), z = high16<BF>(u);
-                const float v = real ? fmaxf(fabsf(z), fabsf(fmaf(15.f, s, z))) : 0.f;
-                bad[g] = __ballot(real && !(s < INFINITY && fabsf(z) < INFINITY));
-                const float c = wave_max_dpp(v < INFINITY ? v : 0.f);
-                const int e = (int)((__float_as_uint(c) >> 23) & 0xffu) - 126;  // c < 2^e
-                if (e > vexp[g]) {
-                    const int now = min(e, 126);
-                    const float f = ldexpf(1.f, vexp[g] - now);
-                    vexp[g] = now;
+                pair[g] = real ? pair[g] & 0x7fff7fffu : 0;
+                most[g] = pair[g];
+                bad_next[g] = 0;
+            }
+            pair_max(most);
+#pragma unroll
+            for (int g = 0; g < G; ++g) {
+                if ((most[g] & 0xffffu) >= kInf || (most[g] >> 16) >= kInf) {
+                    const bool b = (pair[g] & 0x7fffu) >= kInf || (pair[g] >> 16) >= kInf;
+                    bad_next[g] = __ballot(b);
+                    odd_ones = true;
+                    uint32_t rest[1] = {b ? 0 : pair[g]};
+                    pair_max(rest);
+                    most[g] = rest[0];
+                }
+                // |zero + 15 scale| < 2 max(|zero|, 16 scale)
+                const float c = fmaxf(16.f * low16<BF>(most[g]), high16<BF>(most[g]));
+                const int e = __builtin_amdgcn_readfirstlane((int)((__float_as_uint(c) >> 23) & 0xffu) - 125);
+                vnext[g] = max(vnext[g], min(e, 126));
+            }
+            if (odd_ones) {  // (what no row sees, and what makes rows NaN further down)
+                uint64_t keep = ~0ull;
+#pragma unroll
+                for (int g = 0; g < G; ++g) keep = vg == g ? ~bad_next[g] : keep;
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (tb + 8 * wave + i >= rq.len || !((ok >> (wave >> 1)) & 1) || !((keep >> (8 * wave + i)) & 1))
+                        vm[i] = 0;
+            }
+            int e = vnext[0];
+#pragma unroll
+            for (int g = 1; g < G; ++g) e = vg == g ? vnext[g] : e;
+            const float fs = exp2i(18 - e), fz = ldexpf(1.f, -6 - e), fs_odd = fs * 0x1p-4f;
+            half8_t sc, ze;  // codes of odd pairs count 16 times
+#pragma unroll
+            for (int i = 0; i < 8; i += 2) {
+                const float f = (i & 2) ? fs_odd : fs;
+                const half2_t s2 = __builtin_convertvector(float2_t{low16<BF>(vm[i]) * f, low16<BF>(vm[i + 1]) * f}, half2_t);
+                const half2_t z2 = __builtin_convertvector(float2_t{high16<BF>(vm[i]) * fz, high16<BF>(vm[i + 1]) * fz}, half2_t);
+                sc[i] = s2[0], sc[i + 1] = s2[1], ze[i] = z2[0], ze[i + 1] = z2[1];
+            }
+#pragma unroll
+            for (int k = 0; k < VW; ++k)  // dim NT * m + j at place 32 j + m
+                *reinterpret_cast<half8_t *>(out + PT::kOperands + (wave * D + 32 * (j0 + k) + col) * 16) =
+                    __builtin_elementwise_fma(codes_operand(vw[k]), sc, ze);
+        };
+
+        // One tile: computed from `cur`; the next one prepared from `next` into
+        // `out`; the copy of a later one started into `into`.  (The pointers
+        // differ: no read here waits for that copy.)
+        auto step = [&](char *__restrict into, const char *__restrict next, const char *__restrict cur,
+                        char *__restrict out, int tile) {
+            const int tb = tile * kTokens;
+            if (tile + kSlots < n_tiles)
+                PT::fetch(a.st, h, lane, into + seg * PT::kSeg, own(pages), offset(tile + kSlots), wave >> 2);
+            // Of the two waves of a SIMD, w and w + 4, one prepares first and one
+            // last, so that one's products meet the other's softmax.
+            uint64_t bad[G];
+            int move[G];
+#pragma unroll
+            for (int g = 0; g < G; ++g) bad[g] = bad_next[g], move[g] = vexp[g] - vnext[g], vexp[g] = vnext[g];
+            if (tile + 1 < n_tiles && wave >= 4) prepare(next, out, tb + kTokens, ok[1]);
+#pragma unroll
+            for (int g = 0; g < G; ++g)
+                if (move[g]) {
+                    const float f = ldexpf(1.f, move[g]);
 #pragma unroll
                     for (int j = 0; j < NT; ++j)
 #pragma unroll
                         for (int i = 0; i < 16; ++i)
                             if (group_of(i) == g) o[j][i] *= f;
                 }
-            }
-        };
-        // The tile's values as fp16: [8 blocks][dims][8 tokens], dim NT*m + j at
-        // place 32 j + m, so that neighbouring threads write neighbouring places.
-        auto dequantise = [&](const char *__restrict slot, char *__restrict out, int tb, int ok) {
-            const int blk = threadIdx.x >> 5, m = threadIdx.x & 31, g = m * NT * G / D;
-            const char *seg = slot + (blk >> 1) * PT::kSeg;
-            uint32_t meta[8], w[NT];
-            read_words(seg + 2 * PT::kKeys + (G + g) * 64 + (blk & 1) * 32, meta);
-            read_words(seg + PT::kKeys + ((blk & 1) * D + m * NT) * 4, w);
-            int e = vexp[0];
-#pragma unroll
-            for (int k = 1; k < G; ++k) e = g == k ? vexp[k] : e;
-            const float fs = ldexpf(1.f, 18 - e), fz = ldexpf(1.f, -6 - e);
-            const bool page = (ok >> (blk >> 1)) & 1;
-            half2_t s2[4], z2[4];
-#pragma unroll
-            for (int p = 0; p < 4; ++p) {
-                float s[2], z[2];
-#pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    const uint32_t u = meta[2 * p + k];
-                    s[k] = low16<BF>(u) * fs, z[k] = high16<BF>(u) * fz;
-                    // (what no row sees, and what makes rows NaN further down)
-                    if (!page || tb + blk * 8 + 2 * p + k >= rq.len || !(fabsf(s[k]) + fabsf(z[k]) < INFINITY)) s[k] = z[k] = 0.f;
-                }
-                const float odd = (p & 1) ? 0x1p-4f : 1.f;  // codes of odd pairs count 16 times
-                s2[p] = __builtin_convertvector(float2_t{s[0] * odd, s[1] * odd}, half2_t);
-                z2[p] = __builtin_convertvector(float2_t{z[0], z[1]}, half2_t);
-            }
-#pragma unroll
-            for (int j = 0; j < NT; ++j) {
-                union {
-                    half8_t h;
-                    half2_t p[4];
-                    uint4 u;
-                } x;
-                x.h = codes_operand(w[j]);
-#pragma unroll
-                for (int p = 0; p < 4; ++p) x.p[p] = __builtin_elementwise_fma(x.p[p], s2[p], z2[p]);
-                *reinterpret_cast<uint4 *>(out + ((blk * D) + 32 * j + m) * 16) = x.u;
-            }
-        };
-
-        // One tile: its scores from `cur` and values from `vin`; the next one's
-        // values from `next` into `vout`; the copy of the one after that into
-        // `into`.  (The pointers differ: no read here waits for that copy.)
-        uint64_t bad[G], bad_next[G];
-        auto step = [&](char *__restrict into, const char *__restrict cur, const char *__restrict next,
-                        const char *__restrict vin, char *__restrict vout, int tile, int ok, int ok_next) {
-            const int tb = tile * kTokens;
-            if (tile + 2 < n_tiles) {
-                const int t16 = tb + 2 * kTokens + 16 * wave;
-                PT::fetch(a.st, h, lane, into + wave * PT::kSeg, max(page_at(t16), 0), t16 & in_page);
-            }
-            half8_t p16[4];
-            const bool on = tb < wave_end;
-            if (on) {
-                float x[32];
+            if (tb < wave_end) {
 #pragma unroll
                 for (int y = 0; y < 2; ++y) {
-                    // row col of the A operand: this token, so that a lane's 16
-                    // results are two whole blocks of 8 tokens
-                    const int t = 32 * y + 16 * (col >> 4) + 8 * ((col >> 2) & 1) + 4 * ((col >> 3) & 1) + (col & 3);
-                    const char *seg = cur + (t >> 4) * PT::kSeg;
-                    float16_t z = float16_t{};
+                    float16_t x = float16_t{}, d[G];
 #pragma unroll
-                    for (int k = 0; k < (G + 1) / 2; ++k) {
-                        const int zg = min(2 * k + half, G - 1);
-                        const float zf = high16<BF>(*reinterpret_cast<const uint32_t *>(seg + 2 * PT::kKeys + zg * 64 + (t & 15) * 4));
-                        const uint32_t zh = __float_as_uint(zf) >> 16;
-                        const uint32_t zl = __float_as_uint(zf - __uint_as_float(zh << 16)) >> 16;
-                        union {
-                            uint32_t u[4];
-                            bf8_t b;
-                        } za;
-                        za.u[0] = zh | (zh << 16), za.u[1] = zh | (zl << 16), za.u[2] = zl, za.u[3] = 0;
-                        z = __builtin_amdgcn_mfma_f32_32x32x16_bf16(za.b, qz[k], z, 0, 0, 0);
+                    for (int k = 0; k < PT::kPairs; ++k) {
+                        const bf8_t z = *reinterpret_cast<const bf8_t *>(
+                            cur + 2 * PT::kOperands + (((y * PT::kPairs + k) * 2 + half) * 32 + col) * 16);
+                        x = __builtin_amdgcn_mfma_f32_32x32x16_bf16(z, qz[k], x, 0, 0, 0);
                     }
+                    // the groups' sums side by side: a product waits for the one before it
 #pragma unroll
-                    for (int g = 0; g < G; ++g) {
-                        uint32_t w[HW];
-                        const int c = (g * GW + half * HW) / 4, sw = (t >> 2) % PT::kKP;
-                        if constexpr (HW == 8) {
-                            uint32_t w4[4];
+                    for (int g = 0; g < G; ++g) d[g] = float16_t{};
 #pragma unroll
-                            for (int k = 0; k < 2; ++k) {
-                                read_words(seg + ((t & 15) * PT::kKP + ((c + k) ^ sw)) * 16, w4);
+                    for (int s = 0; s < HW; ++s)
 #pragma unroll
-                                for (int e = 0; e < 4; ++e) w[4 * k + e] = w4[e];
-                            }
-                        } else if constexpr (HW == 4) {
-                            read_words(seg + ((t & 15) * PT::kKP + (c ^ sw)) * 16, w);
-                        } else {
-                            read_words(seg + ((t & 15) * PT::kKP + (c ^ sw)) * 16 + half * 8, w);
+                        for (int g = 0; g < G; ++g) {
+                            const half8_t k = *reinterpret_cast<const half8_t *>(
+                                cur + (((y * (D / 16) + g * HW + s) * 2 + half) * 32 + col) * 16);
+                            d[g] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, qf[g][s], d[g], 0, 0, 0);
                         }
-                        float16_t d = float16_t{};
+                    // element i: token 32y + 16(i/8) + 8 half + i%8
 #pragma unroll
-                        for (int s = 0; s < HW; ++s)
-                            d = __builtin_amdgcn_mfma_f32_32x32x16_f16(codes_operand(w[s]), qf[g][s], d, 0, 0, 0);
-                        // element i: token 32y + 16(i/8) + 8 half + i%8
+                    for (int g = 0; g < G; ++g)
 #pragma unroll
-                        for (int i = 0; i < 16; i += 4) {
+                        for (int i = 0; i < 16; i += 8) {
                             uint32_t m[4];
-                            const int t4 = 16 * (i / 8) + 8 * half + i % 8;
-                            read_words(cur + (2 * y + (t4 >> 4)) * PT::kSeg + 2 * PT::kKeys + g * 64 + (t4 & 15) * 4, m);
+                            read_words(cur + 2 * PT::kOperands + PT::kZeros + (g * kTokens + 32 * y + 2 * i + 8 * half) * 2, m);
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) z[i + e] = fmaf(low16<BF>(m[e]), d[i + e], z[i + e]);
+                            for (int e = 0; e < 8; ++e)
+                                x[i + e] = fmaf((e & 1) ? high16<BF>(m[e / 2]) : low16<BF>(m[e / 2]), d[g][i + e], x[i + e]);
+                        }
+                    if (tb + 32 * y + 32 > all_see || ok[0] != 15) {
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) {
+                            const int t = 32 * y + 16 * (i / 8) + 8 * half + i % 8;
+                            if (tb + t >= limit || !((ok[0] >> (2 * y + i / 8)) & 1)) x[i] = -INFINITY;
                         }
                     }
+                    float m = x[0];
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) x[16 * y + i] = z[i];
-                }
-                if (tb + kTokens > all_see || ok != 15) {
+                    for (int i = 1; i < 16; ++i) m = fmaxf(m, x[i]);
+                    if (__any(m > top + lag)) {
+                        const float now = fmaxf(top, half_max(m));
+                        const float f = now == top ? 1.f : fast_exp2((top - now) * factor);
+                        top = now;
+                        l *= f;
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) {
-                        const int t = 32 * (i / 16) + 16 * (i % 16 / 8) + 8 * half + i % 8;
-                        if (tb + t >= limit || !((ok >> (t >> 4)) & 1)) x[i] = -INFINITY;
+                        for (int j = 0; j < NT; ++j) o[j] *= f;
+                    }
+                    // (times 2^10: a probability below 2^-24 of the largest is one fp16 step)
+                    const float off = 10.f - (top == -INFINITY ? 0.f : top * factor);
+#pragma unroll
+                    for (int b = 0; b < 2; ++b) {
+                        half8_t p16;
+#pragma unroll
+                        for (int i = 0; i < 8; i += 2) {
+                            const float p0 = fast_exp2(fmaf(x[8 * b + i], factor, off));
+                            const float p1 = fast_exp2(fmaf(x[8 * b + i + 1], factor, off));
+                            l += p0 + p1;
+                            const half2_t hh = __builtin_convertvector(float2_t{p0, p1}, half2_t);
+                            p16[i] = hh[0], p16[i + 1] = hh[1];
+                        }
+#pragma unroll
+                        for (int j = 0; j < NT; ++j) {
+                            const int blk = 2 * (2 * y + b) + half;
+                            const half8_t v = *reinterpret_cast<const half8_t *>(cur + PT::kOperands + (blk * D + 32 * j + col) * 16);
+                            o[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, p16, o[j], 0, 0, 0);
+                        }
                     }
                 }
-                const float m = column_max(x);
-                if (__any(m > top + lag)) {
-                    const float now = fmaxf(top, half_max(m));
-                    const float f = now == top ? 1.f : fast_exp2((top - now) * factor);
-                    top = now;
-                    l *= f;
-#pragma unroll
-                    for (int j = 0; j < NT; ++j) o[j] *= f;
-                }
-                // (times 2^10: a probability below 2^-24 of the largest is one fp16 step)
-                const float off = 10.f - (top == -INFINITY ? 0.f : top * factor);
-#pragma unroll
-                for (int i = 0; i < 32; i += 2) {
-                    const float p0 = fast_exp2(fmaf(x[i], factor, off)), p1 = fast_exp2(fmaf(x[i + 1], factor, off));
-                    l += p0 + p1;
-                    const half2_t hh = __builtin_convertvector(float2_t{p0, p1}, half2_t);
-                    p16[i / 8][i % 8] = hh[0], p16[i / 8][i % 8 + 1] = hh[1];
-                }
-#pragma unroll
-                for (int b = 0; b < 4; ++b)
-#pragma unroll
-                    for (int j = 0; j < NT; ++j) {
-                        const half8_t v = *reinterpret_cast<const half8_t *>(vin + ((2 * b + half) * D + 32 * j + col) * 16);
-                        o[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, p16[b], o[j], 0, 0, 0);
-                    }
 #pragma unroll
                 for (int g = 0; g < G; ++g)
                     if (bad[g]) {
@@ -386,66 +513,129 @@ __global__ void __launch_bounds__(256, 2) paged_prompt_kernel(const PagedAttn a)
                                     if (group_of(i) == g) o[j][i] = NAN;
                     }
             }
-            if (tile + 1 < n_tiles) {
-                meet(next, tb + kTokens, ok_next, bad_next);
-                dequantise(next, vout, tb + kTokens, ok_next);
-            }
+            if (tile + 1 < n_tiles && wave < 4) prepare(next, out, tb + kTokens, ok[1]);
         };
 
         wait_loads<0>();
         __syncthreads();
-        int ok = n_tiles > 0 ? pages_ok(0) : 0;
-        if (n_tiles > 0) {
-            meet(raw, 0, ok, bad);
-            dequantise(raw, vals, 0, ok);
-        }
-        for (int i = 0, slot = 0; i < n_tiles; ++i) {
-            const int ok_next = pages_ok(i + 1);
-            wait_loads<0>();  // the next tile's segment
-            __syncthreads();  // everyone's, and this tile's values
-            const int next = slot == 2 ? 0 : slot + 1, after = next == 2 ? 0 : next + 1;
-            step(raw + after * PT::kBytes, raw + slot * PT::kBytes, raw + next * PT::kBytes, vals + (i & 1) * kValues,
-                 vals + (~i & 1) * kValues, i, ok, ok_next);
-            slot = next, ok = ok_next;
+        if (first_tile < n_tiles) prepare(raw, prepared, first_tile * kTokens, ok[0]);
+        int slot = 0, into = 1;  // raw slot and prepared form of the tile computed
+        for (int i = first_tile; i < n_tiles; ++i) {
+            // the wave's copies of the next tile (of the one after it, two loads or
+            // one may be on their way), then everyone's, and this tile's operands
+            if (i + 2 >= n_tiles)
+                wait_loads<0>();
+            else if (wave < 4)
+                wait_loads<2>();
+            else
+                wait_loads<1>();
+            lds_barrier();
+            const int next = slot == kSlots - 1 ? 0 : slot + 1, from = into ^ 1;
+            step(raw + slot * PT::kBytes, raw + next * PT::kBytes, prepared + from * PT::kPrepared,
+                 prepared + into * PT::kPrepared, i);
+            slot = next, into = from;
 #pragma unroll
-            for (int g = 0; g < G; ++g) bad[g] = bad_next[g];
+            for (int k = 0; k < kSlots; ++k) ok[k] = ok[k + 1];
+            ok[kSlots - 1] = mask_of(pages);
+            pages_of(i + kSlots + 1, pages);
         }
 
         const float sum = l + __shfl_xor(l, 32);
-        const float inv = sum == 0.f ? 0.f : 1.f / sum;
-        if (live) {
-            const int64_t at = ((int64_t)(rq.t0 + row / a.rep) * a.hq + h * a.rep + row % a.rep) * D;
+        if (parts == 1) {
+            const float inv = sum == 0.f ? 0.f : 1.f / sum;
+            if (live) {
+                const int64_t at = ((int64_t)(rq.t0 + row / a.rep) * a.hq + h * a.rep + row % a.rep) * D;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const int m = 8 * (i / 4) + 4 * half + i % 4;
+                    const int e = vexp[group_of(i)] + 6;
+                    if constexpr (NT == 4) {
+                        store_out4(a, at + NT * m, ldexpf(o[0][i] * inv, e), ldexpf(o[1][i] * inv, e),
+                                   ldexpf(o[2][i] * inv, e), ldexpf(o[3][i] * inv, e));
+                    } else if (i % 2 == 0) {  // (two rows of the A operand are neighbours)
+                        store_out4(a, at + NT * m, ldexpf(o[0][i] * inv, e), ldexpf(o[1][i] * inv, e),
+                                   ldexpf(o[0][i + 1] * inv, e), ldexpf(o[1][i + 1] * inv, e));
+                    }
+                }
+            }
+        } else {
+            // a part: the sums as they are (times 2^10), for prompt_merge_kernel
+            if (part == 0) cut = make_int4(parts, r, h, row_tile);
+            const int64_t at = (int64_t)item * kRows + wave * 32 + col;
+            if (half == 0) *reinterpret_cast<float2 *>(a.ml + at * 2) = make_float2(top * factor, sum);
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
                 const int m = 8 * (i / 4) + 4 * half + i % 4;
                 const int e = vexp[group_of(i)] + 6;
-                if constexpr (NT == 4) {
-                    store4_from_f32(a.out, a.q_dtype, at + NT * m, ldexpf(o[0][i] * inv, e), ldexpf(o[1][i] * inv, e),
-                                    ldexpf(o[2][i] * inv, e), ldexpf(o[3][i] * inv, e));
-                } else {
 #pragma unroll
-                    for (int j = 0; j < NT; ++j) store_from_f32(a.out, a.q_dtype, at + NT * m + j, ldexpf(o[j][i] * inv, e));
-                }
+                for (int j = 0; j < NT; ++j) a.acc[at * D + NT * m + j] = ldexpf(o[j][i], e);
             }
         }
         __syncthreads();  // (the next item's copies)
+    }
+    if (a.cut && (int)blockIdx.x < a.target && threadIdx.x == 0) a.cut[blockIdx.x] = cut;
+}
+
+// Joins the parts of the column that cut[blockIdx.y] names: part i is at item
+// blockIdx.y + i * heads.  A thread takes four dims of a row.
+template <int D>
+__global__ void __launch_bounds__(256) prompt_merge_kernel(const PagedAttn a) {
+    constexpr int CH = D / 4, AT_ONCE = 256 / CH;
+    const int4 cut = a.cut[blockIdx.y];
+    const int parts = cut.x, r = cut.y, h = cut.z, c = threadIdx.x % CH * 4;
+    if (parts == 0) return;
+    const Request rq = request(a, r);
+    for (int row = blockIdx.x * AT_ONCE + threadIdx.x / CH; row < kRows; row += gridDim.x * AT_ONCE) {
+        const int n = cut.w * kRows + row;
+        if (n >= rq.rows) return;
+        auto at = [&](int i) { return ((int64_t)blockIdx.y + (int64_t)i * a.st.heads) * kRows + row; };
+        float m = -INFINITY, l = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
+        for (int i = 0; i < parts; ++i) m = fmaxf(m, a.ml[at(i) * 2]);
+#pragma unroll 4
+        for (int i = 0; i < parts; ++i) {
+            const float2 e = *reinterpret_cast<const float2 *>(a.ml + at(i) * 2);
+            const float4 v = *reinterpret_cast<const float4 *>(a.acc + at(i) * D + c);
+            const float f = e.x == m ? 1.f : fast_exp2(e.x - m);
+            l += f * e.y;
+            x[0] += f * v.x, x[1] += f * v.y, x[2] += f * v.z, x[3] += f * v.w;
+        }
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        const int64_t o = ((int64_t)(rq.t0 + n / a.rep) * a.hq + h * a.rep + n % a.rep) * D + c;
+        store_out4(a, o, x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
     }
 }
 
 template <int D, int G>
 static void launch_prompt(const PagedAttn &a, bool bf, unsigned groups, hipStream_t st) {
+    const dim3 block(64 * kPWaves);
     if (bf)
-        hipLaunchKernelGGL((paged_prompt_kernel<D, G, true>), dim3(groups), dim3(256), 0, st, a);
+        hipLaunchKernelGGL((paged_prompt_kernel<D, G, true>), dim3(groups), block, 0, st, a);
     else
-        hipLaunchKernelGGL((paged_prompt_kernel<D, G, false>), dim3(groups), dim3(256), 0, st, a);
+        hipLaunchKernelGGL((paged_prompt_kernel<D, G, false>), dim3(groups), block, 0, st, a);
+    if (a.target) hipLaunchKernelGGL(prompt_merge_kernel<D>, dim3(16, a.target), dim3(256), 0, st, a);
 }
 
-int launch_paged_prompt(const PagedAttn &a, const ss_paged_store *s, hipStream_t st) {
+// Workgroups that fill the device (one a compute unit) if the columns alone
+// may not, else 0: then no column is cut.
+static int cut_target(int64_t n_requests, int heads, int64_t rows, int most_rows) {
+    const int64_t least = max((int64_t)0, rows - n_requests * most_rows) / kRows * heads;
+    return 2 * least <= device_cu_count() ? device_cu_count() : 0;
+}
+
+size_t paged_prompt_bytes(const ss_paged_store *s, int64_t n_requests, int64_t rows, int most_rows) {
+    return (size_t)cut_target(n_requests, s->n_kv_heads, rows, most_rows) * (16 + kRows * (s->head_dim + 2) * 4);
+}
+
+int launch_paged_prompt(PagedAttn a, const ss_paged_store *s, void *workspace, hipStream_t st) {
     // at most this many row tiles: whole ones, and one a request of more than most_rows rows
     const int64_t rows = a.n_tokens * a.rep;
     const int64_t tiles = rows / kRows + min((int64_t)a.n_req, rows / (a.most_rows + 1));
-    const unsigned groups = (unsigned)min(tiles * a.st.heads, (int64_t)1 << 20);
-    if (groups == 0) return SS_OK;
+    if (tiles == 0) return SS_OK;
+    a.target = cut_target(a.n_req, a.st.heads, rows, a.most_rows);
+    a.cut = a.target ? static_cast<int4 *>(workspace) : nullptr;
+    a.acc = reinterpret_cast<float *>(a.cut + a.target);
+    a.ml = a.acc + (size_t)a.target * kRows * s->head_dim;
+    const unsigned groups = (unsigned)max(min(tiles * a.st.heads, (int64_t)1 << 20), (int64_t)a.target);
     const bool bf = s->dtype == SS_BF16;
     const int key = s->head_dim * 1000 + s->group_size;
     if (key == 128032) launch_prompt<128, 4>(a, bf, groups, st);

@@ -298,7 +298,7 @@ def paged_attention(queries: torch.Tensor, store: PagedKVStore, block_table: tor
     max_new = max(1, min(n, n - r + 1 if max_new is None else max_new))
     max_length = max(1, min(width * st.page_size, max_length or width * st.page_size))
     at = ctypes.addressof(st)
-    need = _hip.load_library().ss_paged_attn_workspace_bytes(at, r, hq, max_new, max_length)
+    need = _hip.load_library().ss_paged_attn_workspace_bytes(at, n, r, hq, max_new, max_length)
     # of this call alone: calls on other streams and captured graphs have their own
     ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
     _launch("ss_paged_attn", dev, at, q.data_ptr(), _hip.dtype_code(q.dtype), n, q.stride(0),
