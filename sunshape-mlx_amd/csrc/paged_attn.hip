@@ -9,8 +9,6 @@
 // holds, of one column, 4 tokens of each key tile; two key tiles whose token
 // order is chosen so make exactly the lane's 8 tokens of the second product's
 // B operand: the probabilities never leave the lane's registers.
-#include <type_traits>
-
 #include "paged_attn.hpp"
 
 namespace ss {
@@ -318,9 +316,8 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(const PagedAttn a) {
             for (int j = 0; j < VT; ++j) o[s][j] *= f;
         };
 
-        // masked: some row does not see some token of the tile
-        auto compute = [&](const char *slot, int tb, bool ok, auto masked) {
-            constexpr bool mask = decltype(masked)::value;
+        // mask: some row does not see some token of the tile
+        auto compute = [&](const char *slot, int tb, bool ok, bool mask) {
             uint32_t kw[2][KS], vw[VT], km[8], vm[8];
 #pragma unroll
             for (int y = 0; y < 2; ++y) {
@@ -359,27 +356,40 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(const PagedAttn a) {
                 for (int s = 0; s < NS; ++s) rescale(s, ldexpf(1.f, vexp - now));
                 vexp = now;
             }
-            half8_t p16[NS];
+            // (sets inside: an operand's registers serve every set and are free again)
+            float xs[NS][8];
 #pragma unroll
-            for (int s = 0; s < NS; ++s) {
-                float x[8];
+            for (int y = 0; y < 2; ++y) {
+                float4_t d[NS];
 #pragma unroll
-                for (int y = 0; y < 2; ++y) {
-                    float4_t d = {0.f, 0.f, 0.f, 0.f};
+                for (int s = 0; s < NS; ++s) d[s] = float4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                    for (int k = 0; k < KS; ++k)
-                        d = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes_operand(kw[y][k]), qf[s][k], d, 0, 0, 0);
+                for (int k = 0; k < KS; ++k) {
+                    const half8_t key = codes_operand(kw[y][k]);
+#pragma unroll
+                    for (int s = 0; s < NS; ++s)
+                        d[s] = __builtin_amdgcn_mfma_f32_16x16x32_f16(key, qf[s][k], d[s], 0, 0, 0);
+                }
+#pragma unroll
+                for (int s = 0; s < NS; ++s)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const uint32_t m = km[4 * y + i];
-                        x[4 * y + i] = groups_sum<G>(fmaf(low16<BF>(m), d[i], high16<BF>(m) * qz[s]));
+                        xs[s][4 * y + i] = groups_sum<G>(fmaf(low16<BF>(m), d[s][i], high16<BF>(m) * qz[s]));
                     }
-                }
-                if (mask) {
+            }
+            half8_t p16[NS];
+#pragma unroll
+            for (int s = 0; s < NS; ++s) {
+                float(&x)[8] = xs[s];
+                uint32_t v[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[j] = vm[j];
+                if (mask) {  // what the row does not see adds nothing, whatever its value holds
                     const int see = ok ? limit[s] : 0;
 #pragma unroll
                     for (int j = 0; j < 8; ++j)
-                        if (first + j >= see) x[j] = -INFINITY;
+                        if (first + j >= see) x[j] = -INFINITY, v[j] = 0;
                 }
                 const float m = column_max(x);
                 if (__any(m > top[s] + lag[s])) {
@@ -395,9 +405,8 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(const PagedAttn a) {
                     const float p = fast_exp2(fmaf(x[j], factor[s], (j & 2) ? even - 4.f : even));
                     // the value's middle, zero + 7.5 scale, in float32: what is
                     // left for the product, (code - 7.5) scale, is small
-                    float mid = fmaf(low16<BF>(vm[j]), 7.5f, high16<BF>(vm[j]));
-                    w[j] = p * low16<BF>(vm[j]);
-                    if (mask && (!ok || first + j >= limit[s])) mid = w[j] = 0.f;  // (even of NaN)
+                    const float mid = fmaf(low16<BF>(v[j]), 7.5f, high16<BF>(v[j]));
+                    w[j] = p * low16<BF>(v[j]);
                     if (j & 2) {
                         l_odd[s] += p;
                         z_odd[s] = fmaf(p, mid, z_odd[s]);
@@ -434,10 +443,7 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(const PagedAttn a) {
                 wait_loads<0>();
             }
             const bool ok = (quad < 2 ? p0 : p1) >= 0;
-            if (tb + kTile > all_see || p0 < 0 || p1 < 0)
-                compute(slot, tb, ok, std::true_type{});
-            else
-                compute(slot, tb, ok, std::false_type{});
+            compute(slot, tb, ok, tb + kTile > all_see || p0 < 0 || p1 < 0);
         };
         int slot = 0;
         for (int tb = begin + kTile * wave; tb < end; tb += kUnit) {
