@@ -150,7 +150,7 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(const PagedAttn a) {
     const int total = __builtin_amdgcn_readlane(units_scan, 63);
     const int all_columns = __builtin_amdgcn_readlane(wave_scan(columns), 63);
     int u, stop, base, r, share, parts = 0;
-    if (all_columns <= groups / 2) {
+    if (a.cut && all_columns <= groups / 2) {
         // Few columns: each is cut into parts of its own, of at most `share`
         // units, so that no workgroup has more than one.  Sum of ceil(n/share)
         // is at most total/share + columns, and about total/share + columns/2.
@@ -191,7 +191,8 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(const PagedAttn a) {
         }
     } else {
         // Many: the units of all columns in one row, shared out evenly; a run
-        // may end inside a column and may hold several.
+        // may end inside a column and may hold several.  (Without `cut`: a
+        // workgroup takes the columns that begin in its share, whole.)
         share = max(uniform_div(total + groups - 1, groups), kWhole);
         u = min((int64_t)blockIdx.x * share, (int64_t)total);
         stop = min((int64_t)u + share, (int64_t)total);
@@ -212,11 +213,15 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(const PagedAttn a) {
         }
         const int column = uniform_div(u - base, n_units);
         const int c0 = base + column * n_units, c1 = c0 + n_units;
+        if (!a.cut && c0 < first_unit) {
+            u = c1;
+            continue;
+        }
         const int h = uniform_div(column, row_blocks), rb = column - h * row_blocks;
         const int begin = (u - c0) * kUnit;
-        const int part_end = min(stop, c1);
+        const int part_end = a.cut ? min(stop, c1) : c1;
         const int end = min((part_end - c0) * kUnit, rq.len);
-        const bool whole = c0 >= first_unit && c1 <= stop;
+        const bool whole = c0 >= first_unit && (!a.cut || c1 <= stop);
         const int place = c0 < first_unit ? 0 : 1;  // of this part, if it is one
         if (!whole && place == 1)
             cut = make_int4(parts ? parts : uniform_div(c1 - 1, share) - (int)blockIdx.x + 1, r, h, rb);
@@ -501,7 +506,7 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(const PagedAttn a) {
         }
         __syncthreads();
     }
-    if (threadIdx.x == 0) a.cut[blockIdx.x] = cut;
+    if (a.cut && threadIdx.x == 0) a.cut[blockIdx.x] = cut;
 }
 
 // Joins the parts of the column that workgroup blockIdx.y of the kernel above
@@ -569,6 +574,7 @@ __global__ void __launch_bounds__(256) paged_merge_kernel(const PagedAttn a, int
 
 struct PagedPlan {
     int sets, rows, groups;  // column sets, query rows a workgroup takes; workgroups
+    bool cut;                // whether columns may be cut
     size_t bytes;
 };
 
@@ -583,8 +589,10 @@ static PagedPlan paged_plan(const ss_paged_store *s, int64_t n_tokens, int64_t n
     p.rows = p.sets * rs;
     const double units = (double)n_requests * s->n_kv_heads * ((rows + p.rows - 1) / p.rows) *
                          ((max_length + kUnit - 1) / kUnit);
-    p.groups = (int)min((double)(2 * device_cu_count()), units / kMinShare + 1);
-    p.bytes = (size_t)p.groups * (16 + 2 * p.rows * (s->head_dim + 2) * 4);
+    p.cut = max_length > kWhole * kUnit;
+    p.groups = (int)min((double)(2 * device_cu_count()), units / (p.cut ? kMinShare : 1));
+    p.groups = max(p.groups, 1);
+    p.bytes = p.cut ? (size_t)p.groups * (16 + 2 * p.rows * (s->head_dim + 2) * 4) : 0;
     if (max_new * rep > kPromptRows)  // (one after the other: they share it)
         p.bytes = max(p.bytes, paged_prompt_bytes(s, n_requests, n_tokens * rep, kPromptRows));
     return p;
@@ -607,7 +615,7 @@ static void launch_paged(const PagedAttn &a, const PagedPlan &p, hipStream_t st)
         hipLaunchKernelGGL((paged_attn_kernel<D, G, BF, 1>), dim3(p.groups), dim3(256), 0, st, a);
     else
         hipLaunchKernelGGL((paged_attn_kernel<D, G, BF, 2>), dim3(p.groups), dim3(256), 0, st, a);
-    if (p.groups > 1)
+    if (p.cut)
         hipLaunchKernelGGL(paged_merge_kernel<D>, dim3(p.rows, p.groups), dim3(256), 0, st, a, p.rows);
 }
 
@@ -660,7 +668,7 @@ extern "C" int ss_paged_attn(const ss_paged_store *store, const void *q, int q_d
     a.vec = ((uintptr_t)q & 15) == 0 && q_st % 8 == 0 && q_sh % 8 == 0;
     const bool prompts = max_new * a.rep > kPromptRows;
     a.most_rows = prompts ? kPromptRows : INT32_MAX;
-    a.cut = static_cast<int4 *>(workspace);
+    a.cut = p.cut ? static_cast<int4 *>(workspace) : nullptr;
     a.acc = reinterpret_cast<float *>(a.cut + p.groups);
     a.ml = a.acc + (size_t)p.groups * 2 * p.rows * store->head_dim;
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);

@@ -23,6 +23,7 @@ infinity or NaN is held as NaN.
 from __future__ import annotations
 
 import ctypes
+from functools import lru_cache
 from typing import NamedTuple
 
 import torch
@@ -110,51 +111,58 @@ class BlockPlan(NamedTuple):
 
 
 def _struct(store: PagedKVStore) -> _Store:
-    """The store's C form, its tensors' shapes checked against each other."""
+    """The store's C form, its tensors checked (every call: they may have been
+    given other memory in place)."""
     kc, vc, km, vm = store
-    if kc.dim() != 4 or vc.dim() != 4 or km.dim() != 5 or kc.shape[2] < 1:
+    if not (kc.is_cuda and vc.is_cuda and km.is_cuda and vm.is_cuda):
+        _hip.require_gpu(kc, vc, km, vm)
+    shape, meta = kc.shape, km.shape
+    if len(shape) != 4 or len(meta) != 5:
         raise ValueError("a paged store has 4-dim codes and 5-dim scales")
-    n, h, p, _ = kc.shape
-    d = vc.shape[3]
-    g = km.shape[2]
-    meta = (n, h, g, p, 2)
-    if kc.shape != (n, h, p, d // 8) or vc.shape != (n, h, p // 8, d) or km.shape != meta or \
-            vm.shape != meta or g < 1 or d % g or d % 8:
-        raise ValueError(f"store shapes do not agree: {tuple(kc.shape)}, {tuple(vc.shape)}, "
-                         f"{tuple(km.shape)}, {tuple(vm.shape)}")
-    if kc.dtype != torch.int32 or vc.dtype != torch.int32 or km.dtype not in _HALF or \
-            vm.dtype != km.dtype:
+    n, h, p, w = shape
+    d, g = 8 * w, meta[2]
+    if vc.shape != (n, h, p // 8, d) or meta != (n, h, g, p, 2) or vm.shape != meta or \
+            g < 1 or d % g or p % 8:
+        raise ValueError(f"store shapes do not agree: {tuple(shape)}, {tuple(vc.shape)}, "
+                         f"{tuple(meta)}, {tuple(vm.shape)}")
+    dtype = km.dtype
+    if kc.dtype is not torch.int32 or vc.dtype is not torch.int32 or dtype not in _HALF or \
+            vm.dtype is not dtype:
         raise TypeError("a paged store has int32 codes and float16 or bfloat16 scales")
-    _hip.require_gpu(*store)
-    dev = kc.device
-    for t in store:
-        if not t.is_contiguous() or t.device != dev:
-            raise ValueError("store tensors must be contiguous and on one device")
+    dev = kc.get_device()
+    if vc.get_device() != dev or km.get_device() != dev or vm.get_device() != dev or not (
+            kc.is_contiguous() and vc.is_contiguous() and km.is_contiguous() and
+            vm.is_contiguous()):
+        raise ValueError("store tensors must be contiguous and on one device")
     return _Store(kc.data_ptr(), vc.data_ptr(), km.data_ptr(), vm.data_ptr(), n, h, d, d // g, p,
-                  _hip.dtype_code(km.dtype))
+                  _CODE[dtype])
 
 
-def _index(name: str, t: torch.Tensor, shape, device) -> torch.Tensor:
-    """An int32 tensor of the tables, checked."""
-    _hip.require_gpu(t)
-    if t.dtype != torch.int32:
+_CODE = {torch.float32: _hip.SS_F32, torch.float16: _hip.SS_F16, torch.bfloat16: _hip.SS_BF16}
+
+
+def _index(name: str, t: torch.Tensor, shape, dev: int) -> int:
+    """The address of an int32 tensor of the tables, checked."""
+    if not t.is_cuda:
+        _hip.require_gpu(t)
+    if t.dtype is not torch.int32:
         raise TypeError(f"{name} must be int32, not {t.dtype}")
-    if t.shape != shape or not t.is_contiguous() or t.device != device:
-        raise ValueError(f"{name} must be contiguous {tuple(shape)} on {device}, got "
+    if t.shape != shape or not t.is_contiguous() or t.get_device() != dev:
+        raise ValueError(f"{name} must be contiguous {tuple(shape)} on cuda:{dev}, got "
                          f"{tuple(t.shape)} on {t.device}")
-    return t
+    return t.data_ptr()
 
 
-def _launch(name: str, device, *args) -> None:
-    """A C-ABI call on the current stream of ``device``, which need not be
+def _launch(name: str, dev: int, *args) -> None:
+    """A C-ABI call on the current stream of device ``dev``, which need not be
     the current device."""
     fn = getattr(_hip.load_library(), name)
-    if device.index == torch.cuda.current_device():
-        _hip.check(fn(*args, _hip.stream_handle(device)))
+    if dev == torch._C._cuda_getDevice():
+        rc = fn(*args, _hip.stream_handle(dev))
     else:
-        with torch.cuda.device(device):
-            _hip.check(fn(*args, _hip.stream_handle(device)))
-    _hip.record_dispatch(name[3:] + "_hip")
+        with torch.cuda.device(dev):
+            rc = fn(*args, _hip.stream_handle(dev))
+    _hip._launched(name, rc)
 
 
 def build_block_tables(lengths: torch.Tensor, new_lengths: torch.Tensor,
@@ -172,29 +180,32 @@ def build_block_tables(lengths: torch.Tensor, new_lengths: torch.Tensor,
     place; new tensors by default).  All tensors int32 on one device; nothing
     waits for the GPU: a step that is impossible (too few pages, say) changes
     nothing, gives no token a slot and says why in ``status``."""
-    _hip.require_gpu(lengths)
-    dev = lengths.device
     if lengths.dim() != 1 or block_table.dim() != 2 or free_pages.dim() != 1:
         raise ValueError("lengths (R,), block_table (R, W) and free_pages (n_pages,) expected")
-    r = lengths.shape[0]
-    _index("lengths", lengths, (r,), dev)
-    _index("new_lengths", new_lengths, (r,), dev)
-    _index("block_table", block_table, (r, block_table.shape[1]), dev)
-    _index("free_pages", free_pages, free_pages.shape, dev)
-    _index("n_free", n_free, (1,), dev)
     if n_tokens < 0:
         raise ValueError("n_tokens must not be negative")
+    if not lengths.is_cuda:
+        _hip.require_gpu(lengths)
+    dev, size = lengths.get_device(), lengths.shape
+    r, width = size[0], block_table.shape[1]
+    args = (_index("lengths", lengths, size, dev), _index("new_lengths", new_lengths, size, dev), r,
+            _index("block_table", block_table, (r, width), dev), width,
+            _index("free_pages", free_pages, free_pages.shape, dev), free_pages.shape[0],
+            _index("n_free", n_free, (1,), dev), page_size, n_tokens)
     # one allocation for everything that is new
-    buf = torch.empty(2 * r + 3 + 2 * n_tokens, dtype=torch.int32, device=dev)
-    parts = buf.split_with_sizes((r + 1, n_tokens, n_tokens, r, 1, 1))
-    starts, slots, positions, len_out, free_out, status = parts
-    len_out = len_out if lengths_out is None else _index("lengths_out", lengths_out, (r,), dev)
-    free_out = free_out if n_free_out is None else _index("n_free_out", n_free_out, (1,), dev)
-    _launch("ss_block_tables", dev, lengths.data_ptr(), new_lengths.data_ptr(), r,
-            block_table.data_ptr(), block_table.shape[1], free_pages.data_ptr(),
-            free_pages.shape[0], n_free.data_ptr(), page_size, n_tokens, len_out.data_ptr(),
-            free_out.data_ptr(), starts.data_ptr(), slots.data_ptr(), positions.data_ptr(),
-            status.data_ptr())
+    buf = torch.empty(2 * r + 3 + 2 * n_tokens, dtype=torch.int32, device=lengths.device)
+    starts, slots, positions, len_out, free_out, status = buf.split_with_sizes(
+        (r + 1, n_tokens, n_tokens, r, 1, 1))
+    at = buf.data_ptr()
+    at_len = at + 4 * (r + 1 + 2 * n_tokens)
+    at_free, at_status = at_len + 4 * r, at_len + 4 * r + 4
+    if lengths_out is not None:
+        len_out, at_len = lengths_out, _index("lengths_out", lengths_out, size, dev)
+    if n_free_out is not None:
+        free_out, at_free = n_free_out, _index("n_free_out", n_free_out, (1,), dev)
+    at_slots = at + 4 * (r + 1)
+    _launch("ss_block_tables", dev, *args, at_len, at_free, at, at_slots, at_slots + 4 * n_tokens,
+            at_status)
     return BlockPlan(len_out, free_out, starts, slots, positions, status)
 
 
@@ -210,11 +221,12 @@ def check_plan(plan: BlockPlan) -> None:
         raise RuntimeError("block tables: " + ", ".join(t for b, t in _STATUS if status & b))
 
 
-def _rows(name: str, t: torch.Tensor, shape, device) -> torch.Tensor:
-    """(N, H, D) rows of a kernel's type with unit last stride."""
-    _hip.require_gpu(t)
-    if t.shape != shape or t.device != device:
-        raise ValueError(f"{name} must be {tuple(shape)} on {device}, got {tuple(t.shape)} on "
+def _rows(name: str, t: torch.Tensor, shape, dev: int) -> torch.Tensor:
+    """(N, H, D) rows with unit last stride."""
+    if not t.is_cuda:
+        _hip.require_gpu(t)
+    if t.shape != shape or t.get_device() != dev:
+        raise ValueError(f"{name} must be {tuple(shape)} on cuda:{dev}, got {tuple(t.shape)} on "
                          f"{t.device}")
     return t if t.stride(2) == 1 else t.contiguous()
 
@@ -226,29 +238,41 @@ def append_paged(store: PagedKVStore, keys: torch.Tensor, values: torch.Tensor,
     Tokens whose slot is negative or outside the pool are left out; the slots
     of the others have to differ from each other."""
     st = _struct(store)
-    dev = store.k_codes.device
-    shape = (slots.shape[0], st.n_kv_heads, st.head_dim) if slots.dim() == 1 else None
-    _index("slots", slots, slots.shape[:1], dev)
-    if keys.dtype != values.dtype:
+    dev = store[0].get_device()
+    n = slots.shape[0]
+    at_slots = _index("slots", slots, (n,), dev)
+    if keys.dtype is not values.dtype:
         raise TypeError("keys and values must share a dtype")
     code = _hip.dtype_code(keys.dtype)
+    shape = (n, st.n_kv_heads, st.head_dim)
     k, v = _rows("keys", keys, shape, dev), _rows("values", values, shape, dev)
-    _launch("ss_append_paged", dev, ctypes.addressof(st), k.data_ptr(), v.data_ptr(), code,
-            shape[0], k.stride(0), k.stride(1), v.stride(0), v.stride(1), slots.data_ptr())
+    _launch("ss_append_paged", dev, ctypes.addressof(st), k.data_ptr(), v.data_ptr(), code, n,
+            k.stride(0), k.stride(1), v.stride(0), v.stride(1), at_slots)
 
 
 def read_paged(store: PagedKVStore, slots: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """(keys, values) that ``slots`` (N,) hold, (N, H, D) in the store's type
     (zeros for a slot outside the pool)."""
     st = _struct(store)
-    dev = store.k_codes.device
-    _index("slots", slots, slots.shape[:1], dev)
     n = slots.shape[0]
-    out = torch.empty((2, n, st.n_kv_heads, st.head_dim), dtype=store.dtype, device=dev)
-    k, v = out.unbind(0)
-    _launch("ss_read_paged", dev, ctypes.addressof(st), slots.data_ptr(), n, k.data_ptr(),
-            v.data_ptr())
+    dev = store[0].get_device()
+    at_slots = _index("slots", slots, (n,), dev)
+    shape = (n, st.n_kv_heads, st.head_dim)
+    dtype, device = store[2].dtype, store[0].device
+    k = torch.empty(shape, dtype=dtype, device=device)
+    v = torch.empty(shape, dtype=dtype, device=device)
+    _launch("ss_read_paged", dev, ctypes.addressof(st), at_slots, n, k.data_ptr(), v.data_ptr())
     return k, v
+
+
+@lru_cache(maxsize=4096)
+def _workspace_bytes(dev: int, shape: tuple, n: int, r: int, hq: int, max_new: int,
+                     max_length: int) -> int:
+    """Workspace of a call of these sizes on device ``dev``."""
+    like = _Store(1 << 20, 1 << 20, 1 << 20, 1 << 20, *shape)  # (addresses are not read)
+    with torch.cuda.device(dev):
+        return _hip.load_library().ss_paged_attn_workspace_bytes(
+            ctypes.addressof(like), n, r, hq, max_new, max_length)
 
 
 def paged_attention(queries: torch.Tensor, store: PagedKVStore, block_table: torch.Tensor,
@@ -269,40 +293,41 @@ def paged_attention(queries: torch.Tensor, store: PagedKVStore, block_table: tor
     a token and a table row is full); the result does not depend on them.
     Queries under autograd are refused: there is no backward pass."""
     st = _struct(store)
-    dev = store.k_codes.device
+    dev = store[0].get_device()
     if queries.dim() != 3 or lengths.dim() != 1 or block_table.dim() != 2:
         raise ValueError("queries (N, Hq, D), lengths (R,) and block_table (R, W) expected")
     n, hq, _ = queries.shape
-    r = lengths.shape[0]
-    if queries.dtype not in _HALF:
-        raise TypeError(f"queries must be float16 or bfloat16, not {queries.dtype}")
+    r, width = block_table.shape
+    dtype = queries.dtype
+    if dtype not in _HALF:
+        raise TypeError(f"queries must be float16 or bfloat16, not {dtype}")
     if queries.requires_grad and torch.is_grad_enabled():
         raise ValueError("paged_attention has no backward pass: call it under torch.no_grad()")
     if hq < 1 or hq % st.n_kv_heads:
         raise ValueError(f"{hq} query heads do not share {st.n_kv_heads} KV heads")
-    q = _rows("queries", queries, (n, hq, st.head_dim), dev)
-    width = block_table.shape[1]
-    _index("lengths", lengths, (r,), dev)
-    _index("block_table", block_table, (r, width), dev)
-    _index("token_starts", token_starts, (r + 1,), dev)
+    shape = (n, hq, st.head_dim)
+    q = _rows("queries", queries, shape, dev)
+    at_lengths = _index("lengths", lengths, (r,), dev)
+    at_table = _index("block_table", block_table, (r, width), dev)
+    at_starts = _index("token_starts", token_starts, (r + 1,), dev)
     zero_rest = out is None
-    if out is None:
-        out = torch.empty((n, hq, st.head_dim), dtype=q.dtype, device=dev)
-    elif out.shape != q.shape or out.dtype != q.dtype or out.device != dev or \
+    if zero_rest:
+        out = torch.empty(shape, dtype=dtype, device=q.device)
+    elif out.shape != shape or out.dtype is not dtype or out.device != q.device or \
             not out.is_contiguous():
-        raise ValueError(f"out must be contiguous {q.dtype} {tuple(q.shape)} on {dev}")
+        raise ValueError(f"out must be contiguous {dtype} {shape} on {q.device}")
     if n == 0:
         return out
     if r == 0:
         return out.zero_() if zero_rest else out
+    most = width * st.page_size
     max_new = max(1, min(n, n - r + 1 if max_new is None else max_new))
-    max_length = max(1, min(width * st.page_size, max_length or width * st.page_size))
-    at = ctypes.addressof(st)
-    need = _hip.load_library().ss_paged_attn_workspace_bytes(at, n, r, hq, max_new, max_length)
+    max_length = max(1, min(most, most if max_length is None else max_length))
+    need = _workspace_bytes(dev, (st.n_pages, st.n_kv_heads, st.head_dim, st.group_size,
+                                  st.page_size, st.dtype), n, r, hq, max_new, max_length)
     # of this call alone: calls on other streams and captured graphs have their own
-    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-    _launch("ss_paged_attn", dev, at, q.data_ptr(), _hip.dtype_code(q.dtype), n, q.stride(0),
-            q.stride(1), hq, block_table.data_ptr(), width, lengths.data_ptr(),
-            token_starts.data_ptr(), r, float(scale), int(causal), max_new, max_length,
-            out.data_ptr(), int(zero_rest), _hip.ptr(ws), need)
+    ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+    _launch("ss_paged_attn", dev, ctypes.addressof(st), q.data_ptr(), _CODE[dtype], n, q.stride(0),
+            q.stride(1), hq, at_table, width, at_lengths, at_starts, r, scale, causal, max_new,
+            max_length, out.data_ptr(), zero_rest, _hip.ptr(ws), need)
     return out

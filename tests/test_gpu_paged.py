@@ -339,9 +339,22 @@ def test_attention_over_many_splits(length):
     for _ in range(3):  # bit for bit the same again
         assert torch.equal(S.paged_attention(q, store, table, le, starts, 0.09, max_new=1,
                                              max_length=length), first)
-    for hint in (1, 200, 100000):
+    for hint in (1, 200, 513, 100000):  # (too short ones too: whole columns, then)
         out = S.paged_attention(q, store, table, le, starts, 0.09, max_length=hint)
         check_attention(out, q, store, table, le, starts, 0.09)
+
+
+@pytest.mark.parametrize("hint", [None, 100])
+@pytest.mark.parametrize("b,most", [(70, 300), (300, 40), (150, 900)])
+def test_attention_of_many_requests(b, most, hint):
+    """More requests than a wave has lanes, more columns than workgroups."""
+    rng = random.Random(b)
+    lengths = [rng.choice([0, 1, rng.randint(1, most), rng.randint(1, most)]) for _ in range(b)]
+    new = [min(n, rng.choice([0, 1, 1, 1, 2])) for n in lengths]
+    store, table, le, starts = world(5, lengths, new, 4, 64, 64, 16, torch.float16)
+    q = rows(9, sum(new), 8, 64, torch.float16, False)
+    out = S.paged_attention(q, store, table, le, starts, 0.125, max_new=2, max_length=hint)
+    check_attention(out, q, store, table, le, starts, 0.125)
 
 
 @pytest.mark.parametrize("new", [1, 80])
