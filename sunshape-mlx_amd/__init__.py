@@ -4,7 +4,8 @@ A from-scratch HIP implementation of the compressed-KV attention path of
 gauravsaini/sunshape-mlx behind that package's Python API: block-VQ key
 encoding, the per-step query x centroid table, fused split-T gather-attention
 decode over uint8 key indices with fp16 or grouped 2/3/4-bit values, KV-cache
-append and value packing.  Compute runs in ``libsunshape_hip.so`` (C ABI in
+append and value packing; and a paged cache of 4-bit keys and values for many
+requests (``PagedKVCache``).  Compute runs in ``libsunshape_hip.so`` (C ABI in
 ``include/sunshape_hip.h``); torch supplies device memory and streams.
 
 The source directory is ``sunshape-mlx_amd/``; it is imported under the name
@@ -58,6 +59,7 @@ from .cache import HybridSunShapeKVCache, SunShapeKVCache, create_kv_cache  # no
 from .value_codecs import GroupedValueCodec, TurboQuantValueCodec, build_value_codec  # noqa: E402
 from .paged import (  # noqa: E402
     BlockPlan,
+    PagedKVCache,
     PagedKVStore,
     append_paged,
     build_block_tables,
@@ -76,6 +78,6 @@ __all__ = [
     "pack_indices", "unpack_indices", "quantize_values", "dequantize_values", "get_kernel_stats",
     "reset_kernel_stats", "apply_permutation", "invert_permutation", "generate_rotation_matrix",
     "covariance_block_permutation", "save_codec", "load_codec", "save_cache", "load_cache",
-    "PagedKVStore", "BlockPlan", "build_block_tables", "check_plan", "append_paged", "read_paged",
+    "PagedKVCache", "PagedKVStore", "BlockPlan", "build_block_tables", "check_plan", "append_paged", "read_paged",
     "paged_attention",
 ]

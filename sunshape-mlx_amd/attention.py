@@ -27,6 +27,7 @@ from torch.autograd import forward_ad as _forward_ad
 from . import _hip
 from .cache import HybridSunShapeKVCache, SunShapeKVCache, _plan_key
 from .codec import PERM_MODES, SunShapeBlockCodec
+from .paged import PagedKVCache
 
 
 def _kernel_query(codec: SunShapeBlockCodec, queries: torch.Tensor, scale: float):
@@ -520,7 +521,8 @@ def _two_pass(cache, queries: torch.Tensor, scale: float, mask,
     return out.reshape(b_, hq, tq, d).to(out_dtype)
 
 
-def sunshape_sdpa(queries: torch.Tensor, cache: SunShapeKVCache | HybridSunShapeKVCache,
+def sunshape_sdpa(queries: torch.Tensor,
+                  cache: SunShapeKVCache | HybridSunShapeKVCache | PagedKVCache,
                   scale: float, mask: torch.Tensor | str | None = None, *,
                   out_dtype: torch.dtype | None = None) -> torch.Tensor:
     """Attention of ``queries`` (B, n_q_heads, T_q, D) against a SunShape cache
@@ -529,7 +531,12 @@ def sunshape_sdpa(queries: torch.Tensor, cache: SunShapeKVCache | HybridSunShape
     or an additive / boolean array broadcastable to (B, n_q_heads, T_q, T_kv).
     Returns (B, n_q_heads, T_q, D) in the query dtype, as the reference does
     (attention.py:292, 304), or in ``out_dtype`` when given (an extension:
-    float32 keeps the kernels' fp32 accumulation in the result)."""
+    float32 keeps the kernels' fp32 accumulation in the result).  A
+    ``PagedKVCache`` takes None and ``"causal"``, in the query dtype."""
+    if isinstance(cache, PagedKVCache):
+        if out_dtype not in (None, queries.dtype):
+            raise ValueError(f"a paged cache's output has the query dtype, not {out_dtype}")
+        return cache.sdpa(queries, scale, mask)
     b_, hq, tq, d = queries.shape
     hkv = cache.n_kv_heads
     if hq % hkv != 0:

@@ -29,6 +29,7 @@ from typing import NamedTuple
 import torch
 
 from . import _hip
+from .cache import DeferredTensor
 
 _HALF = (torch.float16, torch.bfloat16)
 
@@ -138,6 +139,9 @@ def _struct(store: PagedKVStore) -> _Store:
                   _CODE[dtype])
 
 
+# names of the dispatch counters (get_kernel_stats)
+_STATS = {f"ss_{n}": f"{n}_hip" for n in ("block_tables", "append_paged", "read_paged",
+                                          "paged_attn")}
 _CODE = {torch.float32: _hip.SS_F32, torch.float16: _hip.SS_F16, torch.bfloat16: _hip.SS_BF16}
 
 
@@ -162,7 +166,7 @@ def _launch(name: str, dev: int, *args) -> None:
     else:
         with torch.cuda.device(dev):
             rc = fn(*args, _hip.stream_handle(dev))
-    _hip._launched(name, rc)
+    _hip._launched(_STATS[name], rc)
 
 
 def build_block_tables(lengths: torch.Tensor, new_lengths: torch.Tensor,
@@ -331,3 +335,215 @@ def paged_attention(queries: torch.Tensor, store: PagedKVStore, block_table: tor
             q.stride(1), hq, at_table, width, at_lengths, at_starts, r, scale, causal, max_new,
             max_length, out.data_ptr(), zero_rest, _hip.ptr(ws), need)
     return out
+
+
+class PagedKVCache:
+    """The keys and values of up to ``n_requests`` requests in one pool of
+    ``n_pages`` pages (by default enough for ``max_tokens`` of each).
+
+    A serving step is ``step`` (scheduling), ``append`` and ``attend`` on packed
+    tokens, all requests together:
+
+        cache.step(new_lengths, n_tokens)      # how many tokens each adds
+        cache.append(keys, values)             # (N, H, D), request after request
+        out = cache.attend(queries, scale)     # (N, Hq, D)
+
+    Lengths, tables and the stack of free pages live on the GPU and are
+    stepped there in place, so a step needs no synchronisation and can be
+    captured in a graph.  A batch whose sequences all add the same number of
+    tokens may use ``update_and_fetch`` and ``sunshape_sdpa`` (or the SDPA
+    router) instead, as with the other caches."""
+
+    def __init__(self, *, n_requests: int, n_kv_heads: int = 1, head_dim: int = 128,
+                 max_tokens: int, n_pages: int | None = None, page_size: int = 64,
+                 group_size: int = 64, dtype: torch.dtype = torch.float16, device=None,
+                 lazy_fetch: bool = True):
+        if n_requests < 1 or max_tokens < 1:
+            raise ValueError("n_requests and max_tokens must be positive")
+        width = -(-max_tokens // page_size)
+        n_pages = n_requests * width if n_pages is None else n_pages
+        self.store = PagedKVStore.zeros(n_pages, n_kv_heads, head_dim, page_size=page_size,
+                                        group_size=group_size, dtype=dtype, device=device)
+        dev = self.store.k_codes.device
+        self.n_requests, self.n_kv_heads, self.head_dim = n_requests, n_kv_heads, head_dim
+        self.page_size, self.group_size, self.dtype = page_size, group_size, dtype
+        self.max_tokens = max_tokens
+        self.lazy_fetch = lazy_fetch
+        self.block_table = torch.full((n_requests, width), -1, dtype=torch.int32, device=dev)
+        self.lengths = torch.zeros((n_requests,), dtype=torch.int32, device=dev)
+        self.free_pages = torch.arange(n_pages, dtype=torch.int32, device=dev)
+        self.n_free = torch.full((1,), n_pages, dtype=torch.int32, device=dev)
+        self.plan: BlockPlan | None = None  # of the last step
+        self._version = 0                   # bumped by every change of the stored tokens
+        # what the host knows of the lengths: all of them (steps given as
+        # lists), or a bound
+        self._host: list[int] | None = [0] * n_requests
+        self._bound = 0
+        self._max_new = 1
+        self._starts: tuple[int, torch.Tensor] | None = None
+
+    # -------------------------------------------------------------- serving
+    def step(self, new_lengths, n_tokens: int | None = None, *,
+             max_new: int | None = None) -> BlockPlan:
+        """Schedule a step in which request r adds ``new_lengths[r]`` tokens
+        (negative: gives its last ones back; minus its length: ends).  A list
+        of ints is checked here and raises when the step is impossible.  An
+        int32 tensor on the GPU needs ``n_tokens``, at least the sum of what is
+        added (``max_new``, the most one adds, sizes later launches); whether
+        the step was possible is then seen by ``check``."""
+        if isinstance(new_lengths, torch.Tensor):
+            if n_tokens is None:
+                raise ValueError("n_tokens is required with new_lengths on the GPU")
+            new, self._host = new_lengths, None
+            most = min(n_tokens, n_tokens if max_new is None else max_new)
+            self._bound = min(self.max_tokens, self._bound + max(0, most))
+        else:
+            adds = [int(x) for x in new_lengths]
+            if len(adds) != self.n_requests:
+                raise ValueError(f"{len(adds)} lengths for {self.n_requests} requests")
+            total = sum(max(0, x) for x in adds)
+            if n_tokens is not None and n_tokens < total:
+                raise ValueError(f"{total} new tokens do not fit n_tokens {n_tokens}")
+            n_tokens = total if n_tokens is None else n_tokens
+            most = max(adds)
+            if self._host is not None:
+                after = [n + x for n, x in zip(self._host, adds)]
+                pages = sum(-(-n // self.page_size) for n in after)
+                if min(after) < 0 or max(after) > self.max_tokens:
+                    raise ValueError(f"lengths {after} are not within 0 .. {self.max_tokens}")
+                if pages > self.free_pages.shape[0]:
+                    raise RuntimeError(f"{pages} pages needed, {self.free_pages.shape[0]} there")
+                self._host, self._bound = after, max(after)
+            else:
+                self._bound = min(self.max_tokens, self._bound + max(0, most))
+            new = torch.tensor(adds, dtype=torch.int32).to(self.lengths.device)
+        plan = build_block_tables(self.lengths, new, self.block_table, self.free_pages,
+                                  self.n_free, self.page_size, n_tokens,
+                                  lengths_out=self.lengths, n_free_out=self.n_free)
+        self.plan, self._max_new = plan, max(1, most)
+        self._version += 1
+        return plan
+
+    def check(self) -> None:
+        """Raise if the last step was impossible (waits for the GPU)."""
+        if self.plan is not None:
+            check_plan(self.plan)
+
+    def append(self, keys: torch.Tensor, values: torch.Tensor) -> None:
+        """Store the keys and values (N, H, D) of the last step's tokens."""
+        if self.plan is None:
+            raise RuntimeError("append needs a step first")
+        append_paged(self.store, keys, values, self.plan.slots)
+        self._version += 1
+
+    def attend(self, queries: torch.Tensor, scale: float, *, causal: bool = True,
+               out: torch.Tensor | None = None) -> torch.Tensor:
+        """Attention of the last step's tokens' queries (N, Hq, D)."""
+        if self.plan is None:
+            raise RuntimeError("attend needs a step first")
+        return paged_attention(queries, self.store, self.block_table, self.lengths,
+                               self.plan.token_starts, scale, causal=causal,
+                               max_new=self._max_new, max_length=max(1, self._bound), out=out)
+
+    def release(self, requests) -> None:
+        """End these requests: their pages go back to the pool."""
+        at = torch.as_tensor(list(requests), dtype=torch.int64)
+        if at.numel() and (int(at.min()) < 0 or int(at.max()) >= self.n_requests):
+            raise ValueError(f"requests must be within 0 .. {self.n_requests - 1}")
+        if self._host is not None:
+            gone = set(at.tolist())
+            self.step([-n if r in gone else 0 for r, n in enumerate(self._host)])
+            return
+        new = torch.zeros_like(self.lengths)
+        at = at.to(new.device)
+        new[at] = -self.lengths[at]
+        self.step(new, 0)
+
+    def trim(self, n: int) -> None:
+        """Give the last ``n`` tokens of every request back."""
+        if self._host is not None:
+            self.step([-min(n, have) for have in self._host])
+        else:
+            self.step(-self.lengths.clamp(max=n), 0)
+
+    # ------------------------------------------- batches of equal steps
+    def update_and_fetch(self, keys: torch.Tensor, values: torch.Tensor):
+        """Append ``keys`` and ``values`` (B, H, T, D), T tokens to each of the
+        cache's B requests.  Returns them as held, (B, H, offset, D) in the
+        cache's type (read when used, with ``lazy_fetch``), where all requests
+        have one length, else (None, None)."""
+        b_, h_, t_, d = keys.shape
+        if (b_, h_, d) != (self.n_requests, self.n_kv_heads, self.head_dim) or \
+                values.shape != keys.shape:
+            raise ValueError(f"keys and values must be ({self.n_requests}, {self.n_kv_heads}, T, "
+                             f"{self.head_dim}), got {tuple(keys.shape)}, {tuple(values.shape)}")
+        self.step([t_] * b_)
+        rows = (b_ * t_, h_, d)
+        self.append(keys.transpose(1, 2).reshape(rows), values.transpose(1, 2).reshape(rows))
+        if self._host is None or min(self._host) != max(self._host):
+            return None, None
+        shape = (b_, h_, self._host[0], d)
+        if not self.lazy_fetch:
+            return self._held()
+        dev = self.lengths.device
+        return tuple(DeferredTensor(lambda i=i: self._held()[i], shape, self.dtype, dev, self)
+                     for i in range(2))
+
+    def _held(self):
+        """(keys, values) of requests of one length, (B, H, offset, D)."""
+        n = self.offset
+        pos = torch.arange(n, device=self.lengths.device)
+        slots = self.block_table[:, pos // self.page_size] * self.page_size + pos % self.page_size
+        k, v = read_paged(self.store, slots.to(torch.int32).reshape(-1))
+        shape = (self.n_requests, n, self.n_kv_heads, self.head_dim)
+        return k.view(shape).transpose(1, 2), v.view(shape).transpose(1, 2)
+
+    def sdpa(self, queries: torch.Tensor, scale: float, mask=None) -> torch.Tensor:
+        """``sunshape_sdpa`` over this cache: ``queries`` (B, Hq, T, D) are those
+        of each request's last T tokens; ``mask`` is None (every query sees all
+        of its request) or ``"causal"``.  Lengths make the padding masks of
+        other caches unnecessary; arrays are refused."""
+        if mask is not None and not (isinstance(mask, str) and mask in ("causal", "none")):
+            raise ValueError("a paged cache takes no mask array: its requests have lengths of "
+                             "their own (mask None or 'causal')")
+        b_, hq, t_, d = queries.shape
+        if b_ != self.n_requests:
+            raise ValueError(f"queries of {b_} sequences, {self.n_requests} requests")
+        if self._starts is None or self._starts[0] != t_:
+            self._starts = (t_, torch.arange(0, (b_ + 1) * t_, max(1, t_), dtype=torch.int32,
+                                             device=self.lengths.device)
+                            if t_ else torch.zeros_like(torch.cat((self.lengths, self.lengths[:1]))))
+        out = paged_attention(queries.transpose(1, 2).reshape(b_ * t_, hq, d), self.store,
+                              self.block_table, self.lengths, self._starts[1], scale,
+                              causal=mask == "causal", max_new=max(1, t_),
+                              max_length=max(1, self._bound))
+        return out.view(b_, t_, hq, d).transpose(1, 2)
+
+    @property
+    def offset(self) -> int:
+        """Tokens held by every request (raises where they differ or the host
+        does not know them; ``lengths`` has them on the GPU)."""
+        if self._host is None or min(self._host) != max(self._host):
+            raise RuntimeError("the requests have no one length known to the host; see lengths")
+        return self._host[0]
+
+    # -------------------------------------------------------------- protocol
+    def is_trimmable(self) -> bool:
+        return True
+
+    def make_mask(self, N: int, return_array: bool = False, window_size: int | None = None,
+                  **kwargs):
+        """``"causal"``, the mask of new queries (no array: see ``sdpa``)."""
+        if return_array or window_size is not None:
+            raise ValueError("a paged cache has no mask arrays")
+        return "causal"
+
+    @property
+    def nbytes(self) -> int:
+        """Bytes of the pool."""
+        return sum(t.numel() * t.element_size() for t in self.store)
+
+    def __repr__(self) -> str:
+        return (f"PagedKVCache(n_requests={self.n_requests}, n_kv_heads={self.n_kv_heads}, "
+                f"head_dim={self.head_dim}, pages={self.free_pages.shape[0]}x{self.page_size}, "
+                f"group_size={self.group_size}, dtype={self.dtype})")

@@ -18,6 +18,7 @@ import torch
 
 from .attention import sunshape_sdpa
 from .cache import HybridSunShapeKVCache, SunShapeKVCache
+from .paged import PagedKVCache
 
 _BASE_MODULE = "mlx_lm.models.base"
 _ALIAS_MODULES = ["mlx_lm.models.qwen3", "mlx_lm.models.qwen3_next", "mlx_lm.models.qwen3_moe"]
@@ -57,7 +58,7 @@ def _original_sdpa():
 def scaled_dot_product_attention(queries, keys, values, cache, scale, mask, sinks=None):
     """SDPA router: SunShape cache -> ``sunshape_sdpa`` (``sinks`` ignored, as
     the reference does); otherwise the original SDPA (patch.py:58-74)."""
-    if isinstance(cache, (SunShapeKVCache, HybridSunShapeKVCache)):
+    if isinstance(cache, (SunShapeKVCache, HybridSunShapeKVCache, PagedKVCache)):
         return sunshape_sdpa(queries, cache, scale, mask)
     original = _original_sdpa()
     if original is not None:

@@ -287,8 +287,7 @@ def check_attention(out, q, store, table, lengths, starts, scale, causal=True):
     got = out.cpu().double()
     assert torch.isfinite(got).all()
     err = (got - want).abs()
-    worst = float((err / tol.clamp(min=1e-30)).max())
-    assert (err <= tol).all(), f"{worst:.2f} of the bound"
+    assert (err <= tol).all(), f"{float((err / tol.clamp(min=1e-30)).max()):.2f} of the bound"
 
 
 CASES = [  # lengths, new tokens, query / KV heads, page
@@ -586,3 +585,123 @@ def test_refusals_on_the_device():
         S.build_block_tables(le, ints([1]), table, ints([0]), ints([1]), 24, 1)
     with pytest.raises(ValueError):
         S.paged_attention(q, store, table, le, starts.cpu(), 0.1)
+
+
+# ------------------------------------------------------------------- cache
+
+
+def test_cache_serves_requests_of_their_own_lengths():
+    """Steps given as lists and as tensors, speculation, trims, releases: the
+    outputs and what the cache holds against everything appended."""
+    hq, hkv, d, group, page = 8, 2, 128, 64, 32
+    c = S.PagedKVCache(n_requests=3, n_kv_heads=hkv, head_dim=d, max_tokens=400, n_pages=20,
+                       page_size=page, group_size=group, dtype=torch.bfloat16)
+    lengths = [0, 0, 0]
+
+    def go(new, n_tokens=None, seed=0):
+        total = sum(max(0, x) for x in new)
+        plan = c.step(ints(new), n_tokens) if n_tokens is not None else c.step(new)
+        c.check()
+        n = plan.slots.numel()
+        k, v = rows(seed, n, hkv, d, torch.bfloat16), rows(seed + 50, n, hkv, d, torch.bfloat16, False)
+        c.append(k, v)
+        q = rows(seed + 90, n, hq, d, torch.bfloat16, False)
+        out = c.attend(q, 0.09)
+        check_attention(out, q, c.store, c.block_table, c.lengths, plan.token_starts, 0.09)
+        assert (out[total:] == 0).all()
+        for r, x in enumerate(new):
+            lengths[r] += x
+        assert c.lengths.tolist() == lengths
+        check_slots(c.store, k, v, plan.slots, group)
+
+    go([70, 1, 0], seed=1)
+    go([1, 1, 150], seed=2)
+    go([4, 4, 4], seed=3)
+    go([-3, 0, -1], seed=4)
+    c.release([1])
+    lengths[1] = 0
+    assert c.lengths.tolist() == lengths
+    with pytest.raises(RuntimeError, match="no one length"):
+        c.offset
+    go([1, 33, 1], 40, seed=5)   # from here on the host does not know the lengths
+    go([2, -33, 1], 3, seed=6)
+    c.release([0])
+    lengths[0] = 0
+    c.trim(5)
+    lengths = [max(0, x - 5) for x in lengths]
+    assert c.lengths.tolist() == lengths
+    go([9, 9, 1], 19, seed=7)
+    assert int(c.n_free) == 20 - sum(-(-x // page) for x in lengths)
+    # 9 + 400 tokens fit the 13 pages of a row (416) and the 13 that are free
+    # beside the one held; 8 more do not
+    c.step(ints([0, 400, 0]), 400)
+    c.check()
+    lengths[1] += 400
+    assert c.lengths.tolist() == lengths
+    c.step(ints([0, 8, 0]), 8)
+    with pytest.raises(RuntimeError, match="row holds"):
+        c.check()
+    assert c.lengths.tolist() == lengths and (c.plan.slots == -1).all()
+
+
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("t", [1, 3, 40])
+def test_cache_in_the_router(t, dtype):
+    """update_and_fetch and the SDPA router, as a model calls them."""
+    b, hq, hkv, d, group = 2, 8, 2, 64, 32
+    c = S.PagedKVCache(n_requests=b, n_kv_heads=hkv, head_dim=d, max_tokens=300, group_size=group,
+                       dtype=dtype)
+    k, v = (rows(i, b * (90 + t), hkv, d, dtype).view(b, -1, hkv, d).transpose(1, 2) for i in (1, 2))
+    c.update_and_fetch(k[:, :, :90], v[:, :, :90])
+    ks, vs = c.update_and_fetch(k[:, :, 90:], v[:, :, 90:])
+    assert ks.shape == vs.shape == (b, hkv, 90 + t, d) and c.offset == 90 + t
+    for got, x in ((ks, k), (vs, v)):
+        want = R.held(x.cpu(), group)
+        assert ((got.cpu().double() - want).abs() <= R.U16[dtype] * want.abs() + 2.0 ** -22 * 16).all()
+    q = rows(3, b * t, hq, d, dtype, False).view(b, t, hq, d).transpose(1, 2)
+    starts = ints([0, t, 2 * t])
+    for mask in ("causal", None):
+        out = S.patch.scaled_dot_product_attention(q, ks, vs, c, 0.125, mask)
+        assert out.shape == q.shape
+        packed = out.transpose(1, 2).reshape(b * t, hq, d)
+        check_attention(packed, q.transpose(1, 2).reshape(b * t, hq, d), c.store, c.block_table,
+                        c.lengths, starts, 0.125, mask == "causal")
+    c.trim(t)
+    assert c.offset == 90
+    with pytest.raises(RuntimeError, match="changed"):
+        ks2, _ = c.update_and_fetch(k[:, :, 90:], v[:, :, 90:])
+        c.trim(1)
+        ks2 + 0
+    none = S.sunshape_sdpa(q[:, :, :0], c, 0.125)
+    assert none.shape == (b, hq, 0, d)
+    stats = S.get_kernel_stats()
+    assert stats["paged_attn_hip"] > 0 and stats["block_tables_hip"] > 0
+
+
+def test_cache_decode_step_replays_from_a_graph():
+    b, hq, hkv, d = 2, 8, 2, 128
+    c = S.PagedKVCache(n_requests=b, n_kv_heads=hkv, head_dim=d, max_tokens=900)
+    n = 700
+    c.step([n, 300])
+    c.append(rows(1, n + 300, hkv, d, torch.float16), rows(2, n + 300, hkv, d, torch.float16, False))
+    one = ints([1] * b)
+    k, v, q = (torch.zeros((b, h, d), dtype=torch.float16, device=DEV) for h in (hkv, hkv, hq))
+    out = torch.zeros_like(q)
+
+    def step():
+        c.step(one, b, max_new=1)
+        c.append(k, v)
+        c.attend(q, 0.1, out=out)
+
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        step()
+    for i in range(5):
+        for j, x in enumerate((k, v, q)):
+            x.copy_(rows(10 * i + j, b, x.shape[1], d, torch.float16, j == 0))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert c.lengths.tolist() == [n + i + 1, 301 + i]
+        check_attention(out, q, c.store, c.block_table, c.lengths, ints([0, 1, 2]), 0.1)
+        torch.empty(1 << 20, device=DEV).random_()

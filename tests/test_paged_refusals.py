@@ -1,0 +1,228 @@
+"""What the paged cache's entry points refuse, on the CPU: the C ABI checks
+sizes before any launch, the Python layer checks tensors before it calls."""
+
+import ctypes
+
+import pytest
+import torch
+
+import sunshape_mlx_amd as S
+from sunshape_mlx_amd import _hip, paged
+
+FAKE = 1 << 20  # an address that nothing reads
+
+
+def store(**kw):
+    f = dict(k_codes=FAKE, v_codes=FAKE, k_meta=FAKE, v_meta=FAKE, n_pages=4, n_kv_heads=2,
+             head_dim=128, group_size=64, page_size=64, dtype=_hip.SS_F16)
+    f.update(kw)
+    return paged._Store(**f)
+
+
+BAD_STORES = [
+    (dict(k_codes=None), -1), (dict(v_meta=FAKE + 4), -1), (dict(n_pages=0), -1),
+    (dict(n_kv_heads=0), -1), (dict(dtype=_hip.SS_F32), -2), (dict(head_dim=96), -2),
+    (dict(head_dim=256), -2), (dict(group_size=16), -2), (dict(head_dim=64, group_size=128), -2),
+    (dict(page_size=8), -2), (dict(page_size=48), -2), (dict(page_size=2048), -2),
+    (dict(n_pages=1 << 26), -2),
+]
+
+
+@pytest.mark.parametrize("kw,status", BAD_STORES)
+def test_stores_that_are_refused(kw, status):
+    lib, st = _hip.load_library(), store(**kw)
+    at = ctypes.addressof(st)
+    assert lib.ss_append_paged(at, FAKE, FAKE, 1, 1, 256, 128, 256, 128, FAKE, None) == status
+    assert lib.ss_read_paged(at, FAKE, 1, FAKE, FAKE, None) == status
+    assert attention(st) == status
+    assert lib.ss_paged_attn_workspace_bytes(at, 1, 1, 2, 1, 1000) == 0
+
+
+def attention(st=None, q=FAKE, q_dtype=_hip.SS_F16, n=1, hq=2, table=FAKE, width=4, lengths=FAKE,
+              starts=FAKE, r=1, max_new=1, max_length=256, out=FAKE, ws=None, ws_bytes=0):
+    st = store() if st is None else st
+    return _hip.load_library().ss_paged_attn(
+        ctypes.addressof(st), q, q_dtype, n, hq * 128, 128, hq, table, width, lengths, starts, r,
+        0.1, 1, max_new, max_length, out, 0, ws, ws_bytes, None)
+
+
+@pytest.mark.parametrize("kw,status", [
+    (dict(q=None), -1), (dict(q_dtype=_hip.SS_F32), -2), (dict(q_dtype=7), -2), (dict(n=-1), -1),
+    (dict(hq=3), -1), (dict(hq=0), -1), (dict(hq=2048), -2), (dict(table=None), -1),
+    (dict(width=0), -1), (dict(width=1 << 30), -2), (dict(lengths=None), -1),
+    (dict(starts=None), -1), (dict(r=0), -1), (dict(r=70000), -1), (dict(max_new=0), -1),
+    (dict(max_length=0), -1), (dict(out=None), -1), (dict(out=FAKE + 2), -1),
+    (dict(n=1 << 31), -2), (dict(max_length=5000, width=100), -4),
+    (dict(max_length=5000, width=100, ws=FAKE, ws_bytes=64), -4), (dict(n=0), 0),
+])
+def test_attention_calls_that_are_refused(kw, status):
+    assert attention(**kw) == status
+    assert status == 0 or _hip.load_library().ss_last_error()
+
+
+def test_workspace_is_what_the_call_asks_for():
+    lib = _hip.load_library()
+    for n, r, hq, new, length in ((1, 1, 2, 1, 512), (1, 1, 2, 1, 513), (300, 2, 8, 200, 4000),
+                                  (4096, 256, 32, 1, 131072)):
+        st = store()
+        need = lib.ss_paged_attn_workspace_bytes(ctypes.addressof(st), n, r, hq, new, length)
+        assert (need == 0) == (length <= 512 and new == 1)
+        if need:
+            assert attention(n=n, r=r, hq=hq, max_new=new, max_length=length, width=4000,
+                             ws=FAKE, ws_bytes=need - 1) == -4
+
+
+@pytest.mark.parametrize("kw,status", [
+    (dict(n_tokens=-1), -1), (dict(n_requests=0), -1), (dict(n_requests=4097), -2),
+    (dict(width=0), -1), (dict(pool=0), -1), (dict(page_size=24), -2), (dict(page_size=8), -2),
+    (dict(pool=1 << 28), -2), (dict(lengths=None), -1), (dict(slots=None), -1),
+])
+def test_block_table_calls_that_are_refused(kw, status):
+    f = dict(lengths=FAKE, n_requests=2, width=4, pool=8, page_size=64, n_tokens=3, slots=FAKE)
+    f.update(kw)
+    assert _hip.load_library().ss_block_tables(
+        f["lengths"], FAKE, f["n_requests"], FAKE, f["width"], FAKE, f["pool"], FAKE,
+        f["page_size"], f["n_tokens"], FAKE, FAKE, FAKE, f["slots"], None, FAKE, None) == status
+
+
+@pytest.mark.parametrize("n,dtype,keys,status", [(-1, 1, FAKE, -1), (1, 9, FAKE, -1), (1, 1, None, -1), (0, 1, None, 0)])
+def test_append_calls_that_are_refused(n, dtype, keys, status):
+    st = store()
+    assert _hip.load_library().ss_append_paged(ctypes.addressof(st), keys, FAKE, dtype, n, 256, 128,
+                                               256, 128, FAKE, None) == status
+
+
+# ------------------------------------------------------------ Python layer
+
+
+class Launched(Exception):
+    pass
+
+
+@pytest.fixture
+def on_cpu(monkeypatch):
+    """CPU tensors pass for GPU ones; a call that would launch raises Launched."""
+    def launch(name, dev, *args):
+        raise Launched(name)
+
+    monkeypatch.setattr(_hip, "require_gpu", lambda *t: None)
+    monkeypatch.setattr(paged, "_launch", launch)
+    monkeypatch.setattr(paged, "_workspace_bytes", lambda *a: 0)
+
+
+def pool(n=3, h=2, d=128, **kw):
+    return S.PagedKVStore.zeros(n, h, d, device="cpu", **kw)
+
+
+def ints(*v):
+    return torch.tensor(v, dtype=torch.int32)
+
+
+def call(store=None, n=2, **kw):
+    store = pool() if store is None else store
+    f = dict(queries=torch.zeros(n, 4, 128, dtype=torch.float16), store=store,
+             block_table=torch.zeros(1, 3, dtype=torch.int32), lengths=ints(5),
+             token_starts=ints(0, n), scale=0.1)
+    f.update(kw)
+    return S.paged_attention(**f)
+
+
+def test_cpu_tensors_are_refused():
+    with pytest.raises(ValueError, match="no CPU fallback"):
+        call()
+    with pytest.raises(ValueError, match="no CPU fallback"):
+        S.build_block_tables(ints(1), ints(1), torch.zeros(1, 1, dtype=torch.int32), ints(0), ints(1), 16, 1)
+    with pytest.raises(ValueError, match="no CPU fallback"):
+        S.read_paged(pool(), ints(0))
+
+
+def test_a_good_call_gets_to_its_launch(on_cpu):
+    with pytest.raises(Launched, match="ss_paged_attn"):
+        call()
+    z = torch.zeros(2, 2, 128)
+    with pytest.raises(Launched, match="ss_append_paged"):
+        S.append_paged(pool(), z, z, ints(0, 1))
+
+
+@pytest.mark.parametrize("kw,error", [
+    (dict(queries=torch.zeros(2, 4, 128)), TypeError),
+    (dict(queries=torch.zeros(2, 3, 128, dtype=torch.float16)), ValueError),
+    (dict(queries=torch.zeros(2, 4, 64, dtype=torch.float16)), ValueError),
+    (dict(queries=torch.zeros(2, 4, dtype=torch.float16)), ValueError),
+    (dict(queries=torch.zeros(2, 4, 128, dtype=torch.float16, requires_grad=True)), ValueError),
+    (dict(lengths=torch.tensor([5])), TypeError), (dict(lengths=ints(5, 6)), ValueError),
+    (dict(token_starts=ints(0)), ValueError), (dict(token_starts=ints(0, 1, 2)), ValueError),
+    (dict(block_table=torch.zeros(1, 6, dtype=torch.int32)[:, ::2]), ValueError),
+    (dict(out=torch.zeros(2, 4, 128)), ValueError), (dict(out=torch.zeros(1, 4, 128, dtype=torch.float16)), ValueError),
+])
+def test_attention_arguments_that_are_refused(on_cpu, kw, error):
+    with pytest.raises(error):
+        call(**kw)
+
+
+def test_stores_whose_tensors_do_not_agree(on_cpu):
+    good = pool()
+    for i, t in enumerate(good):
+        for bad in (t[:2], t.transpose(0, 1), t.double() if t.is_floating_point() else t.long()):
+            with pytest.raises((ValueError, TypeError)):
+                S.read_paged(S.PagedKVStore(*good[:i], bad, *good[i + 1:]), ints(0))
+    with pytest.raises((ValueError, TypeError)):
+        S.read_paged(S.PagedKVStore(good[0], good[1], good[2], good[3].bfloat16()), ints(0))
+
+
+def test_appends_that_are_refused(on_cpu):
+    z = torch.zeros(2, 2, 128)
+    for k, v, s in ((z[:1], z, ints(0, 1)), (z, z[:, :1], ints(0, 1)), (z, z.half(), ints(0, 1)),
+                    (z.double(), z.double(), ints(0, 1)), (z, z, torch.tensor([0, 1])), (z, z, ints(0, 1, 2))):
+        with pytest.raises((ValueError, TypeError)):
+            S.append_paged(pool(), k, v, s)
+
+
+@pytest.mark.parametrize("kw,error", [
+    (dict(head_dim=96), ValueError), (dict(group_size=48), ValueError), (dict(page_size=40), ValueError),
+    (dict(dtype=torch.float32), TypeError), (dict(n_requests=0), ValueError),
+    (dict(max_tokens=0), ValueError), (dict(n_pages=0), ValueError), (dict(n_kv_heads=0), ValueError),
+])
+def test_caches_that_are_refused(kw, error):
+    f = dict(n_requests=2, n_kv_heads=2, head_dim=128, max_tokens=100, device="cpu")
+    f.update(kw)
+    with pytest.raises(error):
+        S.PagedKVCache(**f)
+
+
+def test_cache_steps_that_are_refused(on_cpu, monkeypatch):
+    monkeypatch.setattr(paged, "_launch", lambda *a: None)
+    c = S.PagedKVCache(n_requests=2, n_kv_heads=2, head_dim=128, max_tokens=100, n_pages=3,
+                       page_size=32, device="cpu")
+    z = torch.zeros(1, 2, 128, dtype=torch.float16)
+    with pytest.raises(RuntimeError, match="step first"):
+        c.append(z, z)
+    with pytest.raises(RuntimeError, match="step first"):
+        c.attend(z, 0.1)
+    for bad in ([1], [1, 2, 3], [101, 0], [-1, 0]):
+        with pytest.raises(ValueError):
+            c.step(bad)
+    with pytest.raises(RuntimeError, match="pages"):
+        c.step([64, 64])
+    with pytest.raises(ValueError):
+        c.step([5, 5], 9)
+    with pytest.raises(ValueError, match="n_tokens"):
+        c.step(ints(1, 1))
+    c.step([5, 3])
+    with pytest.raises(RuntimeError, match="one length"):
+        c.offset
+    q = torch.zeros(2, 4, 1, 128, dtype=torch.float16)
+    with pytest.raises(ValueError, match="mask"):
+        S.sunshape_sdpa(q, c, 0.1, torch.zeros(1))
+    with pytest.raises(ValueError):
+        S.sunshape_sdpa(q[:1], c, 0.1)
+    with pytest.raises(ValueError, match="dtype"):
+        S.sunshape_sdpa(q, c, 0.1, out_dtype=torch.float32)
+    with pytest.raises(ValueError):
+        c.update_and_fetch(q, q)
+    with pytest.raises(ValueError):
+        c.release([2])
+    with pytest.raises(ValueError):
+        c.make_mask(1, return_array=True)
+    with pytest.raises(TypeError):
+        S.save_cache("/nonexistent", c)
