@@ -2,13 +2,13 @@
 // of decode steps and speculative verification (paged_attn.hpp has the
 // formulas, paged_prompt.hip the many rows of prompts).
 //
-// Value codes enter the second product unconverted too, so scales stay out of
-// the operands: the 16 columns of both products are (row r, group g), a query
-// entering column (r, g) with the dims of group g alone, a probability times
-// the value's scale in g.  Keys are the A operand (16 tokens), so a lane
-// holds, of one column, 4 tokens of each key tile; two key tiles whose token
-// order is chosen so make exactly the lane's 8 tokens of the second product's
-// B operand: the probabilities never leave the lane's registers.
+// Scales stay out of the codes' operands: the 16 columns of both products are
+// (row r, group g), a query entering column (r, g) with the dims of group g
+// alone, a probability times the value's scale in g.  Keys are the A operand
+// (16 tokens), so a lane holds, of one column, 4 tokens of each key tile; two
+// key tiles whose token order is chosen so make exactly the lane's 8 tokens of
+// the second product's B operand: the probabilities never leave the lane's
+// registers.
 #include "paged_attn.hpp"
 
 namespace ss {
@@ -94,8 +94,9 @@ __device__ __forceinline__ float lanes4_sum(float v) {
 // Over the groups of a row (neighbouring columns).
 template <int G>
 __device__ __forceinline__ float groups_sum(float v) {
-    if (G >= 2) v += dpp_mov<0xB1>(v);  // quad_perm [1,0,3,2]
-    if (G >= 4) v += dpp_mov<0x4E>(v);  // quad_perm [2,3,0,1]
+    // (written so that the move is part of the addition)
+    if (G >= 2) v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0xB1, 0xf, 0xf, true));  // quad_perm [1,0,3,2]
+    if (G >= 4) v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x4E, 0xf, 0xf, true));  // quad_perm [2,3,0,1]
     return v;
 }
 
@@ -229,11 +230,10 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(const PagedAttn a) {
         const int32_t *row_table = a.table + (int64_t)r * a.width;
 
         char *ring = lds + wave * kStages * TL::kBytes;
+        const int last_page = (int)min(a.width - 1, (int64_t)INT32_MAX);
         // Page of the 16 tokens from `token`; -1 if the table names none of the pool.
-        auto page_at = [&](int token) {
-            const int p = table_read(row_table, min((int64_t)(token >> log_page), a.width - 1));
-            return (uint32_t)p < (uint32_t)a.st.n_pages ? p : -1;
-        };
+        auto in_pool = [&](int p) { return (uint32_t)p < (uint32_t)a.st.n_pages ? p : -1; };
+        auto page_at = [&](int token) { return table_read(row_table, min(token >> log_page, last_page)); };
         // queries first: what is loaded later would hold them back
         int limit[NS];  // tokens that the column's row sees
         uint4 raw[NS][KS];
@@ -253,7 +253,7 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(const PagedAttn a) {
         int pages[kStages][2];             // of the tiles in flight, the oldest first
 #pragma unroll
         for (int i = 0; i < kStages; ++i) {
-            pages[i][0] = page_at(ahead), pages[i][1] = page_at(ahead + 16);
+            pages[i][0] = in_pool(page_at(ahead)), pages[i][1] = in_pool(page_at(ahead + 16));
             ahead += kUnit;
         }
         // The queries, here and not where they are used: by then they would wait
@@ -291,10 +291,10 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(const PagedAttn a) {
                 for (int e = 0; e < 8; ++e) {
                     const float y = in_group ? x[k][e] * down : 0.f;  // (down: its sign is the scale's)
                     sum += y;
-                    qf[s][k][e] = (_Float16)((e & 2) ? y * 0x1p-4f : y);
+                    qf[s][k][e] = (_Float16)y;
                 }
-            qz[s] = lanes4_sum(sum) * 0x1p-24f;
-            factor[s] = fmaxf(fabsf(a.scale) * kLog2e * 0x1p24f * exp2i(shift), 1e-30f);
+            qz[s] = lanes4_sum(sum);
+            factor[s] = fmaxf(fabsf(a.scale) * kLog2e * 64.f * exp2i(shift), 1e-30f);
             lag[s] = kLag / factor[s];
         }
         // (limits grow with the row: the first row's is the smallest)
@@ -303,19 +303,26 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(const PagedAttn a) {
         // The sums are kept times 2^(10 - vexp): vexp is above every value scale
         // (as a power of two) that the column's group has met, so p * scale
         // stays within fp16 whatever the scales.  top is in units of S.
-        float top[NS], l_even[NS], l_odd[NS], z_even[NS], z_odd[NS];
+        float top[NS], l[NS], z[NS];
         float4_t o[NS][VT], ones[NS];
 #pragma unroll
         for (int s = 0; s < NS; ++s) {
             top[s] = -INFINITY;
-            l_even[s] = l_odd[s] = z_even[s] = z_odd[s] = 0.f;
+            l[s] = z[s] = 0.f;
             ones[s] = float4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int j = 0; j < VT; ++j) o[s][j] = float4_t{0.f, 0.f, 0.f, 0.f};
         }
         int vexp = -60;
+        float offset[NS];  // of the exponents: 10 - vexp less the maximum's
+        auto set_offset = [&](int s) {
+            offset[s] = (float)(10 - vexp) - (top[s] == -INFINITY ? 0.f : top[s] * factor[s]);
+        };
+#pragma unroll
+        for (int s = 0; s < NS; ++s) set_offset(s);
+        const CodeBits code_bits;
         auto rescale = [&](int s, float f) {
-            l_even[s] *= f, l_odd[s] *= f, z_even[s] *= f, z_odd[s] *= f;
+            l[s] *= f, z[s] *= f;
             ones[s] *= f;
 #pragma unroll
             for (int j = 0; j < VT; ++j) o[s][j] *= f;
@@ -350,9 +357,10 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(const PagedAttn a) {
                 for (int j = 0; j < 8; ++j)
                     if (!ok || first + j >= rq.len) vm[j] = 0;
             }
-            float vtop = low16<BF>(vm[0]);
+            float vs[8];
 #pragma unroll
-            for (int j = 1; j < 8; ++j) vtop = fmaxf(vtop, low16<BF>(vm[j]));
+            for (int j = 0; j < 8; ++j) vs[j] = low16<BF>(vm[j]);
+            const float vtop = column_max(vs);
             if (__any(vtop > exp2i(vexp))) {
                 const float c = lanes4_max(vtop);
                 const int e = (int)((__float_as_uint(c) >> 23) & 0xffu) - 126;  // c < 2^e
@@ -360,6 +368,8 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(const PagedAttn a) {
 #pragma unroll
                 for (int s = 0; s < NS; ++s) rescale(s, ldexpf(1.f, vexp - now));
                 vexp = now;
+#pragma unroll
+                for (int s = 0; s < NS; ++s) set_offset(s);
             }
             // (sets inside: an operand's registers serve every set and are free again)
             float xs[NS][8];
@@ -367,10 +377,10 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(const PagedAttn a) {
             for (int y = 0; y < 2; ++y) {
                 float4_t d[NS];
 #pragma unroll
-                for (int s = 0; s < NS; ++s) d[s] = float4_t{0.f, 0.f, 0.f, 0.f};
+                for (int s = 0; s < NS; ++s) d[s] = float4_t{-qz[s], -qz[s], -qz[s], -qz[s]};
 #pragma unroll
                 for (int k = 0; k < KS; ++k) {
-                    const half8_t key = codes_operand(kw[y][k]);
+                    const half8_t key = codes_operand(kw[y][k], code_bits);
 #pragma unroll
                     for (int s = 0; s < NS; ++s)
                         d[s] = __builtin_amdgcn_mfma_f32_16x16x32_f16(key, qf[s][k], d[s], 0, 0, 0);
@@ -380,58 +390,51 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(const PagedAttn a) {
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const uint32_t m = km[4 * y + i];
-                        xs[s][4 * y + i] = groups_sum<G>(fmaf(low16<BF>(m), d[s][i], high16<BF>(m) * qz[s]));
+                        xs[s][4 * y + i] = groups_sum<G>(fmaf(low16<BF>(m), d[s][i], high16<BF>(m) * (qz[s] / 64.f)));
                     }
             }
             half8_t p16[NS];
 #pragma unroll
             for (int s = 0; s < NS; ++s) {
                 float(&x)[8] = xs[s];
-                uint32_t v[8];
+                float v[8], mid[8];
 #pragma unroll
-                for (int j = 0; j < 8; ++j) v[j] = vm[j];
+                for (int j = 0; j < 8; ++j) v[j] = vs[j], mid[j] = fmaf(vs[j], 7.5f, high16<BF>(vm[j]));
                 if (mask) {  // what the row does not see adds nothing, whatever its value holds
                     const int see = ok ? limit[s] : 0;
 #pragma unroll
                     for (int j = 0; j < 8; ++j)
-                        if (first + j >= see) x[j] = -INFINITY, v[j] = 0;
+                        if (first + j >= see) x[j] = -INFINITY, v[j] = mid[j] = 0.f;
                 }
                 const float m = column_max(x);
                 if (__any(m > top[s] + lag[s])) {
                     const float now = fmaxf(top[s], lanes4_max(m));
                     rescale(s, now == top[s] ? 1.f : fast_exp2((top[s] - now) * factor[s]));
                     top[s] = now;
+                    set_offset(s);
                 }
-                // pairs (2,3) and (6,7), whose codes count 16 times, at 2^-4
-                const float even = (float)(10 - vexp) - (top[s] == -INFINITY ? 0.f : top[s] * factor[s]);
                 float w[8];
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
-                    const float p = fast_exp2(fmaf(x[j], factor[s], (j & 2) ? even - 4.f : even));
+                    const float p = fast_exp2(fmaf(x[j], factor[s], offset[s]));
                     // the value's middle, zero + 7.5 scale, in float32: what is
                     // left for the product, (code - 7.5) scale, is small
-                    const float mid = fmaf(low16<BF>(v[j]), 7.5f, high16<BF>(v[j]));
-                    w[j] = p * low16<BF>(v[j]);
-                    if (j & 2) {
-                        l_odd[s] += p;
-                        z_odd[s] = fmaf(p, mid, z_odd[s]);
-                    } else {
-                        l_even[s] += p;
-                        z_even[s] = fmaf(p, mid, z_even[s]);
-                    }
+                    l[s] += p;
+                    z[s] = fmaf(p, mid[j], z[s]);
+                    w[j] = p * v[j];
                 }
-                // one rounding to fp16, 2^-11 of w (code - 7.5): 7.5 times the
-                // sum of the rounded w is taken off again at the end
+                // one rounding to fp16, 2^-11 of w (code - 7.5): the sum of the
+                // rounded w is taken off again at the end
 #pragma unroll
                 for (int j = 0; j < 8; j += 2) {
                     const half2_t hh = __builtin_convertvector(float2_t{w[j], w[j + 1]}, half2_t);
                     p16[s][j] = hh[0], p16[s][j + 1] = hh[1];
                 }
-                ones[s] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes_operand(0x11111111u), p16[s], ones[s], 0, 0, 0);
+                ones[s] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes_operand(0, code_bits), p16[s], ones[s], 0, 0, 0);
             }
 #pragma unroll
             for (int j = 0; j < VT; ++j) {
-                const half8_t v = codes_operand(vw[j]);
+                const half8_t v = codes_operand(vw[j], code_bits);
 #pragma unroll
                 for (int s = 0; s < NS; ++s)
                     o[s][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, p16[s], o[s][j], 0, 0, 0);
@@ -453,12 +456,14 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(const PagedAttn a) {
         int slot = 0;
         for (int tb = begin + kTile * wave; tb < end; tb += kUnit) {
             constexpr int last = kStages - 1;
+            // (read here and looked at below: their wait is then the codes' own)
+            const int new0 = page_at(ahead), new1 = page_at(ahead + 16);
             step(ring + (slot + last) % kStages * TL::kBytes, ring + slot * TL::kBytes, tb, pages[0][0], pages[0][1],
                  pages[last][0], pages[last][1]);
             slot = (slot + 1) % kStages;
 #pragma unroll
             for (int i = 0; i < last; ++i) pages[i][0] = pages[i + 1][0], pages[i][1] = pages[i + 1][1];
-            pages[last][0] = page_at(ahead), pages[last][1] = page_at(ahead + 16);
+            pages[last][0] = in_pool(new0), pages[last][1] = in_pool(new1);
             ahead += kUnit;
         }
         __syncthreads();  // the ring's memory takes the results
@@ -466,17 +471,17 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(const PagedAttn a) {
         // the waves' results, joined
 #pragma unroll
         for (int s = 0; s < NS; ++s) {
-            const float l = ldexpf(lanes4_sum(l_even[s] + 16.f * l_odd[s]), vexp - 10);
-            const float z = ldexpf(lanes4_sum(z_even[s] + 16.f * z_odd[s]), vexp - 10);
+            const float lsum = ldexpf(lanes4_sum(l[s]), vexp - 10);
+            const float zsum = ldexpf(lanes4_sum(z[s]), vexp - 10);
             const int row = s * RS + col / G;
-            if (g == 0 && quad == 0) stats[wave][row][0] = top[s] * factor[s], stats[wave][row][1] = l;
+            if (g == 0 && quad == 0) stats[wave][row][0] = top[s] * factor[s], stats[wave][row][1] = lsum;
             if (in_group) {
                 // tile j, element i: dim (4 * quad + i) * D/16 + j
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
 #pragma unroll
                     for (int j = 0; j < VT; ++j)
-                        part[wave][row][(4 * quad + i) * VT + j] = ldexpf(o[s][j][i] - 7.5f * ones[s][i], vexp + 14) + z;
+                        part[wave][row][(4 * quad + i) * VT + j] = ldexpf(64.f * o[s][j][i] - 71.5f * ones[s][i], vexp - 10) + zsum;
             }
         }
         __syncthreads();

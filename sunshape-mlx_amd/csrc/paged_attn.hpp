@@ -5,14 +5,14 @@
 //   O[r][d] = sum_t p_rt (s'_tg c'_td + z'_tg),   g = d's group
 //
 // with c the keys' codes, s and z their scales and zeros (primed: the
-// values').  Key codes enter the matrix cores as they are: a 4-bit code in the
-// low bits of a 16-bit half is the fp16 subnormal c * 2^-24, one place
-// further left c * 2^-20, and the fp16 matrix products take subnormals
-// exactly, so two masks and half a shift turn eight codes into the four
-// registers of an operand and no code is ever converted.  The factor 16
-// between the places is taken from the other operand (queries, respectively
-// probabilities, of odd pairs times 2^-4); 2^24 goes into the factors that
-// the sums are multiplied by in any case.
+// values').  A code enters the fp16 matrix products as 1 + c/64: put into the
+// middle of the mantissa of a 1 it needs no conversion, 7 operations for 8
+// codes, and sum(x c) = 64 (sum(x (1 + c/64)) - sum(x)), where the sum of the
+// other operand starts the accumulator, joins the zero's part or is taken off
+// at the end.  (5 operations would make it the fp16 subnormal c * 2^-24; but
+// the matrix cores align products by their operands' exponent fields, so that
+// subnormals lost up to 10 bits: sums of 64 were off by 1.1e-5 of their terms,
+// against 1.2e-7.)
 #pragma once
 
 #include "paged_common.hpp"
@@ -115,18 +115,22 @@ __device__ __forceinline__ lds_ptr<T> as_lds(void *p) {
     return reinterpret_cast<lds_ptr<T>>(static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p)));
 }
 
-// A word's eight codes as the four registers of an operand: pairs (0,1) and
-// (4,5) times 2^-24, (2,3) and (6,7) times 2^-20.
-__device__ __forceinline__ half8_t codes_operand(uint32_t w) {
+// A word's eight codes c as the four registers of an operand, 1 + c/64 each.
+// (The constants in registers that the compiler does not see through: as
+// literals they would take an and, an or where one instruction does both.)
+struct CodeBits {
+    uint32_t bits = 0x00f000f0u, one = 0x3c003c00u;
+    __device__ CodeBits() { asm volatile("" : "+s"(bits), "+v"(one)); }
+};
+__device__ __forceinline__ half8_t codes_operand(uint32_t w, const CodeBits &k) {
     union {
         uint32_t u[4];
         half8_t h;
     } x;
-    const uint32_t hi = w >> 8;
-    x.u[0] = w & 0x000f000fu;
-    x.u[1] = w & 0x00f000f0u;
-    x.u[2] = hi & 0x000f000fu;
-    x.u[3] = hi & 0x00f000f0u;
+    x.u[0] = ((w << 4) & k.bits) | k.one;
+    x.u[1] = (w & k.bits) | k.one;
+    x.u[2] = ((w >> 4) & k.bits) | k.one;
+    x.u[3] = ((w >> 8) & k.bits) | k.one;
     return x.h;
 }
 

@@ -4,17 +4,16 @@
 // A workgroup of eight waves takes 256 query rows of one KV head (its group's
 // heads at consecutive positions), 32 a wave, over 64-token tiles.  While a
 // tile is computed the next one is prepared, once for all rows: its key codes
-// are spread to 16-bit halves (not converted: see paged_attn.hpp) and its
-// values dequantised to fp16, both in the operand order of
+// become 16-bit operands (see paged_attn.hpp) and its values are dequantised to fp16, both in the operand order of
 // v_mfma_f32_32x32x16_f16, and the one after that is copied from HBM.
 //
 // Scores are exact: code products are summed group by group and each sum is
 // multiplied by its token's scale in float32; the zeros' part is one more
-// product, of the zeros and the queries' sums, both split into bf16 parts.
-// Values are rounded to fp16 times a power of two a group that keeps the
-// largest value met below 2^-6 (a code's factor then stays within fp16: code *
-// 2^-24 times scale * 2^18): 2^-11 of a value, as the probabilities' rounding
-// costs; statistics and sums are float32.
+// product, of zero/64 - scale and the queries' sums, both split into bf16
+// parts.  Values are rounded to fp16 (2^-11 of a value, as the probabilities'
+// rounding costs), times a power of two a group that keeps the largest value
+// met below 2^-6: packed fp16 arithmetic takes a code as the subnormal code *
+// 2^-24, exactly, times scale * 2^18.  Statistics and sums are float32.
 //
 // The vector ALUs bound it (per 32 rows and 64 tokens: 2 x 32 products of
 // scale and sum, 32 exponentials), so what does not depend on the row is done
@@ -72,6 +71,21 @@ struct PromptTile {
         }
     }
 };
+
+// A word's eight codes as fp16 subnormals: pairs (0,1) and (4,5) times 2^-24,
+// (2,3) and (6,7) times 2^-20.
+__device__ __forceinline__ half8_t codes_subnormal(uint32_t w) {
+    union {
+        uint32_t u[4];
+        half8_t h;
+    } x;
+    const uint32_t hi = w >> 8;
+    x.u[0] = w & 0x000f000fu;
+    x.u[1] = w & 0x00f000f0u;
+    x.u[2] = hi & 0x000f000fu;
+    x.u[3] = hi & 0x00f000f0u;
+    return x.h;
+}
 
 // Row tiles of a request that are this kernel's.
 __device__ __forceinline__ int tiles_of(const PagedAttn &a, const Request &q) {
@@ -259,7 +273,7 @@ __global__ void __launch_bounds__(64 * kPWaves, 2) paged_prompt_kernel(const Pag
                 }
             const int shift = row_exp_shift(half_max(top));
             const float down = a.scale < 0.f ? -exp2i(-shift) : exp2i(-shift);
-            factor = fmaxf(fabsf(a.scale) * kLog2e * 0x1p24f * exp2i(shift), 1e-30f);
+            factor = fmaxf(fabsf(a.scale) * kLog2e * 64.f * exp2i(shift), 1e-30f);
             lag = kLag / factor;
             float sums[G];
 #pragma unroll
@@ -271,12 +285,12 @@ __global__ void __launch_bounds__(64 * kPWaves, 2) paged_prompt_kernel(const Pag
                     for (int e = 0; e < 8; ++e) {
                         const float y = x[g][s][e] * down;
                         sum += y;
-                        qf[g][s][e] = (_Float16)((e & 2) ? y * 0x1p-4f : y);
+                        qf[g][s][e] = (_Float16)y;
                     }
-                sums[g] = (sum + __shfl_xor(sum, 32)) * 0x1p-24f;
+                sums[g] = sum + __shfl_xor(sum, 32);
             }
-            // the sum of group 2y + half as three bf16 parts, for the zero's two:
-            // (zh, zh, zh, zl, zl) . (q1, q2, q3, q1, q2)
+            // the sum of group 2y + half as three bf16 parts, for the zero's three:
+            // (z1, z1, z1, z2, z2, z3) . (q1, q2, q3, q1, q2, q1)
 #pragma unroll
             for (int y = 0; y < (G + 1) / 2; ++y) {
                 float v = half == 0 ? sums[2 * y] : (2 * y + 1 < G ? sums[2 * y + 1 < G ? 2 * y + 1 : 0] : 0.f);
@@ -286,7 +300,7 @@ __global__ void __launch_bounds__(64 * kPWaves, 2) paged_prompt_kernel(const Pag
                     part[k] = __bfloat162float(__float2bfloat16(v));
                     v -= part[k];
                 }
-                const float b[8] = {part[0], part[1], part[2], part[0], part[1], 0.f, 0.f, 0.f};
+                const float b[8] = {part[0], part[1], part[2], part[0], part[1], part[0], 0.f, 0.f};
 #pragma unroll
                 for (int e = 0; e < 8; ++e) qz[y][e] = (__bf16)b[e];
             }
@@ -310,6 +324,7 @@ __global__ void __launch_bounds__(64 * kPWaves, 2) paged_prompt_kernel(const Pag
         // t's group g is not finite.
         uint64_t bad_next[G];
         auto prepare = [&](const char *__restrict slot, char *__restrict out, int tb, int ok) {
+            const CodeBits code_bits;
             constexpr uint32_t kInf = BF ? 0x7f80u : 0x7c00u;
             constexpr int KW = D / 64, VW = NT / 2;  // words of keys and values that a lane takes
             // everything that is read first
@@ -339,15 +354,18 @@ __global__ void __launch_bounds__(64 * kPWaves, 2) paged_prompt_kernel(const Pag
             for (int k = 0; k < KW; ++k) {
                 const int g = (w0 + k) / GW, in = (w0 + k) % GW;
                 const int place = (((lane >> 5) * (D / 16) + g * HW + in % HW) * 2 + in / HW) * 32 + row;
-                *reinterpret_cast<half8_t *>(out + place * 16) = codes_operand(kw[k]);
+                *reinterpret_cast<half8_t *>(out + place * 16) = codes_operand(kw[k], code_bits);
             }
             if (wave < 2 * PT::kPairs) {  // zeros and scales of the keys' group `wave` (one past an odd number: 0)
-                const float zf = high16<BF>(km);
-                const uint32_t zh = __float_as_uint(zf) >> 16;
-                const uint32_t zl = __float_as_uint(zf - __uint_as_float(zh << 16)) >> 16;
+                // (truncated parts: what is left is exact)
+                const float zero = fmaf(high16<BF>(km), 1.f / 64.f, -low16<BF>(km));
+                const uint32_t z1 = __float_as_uint(zero) >> 16;
+                const float rest = zero - __uint_as_float(z1 << 16);
+                const uint32_t z2 = __float_as_uint(rest) >> 16;
+                const uint32_t z3 = __float_as_uint(rest - __uint_as_float(z2 << 16)) >> 16;
                 const int place = (((lane >> 5) * PT::kPairs + (wave >> 1)) * 2 + (wave & 1)) * 32 + row;
                 *reinterpret_cast<uint4 *>(out + 2 * PT::kOperands + place * 16) =
-                    make_uint4(zh | (zh << 16), zh | (zl << 16), zl, 0);
+                    make_uint4(z1 | (z1 << 16), z1 | (z2 << 16), z2 | (z3 << 16), 0);
                 if (wave < G)
                     reinterpret_cast<uint16_t *>(out + 2 * PT::kOperands + PT::kZeros)[wave * kTokens + lane] = (uint16_t)km;
             }
@@ -401,7 +419,7 @@ __global__ void __launch_bounds__(64 * kPWaves, 2) paged_prompt_kernel(const Pag
 #pragma unroll
             for (int k = 0; k < VW; ++k)  // dim NT * m + j at place 32 j + m
                 *reinterpret_cast<half8_t *>(out + PT::kOperands + (wave * D + 32 * (j0 + k) + col) * 16) =
-                    __builtin_elementwise_fma(codes_operand(vw[k]), sc, ze);
+                    __builtin_elementwise_fma(codes_subnormal(vw[k]), sc, ze);
         };
 
         // One tile: computed from `cur`; the next one prepared from `next` into

@@ -63,15 +63,16 @@ def attend(q, store, table, lengths, starts, scale, causal=True, n_pages=None):
     """(out, tol): the attention in 64 bits and how far the kernels' roundings
     may take them from it.
 
-    Per row: a score is a sum of D products of a 16-bit and a 4-bit number, in
-    float32, times a scale, plus a zero times a sum of D numbers: off by at
-    most (D + 8) 2^-24 of the sum B of its terms' magnitudes (first order).
-    exp2 and the running maximum add 2^-21; the sums over tokens at most one
-    rounding a 32-token tile and 64 more.  A relative change e of every
-    probability moves an output by 2 e max|v|.  The output's own rounding is
-    half a step of its type.  Up to 64 rows a KV head, p s is rounded to fp16
-    (2^-11) and multiplied by code - 7.5; more rows round p and the value
-    itself, the value to at least 2^-18 of the largest of the request.""" 
+    Per row: a score is s 64 (sum q (1 + c/64)) + (z - 64 s) sum q, sums of D
+    exact products in float32: off by at most (D + 8) 2^-24 of the sum B of
+    the terms' magnitudes (first order).  exp2 and the running maximum add
+    2^-21; the sums over tokens at most one rounding a 32-token tile and 64
+    more.  A relative change e of every probability moves an output by 2 e
+    max|v|.  The output's own rounding is half a step of its type.  Up to 64
+    rows a KV head, p s is rounded to fp16 (2^-11) and multiplied by code -
+    7.5, as the difference of two sums of 64 p s and 72 p s; more rows round p
+    and the value itself, the value to at least 2^-18 of the largest of the
+    request."""
     k_c, v_c, k_m, v_m = unpack(store)
     page = store[0].shape[2]
     k_all, v_all = values_of(k_c, k_m), values_of(v_c, v_m)
@@ -94,7 +95,7 @@ def attend(q, store, table, lengths, starts, scale, causal=True, n_pages=None):
         for h in range(hkv):
             k, v = k_all[at, h], v_all[at, h]
             kt = k_m[at, h].double().repeat_interleave(d // k_m.shape[2], 1)
-            kmag = kt[..., 0] * k_c[at, h] + kt[..., 1].abs()
+            kmag = kt[..., 0] * (64 + k_c[at, h]) + (kt[..., 1] - 64 * kt[..., 0]).abs()
             vt = v_m[at, h].double().repeat_interleave(d // v_m.shape[2], 1)
             middle = vt[..., 0] * (v_c[at, h] - 7.5).abs()
             largest = v.abs().nan_to_num(0.0).amax(0)
@@ -112,7 +113,8 @@ def attend(q, store, table, lengths, starts, scale, causal=True, n_pages=None):
                 e = (d + 8) * 2.0 ** -24 * b + 2.0 ** -21 + (length / 32 + 64) * 2.0 ** -24
                 vmax = (vt[..., 0] * v_c[at, h] + vt[..., 1].abs())[see].amax(0)
                 if n * rep <= 64:
-                    half = 2.0 ** -11 * (p @ middle[see])
+                    half = 2.0 ** -11 * (p @ middle[see]) + \
+                        (length / 32 + 64) * 2.0 ** -24 * 152 * (p @ vt[see][..., 0])
                 else:
                     half = 2.001 * 2.0 ** -11 * (p @ v[see].abs()) + 2.0 ** -18 * largest
                 tol[row, h * rep:(h + 1) * rep] = u * o.abs() + half + 2 * e * vmax + \
