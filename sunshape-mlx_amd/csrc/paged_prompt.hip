@@ -97,6 +97,14 @@ __device__ __forceinline__ int parts_of_tiles(const Request &q, int share) {
     return max(1, (int)(((int64_t)(q.len + kTokens - 1) / kTokens + share - 1) / share));
 }
 
+// The bits of the 16-bit float 2^k, k >= -126 (positive ones compare as
+// integers); above the finite ones those of infinity, below all of them 1.
+template <bool BF>
+__device__ __forceinline__ uint32_t bits_of_exp2(int k) {
+    if (BF) return (uint32_t)min(k + 127, 255) << 7;
+    return k >= -14 ? (uint32_t)min(k + 15, 31) << 10 : 1u << max(k + 24, 0);
+}
+
 // Largest low and largest high half of the lanes' pairs, N sets side by side.
 template <int N>
 __device__ __forceinline__ void pair_max(uint32_t (&v)[N]) {
@@ -275,7 +283,9 @@ __global__ void __launch_bounds__(64 * kPWaves, 2) paged_prompt_kernel(const Pag
             const float down = a.scale < 0.f ? -exp2i(-shift) : exp2i(-shift);
             factor = fmaxf(fabsf(a.scale) * kLog2e * 64.f * exp2i(shift), 1e-30f);
             lag = kLag / factor;
-            float sums[G];
+            float sums[(G + 1) / 2];  // of group 2y + half
+#pragma unroll
+            for (int y = 0; y < (G + 1) / 2; ++y) sums[y] = 0.f;
 #pragma unroll
             for (int g = 0; g < G; ++g) {
                 float sum = 0.f;
@@ -287,13 +297,14 @@ __global__ void __launch_bounds__(64 * kPWaves, 2) paged_prompt_kernel(const Pag
                         sum += y;
                         qf[g][s][e] = (_Float16)y;
                     }
-                sums[g] = sum + __shfl_xor(sum, 32);
+                sum += __shfl_xor(sum, 32);
+                sums[g / 2] = half == g % 2 ? sum : sums[g / 2];
             }
             // the sum of group 2y + half as three bf16 parts, for the zero's three:
             // (z1, z1, z1, z2, z2, z3) . (q1, q2, q3, q1, q2, q1)
 #pragma unroll
             for (int y = 0; y < (G + 1) / 2; ++y) {
-                float v = half == 0 ? sums[2 * y] : (2 * y + 1 < G ? sums[2 * y + 1 < G ? 2 * y + 1 : 0] : 0.f);
+                float v = sums[y];
                 float part[3];
 #pragma unroll
                 for (int k = 0; k < 3; ++k) {
@@ -315,6 +326,11 @@ __global__ void __launch_bounds__(64 * kPWaves, 2) paged_prompt_kernel(const Pag
         int vexp[G], vnext[G];
 #pragma unroll
         for (int g = 0; g < G; ++g) vexp[g] = vnext[g] = -60;
+        // The bits from which zeros and scales would pass 2^vnext: few tiles
+        // after the first have any, and a look at a tile's largest is skipped.
+        uint32_t zero_top[G], scale_top[G];
+#pragma unroll
+        for (int g = 0; g < G; ++g) zero_top[g] = scale_top[g] = 1;
 
         // Element i of a product's 16: its value's group, as NT dims a row of
         // the A operand make neighbours (row m of tile j is dim NT*m + j).
@@ -372,28 +388,34 @@ __global__ void __launch_bounds__(64 * kPWaves, 2) paged_prompt_kernel(const Pag
 
             const bool real = tb + lane < rq.len && (ok >> (lane >> 4) & 1);
             bool odd_ones = tb + kTokens > rq.len || ok != 15;
-            uint32_t most[G];
+            bool more = false;
 #pragma unroll
             for (int g = 0; g < G; ++g) {
                 pair[g] = real ? pair[g] & 0x7fff7fffu : 0;
-                most[g] = pair[g];
                 bad_next[g] = 0;
+                more |= pair[g] >= zero_top[g] << 16 || (pair[g] & 0x7fffu) >= scale_top[g];
             }
-            pair_max(most);
+            if (__any(more)) {
+                uint32_t most[G];
 #pragma unroll
-            for (int g = 0; g < G; ++g) {
-                if ((most[g] & 0xffffu) >= kInf || (most[g] >> 16) >= kInf) {
-                    const bool b = (pair[g] & 0x7fffu) >= kInf || (pair[g] >> 16) >= kInf;
-                    bad_next[g] = __ballot(b);
-                    odd_ones = true;
-                    uint32_t rest[1] = {b ? 0 : pair[g]};
-                    pair_max(rest);
-                    most[g] = rest[0];
+                for (int g = 0; g < G; ++g) most[g] = pair[g];
+                pair_max(most);
+#pragma unroll
+                for (int g = 0; g < G; ++g) {
+                    if ((most[g] & 0xffffu) >= kInf || (most[g] >> 16) >= kInf) {
+                        const bool b = (pair[g] & 0x7fffu) >= kInf || (pair[g] >> 16) >= kInf;
+                        bad_next[g] = __ballot(b);
+                        odd_ones = true;
+                        uint32_t rest[1] = {b ? 0 : pair[g]};
+                        pair_max(rest);
+                        most[g] = rest[0];
+                    }
+                    // |zero + 15 scale| < 2 max(|zero|, 16 scale)
+                    const float c = fmaxf(16.f * low16<BF>(most[g]), high16<BF>(most[g]));
+                    const int e = __builtin_amdgcn_readfirstlane((int)((__float_as_uint(c) >> 23) & 0xffu) - 125);
+                    vnext[g] = max(vnext[g], min(e, 126));
+                    zero_top[g] = bits_of_exp2<BF>(vnext[g] - 1), scale_top[g] = bits_of_exp2<BF>(vnext[g] - 5);
                 }
-                // |zero + 15 scale| < 2 max(|zero|, 16 scale)
-                const float c = fmaxf(16.f * low16<BF>(most[g]), high16<BF>(most[g]));
-                const int e = __builtin_amdgcn_readfirstlane((int)((__float_as_uint(c) >> 23) & 0xffu) - 125);
-                vnext[g] = max(vnext[g], min(e, 126));
             }
             if (odd_ones) {  // (what no row sees, and what makes rows NaN further down)
                 uint64_t keep = ~0ull;
@@ -404,9 +426,10 @@ __global__ void __launch_bounds__(64 * kPWaves, 2) paged_prompt_kernel(const Pag
                     if (tb + 8 * wave + i >= rq.len || !((ok >> (wave >> 1)) & 1) || !((keep >> (8 * wave + i)) & 1))
                         vm[i] = 0;
             }
-            int e = vnext[0];
+            // (read as scalars: as elements the compiler would index an array in memory)
+            int e = __builtin_amdgcn_readfirstlane(vnext[0]);
 #pragma unroll
-            for (int g = 1; g < G; ++g) e = vg == g ? vnext[g] : e;
+            for (int g = 1; g < G; ++g) e = vg == g ? __builtin_amdgcn_readfirstlane(vnext[g]) : e;
             const float fs = exp2i(18 - e), fz = ldexpf(1.f, -6 - e), fs_odd = fs * 0x1p-4f;
             half8_t sc, ze;  // codes of odd pairs count 16 times
 #pragma unroll
