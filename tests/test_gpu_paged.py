@@ -107,6 +107,21 @@ def test_block_tables_of_many_requests(b, most, add, page):
     check_tables(plan, t, f, ref, before, new, n)
 
 
+@pytest.mark.parametrize("b,page", [(64, 16), (4096, 32)])
+def test_block_tables_of_which_few_requests_move(b, page):
+    """The pages given back and taken lie far apart, in runs from one page to
+    many times what the lanes of a wave hold."""
+    lengths, new = [5] * b, [0] * b
+    lengths[0], new[0] = 700 * page + 1, -(700 * page)
+    lengths[1], new[1] = 2 * page, -page
+    lengths[b // 2], new[b // 2] = 3, 130 * page
+    lengths[b - 2], new[b - 2] = page, 1
+    lengths[b - 1], new[b - 1] = 300 * page - 7, -(300 * page - 7)
+    n = 130 * page + 1
+    plan, t, f, ref, before = tables(lengths, new, page, 701, 1200 + 5 * b, n, seed=page)
+    check_tables(plan, t, f, ref, before, new, n)
+
+
 @pytest.mark.parametrize("lengths,new,pages,n,bits", [
     ([5], [-6], 4, 9, 1), ([-1], [0], 4, 9, 1), ([100], [200], 4, 300, 2), ([16, 16], [40, 40], 6, 99, 4),
     ([16, 0], [3, 5], 4, 7, 8), ([2000000000], [2000000000], 4, 9, 2 + 8),
