@@ -17,11 +17,24 @@ constexpr int kTile = 32;          // tokens a wave takes at a time
 constexpr int kWaves = 4;          // waves of a workgroup
 constexpr int kUnit = kTile * kWaves;
 constexpr int kStages = 4;         // tiles of a wave in LDS, one computed while the others arrive
-constexpr int kNt = 2;             // cache policy of the stream: non-temporal
-// Query rows a KV head up to which a request is this kernel's.
+// Cache policy of the stream: non-temporal (8 requests of 32768 tokens: 66 us;
+// cached: 75 us.  1 request: 20.6 and 21.1 us).
+constexpr int kNt = 2;
+// Query rows a KV head up to which a request is this kernel's.  At 8192 tokens
+// and 64 (request, head) columns: 64 rows take 88 us here and 113 us in the
+// prompt kernel, 96 rows 131 and 114 us.  (8 columns fill the device only
+// here: 32 and 52 us at 96 rows, 83 and 74 us at 512; the rule is for the
+// fuller device.)
 constexpr int kPromptRows = 64;
-// Columns of at most kWhole units are not cut; parts have at least kMinShare.
-constexpr int kWhole = 4, kMinShare = 2;
+// Columns of at most kWhole units are not cut, twice that if there are enough
+// of them to give every second compute unit one: a cut adds a launch and a
+// pass over the parts.  1 request of 8 heads, 640 tokens: 9.8 us whole, 11.7
+// cut; 1536 tokens: 15.8 and 11.7.  16 requests: 640 tokens 10.5 and 15.7,
+// 1536 tokens 16.7 and 18.8, 4096 tokens 33.9 and 30.0.
+constexpr int kWhole = 8;
+// Units of a run that may hold several columns (1 and 8 differ by less than
+// runs of the same code do).
+constexpr int kMinRun = 4;
 
 // Blocks of `rows` query rows a KV head of a request that are this kernel's,
 // and units of its tokens.
@@ -163,10 +176,10 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(const PagedAttn a) {
             }
             return n;
         };
-        share = max(uniform_div(total + groups - all_columns / 2 - 1, groups - all_columns / 2), kMinShare);
+        share = max(uniform_div(total + groups - all_columns / 2 - 1, groups - all_columns / 2), 1);
         int scan = wave_scan(items(share));
         if (__builtin_amdgcn_readlane(scan, 63) > groups) {
-            share = max(uniform_div(total + groups - all_columns - 1, groups - all_columns), kMinShare);
+            share = uniform_div(total + groups - all_columns - 1, groups - all_columns);
             scan = wave_scan(items(share));
         }
         const int item = blockIdx.x;
@@ -194,7 +207,7 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(const PagedAttn a) {
         // Many: the units of all columns in one row, shared out evenly; a run
         // may end inside a column and may hold several.  (Without `cut`: a
         // workgroup takes the columns that begin in its share, whole.)
-        share = max(uniform_div(total + groups - 1, groups), kWhole);
+        share = max(uniform_div(total + groups - 1, groups), a.cut ? kMinRun : 1);
         u = min((int64_t)blockIdx.x * share, (int64_t)total);
         stop = min((int64_t)u + share, (int64_t)total);
         const uint64_t holds = __ballot(u < units_scan);
@@ -592,10 +605,10 @@ static PagedPlan paged_plan(const ss_paged_store *s, int64_t n_tokens, int64_t n
     const int64_t rows = min(max_new * rep, (int64_t)kPromptRows);
     p.sets = rows > rs ? 2 : 1;
     p.rows = p.sets * rs;
-    const double units = (double)n_requests * s->n_kv_heads * ((rows + p.rows - 1) / p.rows) *
-                         ((max_length + kUnit - 1) / kUnit);
-    p.cut = max_length > kWhole * kUnit;
-    p.groups = (int)min((double)(2 * device_cu_count()), units / (p.cut ? kMinShare : 1));
+    const double columns = (double)n_requests * s->n_kv_heads * ((rows + p.rows - 1) / p.rows);
+    const int64_t units = (max_length + kUnit - 1) / kUnit;
+    p.cut = units > (2 * columns < device_cu_count() ? kWhole : 2 * kWhole);
+    p.groups = (int)min((double)(2 * device_cu_count()), columns * (p.cut ? (double)units : 1.));
     p.groups = max(p.groups, 1);
     p.bytes = p.cut ? (size_t)p.groups * (16 + 2 * p.rows * (s->head_dim + 2) * 4) : 0;
     if (max_new * rep > kPromptRows)  // (one after the other: they share it)
