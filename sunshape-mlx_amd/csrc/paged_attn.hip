@@ -162,9 +162,15 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(const PagedAttn a) {
     }
     const int units_scan = wave_scan(units);
     const int total = __builtin_amdgcn_readlane(units_scan, 63);
-    const int all_columns = __builtin_amdgcn_readlane(wave_scan(columns), 63);
+    const int columns_scan = wave_scan(columns);
+    const int all_columns = __builtin_amdgcn_readlane(columns_scan, 63);
     int u, stop, base, r, share, parts = 0;
-    if (a.cut && all_columns <= groups / 2) {
+    // Columns to be joined are listed for the merge, (parts, request, first
+    // workgroup, column of the request) at `list`: by column where they are few.
+    const bool few = a.cut && all_columns <= groups / 2;
+    int list = blockIdx.x;
+    int4 cut = make_int4(0, 0, 0, 0);
+    if (few) {
         // Few columns: each is cut into parts of its own, of at most `share`
         // units, so that no workgroup has more than one.  Sum of ceil(n/share)
         // is at most total/share + columns, and about total/share + columns/2.
@@ -189,6 +195,7 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(const PagedAttn a) {
             const int holder = __ffsll((unsigned long long)__ballot(item < scan)) - 1;
             int left = item - (holder ? __builtin_amdgcn_readlane(scan, holder - 1) : 0);
             base = holder ? __builtin_amdgcn_readlane(units_scan, holder - 1) : 0;
+            list = holder ? __builtin_amdgcn_readlane(columns_scan, holder - 1) : 0;
             for (r = holder * per;; ++r) {
                 const Request q = request(a, r);
                 const int n = blocks_of(a, q, ROWS) * heads, n_units = units_of(q);
@@ -198,9 +205,12 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(const PagedAttn a) {
                     u = base + column * n_units;
                     stop = u + uniform_div((part + 1) * n_units, parts);
                     u += uniform_div(part * n_units, parts);
+                    list += column;
+                    if (part == 0 && threadIdx.x == 0)
+                        a.cut[list] = make_int4(parts > 1 ? parts : 0, r, blockIdx.x, column);
                     break;
                 }
-                left -= n * parts, base += n * n_units;
+                left -= n * parts, base += n * n_units, list += n;
             }
         }
     } else {
@@ -216,7 +226,6 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(const PagedAttn a) {
         r = holder * per;
     }
     const int first_unit = u;
-    int4 cut = make_int4(0, 0, 0, 0);
 
     while (u < stop) {
         const Request rq = request(a, r);
@@ -237,8 +246,8 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(const PagedAttn a) {
         const int end = min((part_end - c0) * kUnit, rq.len);
         const bool whole = c0 >= first_unit && (!a.cut || c1 <= stop);
         const int place = c0 < first_unit ? 0 : 1;  // of this part, if it is one
-        if (!whole && place == 1)
-            cut = make_int4(parts ? parts : uniform_div(c1 - 1, share) - (int)blockIdx.x + 1, r, h, rb);
+        if (!few && !whole && place == 1)
+            cut = make_int4(uniform_div(c1 - 1, share) - (int)blockIdx.x + 1, r, blockIdx.x, column);
         u = part_end;
         const int32_t *row_table = a.table + (int64_t)r * a.width;
 
@@ -524,67 +533,81 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(const PagedAttn a) {
         }
         __syncthreads();
     }
-    if (a.cut && threadIdx.x == 0) a.cut[blockIdx.x] = cut;
+    if (a.cut && threadIdx.x == 0) {
+        if (!few) a.cut[blockIdx.x] = cut;
+        if (blockIdx.x == 0) a.cut[groups] = make_int4(few ? all_columns : groups, 0, 0, 0);
+    }
 }
 
-// Joins the parts of the column that workgroup blockIdx.y of the kernel above
-// began and did not end (its second place, then the first place of those that
-// follow), one row (blockIdx.x) a workgroup: every thread loads four dims of
-// its parts at once, 8 (D 128) or 16 threads a dim.
+// Joins the parts of the columns listed (the second place of the workgroup
+// that began one, the first place of those that follow), one row (blockIdx.x)
+// a workgroup: every thread loads four dims of its parts at once, 8 (D 128) or
+// 16 threads a dim.  The host knows how many columns there can be and launches
+// no more workgroups than that: 4.4 us for 8 columns of 64 parts, of which the
+// launch and four reads in a row are nearly all (a workgroup for each of 512
+// possible parts: 4.9 us).
 template <int D>
-__global__ void __launch_bounds__(256) paged_merge_kernel(const PagedAttn a, int rows_per_block) {
+__global__ void __launch_bounds__(256) paged_merge_kernel(const PagedAttn a, int rows_per_block,
+                                                          int groups) {
     constexpr int CH = D / 4, PARTS = 256 / CH, PER = 8, STEP = PARTS * PER;
     __shared__ float red[PARTS][D + 4];
     __shared__ float total[PARTS], tops[kWaves];
-    const int4 cut = a.cut[blockIdx.y];
-    const int parts = cut.x, r = cut.y, h = cut.z, row = blockIdx.x, n = cut.w * rows_per_block + row;
-    if (parts == 0) return;
-    const Request rq = request(a, r);
-    if (n >= rq.rows) return;
-    auto at = [&](int i) { return (((int64_t)blockIdx.y + i) * 2 + (i == 0 ? 1 : 0)) * rows_per_block + row; };
-    const int c = threadIdx.x % CH * 4, p = threadIdx.x / CH, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    float4 v[PER];
+    const int4 begin = a.cut[blockIdx.y];  // (not after the count: one wait for both)
+    const int n_list = a.cut[groups].x;
+    for (int k = blockIdx.y; k < n_list; k += gridDim.y) {
+        const int4 cut = k == (int)blockIdx.y ? begin : a.cut[k];
+        const int parts = cut.x, row = blockIdx.x;
+        if (parts == 0) continue;
+        const Request rq = request(a, cut.y);
+        const int row_blocks = blocks_of(a, rq, rows_per_block);
+        const int h = uniform_div(cut.w, row_blocks), n = (cut.w - h * row_blocks) * rows_per_block + row;
+        if (n >= rq.rows) continue;
+        auto at = [&](int i) { return (((int64_t)cut.z + i) * 2 + (i == 0 ? 1 : 0)) * rows_per_block + row; };
+        const int c = threadIdx.x % CH * 4, p = threadIdx.x / CH, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+        float4 v[PER];
 #pragma unroll
-    for (int i = 0; i < PER; ++i)
-        v[i] = *reinterpret_cast<const float4 *>(a.acc + at(min(p + i * PARTS, parts - 1)) * D + c);
-    float m = -INFINITY;
-    for (int i = threadIdx.x; i < parts; i += 256) m = fmaxf(m, a.ml[at(i) * 2]);
-    m = wave_max(m);
-    if (lane == 0) tops[wave] = m;
-    __syncthreads();
+        for (int i = 0; i < PER; ++i)
+            v[i] = *reinterpret_cast<const float4 *>(a.acc + at(min(p + i * PARTS, parts - 1)) * D + c);
+        float m = -INFINITY;
+        for (int i = threadIdx.x; i < parts; i += 256) m = fmaxf(m, a.ml[at(i) * 2]);
+        m = wave_max(m);
+        if (lane == 0) tops[wave] = m;
+        __syncthreads();
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) m = fmaxf(m, tops[w]);
-    float x[4] = {0.f, 0.f, 0.f, 0.f}, l = 0.f;
-    for (int from = 0; from < parts; from += STEP) {
+        for (int w = 0; w < kWaves; ++w) m = fmaxf(m, tops[w]);
+        float x[4] = {0.f, 0.f, 0.f, 0.f}, l = 0.f;
+        for (int from = 0; from < parts; from += STEP) {
 #pragma unroll
-        for (int i = 0; i < PER; ++i) {
-            const int s = from + p + i * PARTS;
-            if (s >= parts) break;
-            const float2 e = *reinterpret_cast<const float2 *>(a.ml + at(s) * 2);
-            const float f = e.x == m ? 1.f : fast_exp2(e.x - m);
-            l += f * e.y;
-            x[0] += f * v[i].x, x[1] += f * v[i].y, x[2] += f * v[i].z, x[3] += f * v[i].w;
+            for (int i = 0; i < PER; ++i) {
+                const int s = from + p + i * PARTS;
+                if (s >= parts) break;
+                const float2 e = *reinterpret_cast<const float2 *>(a.ml + at(s) * 2);
+                const float f = e.x == m ? 1.f : fast_exp2(e.x - m);
+                l += f * e.y;
+                x[0] += f * v[i].x, x[1] += f * v[i].y, x[2] += f * v[i].z, x[3] += f * v[i].w;
+            }
+            if (from + STEP < parts)
+#pragma unroll
+                for (int i = 0; i < PER; ++i)
+                    v[i] = *reinterpret_cast<const float4 *>(a.acc + at(min(from + STEP + p + i * PARTS, parts - 1)) * D + c);
         }
-        if (from + STEP < parts)
 #pragma unroll
-            for (int i = 0; i < PER; ++i)
-                v[i] = *reinterpret_cast<const float4 *>(a.acc + at(min(from + STEP + p + i * PARTS, parts - 1)) * D + c);
-    }
+        for (int k = 0; k < 4; ++k) red[p][c + k] = x[k];
+        if (c == 0) total[p] = l;
+        __syncthreads();
+        if (threadIdx.x < CH) {
+            float y[4] = {0.f, 0.f, 0.f, 0.f}, t = 0.f;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) red[p][c + k] = x[k];
-    if (c == 0) total[p] = l;
-    __syncthreads();
-    if (threadIdx.x < CH) {
-        float y[4] = {0.f, 0.f, 0.f, 0.f}, t = 0.f;
+            for (int i = 0; i < PARTS; ++i) {
+                t += total[i];
 #pragma unroll
-        for (int i = 0; i < PARTS; ++i) {
-            t += total[i];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) y[k] += red[i][c + k];
+                for (int k = 0; k < 4; ++k) y[k] += red[i][c + k];
+            }
+            const float inv = t == 0.f ? 0.f : 1.f / t;
+            const int64_t o = ((int64_t)(rq.t0 + n / a.rep) * a.hq + h * a.rep + n % a.rep) * D + c;
+            store_out4(a, o, y[0] * inv, y[1] * inv, y[2] * inv, y[3] * inv);
         }
-        const float inv = t == 0.f ? 0.f : 1.f / t;
-        const int64_t o = ((int64_t)(rq.t0 + n / a.rep) * a.hq + h * a.rep + n % a.rep) * D + c;
-        store_out4(a, o, y[0] * inv, y[1] * inv, y[2] * inv, y[3] * inv);
+        __syncthreads();  // (the next column's sums)
     }
 }
 
@@ -592,6 +615,7 @@ __global__ void __launch_bounds__(256) paged_merge_kernel(const PagedAttn a, int
 
 struct PagedPlan {
     int sets, rows, groups;  // column sets, query rows a workgroup takes; workgroups
+    int columns;             // that there can be, at most `groups`
     bool cut;                // whether columns may be cut
     size_t bytes;
 };
@@ -610,7 +634,8 @@ static PagedPlan paged_plan(const ss_paged_store *s, int64_t n_tokens, int64_t n
     p.cut = units > (2 * columns < device_cu_count() ? kWhole : 2 * kWhole);
     p.groups = (int)min((double)(2 * device_cu_count()), columns * (p.cut ? (double)units : 1.));
     p.groups = max(p.groups, 1);
-    p.bytes = p.cut ? (size_t)p.groups * (16 + 2 * p.rows * (s->head_dim + 2) * 4) : 0;
+    p.columns = (int)min(columns, (double)p.groups);
+    p.bytes = p.cut ? 16 + (size_t)p.groups * (16 + 2 * p.rows * (s->head_dim + 2) * 4) : 0;
     if (max_new * rep > kPromptRows)  // (one after the other: they share it)
         p.bytes = max(p.bytes, paged_prompt_bytes(s, n_requests, n_tokens * rep, kPromptRows));
     return p;
@@ -634,7 +659,7 @@ static void launch_paged(const PagedAttn &a, const PagedPlan &p, hipStream_t st)
     else
         hipLaunchKernelGGL((paged_attn_kernel<D, G, BF, 2>), dim3(p.groups), dim3(256), 0, st, a);
     if (p.cut)
-        hipLaunchKernelGGL(paged_merge_kernel<D>, dim3(p.rows, p.groups), dim3(256), 0, st, a, p.rows);
+        hipLaunchKernelGGL(paged_merge_kernel<D>, dim3(p.rows, p.columns), dim3(256), 0, st, a, p.rows, p.groups);
 }
 
 }  // namespace ss
@@ -687,7 +712,7 @@ extern "C" int ss_paged_attn(const ss_paged_store *store, const void *q, int q_d
     const bool prompts = max_new * a.rep > kPromptRows;
     a.most_rows = prompts ? kPromptRows : INT32_MAX;
     a.cut = p.cut ? static_cast<int4 *>(workspace) : nullptr;
-    a.acc = reinterpret_cast<float *>(a.cut + p.groups);
+    a.acc = reinterpret_cast<float *>(a.cut + p.groups + 1);
     a.ml = a.acc + (size_t)p.groups * 2 * p.rows * store->head_dim;
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
     const bool bf = store->dtype == SS_BF16;

@@ -39,7 +39,7 @@ struct PagedAttn {
     float scale;
     int most_rows;      // requests with more query rows a KV head are the prompt kernel's
     int target;         // of the prompt kernel: workgroups that its parts fill
-    int4 *cut;          // [workgroups]: (parts, request, head, row block) of a column to be joined
+    int4 *cut;          // columns to be joined (each kernel's merge says what it lists)
     float *acc;         // [workgroups][2][rows of a workgroup][D]
     float *ml;          // [workgroups][2][rows of a workgroup][2]
 };
