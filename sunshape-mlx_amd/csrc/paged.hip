@@ -231,47 +231,48 @@ __device__ __forceinline__ int group_reduce(int v, F op) {
 // returns their codes as a word, (scale, zero) as `meta`.
 // zero = min, scale = round16((max - min) / 15), code = the nearest of
 // 0 .. 15 to (x - zero) / scale, ties to even.  x - zero is one rounding;
-// the quotient is never rounded: rcp guesses a code and the exact remainder
-// (an fma) moves it by one where it is past half a step.
+// the quotient is never rounded: rcp guesses its integer part c, at most one
+// off and then next to an integer, and the exact remainder r = d - c scale (an
+// fma) adds one if r > scale/2, or r = scale/2 and c is odd.  Positive floats
+// compare as integers, so that both are one test: bits(r) + (c odd) >
+// bits(scale/2).
 template <int LANES, bool BF>
 __device__ __forceinline__ uint32_t quantize8(const float (&x)[8], uint32_t &meta) {
-    int hi = ord_key(x[0]), lo = hi;
-    uint32_t top = 0;
+    float most = x[0], least = x[0];
+    bool nan = false;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-        const int k = ord_key(x[e]);
-        hi = max(hi, k);
-        lo = min(lo, k);
-        top = max(top, __float_as_uint(x[e]) & 0x7fffffffu);
+        most = fmaxf(most, x[e]);
+        least = fminf(least, x[e]);
+        nan |= x[e] != x[e];
     }
+    // (a NaN's key is above every number's: the range is NaN then)
+    int hi = nan ? INT32_MAX : ord_key(most), lo = ord_key(least);
     hi = group_reduce<LANES>(hi, [](int a, int b) { return max(a, b); });
     lo = group_reduce<LANES>(lo, [](int a, int b) { return min(a, b); });
-    top = (uint32_t)group_reduce<LANES>((int)top, [](int a, int b) { return max(a, b); });
     const float zero = ord_float(lo);
     const float range = __fdiv_rn(__fsub_rn(ord_float(hi), zero), 15.f);
     const uint32_t sb = to_bits16<BF>(range);
     const float scale = from_bits16<BF>(sb);
-    if (top >= 0x7f800000u || !(scale < INFINITY)) {  // a value, or the range, is not finite
+    if (!(scale < INFINITY)) {  // a value, or the range, is not finite
         meta = kNan16<BF> | (kNan16<BF> << 16);
         return 0;
     }
     meta = sb | (to_bits16<BF>(zero) << 16);
     if (!(scale > 0.f)) return 0;
-    // (a scale below 2^-100 has no normal reciprocal: both sides times 2^64)
-    const float up = scale < 0x1p-100f ? 0x1p64f : 1.f;
-    const float sc = scale * up, half = 0.5f * sc, inv = __builtin_amdgcn_rcpf(sc);
+    // (a bfloat16 scale below 2^-100 has no normal reciprocal: both sides times 2^64)
+    const float up = BF && scale < 0x1p-100f ? 0x1p64f : 1.f;
+    const float sc = scale * up, inv = __builtin_amdgcn_rcpf(sc);
+    const int half = __float_as_int(0.5f * sc);
     uint32_t word = 0;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-        const float d = __fsub_rn(x[e], zero) * up;
-        float c = rintf(d * inv);
-        const float rem = fmaf(-c, sc, d);
-        if (fabsf(rem) >= half) {
-            const bool odd = ((int)c & 1) != 0;
-            if (fabsf(rem) > half || odd) c += rem > 0.f ? 1.f : -1.f;
-        }
-        c = fminf(fmaxf(c, 0.f), 15.f);
-        word |= (uint32_t)c << nibble_bit(e);
+        float d = __fsub_rn(x[e], zero);
+        if (BF) d *= up;
+        const float f = floorf(d * inv);
+        uint32_t c = (uint32_t)f;
+        c += __float_as_int(fmaf(-f, sc, d)) + (int)(c & 1) > half;
+        word |= min(c, 15u) << nibble_bit(e);
     }
     return word;
 }
@@ -282,24 +283,26 @@ __device__ __forceinline__ uint32_t quantize8(const float (&x)[8], uint32_t &met
 // where its tokens are one whole block it stores the words; otherwise it
 // clears and sets their bits with two atomics per block (bits of other tokens,
 // which other waves may be writing, are kept; no order changes the result as
-// long as no slot is given twice).  HBM bounds long prompts, the latency of
-// load -> reduce -> store short ones.
+// long as no slot is given twice).  Vector operations bound long prompts (some
+// 11 to quantise a value, and the 8 x 8 transposes), the latency of load ->
+// reduce -> store short ones: 8192 tokens of 8 heads x 128 dims take 16 us
+// (43 MB, 2.7 TB/s; the bytes alone would take 8.3 us), 16 tokens 7 us.
 template <int D, int GROUP, bool BF>
 __global__ void __launch_bounds__(256)
     append_paged_kernel(PagedStore st, const void *keys, const void *values, int in_dtype, int vec, int64_t k_st,
                         int64_t k_sh, int64_t v_st, int64_t v_sh, const int32_t *slots, int64_t n_tok,
-                        int64_t n_items) {
+                        uint32_t n_items) {
     constexpr int LPR = D / 8;          // lanes a row
     constexpr int RPP = 64 / LPR;       // rows a pass
     constexpr int PASSES = 8 / RPP;
     constexpr int G = D / GROUP;
     __shared__ uint32_t tile[4][8][LPR + 1];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int64_t item = (int64_t)blockIdx.x * 4 + wave;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t item = blockIdx.x * 4 + wave;
     if (item >= n_items) return;  // whole waves leave; no barrier follows
-    const int64_t win = item / st.heads;
-    const int h = (int)(item - win * st.heads);
-    const int64_t t0 = win * 8;
+    const uint32_t win = item / (uint32_t)st.heads;
+    const int h = (int)(item - win * (uint32_t)st.heads);
+    const int64_t t0 = (int64_t)win * 8;
     const int n_slots = st.n_pages << st.log_page;
     // lane e < 8 holds the slot of token t0 + e (-1: not stored)
     int my_slot = -1;
@@ -310,13 +313,31 @@ __global__ void __launch_bounds__(256)
     const int w = lane % LPR, g = (w * 8) / GROUP;
     float x[2][PASSES][8];
     int slot_of[PASSES];
+    const bool half = in_dtype != SS_F32 && vec;  // one wide load for 8 values
+    uint4 raw[2][PASSES];
+    auto row_of = [&](int p) { return min(t0 + p * RPP + lane / LPR, n_tok - 1); };
+    if (half) {  // (all before the first is looked at)
 #pragma unroll
-    for (int p = 0; p < PASSES; ++p) {
-        const int e = p * RPP + lane / LPR;
-        const int64_t t = min(t0 + e, n_tok - 1);
-        load8_f32(keys, in_dtype, vec, t * k_st + h * k_sh + w * 8, x[0][p]);
-        load8_f32(values, in_dtype, vec, t * v_st + h * v_sh + w * 8, x[1][p]);
-        slot_of[p] = __shfl(my_slot, e);
+        for (int p = 0; p < PASSES; ++p) {
+            raw[0][p] = *reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(keys) + row_of(p) * k_st + h * k_sh + w * 8);
+            raw[1][p] = *reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(values) + row_of(p) * v_st + h * v_sh + w * 8);
+        }
+    } else {
+#pragma unroll
+        for (int p = 0; p < PASSES; ++p) {
+            load8_f32(keys, in_dtype, vec, row_of(p) * k_st + h * k_sh + w * 8, x[0][p]);
+            load8_f32(values, in_dtype, vec, row_of(p) * v_st + h * v_sh + w * 8, x[1][p]);
+        }
+    }
+#pragma unroll
+    for (int p = 0; p < PASSES; ++p) slot_of[p] = __shfl(my_slot, p * RPP + lane / LPR);
+    if (half) {
+        if (in_dtype == SS_F16)
+#pragma unroll
+            for (int i = 0; i < 2 * PASSES; ++i) unpack16<__half>(raw[i / PASSES][i % PASSES], x[i / PASSES][i % PASSES]);
+        else
+#pragma unroll
+            for (int i = 0; i < 2 * PASSES; ++i) unpack16<__hip_bfloat16>(raw[i / PASSES][i % PASSES], x[i / PASSES][i % PASSES]);
     }
 #pragma unroll
     for (int p = 0; p < PASSES; ++p) {
@@ -325,8 +346,12 @@ __global__ void __launch_bounds__(256)
         const int off = slot & ((1 << st.log_page) - 1);
 #pragma unroll
         for (int kv = 0; kv < 2; ++kv) {
+            if (in_dtype != (BF ? SS_BF16 : SS_F16))
 #pragma unroll
-            for (int i = 0; i < 8; ++i) x[kv][p][i] = round16<BF>(x[kv][p][i]);
+                for (int i = 0; i < 8; i += 2) {
+                    const uint32_t u = pack16<BF>(x[kv][p][i], x[kv][p][i + 1]);
+                    x[kv][p][i] = from_bits16<BF>(u & 0xffffu), x[kv][p][i + 1] = from_bits16<BF>(u >> 16);
+                }
             uint32_t meta;
             const uint32_t word = quantize8<GROUP / 8, BF>(x[kv][p], meta);
             if (kv) tile[wave][e][w] = word;
@@ -392,47 +417,45 @@ __global__ void __launch_bounds__(256)
 
 // -------------------------------------------------------------------- read
 
-// A thread takes 8 dims of one token and head, of the keys or the values:
+// A thread takes 8 dims of the keys and of the values of one token and head:
 // value = zero + code * scale, one rounding to the cache's type.  Tokens
-// without a slot read as zeros.
-template <bool BF>
+// without a slot read as zeros.  A value word's 8 tokens are 8 threads', whose
+// reads of it meet in the caches; 8192 tokens of 8 heads x 128 dims take 11.3
+// us (43 MB, 3.8 TB/s), a copy of as many bytes 8.3 us.
+template <int D, bool BF>
 __global__ void __launch_bounds__(256)
-    read_paged_kernel(PagedStore st, const int32_t *slots, int64_t n_tok, int d, int group, int64_t n_items,
-                      uint16_t *keys, uint16_t *values) {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i >= n_items) return;
-    const int words = d / 8, groups = d / group;
-    const int64_t half = n_items / 2;
-    const bool v = i >= half;
-    const int64_t e = v ? i - half : i;  // (token, head, word)
-    const int64_t th = e / words;
-    const int w = (int)(e - th * words);
-    const int64_t t = th / st.heads;
-    const int h = (int)(th - t * st.heads);
+    read_paged_kernel(PagedStore st, const int32_t *slots, int log_group, uint32_t n_rows, uint16_t *keys,
+                      uint16_t *values) {
+    constexpr int W = D / 8;
+    const uint32_t th = blockIdx.x * (256 / W) + threadIdx.x / W;  // (token, head)
+    if (th >= n_rows) return;
+    const int w = threadIdx.x % W;
+    const uint32_t t = th / (uint32_t)st.heads;
+    const int h = (int)(th - t * (uint32_t)st.heads);
     const int slot = slots[t];
-    uint32_t out[4] = {0, 0, 0, 0};
-    if ((uint32_t)slot < (uint32_t)(st.n_pages << st.log_page)) {
-        const int64_t row = (int64_t)(slot >> st.log_page) * st.heads + h;
-        const int off = slot & ((1 << st.log_page) - 1);
-        const uint32_t m = (v ? st.v_meta : st.k_meta)[((row * groups + w * 8 / group) << st.log_page) + off];
-        const float s = from_bits16<BF>(m & 0xffffu), z = from_bits16<BF>(m >> 16);
-        uint32_t c[8];
-        if (v) {
-            const uint32_t *p = st.v_codes + (((row << st.log_page) + off) >> 3) * d + w * 8;
-            const uint4 a = *reinterpret_cast<const uint4 *>(p), b = *reinterpret_cast<const uint4 *>(p + 4);
-            const uint32_t u[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-#pragma unroll
-            for (int j = 0; j < 8; ++j) c[j] = (u[j] >> nibble_bit(off & 7)) & 15u;
-        } else {
-            const uint32_t u = st.k_codes[((row << st.log_page) + off) * words + w];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) c[j] = (u >> nibble_bit(j)) & 15u;
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-            out[j] = to_bits16<BF>(fmaf((float)c[2 * j], s, z)) | (to_bits16<BF>(fmaf((float)c[2 * j + 1], s, z)) << 16);
+    uint4 *const to_k = reinterpret_cast<uint4 *>(keys + (int64_t)th * D) + w;
+    uint4 *const to_v = reinterpret_cast<uint4 *>(values + (int64_t)th * D) + w;
+    if ((uint32_t)slot >= (uint32_t)(st.n_pages << st.log_page)) {
+        *to_k = *to_v = make_uint4(0, 0, 0, 0);
+        return;
     }
-    *reinterpret_cast<uint4 *>((v ? values : keys) + e * 8) = make_uint4(out[0], out[1], out[2], out[3]);
+    const int64_t row = (int64_t)(slot >> st.log_page) * st.heads + h;
+    const int off = slot & ((1 << st.log_page) - 1), bit = nibble_bit(off & 7);
+    const int64_t at = ((((row * D) >> log_group) + ((w * 8) >> log_group)) << st.log_page) + off;
+    const uint32_t km = st.k_meta[at], vm = st.v_meta[at];
+    const uint32_t kw = st.k_codes[((row << st.log_page) + off) * W + w];
+    const uint32_t *const p = st.v_codes + (((row << st.log_page) + off) >> 3) * D + w * 8;
+    const uint4 a = *reinterpret_cast<const uint4 *>(p), b = *reinterpret_cast<const uint4 *>(p + 4);
+    const float ks = from_bits16<BF>(km & 0xffffu), kz = from_bits16<BF>(km >> 16);
+    const float vs = from_bits16<BF>(vm & 0xffffu), vz = from_bits16<BF>(vm >> 16);
+    // even pairs' codes as the bytes (0, 4, 1, 5) of one word, odd ones' (2, 6, 3, 7)
+    const uint32_t even = kw & 0x0f0f0f0fu, odd = (kw >> 4) & 0x0f0f0f0fu;
+    auto byte = [](uint32_t u, int i) { return (float)((u >> (8 * i)) & 0xffu); };
+    auto key = [&](uint32_t u, int i) { return pack16<BF>(fmaf(byte(u, i), ks, kz), fmaf(byte(u, i + 2), ks, kz)); };
+    *to_k = make_uint4(key(even, 0), key(odd, 0), key(even, 1), key(odd, 1));
+    auto value = [&](uint32_t u) { return fmaf((float)((u >> bit) & 15u), vs, vz); };
+    *to_v = make_uint4(pack16<BF>(value(a.x), value(a.y)), pack16<BF>(value(a.z), value(a.w)),
+                       pack16<BF>(value(b.x), value(b.y)), pack16<BF>(value(b.z), value(b.w)));
 }
 
 // -------------------------------------------------------------------- host
@@ -504,7 +527,7 @@ extern "C" int ss_append_paged(const ss_paged_store *store, const void *keys, co
     if (n_tokens == 0) return SS_OK;
     SS_REQUIRE(keys && values && slots, "null pointer argument");
     const int64_t items = (n_tokens + 7) / 8 * ps.heads;
-    SS_UNSUPPORTED(n_tokens <= INT32_MAX && items < (1LL << 33), "too many tokens for one launch");
+    SS_UNSUPPORTED(n_tokens <= INT32_MAX && items <= INT32_MAX, "too many tokens for one launch");
     // 16-byte loads where every row starts on 16 bytes
     const int per = in_dtype == SS_F32 ? 4 : 8;
     const int vec = (((uintptr_t)keys | (uintptr_t)values) & 15) == 0 && k_st % per == 0 && k_sh % per == 0 &&
@@ -513,7 +536,7 @@ extern "C" int ss_append_paged(const ss_paged_store *store, const void *keys, co
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
     auto launch = [&](auto kernel) {
         hipLaunchKernelGGL(kernel, grid, dim3(256), 0, st, ps, keys, values, in_dtype, vec, k_st, k_sh, v_st, v_sh,
-                           slots, n_tokens, items);
+                           slots, n_tokens, (uint32_t)items);
     };
     const bool bf = store->dtype == SS_BF16;
     const int key = store->head_dim * 1000 + store->group_size;
@@ -535,15 +558,18 @@ extern "C" int ss_read_paged(const ss_paged_store *store, const int32_t *slots, 
     if (n_tokens == 0) return SS_OK;
     SS_REQUIRE(keys && values && slots, "null pointer argument");
     SS_REQUIRE((((uintptr_t)keys | (uintptr_t)values) & 15) == 0, "outputs must be 16-byte aligned");
-    const int64_t items = n_tokens * ps.heads * (store->head_dim / 8) * 2;
-    SS_UNSUPPORTED(n_tokens <= INT32_MAX && items < (1LL << 39), "too many tokens for one launch");
-    const dim3 grid((unsigned)((items + 255) / 256));
+    SS_UNSUPPORTED(n_tokens <= INT32_MAX && n_tokens * ps.heads <= INT32_MAX, "too many tokens for one launch");
+    const int rows = 256 / (store->head_dim / 8);  // of a workgroup
+    const dim3 grid((unsigned)((n_tokens * ps.heads + rows - 1) / rows));
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
     auto launch = [&](auto kernel) {
-        hipLaunchKernelGGL(kernel, grid, dim3(256), 0, st, ps, slots, n_tokens, store->head_dim, store->group_size,
-                           items, static_cast<uint16_t *>(keys), static_cast<uint16_t *>(values));
+        hipLaunchKernelGGL(kernel, grid, dim3(256), 0, st, ps, slots, __builtin_ctz((unsigned)store->group_size),
+                           (uint32_t)(n_tokens * ps.heads), static_cast<uint16_t *>(keys),
+                           static_cast<uint16_t *>(values));
     };
-    store->dtype == SS_BF16 ? launch(read_paged_kernel<true>) : launch(read_paged_kernel<false>);
+    const bool bf = store->dtype == SS_BF16;
+    if (store->head_dim == 128) bf ? launch(read_paged_kernel<128, true>) : launch(read_paged_kernel<128, false>);
+    else bf ? launch(read_paged_kernel<64, true>) : launch(read_paged_kernel<64, false>);
     SS_LAUNCH_CHECK("read_paged_kernel launch");
     return SS_OK;
 }

@@ -35,9 +35,14 @@ __device__ __forceinline__ uint32_t to_bits16(float x) {
     return __half_as_ushort(__float2half(x));
 }
 
+// Two nearest 16-bit floats (one instruction), `a` in the low half.
 template <bool BF>
-__device__ __forceinline__ float round16(float x) {
-    return from_bits16<BF>(to_bits16<BF>(x));
+__device__ __forceinline__ uint32_t pack16(float a, float b) {
+    typedef float f2 __attribute__((ext_vector_type(2)));
+    typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+    typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+    if (BF) return __builtin_bit_cast(uint32_t, __builtin_convertvector((f2{a, b}), b2));
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f2{a, b}), h2));
 }
 
 }  // namespace ss
