@@ -1100,7 +1100,7 @@ int ss_read_paged(const ss_paged_store *store, const int32_t *slots, int64_t n_t
  * Softmax statistics and sums are float32; probabilities times scales enter
  * the matrix cores in 16 bits.  Table entries outside the pool hold no
  * tokens.  max_new and max_length (the most new tokens and the longest
- * length) size the launch: results do not depend on them.  workspace:
+ * length) size the launch: wrong ones change roundings only.  workspace:
  * ss_paged_attn_workspace_bytes of the same arguments, uninitialised, not
  * shared with a call that may run at the same time.
  */

@@ -4,8 +4,9 @@
 // A workgroup of eight waves takes 256 query rows of one KV head (its group's
 // heads at consecutive positions), 32 a wave, over 64-token tiles.  While a
 // tile is computed the next one is prepared, once for all rows: its key codes
-// become 16-bit operands (see paged_attn.hpp) and its values are dequantised to fp16, both in the operand order of
-// v_mfma_f32_32x32x16_f16, and the one after that is copied from HBM.
+// become 16-bit operands (see paged_attn.hpp) and its values are dequantised
+// to fp16, both in the operand order of v_mfma_f32_32x32x16_f16, and the one
+// after that is copied from HBM.
 //
 // Scores are exact: code products are summed group by group and each sum is
 // multiplied by its token's scale in float32; the zeros' part is one more

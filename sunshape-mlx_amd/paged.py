@@ -294,7 +294,8 @@ def paged_attention(queries: torch.Tensor, store: PagedKVStore, block_table: tor
 
     ``max_new`` and ``max_length``, the most new tokens and the longest length
     if the caller knows them, size the launch (by default every request adds
-    a token and a table row is full); the result does not depend on them.
+    a token and a table row is full); wrong ones cost time and change roundings
+    only.
     Queries under autograd are refused: there is no backward pass."""
     st = _struct(store)
     dev = store[0].get_device()
@@ -397,6 +398,8 @@ class PagedKVCache:
             new, self._host = new_lengths, None
             most = min(n_tokens, n_tokens if max_new is None else max_new)
             self._bound = min(self.max_tokens, self._bound + max(0, most))
+            if torch.cuda.is_current_stream_capturing():  # (replays add to the lengths too)
+                self._bound = self.max_tokens
         else:
             adds = [int(x) for x in new_lengths]
             if len(adds) != self.n_requests:
@@ -461,6 +464,7 @@ class PagedKVCache:
 
     def trim(self, n: int) -> None:
         """Give the last ``n`` tokens of every request back."""
+        n = max(0, n)
         if self._host is not None:
             self.step([-min(n, have) for have in self._host])
         else:
@@ -509,12 +513,16 @@ class PagedKVCache:
         b_, hq, t_, d = queries.shape
         if b_ != self.n_requests:
             raise ValueError(f"queries of {b_} sequences, {self.n_requests} requests")
-        if self._starts is None or self._starts[0] != t_:
-            self._starts = (t_, torch.arange(0, (b_ + 1) * t_, max(1, t_), dtype=torch.int32,
-                                             device=self.lengths.device)
-                            if t_ else torch.zeros_like(torch.cat((self.lengths, self.lengths[:1]))))
+        dev = self.lengths.device
+        if torch.cuda.is_current_stream_capturing():  # (the graph's own, filled by its replays)
+            starts = torch.arange(b_ + 1, dtype=torch.int32, device=dev) * t_
+        else:
+            if self._starts is None or self._starts[0] != t_:
+                # copied from the host, which waits: any stream may read it
+                self._starts = (t_, (torch.arange(b_ + 1, dtype=torch.int32) * t_).to(dev))
+            starts = self._starts[1]
         out = paged_attention(queries.transpose(1, 2).reshape(b_ * t_, hq, d), self.store,
-                              self.block_table, self.lengths, self._starts[1], scale,
+                              self.block_table, self.lengths, starts, scale,
                               causal=mask == "causal", max_new=max(1, t_),
                               max_length=max(1, self._bound))
         return out.view(b_, t_, hq, d).transpose(1, 2)

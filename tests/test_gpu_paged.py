@@ -572,6 +572,56 @@ def test_a_step_replays_from_a_graph():
     check_attention(other["out"], other["q"], other["store"], other["table"], other["lengths"], starts, 0.1)
 
 
+@pytest.mark.parametrize("max_length", [100, 1100, 3000])
+def test_more_rows_than_the_hint_says(max_length):
+    """Columns beyond those that the merge is launched for, cut and whole."""
+    new = [15, 9, 0, 1, 60]
+    store, table, le, starts = world(21, [3000, 2000, 700, 1500, 1300], new, 2, 128, 64, 16, torch.float16)
+    q = rows(22, sum(new), 8, 128, torch.float16, False)
+    for max_new in (1, 4, 16):
+        out = S.paged_attention(q, store, table, le, starts, 0.1, max_new=max_new, max_length=max_length)
+        check_attention(out, q, store, table, le, starts, 0.1)
+
+
+def test_a_cache_steps_in_a_graph():
+    """Lengths on the GPU, columns cut and joined, and every replay the same as
+    the steps run eagerly; then eager sdpa calls beside a captured one."""
+    hq, hkv, d, b = 8, 2, 128, 2
+    caches = [S.PagedKVCache(n_requests=b, n_kv_heads=hkv, head_dim=d, max_tokens=4096, page_size=32)
+              for _ in range(2)]
+    given = [torch.zeros((b, h, d), dtype=torch.float16, device=DEV) for h in (hkv, hkv, hq)]
+    new, outs = ints([1] * b), [None, None]
+    for c in caches:
+        c.step(ints([2500, 2500]), 5000)
+        c.append(rows(1, 5000, hkv, d, torch.float16), rows(2, 5000, hkv, d, torch.float16, False))
+
+    def step(i):
+        caches[i].step(new, b, max_new=1)
+        caches[i].append(given[0], given[1])
+        outs[i] = caches[i].attend(given[2], 0.1)
+        return caches[i].sdpa(given[2].view(b, 1, hq, d).transpose(1, 2), 0.1)
+
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        last = step(1)
+    for i in range(6):
+        for j, h in enumerate((hkv, hkv, hq)):
+            given[j].copy_(rows(30 * j + i, b, h, d, torch.float16, j == 0))
+        step(0)
+        graph.replay()
+        torch.cuda.synchronize()
+        c = caches[1]
+        assert c.lengths.tolist() == [2501 + i] * b == caches[0].lengths.tolist()
+        starts = ints([0, 1, 2])
+        for out in (outs[0], outs[1], last.transpose(1, 2).reshape(b, hq, d)):
+            check_attention(out, given[2], c.store, c.block_table, c.lengths, starts, 0.1)
+        beside = c.sdpa(given[2].view(b, 1, hq, d).transpose(1, 2), 0.1)
+        check_attention(beside.transpose(1, 2).reshape(b, hq, d), given[2], c.store, c.block_table,
+                        c.lengths, starts, 0.1)
+        torch.empty(1 << 20, device=DEV).random_()
+
+
 def test_calls_on_other_streams():
     """Two streams at once over one store, each with its own workspace."""
     store, table, le, starts = world(14, [3000, 500], [1, 1], 2, 128, 64, 16, torch.float16)
@@ -603,6 +653,17 @@ def test_refusals_on_the_device():
 
 
 # ------------------------------------------------------------------- cache
+
+
+def test_a_trim_of_a_negative_number_gives_nothing_back():
+    c = S.PagedKVCache(n_requests=2, n_kv_heads=1, head_dim=64, max_tokens=64)
+    c.step([5, 9])
+    c.trim(-3)
+    assert c.lengths.tolist() == [5, 9]
+    c.step(ints([1, 1]), 2)
+    c.trim(-3)
+    c.trim(0)
+    assert c.lengths.tolist() == [6, 10]
 
 
 def test_cache_serves_requests_of_their_own_lengths():
