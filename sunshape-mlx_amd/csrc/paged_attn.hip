@@ -20,12 +20,14 @@ constexpr int kStages = 4;         // tiles of a wave in LDS, one computed while
 // Cache policy of the stream: non-temporal (8 requests of 32768 tokens: 66 us;
 // cached: 75 us.  1 request: 20.6 and 21.1 us).
 constexpr int kNt = 2;
-// Query rows a KV head up to which a request is this kernel's.  At 8192 tokens
-// and 64 (request, head) columns: 64 rows take 88 us here and 113 us in the
-// prompt kernel, 96 rows 131 and 114 us.  (8 columns fill the device only
-// here: 32 and 52 us at 96 rows, 83 and 74 us at 512; the rule is for the
-// fuller device.)
-constexpr int kPromptRows = 64;
+// Requests of more than kPromptRows query rows a KV head are the prompt
+// kernel's, where this one would have more than kPromptUnits units a compute
+// unit (twice that at 64 dims).  At 8192 tokens and 64 (request, head) columns
+// 64 rows take 88 us here and 113 us there, 96 rows 131 and 114 us.  Smaller
+// calls, here and there: a prompt of 128 tokens and 32 heads 8.8 and 21 us,
+// 512 tokens (16 units) 32 and 39, 640 tokens (25) 52 and 43; 24 tokens at
+// 8192 (12) 31 and 49 us; at 64 dims, 1024 tokens of 16 heads (32) 21 and 36.
+constexpr int kPromptRows = 64, kPromptUnits = 16;
 // Columns of at most kWhole units are not cut, twice that if there are enough
 // of them to give every second compute unit one: a cut adds a launch and a
 // pass over the parts.  1 request of 8 heads, 640 tokens: 9.8 us whole, 11.7
@@ -617,6 +619,7 @@ struct PagedPlan {
     int sets, rows, groups;  // column sets, query rows a workgroup takes; workgroups
     int columns;             // that there can be, at most `groups`
     bool cut;                // whether columns may be cut
+    bool prompts;            // whether requests of many rows are the prompt kernel's
     size_t bytes;
 };
 
@@ -626,17 +629,25 @@ static PagedPlan paged_plan(const ss_paged_store *s, int64_t n_tokens, int64_t n
                             int64_t max_new, int64_t max_length) {
     PagedPlan p;
     const int rep = n_q_heads / s->n_kv_heads, rs = 16 / (s->head_dim / s->group_size);
-    const int64_t rows = min(max_new * rep, (int64_t)kPromptRows);
+    int64_t rows = max_new * rep;
     p.sets = rows > rs ? 2 : 1;
     p.rows = p.sets * rs;
-    const double columns = (double)n_requests * s->n_kv_heads * ((rows + p.rows - 1) / p.rows);
     const int64_t units = (max_length + kUnit - 1) / kUnit;
+    // columns of requests of at most `rows` rows each
+    auto columns_of = [&](int64_t rows) {
+        return s->n_kv_heads * min((double)n_requests * ((rows + p.rows - 1) / p.rows),
+                                   (double)(n_tokens * rep / p.rows) + (double)n_requests);
+    };
+    p.prompts = rows > kPromptRows && columns_of(rows) * units * s->head_dim >
+                                           128. * kPromptUnits * device_cu_count();
+    if (p.prompts) rows = kPromptRows;
+    const double columns = columns_of(rows);
     p.cut = units > (2 * columns < device_cu_count() ? kWhole : 2 * kWhole);
     p.groups = (int)min((double)(2 * device_cu_count()), columns * (p.cut ? (double)units : 1.));
     p.groups = max(p.groups, 1);
     p.columns = (int)min(columns, (double)p.groups);
     p.bytes = p.cut ? 16 + (size_t)p.groups * (16 + 2 * p.rows * (s->head_dim + 2) * 4) : 0;
-    if (max_new * rep > kPromptRows)  // (one after the other: they share it)
+    if (p.prompts)  // (one after the other: they share it)
         p.bytes = max(p.bytes, paged_prompt_bytes(s, n_requests, n_tokens * rep, kPromptRows));
     return p;
 }
@@ -709,8 +720,7 @@ extern "C" int ss_paged_attn(const ss_paged_store *store, const void *q, int q_d
     a.hq = n_q_heads, a.rep = n_q_heads / store->n_kv_heads;
     a.q_dtype = q_dtype, a.causal = causal, a.zero_rest = zero_rest, a.scale = scale;
     a.vec = ((uintptr_t)q & 15) == 0 && q_st % 8 == 0 && q_sh % 8 == 0;
-    const bool prompts = max_new * a.rep > kPromptRows;
-    a.most_rows = prompts ? kPromptRows : INT32_MAX;
+    a.most_rows = p.prompts ? kPromptRows : INT32_MAX;
     a.cut = p.cut ? static_cast<int4 *>(workspace) : nullptr;
     a.acc = reinterpret_cast<float *>(a.cut + p.groups + 1);
     a.ml = a.acc + (size_t)p.groups * 2 * p.rows * store->head_dim;
@@ -723,5 +733,5 @@ extern "C" int ss_paged_attn(const ss_paged_store *store, const void *q, int q_d
     else if (key == 64032) bf ? launch_paged<64, 2, true>(a, p, st) : launch_paged<64, 2, false>(a, p, st);
     else bf ? launch_paged<64, 1, true>(a, p, st) : launch_paged<64, 1, false>(a, p, st);
     SS_LAUNCH_CHECK("paged_attn_kernel launch");
-    return prompts ? launch_paged_prompt(a, store, workspace, st) : SS_OK;
+    return p.prompts ? launch_paged_prompt(a, store, workspace, st) : SS_OK;
 }

@@ -68,10 +68,11 @@ def attend(q, store, table, lengths, starts, scale, causal=True, n_pages=None):
     the terms' magnitudes (first order).  exp2 and the running maximum add
     2^-21; the sums over tokens at most one rounding a 32-token tile and 64
     more.  A relative change e of every probability moves an output by 2 e
-    max|v|.  The output's own rounding is half a step of its type.  Up to 64
-    rows a KV head, p s is rounded to fp16 (2^-11) and multiplied by code -
-    7.5, as the difference of two sums of 64 p s and 72 p s; more rows round p
-    and the value itself, the value to at least 2^-18 of the largest of the
+    max|v|.  The output's own rounding is half a step of its type.  p s is
+    rounded to fp16 (2^-11) and multiplied by code - 7.5, as the difference of
+    two sums of 64 p s and 72 p s; more than 64 rows a KV head may take either
+    that way or, where the call's sizes make a large one, have p and the value
+    itself rounded, the value to at least 2^-18 of the largest of the
     request."""
     k_c, v_c, k_m, v_m = unpack(store)
     page = store[0].shape[2]
@@ -112,11 +113,11 @@ def attend(q, store, table, lengths, starts, scale, causal=True, n_pages=None):
                 b = ((qr.abs() @ kmag[see].t()) * scale).amax(-1, keepdim=True)
                 e = (d + 8) * 2.0 ** -24 * b + 2.0 ** -21 + (length / 32 + 64) * 2.0 ** -24
                 vmax = (vt[..., 0] * v_c[at, h] + vt[..., 1].abs())[see].amax(0)
-                if n * rep <= 64:
-                    half = 2.0 ** -11 * (p @ middle[see]) + \
-                        (length / 32 + 64) * 2.0 ** -24 * 152 * (p @ vt[see][..., 0])
-                else:
-                    half = 2.001 * 2.0 ** -11 * (p @ v[see].abs()) + 2.0 ** -18 * largest
+                half = 2.0 ** -11 * (p @ middle[see]) + \
+                    (length / 32 + 64) * 2.0 ** -24 * 152 * (p @ vt[see][..., 0])
+                if n * rep > 64:  # (either kernel's, as the call's size and hints decide)
+                    half = torch.maximum(
+                        half, 2.001 * 2.0 ** -11 * (p @ v[see].abs()) + 2.0 ** -18 * largest)
                 tol[row, h * rep:(h + 1) * rep] = u * o.abs() + half + 2 * e * vmax + \
                     2.0 ** -24 * (1 if q.dtype == torch.float16 else 2.0 ** -100)
     return out, tol

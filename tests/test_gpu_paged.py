@@ -572,6 +572,52 @@ def test_a_step_replays_from_a_graph():
     check_attention(other["out"], other["q"], other["store"], other["table"], other["lengths"], starts, 0.1)
 
 
+# ------------------------------------- the same, in a call that looks large
+
+
+@pytest.fixture
+def wide(monkeypatch):
+    """Tables of 2^20 tokens a row and no hint of the lengths: requests of many
+    rows go to the kernel that is for large calls."""
+    narrow = S.paged_attention
+
+    def call(q, store, table, lengths, starts, scale, *, max_length=None, **kw):
+        more = (1 << 20) // store.page_size - table.shape[1]
+        table = torch.nn.functional.pad(table, (0, more), value=-1)
+        return narrow(q, store, table, lengths, starts, scale, **kw)
+
+    monkeypatch.setattr(S, "paged_attention", call)
+
+
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("d,group", SHAPES)
+@pytest.mark.parametrize("lengths,new,hq,hkv,page",
+                         [c for c in CASES if max(c[1]) * c[2] // c[3] > 64] +
+                         [([500, 65], [400, 65], 4, 4, 16), ([1100], [1030], 2, 1, 64)])
+def test_large_attention(wide, lengths, new, hq, hkv, page, d, group, dtype):
+    test_attention(lengths, new, hq, hkv, page, d, group, dtype)
+
+
+def test_large_attention_without_a_causal_limit(wide):
+    test_attention_without_a_causal_limit(70)
+
+
+@pytest.mark.parametrize("step", [40.0, 600.0])
+def test_large_attention_with_scores_that_rise(wide, step):
+    test_attention_with_scores_that_rise_along_the_cache(step, 80)
+
+
+def test_large_attention_with_values_and_queries_of_all_sizes(wide):
+    test_attention_with_value_scales_of_all_sizes(40)
+    test_attention_with_queries_of_all_sizes(33)
+
+
+@pytest.mark.parametrize("dtype", HALF)
+def test_large_attention_and_what_a_row_does_not_see(wide, dtype):
+    test_what_a_row_does_not_see_does_not_reach_it(dtype, 50)
+    test_pages_outside_the_pool_hold_no_tokens((80, 40))
+
+
 @pytest.mark.parametrize("max_length", [100, 1100, 3000])
 def test_more_rows_than_the_hint_says(max_length):
     """Columns beyond those that the merge is launched for, cut and whole."""
