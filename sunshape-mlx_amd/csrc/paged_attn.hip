@@ -126,6 +126,11 @@ __device__ __forceinline__ float groups_sum(float v) {
 // through a ring of its own in LDS that HBM streams into while older tiles
 // are computed; their results are joined through LDS at the end.  NS sets of
 // 16/G query rows share the stream.
+//
+// Long caches are bound by HBM and, nearly as much, by the vector ALUs (65 % of
+// the cycles): 8 requests of up to 32768 tokens, 8 heads, 195 MB, take 41 us,
+// 4.7 TB/s.  One such request, 38 MB, takes 17 us: tables, queries, four tiles
+// a wave and the join follow each other.
 template <int D, int G, bool BF, int NS>
 __global__ void __launch_bounds__(256, 2) paged_attn_kernel(const PagedAttn a) {
     constexpr int RS = 16 / G;       // rows of a column set
