@@ -94,6 +94,15 @@ def test_append_calls_that_are_refused(n, dtype, keys, status):
                                                256, 128, FAKE, None) == status
 
 
+def test_more_tokens_than_a_launch_counts_are_refused():
+    """Pairs of (token, head) are counted in 32 bits when read back, blocks of
+    8 tokens of a head when written."""
+    lib, st = _hip.load_library(), store(n_kv_heads=1024, n_pages=64)
+    at = ctypes.addressof(st)
+    assert lib.ss_read_paged(at, FAKE, 1 << 21, FAKE, FAKE, None) == -2
+    assert lib.ss_append_paged(at, FAKE, FAKE, 1, 1 << 24, 256, 128, 256, 128, FAKE, None) == -2
+
+
 # ------------------------------------------------------------ Python layer
 
 
