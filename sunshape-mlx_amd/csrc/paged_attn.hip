@@ -149,11 +149,13 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(const PagedAttn a) {
     const int g = col % G;
     const bool in_group = quad * G / 4 == g;  // the lane's dims, and its rows of O, are in the column's group
     const int heads = a.st.heads, log_page = a.st.log_page;
-    if (a.zero_rest) {
-        const int64_t from = max(0, table_read(a.starts, a.n_req));
+    if (a.zero_rest) {  // the rows before the first request's, and those behind the last one's
         const int64_t row = (int64_t)a.hq * D;
-        for (int64_t e = from * row + blockIdx.x * 256 + threadIdx.x; e < a.n_tokens * row; e += gridDim.x * 256)
-            store_from_f32(a.out, a.q_dtype, e, 0.f);
+        const int64_t first = min((int64_t)max(0, table_read(a.starts, 0)), a.n_tokens) * row;
+        const int64_t last = min((int64_t)max(0, table_read(a.starts, a.n_req)), a.n_tokens) * row;
+        const int64_t theirs = max(last - first, (int64_t)0);
+        for (int64_t e = blockIdx.x * 256 + threadIdx.x; e < a.n_tokens * row - theirs; e += gridDim.x * 256)
+            store_from_f32(a.out, a.q_dtype, e < first ? e : e + theirs, 0.f);
     }
 
     // This workgroup's run of units [u, stop), and the request r it starts in,
