@@ -27,6 +27,7 @@ from functools import lru_cache
 from typing import NamedTuple
 
 import torch
+from torch.autograd import forward_ad as _forward_ad
 
 from . import _hip
 from .cache import DeferredTensor
@@ -296,7 +297,8 @@ def paged_attention(queries: torch.Tensor, store: PagedKVStore, block_table: tor
     if the caller knows them, size the launch (by default every request adds
     a token and a table row is full); wrong ones cost time and change roundings
     only.
-    Queries under autograd are refused: there is no backward pass."""
+    Queries under autograd, forward mode too, are refused: there is no
+    derivative."""
     st = _struct(store)
     dev = store[0].get_device()
     if queries.dim() != 3 or lengths.dim() != 1 or block_table.dim() != 2:
@@ -308,6 +310,8 @@ def paged_attention(queries: torch.Tensor, store: PagedKVStore, block_table: tor
         raise TypeError(f"queries must be float16 or bfloat16, not {dtype}")
     if queries.requires_grad and torch.is_grad_enabled():
         raise ValueError("paged_attention has no backward pass: call it under torch.no_grad()")
+    if _forward_ad._current_level >= 0 and _forward_ad.unpack_dual(queries).tangent is not None:
+        raise ValueError("paged_attention has no forward-mode derivative: unpack its dual queries")
     if hq < 1 or hq % st.n_kv_heads:
         raise ValueError(f"{hq} query heads do not share {st.n_kv_heads} KV heads")
     shape = (n, hq, st.head_dim)

@@ -237,3 +237,37 @@ def test_cache_steps_that_are_refused(on_cpu, monkeypatch):
         c.make_mask(1, return_array=True)
     with pytest.raises(TypeError):
         S.save_cache("/nonexistent", c)
+
+
+@pytest.mark.parametrize("shape", [(2, 4, 128), (0, 4, 128)])
+def test_queries_with_a_tangent_are_refused(on_cpu, shape):
+    """Forward mode: the kernel would drop the tangent.  Queries without one
+    pass, inside a level too."""
+    from torch.autograd import forward_ad
+
+    q = torch.zeros(shape, dtype=torch.float16)
+    n = shape[0]
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(q, torch.ones_like(q))
+        for grad in (True, False):  # (no_grad does not reach forward mode)
+            with torch.set_grad_enabled(grad), pytest.raises(ValueError, match="forward-mode"):
+                call(n=n, queries=dual)
+        if n:
+            with pytest.raises(Launched):
+                call(n=n, queries=q)
+            with pytest.raises(Launched):
+                call(n=n, queries=forward_ad.unpack_dual(dual).primal)
+
+
+def test_sdpa_queries_with_a_tangent_are_refused(on_cpu, monkeypatch):
+    from torch.autograd import forward_ad
+
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    c = S.PagedKVCache(n_requests=2, n_kv_heads=2, head_dim=128, max_tokens=100, device="cpu")
+    q = torch.zeros(2, 4, 1, 128, dtype=torch.float16)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(q, torch.ones_like(q))
+        with pytest.raises(ValueError, match="forward-mode"):
+            S.sunshape_sdpa(dual, c, 0.1, "causal")
+        with pytest.raises(Launched):
+            S.sunshape_sdpa(q, c, 0.1, "causal")
