@@ -13,8 +13,10 @@
 // product, of zero/64 - scale and the queries' sums, both split into bf16
 // parts.  Values are rounded to fp16 (2^-11 of a value, as the probabilities'
 // rounding costs), times a power of two a group that keeps the largest value
-// met below 2^-6: packed fp16 arithmetic takes a code as the subnormal code *
-// 2^-24, exactly, times scale * 2^18.  Statistics and sums are float32.
+// met below 2^15: values keep all 11 bits down to 2^-29 of it, and below that
+// are off by 2^-40 of it.  (Codes as they lie, fp16's subnormals, would save
+// 4 operations a word, but hold values below 2^-4 and cost those below 1/256
+// of the largest their bits.)  Statistics and sums are float32.
 //
 // The vector ALUs bound it (per 32 rows and 64 tokens: 2 x 32 products of
 // scale and sum, 32 exponentials), so what does not depend on the row is done
@@ -77,19 +79,24 @@ struct PromptTile {
     }
 };
 
-// A word's eight codes as fp16 subnormals: pairs (0,1) and (4,5) times 2^-24,
-// (2,3) and (6,7) times 2^-20.
-__device__ __forceinline__ half8_t codes_subnormal(uint32_t w) {
+// A word's eight codes as fp16 numbers, pairs (0,1) and (4,5) as they are, (2,3)
+// and (6,7) times 16: put into the low bits of 1024, which is taken off again.
+// (The constants as in CodeBits.)
+struct CodeNumber {
+    uint32_t low = 0x000f000fu, high = 0x00f000f0u, base = 0x64006400u;
+    __device__ CodeNumber() { asm volatile("" : "+s"(low), "+s"(high), "+v"(base)); }
+};
+__device__ __forceinline__ half8_t codes_number(uint32_t w, const CodeNumber &k) {
     union {
         uint32_t u[4];
         half8_t h;
     } x;
     const uint32_t hi = w >> 8;
-    x.u[0] = w & 0x000f000fu;
-    x.u[1] = w & 0x00f000f0u;
-    x.u[2] = hi & 0x000f000fu;
-    x.u[3] = hi & 0x00f000f0u;
-    return x.h;
+    x.u[0] = (w & k.low) | k.base;
+    x.u[1] = (w & k.high) | k.base;
+    x.u[2] = (hi & k.low) | k.base;
+    x.u[3] = (hi & k.high) | k.base;
+    return x.h - (_Float16)1024.f;
 }
 
 // Row tiles of a request that are this kernel's.
@@ -435,19 +442,20 @@ __global__ void __launch_bounds__(64 * kPWaves, 2) paged_prompt_kernel(const Pag
             int e = __builtin_amdgcn_readfirstlane(vnext[0]);
 #pragma unroll
             for (int g = 1; g < G; ++g) e = vg == g ? __builtin_amdgcn_readfirstlane(vnext[g]) : e;
-            const float fs = exp2i(18 - e), fz = ldexpf(1.f, -6 - e), fs_odd = fs * 0x1p-4f;
+            const float up = exp2i(15 - e), up_odd = exp2i(11 - e);  // (-60 <= e <= 126)
+            const CodeNumber number;
             half8_t sc, ze;  // codes of odd pairs count 16 times
 #pragma unroll
             for (int i = 0; i < 8; i += 2) {
-                const float f = (i & 2) ? fs_odd : fs;
+                const float f = (i & 2) ? up_odd : up;
                 const half2_t s2 = __builtin_convertvector(float2_t{low16<BF>(vm[i]) * f, low16<BF>(vm[i + 1]) * f}, half2_t);
-                const half2_t z2 = __builtin_convertvector(float2_t{high16<BF>(vm[i]) * fz, high16<BF>(vm[i + 1]) * fz}, half2_t);
+                const half2_t z2 = __builtin_convertvector(float2_t{high16<BF>(vm[i]) * up, high16<BF>(vm[i + 1]) * up}, half2_t);
                 sc[i] = s2[0], sc[i + 1] = s2[1], ze[i] = z2[0], ze[i + 1] = z2[1];
             }
 #pragma unroll
             for (int k = 0; k < VW; ++k)  // dim NT * m + j at place 32 j + m
                 *reinterpret_cast<half8_t *>(out + PT::kOperands + (wave * D + 32 * (j0 + k) + col) * 16) =
-                    __builtin_elementwise_fma(codes_subnormal(vw[k]), sc, ze);
+                    __builtin_elementwise_fma(codes_number(vw[k], number), sc, ze);
         };
 
         // One tile: computed from `cur`; the next one prepared from `next` into
@@ -599,7 +607,7 @@ __global__ void __launch_bounds__(64 * kPWaves, 2) paged_prompt_kernel(const Pag
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
                     const int m = 8 * (i / 4) + 4 * half + i % 4;
-                    const int e = vexp[group_of(i)] + 6;
+                    const int e = vexp[group_of(i)] - 15;
                     if constexpr (NT == 4) {
                         store_out4(a, at + NT * m, ldexpf(o[0][i] * inv, e), ldexpf(o[1][i] * inv, e),
                                    ldexpf(o[2][i] * inv, e), ldexpf(o[3][i] * inv, e));
@@ -617,7 +625,7 @@ __global__ void __launch_bounds__(64 * kPWaves, 2) paged_prompt_kernel(const Pag
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
                 const int m = 8 * (i / 4) + 4 * half + i % 4;
-                const int e = vexp[group_of(i)] + 6;
+                const int e = vexp[group_of(i)] - 15;
 #pragma unroll
                 for (int j = 0; j < NT; ++j) a.acc[at * D + NT * m + j] = ldexpf(o[j][i], e);
             }

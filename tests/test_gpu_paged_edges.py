@@ -4,9 +4,10 @@ against the 64-bit restatement (tests/paged_reference.py)."""
 
 import math
 
+import paged_reference as R
 import pytest
 import torch
-from test_gpu_paged import DEV, check_attention, ints, rows, world
+from test_gpu_paged import DEV, HALF, check_attention, fresh, ints, rows, wide, world  # noqa: F401
 
 import sunshape_mlx_amd as S
 
@@ -39,3 +40,45 @@ def test_rows_before_the_first_request_are_zero(new):
     # starts past the queries: no request has a row, so all are zero
     poisoned(q.shape, q.dtype)
     assert (S.paged_attention(q, store, table, le, starts + 10 ** 6, 0.125) == 0).all()
+
+
+def beside_a_large_value(dtype, factor, new, d=64, group=32, n=300):
+    """(call arguments, the output in 64 bits, the scale of its values'
+    groups) of rows that rest on one ordinary token, 2^-40 of them on each of
+    the others, one of which, in another tile, holds `factor` times the
+    ordinary values."""
+    g = [rows(40 + i, n, 1, d, torch.float32, False) for i in range(2)]
+    k = torch.zeros((n, 1, d), device=DEV)
+    k[150, 0, 0] = 1.0
+    v = g[0].to(dtype)
+    v[9] = (g[1][9] * factor).to(dtype)
+    store = fresh(dtype, 19, 1, d, group, 16)
+    S.append_paged(store, k.to(dtype), v, torch.arange(n, dtype=torch.int32, device=DEV))
+    table = torch.arange(19, dtype=torch.int32, device=DEV)[None]
+    q = torch.zeros((new, 4, d), dtype=dtype, device=DEV)
+    q[..., 0] = 8.0
+    args = (q, store, table, ints([n]), ints([0, new]), 5 * math.log(2))
+    scale = R.unpack(store)[3][150, 0, :, 0].double().repeat_interleave(group)
+    return args, R.attend(*args)[0], scale
+
+
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("factor", [64.0, 256.0, 1000.0])
+def test_ordinary_values_keep_their_bits_beside_a_large_one(factor, dtype):
+    """p scale is rounded to fp16 (2^-11) and meets code - 7.5; 299 tokens of
+    2^-40, one of them `factor` times as large as 4, are below 2^-28."""
+    args, want, scale = beside_a_large_value(dtype, factor, 2)
+    err = (S.paged_attention(*args).cpu().double() - want).abs()
+    assert (err <= (R.U16[dtype] + 2.0 ** -20) * want.abs() + 2.0 ** -11 * 7.5 * scale + 2.0 ** -24).all()
+
+
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("factor", [64.0, 256.0, 1000.0])
+@pytest.mark.parametrize("d,group", [(64, 32), (128, 64), (128, 128), (128, 32), (64, 64)])
+def test_large_attention_and_ordinary_values_beside_a_large_one(wide, d, group, factor, dtype):
+    """The probability and the value are rounded to fp16, 2^-11 of each and
+    their product 2^-22 more."""
+    args, want, _ = beside_a_large_value(dtype, factor, 80, d, group)
+    err = (S.paged_attention(*args).cpu().double() - want).abs()
+    assert (err <= (R.U16[dtype] + 2.001 * 2.0 ** -11) * want.abs() + 2.0 ** -24).all(), \
+        f"{float((err / want.abs().clamp(min=1e-3)).max()):.1e}"
