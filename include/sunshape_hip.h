@@ -1103,6 +1103,12 @@ int ss_read_paged(const ss_paged_store *store, const int32_t *slots, int64_t n_t
  * length) size the launch: wrong ones change roundings only.  workspace:
  * ss_paged_attn_workspace_bytes of the same arguments, uninitialised, not
  * shared with a call that may run at the same time.
+ * Limits: n_tokens * n_q_heads below 2^31, a table row of at most 2^30 tokens,
+ * at most 1024 query heads and 65535 requests; and, as blocks of 128 tokens
+ * are counted in 32 bits, b * n_kv_heads * table_width * page_size / 128 below
+ * 2^31, where b, blocks of query rows, is at most one a request that has
+ * tokens and one more in four rows of a KV head (n_tokens * n_q_heads /
+ * n_kv_heads), and at most 16 a request.
  */
 size_t ss_paged_attn_workspace_bytes(const ss_paged_store *store, int64_t n_tokens,
                                      int64_t n_requests, int n_q_heads, int64_t max_new,

@@ -659,14 +659,26 @@ static PagedPlan paged_plan(const ss_paged_store *s, int64_t n_tokens, int64_t n
     return p;
 }
 
+// Units that tables of this width can ask of the decode kernel, which counts
+// them in 32 bits: a request of r rows, up to kPromptRows with the prompt
+// kernel beside it, is (r + rows - 1) / rows blocks.
+constexpr double kCounted = 2147483648.0;
+static double most_units(const ss_paged_store *s, const PagedPlan &p, int64_t n_tokens, int64_t n_requests, int rep,
+                         int64_t table_width) {
+    const double requests = (double)min(n_requests, n_tokens);
+    double blocks = requests + (double)n_tokens * rep / p.rows;
+    if (p.prompts) blocks = min(blocks, requests * ((kPromptRows + p.rows - 1) / p.rows));
+    return blocks * s->n_kv_heads * (double)((table_width * s->page_size + kUnit - 1) / kUnit);
+}
+
 static int check_hints(const ss_paged_store *s, int64_t n_requests, int n_q_heads, int64_t max_new,
                        int64_t max_length) {
     SS_REQUIRE(n_requests >= 1 && n_requests <= 65535, "n_requests must be 1 .. 65535");
     SS_REQUIRE(n_q_heads >= 1 && n_q_heads % s->n_kv_heads == 0,
                "query heads must be a multiple of the KV heads");
     SS_UNSUPPORTED(n_q_heads <= 1024, "more than 1024 query heads");
-    SS_REQUIRE(max_new >= 1 && max_new <= INT32_MAX / 1024 && max_length >= 1 && max_length <= INT32_MAX,
-               "max_new and max_length must be positive");
+    SS_REQUIRE(max_new >= 1 && max_new <= INT32_MAX && max_length >= 1 && max_length <= INT32_MAX,
+               "max_new and max_length must be 1 .. 2^31 - 1");
     return SS_OK;
 }
 
@@ -710,12 +722,14 @@ extern "C" int ss_paged_attn(const ss_paged_store *store, const void *q, int q_d
     SS_REQUIRE(((uintptr_t)out & 7) == 0, "out must be 8-byte aligned");
     SS_REQUIRE(table_width >= 1, "bad block table width");
     SS_UNSUPPORTED(table_width <= (1 << 30) / store->page_size, "a table row of more than 2^30 tokens");
-    // every unit of every column is counted in 32 bits
-    SS_UNSUPPORTED(((double)n_requests + (double)n_tokens * (n_q_heads / store->n_kv_heads)) * store->n_kv_heads *
-                           ((double)table_width * store->page_size / kUnit + 1) <
-                       2147483648.0,
-                   "too many requests and tokens for one launch");
-    const PagedPlan p = paged_plan(store, n_tokens, n_requests, n_q_heads, max_new, max_length);
+    PagedPlan p = paged_plan(store, n_tokens, n_requests, n_q_heads, max_new, max_length);
+    // (hints that are too low for the tables)
+    const int rep = n_q_heads / store->n_kv_heads;
+    p.prompts |= most_units(store, p, n_tokens, n_requests, rep, table_width) >= kCounted;
+    SS_UNSUPPORTED(most_units(store, p, n_tokens, n_requests, rep, table_width) < kCounted,
+                   "%lld requests, %lld tokens and %lld pages a table row: more blocks of query rows and of %d tokens "
+                   "than 32 bits count",
+                   (long long)n_requests, (long long)n_tokens, (long long)table_width, kUnit);
     if (p.bytes > workspace_bytes || (p.bytes && !workspace)) {
         set_error("workspace of %zu bytes, %zu needed", workspace_bytes, p.bytes);
         return SS_ERR_WORKSPACE;
@@ -724,7 +738,7 @@ extern "C" int ss_paged_attn(const ss_paged_store *store, const void *q, int q_d
     a.q = q, a.q_st = q_st, a.q_sh = q_sh, a.out = out;
     a.table = block_table, a.lengths = lengths, a.starts = token_starts;
     a.width = table_width, a.n_tokens = n_tokens, a.n_req = (int)n_requests;
-    a.hq = n_q_heads, a.rep = n_q_heads / store->n_kv_heads;
+    a.hq = n_q_heads, a.rep = rep;
     a.q_dtype = q_dtype, a.causal = causal, a.zero_rest = zero_rest, a.scale = scale;
     a.vec = ((uintptr_t)q & 15) == 0 && q_st % 8 == 0 && q_sh % 8 == 0;
     a.most_rows = p.prompts ? kPromptRows : INT32_MAX;
@@ -740,5 +754,5 @@ extern "C" int ss_paged_attn(const ss_paged_store *store, const void *q, int q_d
     else if (key == 64032) bf ? launch_paged<64, 2, true>(a, p, st) : launch_paged<64, 2, false>(a, p, st);
     else bf ? launch_paged<64, 1, true>(a, p, st) : launch_paged<64, 1, false>(a, p, st);
     SS_LAUNCH_CHECK("paged_attn_kernel launch");
-    return p.prompts ? launch_paged_prompt(a, store, workspace, st) : SS_OK;
+    return p.prompts ? launch_paged_prompt(a, store, workspace, workspace_bytes, st) : SS_OK;
 }

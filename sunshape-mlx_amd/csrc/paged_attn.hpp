@@ -169,8 +169,10 @@ __device__ __forceinline__ float column_max(const float (&x)[N]) {
 }
 
 // The requests with more than most_rows query rows a KV head (paged_prompt.hip),
-// with `workspace` of paged_prompt_bytes for n_tokens * rep rows in all.
+// with `workspace` of paged_prompt_bytes for n_tokens * rep rows in all (with
+// less no column is cut).
 size_t paged_prompt_bytes(const ss_paged_store *s, int64_t n_requests, int64_t rows, int most_rows);
-int launch_paged_prompt(PagedAttn a, const ss_paged_store *s, void *workspace, hipStream_t st);
+int launch_paged_prompt(PagedAttn a, const ss_paged_store *s, void *workspace, size_t workspace_bytes,
+                        hipStream_t st);
 
 }  // namespace ss

@@ -686,12 +686,14 @@ size_t paged_prompt_bytes(const ss_paged_store *s, int64_t n_requests, int64_t r
     return (size_t)cut_target(n_requests, s->n_kv_heads, rows, most_rows) * (16 + kRows * (s->head_dim + 2) * 4);
 }
 
-int launch_paged_prompt(PagedAttn a, const ss_paged_store *s, void *workspace, hipStream_t st) {
+int launch_paged_prompt(PagedAttn a, const ss_paged_store *s, void *workspace, size_t workspace_bytes,
+                        hipStream_t st) {
     // at most this many row tiles: whole ones, and one a request of more than most_rows rows
     const int64_t rows = a.n_tokens * a.rep;
     const int64_t tiles = rows / kRows + min((int64_t)a.n_req, rows / (a.most_rows + 1));
     if (tiles == 0) return SS_OK;
     a.target = cut_target(a.n_req, a.st.heads, rows, a.most_rows);
+    if (paged_prompt_bytes(s, a.n_req, rows, a.most_rows) > workspace_bytes) a.target = 0;
     a.cut = a.target ? static_cast<int4 *>(workspace) : nullptr;
     a.acc = reinterpret_cast<float *>(a.cut + a.target);
     a.ml = a.acc + (size_t)a.target * kRows * s->head_dim;

@@ -82,3 +82,30 @@ def test_large_attention_and_ordinary_values_beside_a_large_one(wide, d, group, 
     err = (S.paged_attention(*args).cpu().double() - want).abs()
     assert (err <= (R.U16[dtype] + 2.001 * 2.0 ** -11) * want.abs() + 2.0 ** -24).all(), \
         f"{float((err / want.abs().clamp(min=1e-3)).max()):.1e}"
+
+
+def check_some_rows(out, q, store, table, lengths, starts, scale, some, bound=2.0 ** -9):
+    """Rows (request, new token, KV head) against the 64-bit form: relative
+    L2 error of each query head.  fp16: 2^-11 each of the output, the
+    probabilities and the values is below 2^-9."""
+    rep = q.shape[1] // store.n_kv_heads
+    at, le = starts.tolist(), lengths.tolist()
+    for r, i, h in some:
+        row, n, heads = at[r] + i, at[r + 1] - at[r], slice(h * rep, (h + 1) * rep)
+        one = S.PagedKVStore(*(t[:, h:h + 1] for t in store))
+        want, _ = R.attend(q[row:row + 1, heads], one, table[r:r + 1], ints([le[r] - n + i + 1]), ints([0, 1]), scale)
+        err = (out[row:row + 1, heads].cpu().double() - want).norm(dim=-1)
+        assert (err <= bound * want.norm(dim=-1)).all(), (r, i, h, float((err / want.norm(dim=-1)).max()))
+
+
+@pytest.mark.parametrize("n,hq,hkv,d,max_new", [(33001, 8, 2, 128, None), (32768, 64, 64, 64, 1)])
+def test_long_prompts_in_tables_of_many_pages(n, hq, hkv, d, max_new):
+    """Prompts in tables of 2^20 tokens a row, with and without the hint that
+    there are many rows."""
+    page = 128
+    store, table, le, starts = world(51, [n], [n], hkv, d, 64, page, torch.float16)
+    table = torch.nn.functional.pad(table, (0, 2 ** 20 // page - table.shape[1]), value=-1)
+    q = rows(52, n, hq, d, torch.float16, False)
+    out = S.paged_attention(q, store, table, le, starts, d ** -0.5, max_new=max_new)
+    some = [(0, i, h) for i in (0, 5, 130, n // 2, n - 1) for h in (0, hkv - 1)]
+    check_some_rows(out, q, store, table, le, starts, d ** -0.5, some)

@@ -271,3 +271,37 @@ def test_sdpa_queries_with_a_tangent_are_refused(on_cpu, monkeypatch):
             S.sunshape_sdpa(dual, c, 0.1, "causal")
         with pytest.raises(Launched):
             S.sunshape_sdpa(q, c, 0.1, "causal")
+
+
+def sized(n, r, tokens, hq=32, hkv=8, page=64, max_new=None, max_length=None, **kw):
+    """Status of a call of these sizes that has no workspace: -4 where the
+    sizes are taken."""
+    return attention(store(n_kv_heads=hkv, page_size=page, **kw), n=n, r=r, hq=hq, width=tokens // page,
+                     max_new=max_new or n - r + 1, max_length=max_length or tokens)
+
+
+@pytest.mark.parametrize("n,r,tokens,hq", [
+    # prompts and chunks of tables that hold 131072 and 2^20 tokens a row
+    (65536, 1, 131072, 32), (65536, 16, 131072, 32), (65536, 32, 131072, 32), (131072, 1, 131072, 32),
+    (32768, 1, 131072, 64), (32768, 8, 131072, 64), (92161, 1, 131072, 32), (8192, 1, 1 << 20, 32),
+    (1 << 20, 1, 1 << 20, 32), (1 << 22, 1, 1 << 22, 32), (3000, 1000, 1 << 20, 32), (1000, 1000, 1 << 20, 32),
+    (4096, 4096, 131072, 32), (65535, 65535, 16384, 32),
+])
+@pytest.mark.parametrize("group", [32, 64, 128])
+def test_prompts_and_batches_that_are_taken(n, r, tokens, hq, group):
+    assert sized(n, r, tokens, hq, group_size=group) == -4
+    # hints that are too low for these tables cost time, not the call
+    assert sized(n, r, tokens, hq, group_size=group, max_new=1) == -4
+
+
+def test_counts_past_32_bits_are_refused():
+    """128 requests of one row a KV head, 8 rows a block: at most 128 + 128/8
+    blocks of rows, over as many blocks of 128 tokens as fit 32 bits, and one more."""
+    for heads in (2, 4):
+        most = (2 ** 31 - 1) // ((128 + 16) * heads)
+        for blocks, status in ((most, -4), (most + 1, -2)):
+            assert sized(128, 128, blocks * 128, heads, heads, page=16, max_new=1) == status
+    # the decode kernel's part of many long prompts: 16 blocks a request at most
+    assert sized(1 << 20, 1000, 1 << 20, group_size=32) == -4
+    assert sized(1 << 20, 4097, 1 << 20, group_size=32) == -2
+    assert b"32 bits" in _hip.load_library().ss_last_error()
