@@ -396,14 +396,15 @@ class PagedKVCache:
         int32 tensor on the GPU needs ``n_tokens``, at least the sum of what is
         added (``max_new``, the most one adds, sizes later launches); whether
         the step was possible is then seen by ``check``."""
+        host, bound = None, self._bound
         if isinstance(new_lengths, torch.Tensor):
             if n_tokens is None:
                 raise ValueError("n_tokens is required with new_lengths on the GPU")
-            new, self._host = new_lengths, None
+            new = new_lengths
             most = min(n_tokens, n_tokens if max_new is None else max_new)
-            self._bound = min(self.max_tokens, self._bound + max(0, most))
+            bound = min(self.max_tokens, bound + max(0, most))
             if torch.cuda.is_current_stream_capturing():  # (replays add to the lengths too)
-                self._bound = self.max_tokens
+                bound = self.max_tokens
         else:
             adds = [int(x) for x in new_lengths]
             if len(adds) != self.n_requests:
@@ -414,19 +415,21 @@ class PagedKVCache:
             n_tokens = total if n_tokens is None else n_tokens
             most = max(adds)
             if self._host is not None:
-                after = [n + x for n, x in zip(self._host, adds)]
-                pages = sum(-(-n // self.page_size) for n in after)
-                if min(after) < 0 or max(after) > self.max_tokens:
-                    raise ValueError(f"lengths {after} are not within 0 .. {self.max_tokens}")
+                host = [n + x for n, x in zip(self._host, adds)]
+                pages = sum(-(-n // self.page_size) for n in host)
+                if min(host) < 0 or max(host) > self.max_tokens:
+                    raise ValueError(f"lengths {host} are not within 0 .. {self.max_tokens}")
                 if pages > self.free_pages.shape[0]:
                     raise RuntimeError(f"{pages} pages needed, {self.free_pages.shape[0]} there")
-                self._host, self._bound = after, max(after)
+                bound = max(host)
             else:
-                self._bound = min(self.max_tokens, self._bound + max(0, most))
+                bound = min(self.max_tokens, bound + max(0, most))
             new = torch.tensor(adds, dtype=torch.int32).to(self.lengths.device)
         plan = build_block_tables(self.lengths, new, self.block_table, self.free_pages,
                                   self.n_free, self.page_size, n_tokens,
                                   lengths_out=self.lengths, n_free_out=self.n_free)
+        # (only now: a step that was refused has changed nothing here either)
+        self._host, self._bound = host, bound
         self.plan, self._max_new = plan, max(1, most)
         self._version += 1
         return plan

@@ -305,3 +305,37 @@ def test_counts_past_32_bits_are_refused():
     assert sized(1 << 20, 1000, 1 << 20, group_size=32) == -4
     assert sized(1 << 20, 4097, 1 << 20, group_size=32) == -2
     assert b"32 bits" in _hip.load_library().ss_last_error()
+
+
+def known(c):
+    """What a cache knows on the host."""
+    return c._host, c._bound, c._max_new, c._version, c.plan
+
+
+def small_cache(**kw):
+    f = dict(n_requests=2, n_kv_heads=2, head_dim=128, max_tokens=100, page_size=32, device="cpu")
+    f.update(kw)
+    return S.PagedKVCache(**f)
+
+
+@pytest.mark.parametrize("step", [
+    lambda c: c.step(torch.tensor([1, 1]), 2), lambda c: c.step(ints(1), 2), lambda c: c.step(ints(1, 1, 1), 3),
+    lambda c: c.step(ints(1, 2)[::2], 2), lambda c: c.step(ints(1, 1), -1), lambda c: c.step(ints(1, 1)),
+    lambda c: c.step([1, 1], 1), lambda c: c.step([1, "x"]), lambda c: c.step([200, 0]), lambda c: c.step([1, 1]),
+    lambda c: c.step(ints(1, 1), 2), lambda c: c.trim(1), lambda c: c.release([0]),
+])
+def test_steps_that_fail_leave_the_cache_as_it_was(on_cpu, monkeypatch, step):
+    """Refused arguments, and launches that raise."""
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    refuse = paged._launch
+    c = small_cache()
+    monkeypatch.setattr(paged, "_launch", lambda *a: None)
+    c.step([5, 3])
+    c.step([-2, 1])
+    monkeypatch.setattr(paged, "_launch", refuse)
+    before = known(c)
+    assert before[:3] == ([3, 4], 4, 1)
+    with pytest.raises((ValueError, TypeError, Launched)):
+        step(c)
+    assert known(c) == before
+    assert c.plan is before[-1]
