@@ -170,6 +170,11 @@ def _launch(name: str, dev: int, *args) -> None:
     _hip._launched(_STATS[name], rc)
 
 
+def _capturing(t: torch.Tensor) -> bool:
+    """Whether calls on this tensor go into a graph."""
+    return t.is_cuda and torch.cuda.is_current_stream_capturing()
+
+
 def build_block_tables(lengths: torch.Tensor, new_lengths: torch.Tensor,
                        block_table: torch.Tensor, free_pages: torch.Tensor,
                        n_free: torch.Tensor, page_size: int, n_tokens: int, *,
@@ -392,10 +397,11 @@ class PagedKVCache:
              max_new: int | None = None) -> BlockPlan:
         """Schedule a step in which request r adds ``new_lengths[r]`` tokens
         (negative: gives its last ones back; minus its length: ends).  A list
-        of ints is checked here and raises when the step is impossible.  An
-        int32 tensor on the GPU needs ``n_tokens``, at least the sum of what is
-        added (``max_new``, the most one adds, sizes later launches); whether
-        the step was possible is then seen by ``check``."""
+        of ints is checked here and raises when the step is impossible; it
+        cannot be captured.  An int32 tensor on the GPU needs ``n_tokens``, at
+        least the sum of what is added (``max_new``, the most one adds, sizes
+        later launches); whether the step was possible is then seen by
+        ``check``."""
         host, bound = None, self._bound
         if isinstance(new_lengths, torch.Tensor):
             if n_tokens is None:
@@ -403,9 +409,12 @@ class PagedKVCache:
             new = new_lengths
             most = min(n_tokens, n_tokens if max_new is None else max_new)
             bound = min(self.max_tokens, bound + max(0, most))
-            if torch.cuda.is_current_stream_capturing():  # (replays add to the lengths too)
+            if _capturing(self.lengths):  # (replays add to the lengths too)
                 bound = self.max_tokens
         else:
+            if _capturing(self.lengths):
+                raise RuntimeError("a step given as a list cannot be captured (its replays would not "
+                                   "reach the host's lengths): give new_lengths on the GPU")
             adds = [int(x) for x in new_lengths]
             if len(adds) != self.n_requests:
                 raise ValueError(f"{len(adds)} lengths for {self.n_requests} requests")
@@ -521,7 +530,7 @@ class PagedKVCache:
         if b_ != self.n_requests:
             raise ValueError(f"queries of {b_} sequences, {self.n_requests} requests")
         dev = self.lengths.device
-        if torch.cuda.is_current_stream_capturing():  # (the graph's own, filled by its replays)
+        if _capturing(self.lengths):  # (the graph's own, filled by its replays)
             starts = torch.arange(b_ + 1, dtype=torch.int32, device=dev) * t_
         else:
             if self._starts is None or self._starts[0] != t_:

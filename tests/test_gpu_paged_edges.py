@@ -109,3 +109,18 @@ def test_long_prompts_in_tables_of_many_pages(n, hq, hkv, d, max_new):
     out = S.paged_attention(q, store, table, le, starts, d ** -0.5, max_new=max_new)
     some = [(0, i, h) for i in (0, 5, 130, n // 2, n - 1) for h in (0, hkv - 1)]
     check_some_rows(out, q, store, table, le, starts, d ** -0.5, some)
+
+
+@pytest.mark.filterwarnings("ignore:The CUDA Graph is empty")
+def test_a_list_step_in_a_capture_is_refused():
+    """The capture ends, cache and device go on."""
+    c = S.PagedKVCache(n_requests=2, n_kv_heads=1, head_dim=64, max_tokens=64)
+    c.step([5, 9])
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="captured"):
+        with torch.cuda.graph(graph):
+            c.step([1, 1])
+    assert c._host == [5, 9]
+    c.step([1, 2])
+    assert c.lengths.tolist() == [6, 11] == c._host

@@ -339,3 +339,19 @@ def test_steps_that_fail_leave_the_cache_as_it_was(on_cpu, monkeypatch, step):
         step(c)
     assert known(c) == before
     assert c.plan is before[-1]
+
+
+def test_steps_given_as_lists_are_not_captured(on_cpu, monkeypatch):
+    launch = paged._launch
+    c = small_cache()
+    monkeypatch.setattr(paged, "_launch", lambda *a: None)
+    c.step([5, 5])
+    monkeypatch.setattr(paged, "_launch", launch)
+    monkeypatch.setattr(paged, "_capturing", lambda t: True)
+    before = known(c)
+    z = torch.zeros(2, 2, 1, 128, dtype=torch.float16)
+    for call_ in (lambda: c.step([1, 1]), lambda: c.trim(1), lambda: c.release([0]),
+                  lambda: c.update_and_fetch(z, z)):
+        with pytest.raises(RuntimeError, match="captured"):
+            call_()
+        assert known(c) == before
