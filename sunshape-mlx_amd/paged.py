@@ -241,6 +241,14 @@ def _rows(name: str, t: torch.Tensor, shape, dev: int) -> torch.Tensor:
     return t if t.stride(2) == 1 else t.contiguous()
 
 
+def _new_rows(keys: torch.Tensor, values: torch.Tensor, shape, dev: int):
+    """(keys, values, type code) of new tokens, as the append takes them."""
+    if keys.dtype is not values.dtype:
+        raise TypeError("keys and values must share a dtype")
+    code = _hip.dtype_code(keys.dtype)
+    return _rows("keys", keys, shape, dev), _rows("values", values, shape, dev), code
+
+
 def append_paged(store: PagedKVStore, keys: torch.Tensor, values: torch.Tensor,
                  slots: torch.Tensor) -> None:
     """Quantise ``keys`` and ``values`` (N, H, D), float16, bfloat16 or
@@ -251,11 +259,7 @@ def append_paged(store: PagedKVStore, keys: torch.Tensor, values: torch.Tensor,
     dev = store[0].get_device()
     n = slots.shape[0]
     at_slots = _index("slots", slots, (n,), dev)
-    if keys.dtype is not values.dtype:
-        raise TypeError("keys and values must share a dtype")
-    code = _hip.dtype_code(keys.dtype)
-    shape = (n, st.n_kv_heads, st.head_dim)
-    k, v = _rows("keys", keys, shape, dev), _rows("values", values, shape, dev)
+    k, v, code = _new_rows(keys, values, (n, st.n_kv_heads, st.head_dim), dev)
     _launch("ss_append_paged", dev, ctypes.addressof(st), k.data_ptr(), v.data_ptr(), code, n,
             k.stride(0), k.stride(1), v.stride(0), v.stride(1), at_slots)
 
@@ -497,9 +501,12 @@ class PagedKVCache:
                 values.shape != keys.shape:
             raise ValueError(f"keys and values must be ({self.n_requests}, {self.n_kv_heads}, T, "
                              f"{self.head_dim}), got {tuple(keys.shape)}, {tuple(values.shape)}")
-        self.step([t_] * b_)
         rows = (b_ * t_, h_, d)
-        self.append(keys.transpose(1, 2).reshape(rows), values.transpose(1, 2).reshape(rows))
+        # refused before the requests grow
+        k, v, _ = _new_rows(keys.transpose(1, 2).reshape(rows), values.transpose(1, 2).reshape(rows),
+                            rows, self.lengths.get_device())
+        self.step([t_] * b_)
+        self.append(k, v)
         if self._host is None or min(self._host) != max(self._host):
             return None, None
         shape = (b_, h_, self._host[0], d)

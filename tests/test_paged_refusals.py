@@ -355,3 +355,30 @@ def test_steps_given_as_lists_are_not_captured(on_cpu, monkeypatch):
         with pytest.raises(RuntimeError, match="captured"):
             call_()
         assert known(c) == before
+
+
+@pytest.mark.parametrize("k,v", [
+    (torch.float16, torch.float32), (torch.float64, torch.float64), (torch.int32, torch.int32), ("meta", None),
+    (None, "meta"),
+])
+def test_updates_that_are_refused_add_no_tokens(monkeypatch, k, v):
+    """Types that the append does not take, keys or values on another device."""
+    def one_device(*tensors):
+        if any(t.is_meta for t in tensors):
+            raise ValueError("another device")
+
+    monkeypatch.setattr(_hip, "require_gpu", one_device)
+    monkeypatch.setattr(paged, "_launch", lambda *a: None)
+    c = small_cache()
+    c.step([5, 5])
+    before = known(c)
+    good = torch.zeros(2, 2, 3, 128, dtype=torch.float16)
+
+    def other(x):
+        return good if x is None else good.to("meta") if x == "meta" else good.to(x)
+
+    with pytest.raises((ValueError, TypeError)):
+        c.update_and_fetch(other(k), other(v))
+    assert known(c) == before
+    c.update_and_fetch(good, good)
+    assert c.offset == 8
