@@ -33,6 +33,7 @@ from . import _hip
 from .cache import DeferredTensor
 
 _HALF = (torch.float16, torch.bfloat16)
+_MAX_REQUESTS = 4096  # of build_block_tables
 
 
 class _Store(ctypes.Structure):
@@ -74,6 +75,9 @@ class PagedKVStore(NamedTuple):
             raise ValueError(f"page_size must be a power of two from 16 to 1024, got {page_size}")
         if n_pages < 1 or n_kv_heads < 1:
             raise ValueError("n_pages and n_kv_heads must be positive")
+        if max(n_pages * page_size, n_pages * n_kv_heads) >= 2 ** 31:
+            raise ValueError(f"a pool of {n_pages} pages of {page_size} tokens and {n_kv_heads} heads: "
+                             f"slots, and heads of pages, are counted in 32 bits")
         dev = torch.device("cuda") if device is None else torch.device(device)
         meta = (n_pages, n_kv_heads, head_dim // group_size, page_size, 2)
         return cls(
@@ -374,7 +378,12 @@ class PagedKVCache:
                  lazy_fetch: bool = True):
         if n_requests < 1 or max_tokens < 1:
             raise ValueError("n_requests and max_tokens must be positive")
-        width = -(-max_tokens // page_size)
+        if n_requests > _MAX_REQUESTS or max_tokens > 2 ** 30:
+            raise ValueError(f"at most {_MAX_REQUESTS} requests of at most 2^30 tokens (got "
+                             f"{n_requests}, {max_tokens})")
+        width = -(-max_tokens // max(1, page_size))
+        if n_requests * width >= 2 ** 31:
+            raise ValueError(f"a block table of {n_requests} rows of {width} pages")
         n_pages = n_requests * width if n_pages is None else n_pages
         self.store = PagedKVStore.zeros(n_pages, n_kv_heads, head_dim, page_size=page_size,
                                         group_size=group_size, dtype=dtype, device=device)

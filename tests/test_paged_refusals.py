@@ -382,3 +382,23 @@ def test_updates_that_are_refused_add_no_tokens(monkeypatch, k, v):
     assert known(c) == before
     c.update_and_fetch(good, good)
     assert c.offset == 8
+
+
+@pytest.mark.parametrize("kw", [
+    dict(n_requests=4097), dict(max_tokens=2 ** 30 + 1, n_pages=1), dict(page_size=0), dict(n_pages=2 ** 26),
+    dict(n_pages=2 ** 21, n_kv_heads=1024, page_size=16), dict(n_requests=4096, max_tokens=2 ** 26, n_pages=1),
+])
+def test_caches_that_no_step_would_take_are_not_built(kw, monkeypatch):
+    def zeros(*a, **k):  # (a pool of this size is not made)
+        raise Launched
+
+    monkeypatch.setattr(torch, "zeros", zeros)
+    monkeypatch.setattr(torch, "full", zeros)
+    with pytest.raises(ValueError):
+        small_cache(**dict(dict(page_size=32), **kw))
+
+
+def test_the_largest_number_of_requests_is_taken(on_cpu):
+    c = small_cache(n_requests=4096, n_pages=1)
+    with pytest.raises(Launched, match="ss_block_tables"):
+        c.step([0] * 4096)
