@@ -212,8 +212,8 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(const PagedAttn a) {
                 if (left < n * parts) {
                     const int column = uniform_div(left, parts), part = left - column * parts;
                     u = base + column * n_units;
-                    stop = u + uniform_div((part + 1) * n_units, parts);
-                    u += uniform_div(part * n_units, parts);
+                    stop = u + part_begin(part + 1, n_units, parts);
+                    u += part_begin(part, n_units, parts);
                     list += column;
                     if (part == 0 && threadIdx.x == 0)
                         a.cut[list] = make_int4(parts > 1 ? parts : 0, r, blockIdx.x, column);

@@ -100,6 +100,13 @@ __device__ __forceinline__ int uniform_div(int a, int b) {
     return __builtin_amdgcn_readfirstlane((int)((uint32_t)a / (uint32_t)b));
 }
 
+// Where part i of `parts` begins in a column of n units: i n / parts rounded
+// down, without the product, which reaches 2^32 (512 parts of 2^23 units).
+__device__ __forceinline__ int part_begin(int i, int n, int parts) {
+    const int each = uniform_div(n, parts);
+    return i * each + uniform_div(i * (n - each * parts), parts);
+}
+
 // s_waitcnt vmcnt(N), the other counters unconstrained.
 template <int N>
 __device__ __forceinline__ void wait_loads() {

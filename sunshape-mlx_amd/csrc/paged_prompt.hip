@@ -168,11 +168,12 @@ __global__ void __launch_bounds__(64 * kPWaves, 2) paged_prompt_kernel(const Pag
     // as many as workgroups, each is cut along its tokens into parts of at most
     // `share` tiles of the request's length.
     const int per = (a.n_req + 63) / 64, r0 = min(lane * per, a.n_req), r1 = min(r0 + per, a.n_req);
-    int columns = 0, all_tiles = 0;
+    int columns = 0;
+    uint32_t all_tiles = 0;  // (up to 128 columns of 2^24; of more it is not used)
     for (int i = r0; i < r1; ++i) {
         const Request q = request(a, i);
         const int n = tiles_of(a, q) * heads;
-        columns += n, all_tiles += n * ((q.len + kTokens - 1) / kTokens);
+        columns += n, all_tiles += (uint32_t)n * ((q.len + kTokens - 1) / kTokens);
     }
     int scan = wave_scan(columns);
     const int n_columns = __builtin_amdgcn_readlane(scan, 63);
@@ -180,10 +181,10 @@ __global__ void __launch_bounds__(64 * kPWaves, 2) paged_prompt_kernel(const Pag
     if (a.cut && 2 * n_columns <= a.target) {
         // sum of ceil(n / share) is at most total / share + columns, and about
         // total / share + columns / 2
-        const int total = __builtin_amdgcn_readlane(wave_scan(all_tiles), 63);
+        const uint32_t total = __builtin_amdgcn_readlane(wave_scan((int)all_tiles), 63);
         for (int spare = n_columns / 2;; spare = n_columns) {
             const int free_groups = a.target - spare;
-            share = max(uniform_div(total + free_groups - 1, free_groups), kMinTiles);
+            share = max(uniform_div((int)(total + free_groups - 1), free_groups), kMinTiles);
             columns = 0;
             for (int i = r0; i < r1; ++i) {
                 const Request q = request(a, i);
@@ -228,8 +229,8 @@ __global__ void __launch_bounds__(64 * kPWaves, 2) paged_prompt_kernel(const Pag
         const int last_row = min(row_tile * kRows + kRows, rq.rows) - 1;
         const int seen_tiles =
             (__builtin_amdgcn_readfirstlane(sees(last_row)) + kTokens - 1) / kTokens;  // by the workgroup
-        const int first_tile = uniform_div(part * seen_tiles, parts);
-        const int n_tiles = uniform_div((part + 1) * seen_tiles, parts);
+        const int first_tile = part_begin(part, seen_tiles, parts);
+        const int n_tiles = part_begin(part + 1, seen_tiles, parts);
         const int wave_last = min(row0 + 31, rq.rows - 1);
         const int wave_end = row0 < rq.rows ? __builtin_amdgcn_readfirstlane(sees(wave_last)) : 0;
         const int all_see = row0 < rq.rows ? __builtin_amdgcn_readfirstlane(sees(row0)) : 0;

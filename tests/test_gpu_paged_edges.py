@@ -10,6 +10,7 @@ import torch
 from test_gpu_paged import DEV, HALF, check_attention, fresh, ints, rows, wide, world  # noqa: F401
 
 import sunshape_mlx_amd as S
+from sunshape_mlx_amd import _hip, paged
 
 pytestmark = pytest.mark.gpu
 
@@ -124,3 +125,23 @@ def test_a_list_step_in_a_capture_is_refused():
     assert c._host == [5, 9]
     c.step([1, 2])
     assert c.lengths.tolist() == [6, 11] == c._host
+
+
+@pytest.mark.parametrize("new", [1, 128])
+def test_a_request_of_2_to_the_30_tokens(new):
+    """The longest table row, whose every page is the same: the page's own
+    attention, but for sums of up to 2^17 float32 numbers, 2^-7 of their size
+    each (values around 3, so that the sums are of one sign).  Memory that no
+    part writes is NaN."""
+    d, page, width = 64, 1024, 2 ** 20
+    store = fresh(torch.float16, 1, 1, d, 64, page)
+    k, v = rows(61, page, 1, d, torch.float16, False), 3 + 0.25 * rows(62, page, 1, d, torch.float16, False)
+    S.append_paged(store, k, v, torch.arange(page, dtype=torch.int32, device=DEV))
+    q = rows(63, new, 1, d, torch.float16, False)
+    table = torch.zeros((1, width), dtype=torch.int32, device=DEV)
+    want, _ = R.attend(q, store, table, ints([page]), ints([0, new]), 0.125, causal=False)
+    need = paged._workspace_bytes(0, (1, 1, d, 64, page, _hip.SS_F16), new, 1, 1, new, page * width)
+    assert need > 0
+    poisoned((need // 2,), torch.float16)
+    out = S.paged_attention(q, store, table, ints([page * width]), ints([0, new]), 0.125)
+    assert ((out.cpu().double() - want).abs() <= 2.0 ** -6 * want.abs()).all()
