@@ -312,20 +312,17 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(const PagedAttn a) {
                     top = fmaxf(top, fabsf(x[k][e]));
                 }
             }
-            // a power of two brings the row into fp16's range: 16-bit
-            // queries stay exact
-            const int shift = row_exp_shift(lanes4_max(top));
-            const float down = a.scale < 0.f ? -exp2i(-shift) : exp2i(-shift);
+            const QueryScale by(lanes4_max(top), a.scale);
 #pragma unroll
             for (int k = 0; k < KS; ++k)
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    const float y = in_group ? x[k][e] * down : 0.f;  // (down: its sign is the scale's)
+                    const float y = in_group ? x[k][e] * by.down : 0.f;
                     sum += y;
                     qf[s][k][e] = (_Float16)y;
                 }
             qz[s] = lanes4_sum(sum);
-            factor[s] = fmaxf(fabsf(a.scale) * kLog2e * 64.f * exp2i(shift), 1e-30f);
+            factor[s] = by.factor;
             lag[s] = kLag / factor[s];
         }
         // (limits grow with the row: the first row's is the smallest)

@@ -85,6 +85,23 @@ __device__ __forceinline__ void store_out4(const PagedAttn &a, int64_t i, float 
         make_uint2(f16 ? __builtin_bit_cast(uint32_t, h0) : b0, f16 ? __builtin_bit_cast(uint32_t, h1) : b1);
 }
 
+// How a query row whose largest magnitude is `top` enters the products: times
+// `down`, a power of two that brings it into fp16's range (16-bit queries stay
+// exact) with the scale's sign; a sum of products times `factor` is then a
+// score in log2 units (codes enter as c/64).  factor is at least 2^-124, or
+// masked scores of -inf and the lag of 4 / factor would not be: rows that are
+// smaller stay smaller in fp16.  A scale of 0 or NaN is in `down`.
+struct QueryScale {
+    float down, factor;
+    __device__ QueryScale(float top, float scale) {
+        const float f = fabsf(scale) * kLog2e * 64.f;
+        const int e = (int)((__float_as_uint(f) >> 23) & 0xffu) - 127;  // f >= 2^e
+        const int shift = max(row_exp_shift(top), min(-124 - e, 126));
+        down = exp2i(-shift) * (scale < 0.f ? -1.f : scale > 0.f ? 1.f : scale);
+        factor = fmaxf(f * exp2i(shift), 0x1p-124f);
+    }
+};
+
 // Inclusive sum over the lanes before (lane moves, no LDS).
 __device__ __forceinline__ int wave_scan(int v) {
     v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);  // row_shr:1

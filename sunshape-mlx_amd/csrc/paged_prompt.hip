@@ -292,9 +292,8 @@ __global__ void __launch_bounds__(64 * kPWaves, 2) paged_prompt_kernel(const Pag
                         top = fmaxf(top, fabsf(x[g][s][e]));
                     }
                 }
-            const int shift = row_exp_shift(half_max(top));
-            const float down = a.scale < 0.f ? -exp2i(-shift) : exp2i(-shift);
-            factor = fmaxf(fabsf(a.scale) * kLog2e * 64.f * exp2i(shift), 1e-30f);
+            const QueryScale by(half_max(top), a.scale);
+            factor = by.factor;
             lag = kLag / factor;
             float sums[(G + 1) / 2];  // of group 2y + half
 #pragma unroll
@@ -306,7 +305,7 @@ __global__ void __launch_bounds__(64 * kPWaves, 2) paged_prompt_kernel(const Pag
                 for (int s = 0; s < HW; ++s)
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
-                        const float y = x[g][s][e] * down;
+                        const float y = x[g][s][e] * by.down;
                         sum += y;
                         qf[g][s][e] = (_Float16)y;
                     }

@@ -145,3 +145,49 @@ def test_a_request_of_2_to_the_30_tokens(new):
     poisoned((need // 2,), torch.float16)
     out = S.paged_attention(q, store, table, ints([page * width]), ints([0, new]), 0.125)
     assert ((out.cpu().double() - want).abs() <= 2.0 ** -6 * want.abs()).all()
+
+
+def small_against_large(q_size, k_size, new):
+    """Call arguments, without the scale, of bfloat16 queries and keys of
+    these sizes."""
+    n, d = 200, 64
+    store = fresh(torch.bfloat16, 13, 1, d, 32, 16)
+    k = (rows(71, n, 1, d, torch.float32, False).clamp(-4, 4) * k_size).to(torch.bfloat16)
+    v = rows(72, n, 1, d, torch.bfloat16, False)
+    S.append_paged(store, k, v, torch.arange(n, dtype=torch.int32, device=DEV))
+    table = torch.arange(13, dtype=torch.int32, device=DEV)[None]
+    q = (rows(73, new, 4, d, torch.float32, False) * q_size).to(torch.bfloat16)
+    return q, store, table, ints([n]), ints([0, new])
+
+
+@pytest.mark.parametrize("new", [1, 80])
+@pytest.mark.parametrize("q_size,k_size", [(1e-30, 1e30), (1e-33, 1e31), (1e-36, 1e31), (1e30, 1e-30),
+                                           (1e36, 1e-36)])
+def test_small_queries_against_large_keys(q_size, k_size, new):
+    args = (*small_against_large(q_size, k_size, new), 0.125)
+    check_attention(S.paged_attention(*args), *args)
+
+
+@pytest.mark.parametrize("q_size,k_size", [(1e-30, 1e30), (1e-33, 1e31)])
+def test_large_attention_of_small_queries(wide, q_size, k_size):
+    test_small_queries_against_large_keys(q_size, k_size, 80)
+
+
+@pytest.mark.parametrize("new", [1, 80])
+@pytest.mark.parametrize("scale", [0.0, -0.0, 1e-38, -1e-40])
+def test_a_scale_of_nothing_gives_the_mean(scale, new):
+    """... of the tokens that a row sees, whatever the keys."""
+    for sizes in ((1.0, 1.0), (1.0, 1e30)):
+        args = (*small_against_large(*sizes, new), scale if sizes[1] == 1.0 else 0.0)
+        check_attention(S.paged_attention(*args), *args)
+
+
+@pytest.mark.parametrize("new", [1, 80])
+def test_a_scale_that_is_no_number_gives_none(new):
+    args = small_against_large(1.0, 1.0, new)
+    assert S.paged_attention(*args, math.nan).isnan().all()
+
+
+def test_large_attention_with_scales_of_nothing(wide):
+    test_a_scale_of_nothing_gives_the_mean(0.0, 80)
+    test_a_scale_that_is_no_number_gives_none(80)
