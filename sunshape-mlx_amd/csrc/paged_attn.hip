@@ -332,11 +332,12 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(const PagedAttn a) {
         // (as a power of two) that the column's group has met, so p * scale
         // stays within fp16 whatever the scales.  top is in units of S.
         float top[NS], l[NS], z[NS];
+        float back[NS];  // added to each group's sum: minus the row's reference / G
         float4_t o[NS][VT], ones[NS];
 #pragma unroll
         for (int s = 0; s < NS; ++s) {
             top[s] = -INFINITY;
-            l[s] = z[s] = 0.f;
+            l[s] = z[s] = back[s] = 0.f;
             ones[s] = float4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int j = 0; j < VT; ++j) o[s][j] = float4_t{0.f, 0.f, 0.f, 0.f};
@@ -418,7 +419,7 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(const PagedAttn a) {
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const uint32_t m = km[4 * y + i];
-                        xs[s][4 * y + i] = groups_sum<G>(fmaf(low16<BF>(m), d[s][i], high16<BF>(m) * (qz[s] / 64.f)));
+                        xs[s][4 * y + i] = groups_sum<G>(fmaf(low16<BF>(m), d[s][i], fmaf(high16<BF>(m), qz[s] / 64.f, back[s])));
                     }
             }
             half8_t p16[NS];
@@ -439,6 +440,12 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(const PagedAttn a) {
                     const float now = fmaxf(top[s], lanes4_max(m));
                     rescale(s, now == top[s] ? 1.f : fast_exp2((top[s] - now) * factor[s]));
                     top[s] = now;
+                    if (__any(is_far(now, factor[s]))) {
+                        const float move = is_far(now, factor[s]) ? now : 0.f;
+                        back[s] -= move / G, top[s] -= move;
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) x[j] -= move;
+                    }
                     set_offset(s);
                 }
                 float w[8];
@@ -502,7 +509,7 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(const PagedAttn a) {
             const float lsum = ldexpf(lanes4_sum(l[s]), vexp - 10);
             const float zsum = ldexpf(lanes4_sum(z[s]), vexp - 10);
             const int row = s * RS + col / G;
-            if (g == 0 && quad == 0) stats[wave][row][0] = top[s] * factor[s], stats[wave][row][1] = lsum;
+            if (g == 0 && quad == 0) stats[wave][row][0] = (top[s] - G * back[s]) * factor[s], stats[wave][row][1] = lsum;
             if (in_group) {
                 // tile j, element i: dim (4 * quad + i) * D/16 + j
 #pragma unroll

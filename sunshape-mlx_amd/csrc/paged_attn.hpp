@@ -28,6 +28,15 @@ typedef float float2_t __attribute__((ext_vector_type(2)));
 // moves: probabilities stay below 2^4, so p * scale stays within fp16 with
 // scales normalised to 2^10.
 constexpr float kLag = 4.f;
+// Scores are kept less a reference of their row, which is 0 until the maximum
+// passes this many log2 units and moves to the maximum then: the maximum times
+// the factor is off by 2^-24 of itself, which scores of 2^28 would turn into
+// infinite probabilities.
+constexpr float kFar = 4096.f;
+__device__ __forceinline__ bool is_far(float top, float factor) {
+    return fabsf(top * factor) > kFar && top > -INFINITY;
+}
+
 struct PagedAttn {
     PagedStore st;
     const void *q;

@@ -313,7 +313,8 @@ __global__ void __launch_bounds__(64 * kPWaves, 2) paged_prompt_kernel(const Pag
                 sums[g / 2] = half == g % 2 ? sum : sums[g / 2];
             }
             // the sum of group 2y + half as three bf16 parts, for the zero's three:
-            // (z1, z1, z1, z2, z2, z3) . (q1, q2, q3, q1, q2, q1)
+            // (z1, z1, z1, z2, z2, z3) . (q1, q2, q3, q1, q2, q1); the first pair's two
+            // places that are left take the row's reference, times 1
 #pragma unroll
             for (int y = 0; y < (G + 1) / 2; ++y) {
                 float v = sums[y];
@@ -332,7 +333,7 @@ __global__ void __launch_bounds__(64 * kPWaves, 2) paged_prompt_kernel(const Pag
         float16_t o[NT];
 #pragma unroll
         for (int j = 0; j < NT; ++j) o[j] = float16_t{};
-        float top = -INFINITY, l = 0.f;
+        float top = -INFINITY, l = 0.f, ref = 0.f;
         // The values met in group g are below 2^vexp; the tile prepared last has
         // vnext, which the sums move to when they come to it.
         int vexp[G], vnext[G];
@@ -393,7 +394,7 @@ __global__ void __launch_bounds__(64 * kPWaves, 2) paged_prompt_kernel(const Pag
                 const uint32_t z3 = __float_as_uint(rest - __uint_as_float(z2 << 16)) >> 16;
                 const int place = (((lane >> 5) * PT::kPairs + (wave >> 1)) * 2 + (wave & 1)) * 32 + row;
                 *reinterpret_cast<uint4 *>(out + 2 * PT::kOperands + place * 16) =
-                    make_uint4(z1 | (z1 << 16), z1 | (z2 << 16), z2 | (z3 << 16), 0);
+                    make_uint4(z1 | (z1 << 16), z1 | (z2 << 16), z2 | (z3 << 16), wave < 2 ? 0x3f803f80u : 0);
                 if (wave < G)
                     reinterpret_cast<uint16_t *>(out + 2 * PT::kOperands + PT::kZeros)[wave * kTokens + lane] = (uint16_t)km;
             }
@@ -533,6 +534,21 @@ __global__ void __launch_bounds__(64 * kPWaves, 2) paged_prompt_kernel(const Pag
                         const float now = fmaxf(top, half_max(m));
                         const float f = now == top ? 1.f : fast_exp2((top - now) * factor);
                         top = now;
+                        if (__any(is_far(now, factor))) {
+                            const float move = is_far(now, factor) ? now : 0.f;
+                            ref += move, top -= move;
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) x[i] -= move;
+                            // minus the reference as three bf16 parts, in the zeros' product
+                            float part[3], rest = -ref;
+#pragma unroll
+                            for (int k = 0; k < 3; ++k) {
+                                part[k] = __bfloat162float(__float2bfloat16(rest));
+                                rest -= part[k];
+                            }
+                            qz[0][6] = (__bf16)(half ? part[2] : part[0]);
+                            qz[0][7] = (__bf16)(half ? 0.f : part[1]);
+                        }
                         l *= f;
 #pragma unroll
                         for (int j = 0; j < NT; ++j) o[j] *= f;
@@ -621,7 +637,7 @@ __global__ void __launch_bounds__(64 * kPWaves, 2) paged_prompt_kernel(const Pag
             // a part: the sums as they are (times 2^10), for prompt_merge_kernel
             if (part == 0) cut = make_int4(parts, r, h, row_tile);
             const int64_t at = (int64_t)item * kRows + wave * 32 + col;
-            if (half == 0) *reinterpret_cast<float2 *>(a.ml + at * 2) = make_float2(top * factor, sum);
+            if (half == 0) *reinterpret_cast<float2 *>(a.ml + at * 2) = make_float2((ref + top) * factor, sum);
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
                 const int m = 8 * (i / 4) + 4 * half + i % 4;

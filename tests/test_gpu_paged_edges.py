@@ -191,3 +191,47 @@ def test_a_scale_that_is_no_number_gives_none(new):
 def test_large_attention_with_scales_of_nothing(wide):
     test_a_scale_of_nothing_gives_the_mean(0.0, 80)
     test_a_scale_that_is_no_number_gives_none(80)
+
+
+def far_scores(dtype, size, new, d=128, n=400):
+    """Call arguments of scores that differ by `size` log2 units from token to
+    token, all of them exact (keys 0 .. 14 in one dim, scale 1), and the 64-bit
+    output: each row's largest tokens alone."""
+    store = fresh(dtype, 25, 1, d, 64, 16)
+    k = torch.zeros((n, 1, d), device=DEV)
+    k[:, 0, 0] = torch.arange(n, device=DEV) * 7 % 15
+    k[:, 0, 1] = 15.0  # (the group's scale)
+    v = rows(81, n, 1, d, dtype, False)
+    S.append_paged(store, k.to(dtype), v, torch.arange(n, dtype=torch.int32, device=DEV))
+    table = torch.arange(25, dtype=torch.int32, device=DEV)[None]
+    q = torch.zeros((new, 4, d), dtype=dtype, device=DEV)
+    q[..., 0] = torch.tensor([1.0, -1.0, 3.0, -0.5], device=DEV)
+    args = (q, store, table, ints([n]), ints([0, new]), size * math.log(2))
+    return args, R.attend(*args)[0]
+
+
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("new", [1, 80])
+@pytest.mark.parametrize("size", [300.0, 2.0 ** 13, 2.0 ** 22, 2.0 ** 27, 2.0 ** 40, 2.0 ** 90])
+def test_scores_of_any_size(size, new, dtype):
+    """The largest scores' tokens are averaged: p is 1 or 0, so only the
+    values' roundings are left, 2^-11 of p scale times 7.5 codes here, 2^-11 of
+    p and of the value in the kernel for large calls."""
+    args, want = far_scores(dtype, size, new)
+    out = S.paged_attention(*args)
+    store = args[1]
+    terms = want.abs() + 7.5 * R.unpack(store)[3][:400, 0, :, 0].double().amax(0).repeat_interleave(64)
+    err = (out.cpu().double() - want).abs()
+    assert (err <= R.U16[dtype] * want.abs() + 2.001 * 2.0 ** -11 * terms + 2.0 ** -16).all(), float(err.max())
+
+
+@pytest.mark.parametrize("dtype", HALF)
+def test_large_attention_with_scores_of_any_size(wide, dtype):
+    for size in (300.0, 2.0 ** 13, 2.0 ** 22, 2.0 ** 27, 2.0 ** 40, 2.0 ** 90):
+        test_scores_of_any_size(size, 80, dtype)
+
+
+@pytest.mark.parametrize("new", [1, 80])
+def test_far_scores_of_small_queries_against_large_keys(new):
+    args = (*small_against_large(1e-20, 1e31, new), 0.125)
+    check_attention(S.paged_attention(*args), *args)
