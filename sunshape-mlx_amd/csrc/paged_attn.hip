@@ -328,9 +328,12 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(const PagedAttn a) {
         // (limits grow with the row: the first row's is the smallest)
         if (a.causal) all_see = max(0, min(rq.len, rq.len - rq.n_all + rb * ROWS / a.rep + 1));
 
-        // The sums are kept times 2^(10 - vexp): vexp is above every value scale
-        // (as a power of two) that the column's group has met, so p * scale
-        // stays within fp16 whatever the scales.  top is in units of S.
+        // Probabilities are kept times 2^kProb, so that a sum of bfloat16's largest
+        // values stays finite; p * scale enters the products times 2^(kScaled -
+        // vexp): vexp is above every value scale (as a power of two) that the
+        // column's group has met, so it stays within fp16 whatever the scales.
+        // top is in units of S.
+        constexpr int kProb = -24, kScaled = 10 - kProb;
         float top[NS], l[NS], z[NS];
         float back[NS];  // added to each group's sum: minus the row's reference / G
         float4_t o[NS][VT], ones[NS];
@@ -342,16 +345,14 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(const PagedAttn a) {
 #pragma unroll
             for (int j = 0; j < VT; ++j) o[s][j] = float4_t{0.f, 0.f, 0.f, 0.f};
         }
-        int vexp = -60;
-        float offset[NS];  // of the exponents: 10 - vexp less the maximum's
-        auto set_offset = [&](int s) {
-            offset[s] = (float)(10 - vexp) - (top[s] == -INFINITY ? 0.f : top[s] * factor[s]);
-        };
+        int vexp = -92;  // (2^(kScaled - vexp) is a float)
+        float up = exp2i(kScaled - vexp);
+        float offset[NS];  // of the exponents: kProb less the maximum's
+        auto set_offset = [&](int s) { offset[s] = kProb - (top[s] == -INFINITY ? 0.f : top[s] * factor[s]); };
 #pragma unroll
         for (int s = 0; s < NS; ++s) set_offset(s);
         const CodeBits code_bits;
-        auto rescale = [&](int s, float f) {
-            l[s] *= f, z[s] *= f;
+        auto rescale = [&](int s, float f) {  // (what is times up)
             ones[s] *= f;
 #pragma unroll
             for (int j = 0; j < VT; ++j) o[s][j] *= f;
@@ -396,9 +397,7 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(const PagedAttn a) {
                 const int now = max(vexp, min(e, 126));
 #pragma unroll
                 for (int s = 0; s < NS; ++s) rescale(s, ldexpf(1.f, vexp - now));
-                vexp = now;
-#pragma unroll
-                for (int s = 0; s < NS; ++s) set_offset(s);
+                vexp = now, up = exp2i(kScaled - vexp);
             }
             // (sets inside: an operand's registers serve every set and are free again)
             float xs[NS][8];
@@ -428,7 +427,7 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(const PagedAttn a) {
                 float(&x)[8] = xs[s];
                 float v[8], mid[8];
 #pragma unroll
-                for (int j = 0; j < 8; ++j) v[j] = vs[j], mid[j] = fmaf(vs[j], 7.5f, high16<BF>(vm[j]));
+                for (int j = 0; j < 8; ++j) v[j] = vs[j] * up, mid[j] = fmaf(vs[j], 7.5f, high16<BF>(vm[j]));
                 if (mask) {  // what the row does not see adds nothing, whatever its value holds
                     const int see = ok ? limit[s] : 0;
 #pragma unroll
@@ -438,7 +437,9 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(const PagedAttn a) {
                 const float m = column_max(x);
                 if (__any(m > top[s] + lag[s])) {
                     const float now = fmaxf(top[s], lanes4_max(m));
-                    rescale(s, now == top[s] ? 1.f : fast_exp2((top[s] - now) * factor[s]));
+                    const float f = now == top[s] ? 1.f : fast_exp2((top[s] - now) * factor[s]);
+                    l[s] *= f, z[s] *= f;
+                    rescale(s, f);
                     top[s] = now;
                     if (__any(is_far(now, factor[s]))) {
                         const float move = is_far(now, factor[s]) ? now : 0.f;
@@ -506,8 +507,7 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(const PagedAttn a) {
         // the waves' results, joined
 #pragma unroll
         for (int s = 0; s < NS; ++s) {
-            const float lsum = ldexpf(lanes4_sum(l[s]), vexp - 10);
-            const float zsum = ldexpf(lanes4_sum(z[s]), vexp - 10);
+            const float lsum = lanes4_sum(l[s]), zsum = lanes4_sum(z[s]);
             const int row = s * RS + col / G;
             if (g == 0 && quad == 0) stats[wave][row][0] = (top[s] - G * back[s]) * factor[s], stats[wave][row][1] = lsum;
             if (in_group) {
@@ -516,7 +516,7 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(const PagedAttn a) {
                 for (int i = 0; i < 4; ++i)
 #pragma unroll
                     for (int j = 0; j < VT; ++j)
-                        part[wave][row][(4 * quad + i) * VT + j] = ldexpf(64.f * o[s][j][i] - 71.5f * ones[s][i], vexp - 10) + zsum;
+                        part[wave][row][(4 * quad + i) * VT + j] = ldexpf(64.f * o[s][j][i] - 71.5f * ones[s][i], vexp - kScaled) + zsum;
             }
         }
         __syncthreads();

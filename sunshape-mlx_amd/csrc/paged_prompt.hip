@@ -338,7 +338,7 @@ __global__ void __launch_bounds__(64 * kPWaves, 2) paged_prompt_kernel(const Pag
         // vnext, which the sums move to when they come to it.
         int vexp[G], vnext[G];
 #pragma unroll
-        for (int g = 0; g < G; ++g) vexp[g] = vnext[g] = -60;
+        for (int g = 0; g < G; ++g) vexp[g] = vnext[g] = -110;
         // The bits from which zeros and scales would pass 2^vnext: few tiles
         // after the first have any, and a look at a tile's largest is skipped.
         uint32_t zero_top[G], scale_top[G];
@@ -426,7 +426,7 @@ __global__ void __launch_bounds__(64 * kPWaves, 2) paged_prompt_kernel(const Pag
                     // |zero + 15 scale| < 2 max(|zero|, 16 scale)
                     const float c = fmaxf(16.f * low16<BF>(most[g]), high16<BF>(most[g]));
                     const int e = __builtin_amdgcn_readfirstlane((int)((__float_as_uint(c) >> 23) & 0xffu) - 125);
-                    vnext[g] = max(vnext[g], min(e, 126));
+                    vnext[g] = max(vnext[g], e);
                     zero_top[g] = bits_of_exp2<BF>(vnext[g] - 1), scale_top[g] = bits_of_exp2<BF>(vnext[g] - 5);
                 }
             }
@@ -443,7 +443,7 @@ __global__ void __launch_bounds__(64 * kPWaves, 2) paged_prompt_kernel(const Pag
             int e = __builtin_amdgcn_readfirstlane(vnext[0]);
 #pragma unroll
             for (int g = 1; g < G; ++g) e = vg == g ? __builtin_amdgcn_readfirstlane(vnext[g]) : e;
-            const float up = exp2i(15 - e), up_odd = exp2i(11 - e);  // (-60 <= e <= 126)
+            const float up = exp2i(15 - e), up_odd = exp2i(11 - e);  // (-110 <= e <= 130)
             const CodeNumber number;
             half8_t sc, ze;  // codes of odd pairs count 16 times
 #pragma unroll

@@ -235,3 +235,30 @@ def test_large_attention_with_scores_of_any_size(wide, dtype):
 def test_far_scores_of_small_queries_against_large_keys(new):
     args = (*small_against_large(1e-20, 1e31, new), 0.125)
     check_attention(S.paged_attention(*args), *args)
+
+
+SIZES = {"constant": lambda v: torch.ones_like(v) * 1e20, "largest": lambda v: torch.full_like(v, 3.3e38),
+         "smallest": lambda v: v * 1e-30, "wide": lambda v: v * 1e37, "raised": lambda v: 1e25 + v * 1e20,
+         "one": lambda v: torch.where(torch.arange(v.shape[0], device=DEV)[:, None, None] == 77, v * 3e37, v)}
+
+
+@pytest.mark.parametrize("new", [1, 3, 80])
+@pytest.mark.parametrize("size", SIZES)
+def test_values_of_any_size(size, new, lengths=(300, 2500)):
+    """bfloat16 values of one size or of all: groups whose scale is 0 or small
+    beside their zero, the largest and the smallest numbers, one token that is
+    far larger than the others.  Keys of 0: every token counts the same."""
+    d, group, page = 64, 32, 16
+    for n in lengths:
+        store = fresh(torch.bfloat16, -(-n // page), 1, d, group, page)
+        v = SIZES[size](rows(91, n, 1, d, torch.float32, False).clamp(-3, 3)).to(torch.bfloat16)
+        S.append_paged(store, torch.zeros_like(v), v, torch.arange(n, dtype=torch.int32, device=DEV))
+        table = torch.arange(-(-n // page), dtype=torch.int32, device=DEV)[None]
+        q = rows(92, new, 4, d, torch.bfloat16, False)
+        args = (q, store, table, ints([n]), ints([0, new]), 0.125)
+        check_attention(S.paged_attention(*args), *args)
+
+
+@pytest.mark.parametrize("size", SIZES)
+def test_large_attention_with_values_of_any_size(wide, size):
+    test_values_of_any_size(size, 80, (300,))
