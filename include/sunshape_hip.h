@@ -1052,7 +1052,8 @@ typedef struct {
  *   - token_starts[n_requests + 1]: where each request's new tokens start in
  *     the packed order (request after request).
  *   - slots[n_tokens], positions[n_tokens] (may be NULL): each packed token's
- *     slot and its position in its request, -1 behind the last one.
+ *     slot and its position in its request, -1 behind the last one.  (A page
+ *     number of the caller's that is negative or past 2^31 slots: slot -1.)
  *   - lengths_out, n_free_out: the counts after the step; they may be the
  *     arrays lengths and n_free themselves.
  * status[0] is 0, or the sum of what makes the step impossible; then nothing

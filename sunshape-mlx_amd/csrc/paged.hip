@@ -51,8 +51,9 @@ __device__ __forceinline__ void write_slot(int64_t tok, const int32_t *starts, i
         const int r = request_of(starts, n_req, (int)tok);
         // ends: lengths after the step; the request's new tokens are its last
         pos = ends[r] - (starts[r + 1] - (int)tok);
-        slot = (int32_t)(((uint32_t)table[r * width + (pos >> log_page)] << log_page) +
-                         (pos & ((1 << log_page) - 1)));
+        // (a page whose slots 32 bits do not hold is in no pool: its tokens have none)
+        const uint32_t page = table[r * width + (pos >> log_page)];
+        if (page <= (uint32_t)INT32_MAX >> log_page) slot = (int32_t)(page << log_page) + (pos & ((1 << log_page) - 1));
     }
     slots[tok] = slot;
     if (positions) positions[tok] = pos;

@@ -262,3 +262,21 @@ def test_values_of_any_size(size, new, lengths=(300, 2500)):
 @pytest.mark.parametrize("size", SIZES)
 def test_large_attention_with_values_of_any_size(wide, size):
     test_values_of_any_size(size, 80, (300,))
+
+
+@pytest.mark.parametrize("n_new", [1, 5000])
+def test_pages_of_no_pool_give_no_slots(n_new):
+    """Page numbers whose slots pass 32 bits do not come back as slots of other
+    pages; for few new tokens and, by the second launch, for many."""
+    page, big = 64, 2 ** 26
+    width = 1 + -(-n_new // page)
+    for number in (big + 3, -big, -1, -big + 3, 2 ** 31 - 1, big // 2 - 1, 7):
+        table = ints([[number] + [-1] * (width - 1), list(range(width))])
+        free = torch.arange(100, 100 + 2 * width, dtype=torch.int32, device=DEV)
+        plan = S.build_block_tables(ints([5, 5]), ints([n_new, 1]), table, free, ints([2 * width]), page, n_new + 1)
+        S.check_plan(plan)
+        slots, first = plan.slots.tolist(), min(n_new, page - 5)
+        real = number >= 0 and (number + 1) * page <= 2 ** 31
+        assert slots[:first] == [number * page + 5 + i if real else -1 for i in range(first)], number
+        assert slots[-1] == 5 and all(s >= 0 for s in slots[first:])
+        assert plan.positions.tolist() == list(range(5, 5 + n_new)) + [5]
