@@ -1097,7 +1097,8 @@ int ss_read_paged(const ss_paged_store *store, const int32_t *slots, int64_t n_t
  * lengths[r] - n + i (causal) or all of them.  Query head hq reads KV head
  * hq / (n_q_heads / n_kv_heads).
  *   out  [n_tokens][n_q_heads][head_dim], q's dtype; rows without a token to
- *        see are zero; rows of no request are zeroed if zero_rest, else left.
+ *        see are zero; rows of no request are zeroed if zero_rest, else left
+ *        (all of them where token_starts descends anywhere).
  * Softmax statistics and sums are float32; probabilities times scales enter
  * the matrix cores in 16 bits.  Table entries outside the pool hold no
  * tokens.  max_new and max_length (the most new tokens and the longest

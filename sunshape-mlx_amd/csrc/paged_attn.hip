@@ -149,25 +149,32 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(const PagedAttn a) {
     const int g = col % G;
     const bool in_group = quad * G / 4 == g;  // the lane's dims, and its rows of O, are in the column's group
     const int heads = a.st.heads, log_page = a.st.log_page;
-    if (a.zero_rest) {  // the rows before the first request's, and those behind the last one's
-        const int64_t row = (int64_t)a.hq * D;
-        const int64_t first = min((int64_t)max(0, table_read(a.starts, 0)), a.n_tokens) * row;
-        const int64_t last = min((int64_t)max(0, table_read(a.starts, a.n_req)), a.n_tokens) * row;
-        const int64_t theirs = max(last - first, (int64_t)0);
+    // Rows but [first, last): those before the first request's and behind the last one's.
+    auto zero_rows = [&](int first, int last) {
+        const int64_t row = (int64_t)a.hq * D, from = min((int64_t)max(0, first), a.n_tokens) * row;
+        const int64_t theirs = max(min((int64_t)max(0, last), a.n_tokens) * row - from, (int64_t)0);
         for (int64_t e = blockIdx.x * 256 + threadIdx.x; e < a.n_tokens * row - theirs; e += gridDim.x * 256)
-            store_from_f32(a.out, a.q_dtype, e < first ? e : e + theirs, 0.f);
-    }
+            store_from_f32(a.out, a.q_dtype, e < from ? e : e + theirs, 0.f);
+    };
+    if (a.zero_rest) zero_rows(table_read(a.starts, 0), table_read(a.starts, a.n_req));
 
     // This workgroup's run of units [u, stop), and the request r it starts in,
     // whose units start at `base`: every wave works it out by itself, a few
     // requests a lane.
     const int groups = gridDim.x, per = (a.n_req + 63) / 64;
-    const int r0 = min(lane * per, a.n_req), r1 = min(r0 + per, a.n_req);
+    const int r0 = min(lane * per, a.n_req);
+    int r1 = min(r0 + per, a.n_req);
     int units = 0, columns = 0;  // of the lane's requests
+    bool down = false;
     for (int i = r0; i < r1; ++i) {
         const Request q = request(a, i);
+        down |= descends(a, i);
         const int n = blocks_of(a, q, ROWS) * heads;
         units += units_of(q) * n, columns += n;
+    }
+    if (__any(down)) {
+        units = columns = 0, r1 = r0;
+        if (a.zero_rest) zero_rows(0, 0);
     }
     const int units_scan = wave_scan(units);
     const int total = __builtin_amdgcn_readlane(units_scan, 63);

@@ -83,6 +83,12 @@ __device__ __forceinline__ Request request(const PagedAttn &a, int r) {
     return q;
 }
 
+// Whether request r ends before it begins.  Starts that descend name no rows at
+// all: requests that overlap might be more than 32 bits count.
+__device__ __forceinline__ bool descends(const PagedAttn &a, int r) {
+    return table_read(a.starts, r + 1) < table_read(a.starts, r);
+}
+
 // Elements i .. i+3 of the output (i a multiple of 4), of q's 16-bit type.
 __device__ __forceinline__ void store_out4(const PagedAttn &a, int64_t i, float x0, float x1, float x2, float x3) {
     const half2_t h0 = __builtin_convertvector(float2_t{x0, x1}, half2_t);

@@ -167,14 +167,17 @@ __global__ void __launch_bounds__(64 * kPWaves, 2) paged_prompt_kernel(const Pag
     // Columns are (request, row tile, KV head).  Where there are fewer than half
     // as many as workgroups, each is cut along its tokens into parts of at most
     // `share` tiles of the request's length.
-    const int per = (a.n_req + 63) / 64, r0 = min(lane * per, a.n_req), r1 = min(r0 + per, a.n_req);
-    int columns = 0;
+    const int per = (a.n_req + 63) / 64, r0 = min(lane * per, a.n_req);
+    int r1 = min(r0 + per, a.n_req), columns = 0;
+    bool down = false;
     uint32_t all_tiles = 0;  // (up to 128 columns of 2^24; of more it is not used)
     for (int i = r0; i < r1; ++i) {
         const Request q = request(a, i);
         const int n = tiles_of(a, q) * heads;
+        down |= descends(a, i);
         columns += n, all_tiles += (uint32_t)n * ((q.len + kTokens - 1) / kTokens);
     }
+    if (__any(down)) columns = 0, all_tiles = 0, r1 = r0;
     int scan = wave_scan(columns);
     const int n_columns = __builtin_amdgcn_readlane(scan, 63);
     int share = INT32_MAX;

@@ -280,3 +280,26 @@ def test_pages_of_no_pool_give_no_slots(n_new):
         assert slots[:first] == [number * page + 5 + i if real else -1 for i in range(first)], number
         assert slots[-1] == 5 and all(s >= 0 for s in slots[first:])
         assert plan.positions.tolist() == list(range(5, 5 + n_new)) + [5]
+
+
+@pytest.mark.parametrize("max_new", [1, 64])
+def test_starts_that_descend_name_no_rows(max_new):
+    """Requests that overlap; as many as pass 32 bits of blocks among them."""
+    store, table, le, _ = world(101, [64, 64, 64], [1, 1, 1], 2, 64, 64, 16, torch.float16)
+    q = rows(102, 40, 8, 64, torch.float16, False)
+    for starts in ([0, 30, 10, 40], [40, 30, 20, 0], [0, 0, 40, 39], [0, 40, -2 ** 31, 40], [5, -2 ** 31, 40, 40]):
+        poisoned(q.shape, q.dtype)
+        assert (S.paged_attention(q, store, table, le, ints(starts), 0.125, max_new=max_new) == 0).all(), starts
+        given = torch.full_like(q, 7.0)
+        S.paged_attention(q, store, table, le, ints(starts), 0.125, max_new=max_new, out=given)
+        assert (given == 7).all()
+    many, page = 4000, 1024
+    big = fresh(torch.float16, 1, 2, 64, 64, page)
+    table = torch.zeros((many, 2 ** 20 // page), dtype=torch.int32, device=DEV)
+    out = S.paged_attention(q, big, table, ints([2 ** 20] * many), ints([0, 40] * (many // 2) + [40]), 0.125,
+                            max_new=max_new)
+    assert (out == 0).all()
+
+
+def test_large_attention_of_starts_that_descend(wide):
+    test_starts_that_descend_name_no_rows(64)
