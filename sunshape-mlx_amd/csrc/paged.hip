@@ -473,7 +473,7 @@ int check_paged_store(const ss_paged_store *s, PagedStore *out, int *log_page) {
                    "group_size %d (32, 64 or 128, at most head_dim)", s->group_size);
     SS_UNSUPPORTED(s->page_size >= 16 && s->page_size <= 1024 && (s->page_size & (s->page_size - 1)) == 0,
                    "page_size %d (a power of two from 16 to 1024)", s->page_size);
-    SS_UNSUPPORTED(s->n_pages * s->page_size <= INT32_MAX && s->n_pages * s->n_kv_heads <= INT32_MAX,
+    SS_UNSUPPORTED(s->n_pages <= INT32_MAX / s->page_size && s->n_pages <= INT32_MAX / s->n_kv_heads,
                    "the pool has more slots than 32 bits count");
     *log_page = __builtin_ctz((unsigned)s->page_size);
     *out = {static_cast<uint32_t *>(s->k_codes), static_cast<uint32_t *>(s->v_codes),
@@ -499,7 +499,7 @@ extern "C" int ss_block_tables(const int32_t *lengths, const int32_t *new_length
     SS_UNSUPPORTED(n_requests <= kMaxRequests, "%lld requests (at most %d)", (long long)n_requests, kMaxRequests);
     SS_UNSUPPORTED(page_size >= 16 && page_size <= 1024 && (page_size & (page_size - 1)) == 0,
                    "page_size %d (a power of two from 16 to 1024)", page_size);
-    SS_UNSUPPORTED(pool * page_size <= INT32_MAX && n_tokens <= INT32_MAX && n_requests * table_width <= INT32_MAX,
+    SS_UNSUPPORTED(pool <= INT32_MAX / page_size && n_tokens <= INT32_MAX && table_width <= INT32_MAX / n_requests,
                    "more slots, tokens or table entries than 32 bits count");
     const int log_page = __builtin_ctz((unsigned)page_size);
     const int in_one = n_tokens <= kSlotsInline;
@@ -527,8 +527,9 @@ extern "C" int ss_append_paged(const ss_paged_store *store, const void *keys, co
     SS_REQUIRE(n_tokens >= 0, "bad sizes");
     if (n_tokens == 0) return SS_OK;
     SS_REQUIRE(keys && values && slots, "null pointer argument");
+    SS_UNSUPPORTED(n_tokens <= INT32_MAX, "too many tokens for one launch");
     const int64_t items = (n_tokens + 7) / 8 * ps.heads;
-    SS_UNSUPPORTED(n_tokens <= INT32_MAX && items <= INT32_MAX, "too many tokens for one launch");
+    SS_UNSUPPORTED(items <= INT32_MAX, "too many tokens for one launch");
     // 16-byte loads where every row starts on 16 bytes
     const int per = in_dtype == SS_F32 ? 4 : 8;
     const int vec = (((uintptr_t)keys | (uintptr_t)values) & 15) == 0 && k_st % per == 0 && k_sh % per == 0 &&

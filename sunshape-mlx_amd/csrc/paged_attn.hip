@@ -711,7 +711,8 @@ extern "C" size_t ss_paged_attn_workspace_bytes(const ss_paged_store *store, int
                                                 int n_q_heads, int64_t max_new, int64_t max_length) {
     PagedStore ps;
     int log_page;
-    if (check_paged_store(store, &ps, &log_page) || check_hints(store, n_requests, n_q_heads, max_new, max_length))
+    if (check_paged_store(store, &ps, &log_page) || check_hints(store, n_requests, n_q_heads, max_new, max_length) ||
+        n_tokens < 0 || n_tokens > INT32_MAX / n_q_heads)
         return 0;
     return paged_plan(store, n_tokens, n_requests, n_q_heads, max_new, max_length).bytes;
 }

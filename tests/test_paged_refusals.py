@@ -402,3 +402,28 @@ def test_the_largest_number_of_requests_is_taken(on_cpu):
     c = small_cache(n_requests=4096, n_pages=1)
     with pytest.raises(Launched, match="ss_block_tables"):
         c.step([0] * 4096)
+
+
+@pytest.mark.parametrize("big", [1 << 62, (1 << 62) + 1, (1 << 60) + 3, (1 << 63) - 1, 1 << 32])
+def test_counts_whose_products_pass_64_bits_are_refused(big):
+    """Products of two sizes that come out small, or negative, in 64 bits."""
+    lib = _hip.load_library()
+    st = store(n_pages=big)
+    at = ctypes.addressof(st)
+    assert lib.ss_read_paged(at, FAKE, 1, FAKE, FAKE, None) == -2
+    assert lib.ss_append_paged(at, FAKE, FAKE, 1, 1, 256, 128, 256, 128, FAKE, None) == -2
+    assert attention(st) == -2
+
+    def tables(r=2, width=4, pool=8, n=3):
+        return lib.ss_block_tables(FAKE, FAKE, r, FAKE, width, FAKE, pool, FAKE, 64, n, FAKE, FAKE, FAKE, FAKE, None,
+                                   FAKE, None)
+
+    assert tables(pool=big) == tables(width=big) == tables(r=4096, width=big) == tables(n=big) == -2
+    st = store()
+    at = ctypes.addressof(st)
+    assert lib.ss_append_paged(at, FAKE, FAKE, 1, big, 256, 128, 256, 128, FAKE, None) == -2
+    assert lib.ss_read_paged(at, FAKE, big, FAKE, FAKE, None) == -2
+    assert attention(n=big) == attention(width=big) == -2
+    assert attention(max_new=big) == attention(max_length=big) == -1
+    for n in (big, -big, -1):
+        assert lib.ss_paged_attn_workspace_bytes(at, n, 1, 2, 1, 100000) == 0
