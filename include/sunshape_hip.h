@@ -1077,6 +1077,7 @@ int ss_block_tables(const int32_t *lengths, const int32_t *new_lengths, int64_t 
  * where the scale is 0).  A group with an infinity or NaN is stored as NaN.
  * Tokens whose slot is negative or outside the pool are not stored.  Slots
  * must be distinct: the content of one that is given twice is undefined.
+ * n_tokens (in whole blocks of 8) * n_kv_heads is at most 2^29 - 32.
  */
 int ss_append_paged(const ss_paged_store *store, const void *keys, const void *values,
                     int in_dtype, int64_t n_tokens, int64_t k_st, int64_t k_sh, int64_t v_st,
@@ -1084,7 +1085,8 @@ int ss_append_paged(const ss_paged_store *store, const void *keys, const void *v
 
 /*
  * What the slots hold: keys and values [n_tokens][n_kv_heads][head_dim] in
- * the store's dtype (zeros for a slot outside the pool).
+ * the store's dtype (zeros for a slot outside the pool).  n_tokens *
+ * n_kv_heads is at most 2^28 - 16 (head_dim 128) or 2^29 - 32 (64).
  */
 int ss_read_paged(const ss_paged_store *store, const int32_t *slots, int64_t n_tokens, void *keys,
                   void *values, void *stream);

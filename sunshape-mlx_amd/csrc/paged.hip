@@ -529,7 +529,8 @@ extern "C" int ss_append_paged(const ss_paged_store *store, const void *keys, co
     SS_REQUIRE(keys && values && slots, "null pointer argument");
     SS_UNSUPPORTED(n_tokens <= INT32_MAX, "too many tokens for one launch");
     const int64_t items = (n_tokens + 7) / 8 * ps.heads;
-    SS_UNSUPPORTED(items <= INT32_MAX, "too many tokens for one launch");
+    SS_UNSUPPORTED((items + 3) / 4 <= kMostGroups, "%lld tokens of %d heads: too many for one launch",
+                   (long long)n_tokens, ps.heads);
     // 16-byte loads where every row starts on 16 bytes
     const int per = in_dtype == SS_F32 ? 4 : 8;
     const int vec = (((uintptr_t)keys | (uintptr_t)values) & 15) == 0 && k_st % per == 0 && k_sh % per == 0 &&
@@ -560,8 +561,9 @@ extern "C" int ss_read_paged(const ss_paged_store *store, const int32_t *slots, 
     if (n_tokens == 0) return SS_OK;
     SS_REQUIRE(keys && values && slots, "null pointer argument");
     SS_REQUIRE((((uintptr_t)keys | (uintptr_t)values) & 15) == 0, "outputs must be 16-byte aligned");
-    SS_UNSUPPORTED(n_tokens <= INT32_MAX && n_tokens * ps.heads <= INT32_MAX, "too many tokens for one launch");
     const int rows = 256 / (store->head_dim / 8);  // of a workgroup
+    SS_UNSUPPORTED(n_tokens <= kMostGroups * rows / ps.heads, "%lld tokens of %d heads: too many for one launch",
+                   (long long)n_tokens, ps.heads);
     const dim3 grid((unsigned)((n_tokens * ps.heads + rows - 1) / rows));
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
     auto launch = [&](auto kernel) {

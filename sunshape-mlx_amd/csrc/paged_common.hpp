@@ -13,6 +13,9 @@ struct PagedStore {
     int n_pages, heads, log_page;
 };
 
+// Workgroups of 256 threads in a launch: the runtime counts its threads in 32 bits.
+constexpr int64_t kMostGroups = UINT32_MAX / 256;
+
 // Checks a caller's store; its shape in *out.
 int check_paged_store(const ss_paged_store *s, PagedStore *out, int *log_page);
 

@@ -427,3 +427,18 @@ def test_counts_whose_products_pass_64_bits_are_refused(big):
     assert attention(max_new=big) == attention(max_length=big) == -1
     for n in (big, -big, -1):
         assert lib.ss_paged_attn_workspace_bytes(at, n, 1, 2, 1, 100000) == 0
+
+
+@pytest.mark.parametrize("heads", [1, 3, 8])
+def test_more_threads_than_a_launch_counts_are_refused(heads):
+    """2^32 threads: 8 of a wave's tokens and a head each in appends, 8 dims of
+    a token and a head in reads."""
+    lib = _hip.load_library()
+    for d, read in ((128, 2 ** 28), (64, 2 ** 29)):
+        st = store(n_kv_heads=heads, head_dim=d)
+        at = ctypes.addressof(st)
+        for n in (-(-2 ** 29 // heads), 2 ** 31 - 1):
+            assert lib.ss_append_paged(at, FAKE, FAKE, 1, n, 256, 128, 256, 128, FAKE, None) == -2
+        for n in (-(-read // heads), 2 ** 31 // heads, 2 ** 31 - 1):
+            assert lib.ss_read_paged(at, FAKE, n, FAKE, FAKE, None) == -2
+        assert b"too many" in lib.ss_last_error()
