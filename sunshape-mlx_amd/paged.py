@@ -571,6 +571,11 @@ class PagedKVCache:
     def is_trimmable(self) -> bool:
         return True
 
+    def empty(self) -> bool:
+        """Whether no request holds a token (waits for the GPU where the host
+        does not know the lengths)."""
+        return not any(self._host) if self._host is not None else not bool(self.lengths.any())
+
     def make_mask(self, N: int, return_array: bool = False, window_size: int | None = None,
                   **kwargs):
         """``"causal"``, the mask of new queries (no array: see ``sdpa``)."""

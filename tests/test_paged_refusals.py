@@ -442,3 +442,18 @@ def test_more_threads_than_a_launch_counts_are_refused(heads):
         for n in (-(-read // heads), 2 ** 31 // heads, 2 ** 31 - 1):
             assert lib.ss_read_paged(at, FAKE, n, FAKE, FAKE, None) == -2
         assert b"too many" in lib.ss_last_error()
+
+
+def test_a_cache_says_whether_it_is_empty(on_cpu, monkeypatch):
+    """As the other caches do; with lengths that the host knows or not."""
+    monkeypatch.setattr(paged, "_launch", lambda *a: None)
+    c = small_cache()
+    assert c.empty()
+    c.step([0, 2])
+    assert not c.empty()
+    c.release([1])
+    assert c.empty()
+    c.step(ints(1, 0), 1)  # (nothing runs here: the lengths on the device are still 0)
+    assert c.empty()
+    c.lengths[1] = 3
+    assert not c.empty()
