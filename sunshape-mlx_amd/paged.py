@@ -409,21 +409,26 @@ class PagedKVCache:
     def step(self, new_lengths, n_tokens: int | None = None, *,
              max_new: int | None = None) -> BlockPlan:
         """Schedule a step in which request r adds ``new_lengths[r]`` tokens
-        (negative: gives its last ones back; minus its length: ends).  A list
-        of ints is checked here and raises when the step is impossible; it
-        cannot be captured.  An int32 tensor on the GPU needs ``n_tokens``, at
-        least the sum of what is added (``max_new``, the most one adds, sizes
-        later launches); whether the step was possible is then seen by
-        ``check``."""
-        host, bound = None, self._bound
+        (negative: gives its last ones back; minus its length: ends).
+
+        A list of ints raises here when the step is impossible, as long as the
+        host knows the lengths: until a first step given as a tensor.  It
+        cannot be captured.
+
+        An int32 tensor on the GPU needs ``n_tokens``, at least the sum of what
+        is added (``max_new``, the most one adds, sizes later launches).  It is
+        held to what a row of the block table takes, ``max_tokens`` rounded up
+        to whole pages; whether it was possible is seen by ``check``, as with a
+        list whose lengths only the GPU knows."""
+        host, bound, row = None, self._bound, self.block_table.shape[1] * self.page_size
         if isinstance(new_lengths, torch.Tensor):
             if n_tokens is None:
                 raise ValueError("n_tokens is required with new_lengths on the GPU")
             new = new_lengths
             most = min(n_tokens, n_tokens if max_new is None else max_new)
-            bound = min(self.max_tokens, bound + max(0, most))
+            bound = min(row, bound + max(0, most))
             if _capturing(self.lengths):  # (replays add to the lengths too)
-                bound = self.max_tokens
+                bound = row
         else:
             if _capturing(self.lengths):
                 raise RuntimeError("a step given as a list cannot be captured (its replays would not "
@@ -445,7 +450,7 @@ class PagedKVCache:
                     raise RuntimeError(f"{pages} pages needed, {self.free_pages.shape[0]} there")
                 bound = max(host)
             else:
-                bound = min(self.max_tokens, bound + max(0, most))
+                bound = min(row, bound + max(0, most))
             new = torch.tensor(adds, dtype=torch.int32).to(self.lengths.device)
         plan = build_block_tables(self.lengths, new, self.block_table, self.free_pages,
                                   self.n_free, self.page_size, n_tokens,

@@ -457,3 +457,18 @@ def test_a_cache_says_whether_it_is_empty(on_cpu, monkeypatch):
     assert c.empty()
     c.lengths[1] = 3
     assert not c.empty()
+
+
+def test_the_bound_follows_what_tensor_steps_may_add(on_cpu, monkeypatch):
+    """Lengths given on the GPU are held to a table row's whole pages, which
+    may pass max_tokens; launches are sized for as many."""
+    monkeypatch.setattr(paged, "_launch", lambda *a: None)
+    for captured, bounds in ((False, (90, 128, 128)), (True, (128, 128, 128))):
+        monkeypatch.setattr(paged, "_capturing", lambda t: captured)
+        c = small_cache()  # (100 tokens, pages of 32)
+        for bound in bounds:
+            c.step(ints(90, 1), 91, max_new=90)
+            assert c._bound == bound
+    monkeypatch.setattr(paged, "_capturing", lambda t: False)
+    with pytest.raises(ValueError, match="within 0 .. 100"):
+        small_cache().step([101, 0])
