@@ -151,3 +151,58 @@ class Pages:
                 positions.append(pos)
             self.lengths[r] += x
         return np.array(slots, np.int64), np.array(positions, np.int64)
+
+
+def attend_l2(q, store, table, lengths, starts, scale, causal=True):
+    """(out, bound): the attention in 64 bits and, per row and query head, how
+    far in L2 the kernels' roundings take it: for ordinary inputs, whose
+    roundings' signs are as good as independent.  ``attend`` adds the largest
+    of every error up and lets half an output pass where many tokens average;
+    here each enters by its square, at its largest (true ones have a third of
+    that in the mean, so a right result lies near 0.6 of the bound):
+
+    - the output's rounding, u |o|;
+    - of token t, p 2^-11 times s |c - 7.5| (p s rounded) or 2 |v| (p and v);
+    - a score's error e, p e |v - o|: sqrt(D) additions' roundings of 2^-24 of
+      sums that are around 80 s |q| (codes enter as 64 + c), and 2^-22 more;
+    - sums over the tokens, sqrt(T / 32 + 64) roundings of 2^-24 of 160 sum(p s)."""
+    k_c, v_c, k_m, v_m = unpack(store)
+    page = store[0].shape[2]
+    k_all, v_all = values_of(k_c, k_m), values_of(v_c, v_m)
+    n_rows, hq, d = q.shape
+    rep = hq // k_c.shape[1]
+    out = torch.zeros((n_rows, hq, d), dtype=torch.float64)
+    bound = torch.zeros((n_rows, hq), dtype=torch.float64)
+    q64, starts, u = q.cpu().double(), starts.cpu().tolist(), U16[q.dtype]
+    for r, length in enumerate(lengths.cpu().tolist()):
+        n = starts[r + 1] - starts[r]
+        if n == 0 or length == 0:
+            continue
+        at = slots_of(table[r], length, page)
+        pos = torch.arange(length)
+        for h in range(k_c.shape[1]):
+            k, v, group = k_all[at, h], v_all[at, h], d // k_m.shape[2]
+            ks = k_m[at, h, :, 0].double()
+            vs = v_m[at, h, :, 0].double().repeat_interleave(group, 1)
+            token = torch.maximum(vs * (v_c[at, h] - 7.5).abs(), 2.002 * v.abs()) * 2.0 ** -11
+            for i in range(n):
+                rows = slice(h * rep, (h + 1) * rep)
+                qr = q64[starts[r] + i, rows]
+                see = pos <= length - n + i if causal else pos >= 0
+                if not bool(see.any()):
+                    continue
+                p = torch.softmax((qr @ k[see].t()) * scale, -1)
+                o = p @ v[see]
+                qg = qr.unflatten(-1, (-1, group)).norm(dim=-1)
+                e = 2.0 ** -24 * d ** 0.5 * 80 * abs(scale) * (qg @ ks[see].t()) + 2.0 ** -22
+                sums = 2.0 ** -24 * (length / 32 + 64) ** 0.5 * 160 * (p @ vs[see])
+                vo = (v[see][None] - o[:, None]).square().sum(-1)
+                square = (u * o).square().sum(-1) + p.square() @ token[see].square().sum(-1) + \
+                    (p * e).square().mul(vo).sum(-1) + sums.square().sum(-1)
+                out[starts[r] + i, rows], bound[starts[r] + i, rows] = o, square.sqrt()
+    return out, bound
+
+
+def within_l2(got, want, bound):
+    """Whether every row and head of ``got`` lies within the bound."""
+    return bool(((got.cpu().double() - want).norm(dim=-1) <= bound).all())
