@@ -97,3 +97,72 @@ def test_large_calls_of_more_requests_than_a_wave_has_lanes(b):
                       max_new=150, max_length=900)
     check_some(given, q, store, table, le, starts, 0.125, some)
     assert (given[sum(new):] == 7).all()
+
+
+@pytest.mark.parametrize("large", [False, True])
+@pytest.mark.parametrize("dtype,other", [HALF, HALF[::-1]])
+@pytest.mark.parametrize("d,group", [(128, 64), (64, 32)])
+def test_queries_of_the_other_type(request, d, group, dtype, other, large):
+    """Queries and stores need not share a type; the output has the queries'."""
+    if large:
+        request.getfixturevalue("wide")
+    store, table, le, starts = world(15, [150, 33, 90], [70, 1, 3], 2, d, group, 16, dtype)
+    q = rows(16, 74, 8, d, other, False)
+    out = S.paged_attention(q, store, table, le, starts, d ** -0.5)
+    assert out.dtype is other and R.within_l2(out, *R.attend_l2(q, store, table, le, starts, d ** -0.5))
+
+
+@pytest.mark.parametrize("large", [False, True])
+@pytest.mark.parametrize("page", [256, 512, 1024])
+def test_large_pages(request, page, large):
+    if large:
+        request.getfixturevalue("wide")
+    store, table, le, starts = world(17, [1500, 1025, 1024, 3], [90, 1, 4, 3], 2, 64, 64, page, torch.float16)
+    q = rows(18, 98, 4, 64, torch.float16, False)
+    out = S.paged_attention(q, store, table, le, starts, 0.125)
+    assert R.within_l2(out, *R.attend_l2(q, store, table, le, starts, 0.125))
+
+
+@pytest.mark.parametrize("large", [False, True])
+@pytest.mark.parametrize("hq", [96, 128, 1024])
+def test_many_query_heads_to_one(request, hq, large):
+    """More rows of one token than a block, or a tile, has."""
+    if large:
+        request.getfixturevalue("wide")
+    store, table, le, starts = world(19, [300, 77], [1, 3], 1, 64, 32, 16, torch.bfloat16)
+    q = rows(20, 4, hq, 64, torch.bfloat16, False)
+    out = S.paged_attention(q, store, table, le, starts, 0.125)
+    assert R.within_l2(out, *R.attend_l2(q, store, table, le, starts, 0.125))
+
+
+@pytest.mark.parametrize("large", [False, True])
+def test_more_new_tokens_than_a_request_holds(request, large):
+    """Rows before the request's first token see nothing and are zero."""
+    if large:
+        request.getfixturevalue("wide")
+    store, table, le, starts = world(21, [3, 40, 1], [70, 2, 100], 2, 64, 64, 16, torch.float16)
+    q = rows(22, 172, 4, 64, torch.float16, False)
+    out = S.paged_attention(q, store, table, le, starts, 0.125)
+    assert R.within_l2(out, *R.attend_l2(q, store, table, le, starts, 0.125))
+    assert (out[:67] == 0).all() and (out[72:171] == 0).all() and (out[67:72] != 0).any(-1).all()
+
+
+def test_thousands_of_requests():
+    """Dozens of requests a lane, most of them without new tokens."""
+    rng = random.Random(3)
+    lengths = [rng.choice([0, 1, 5, 30]) for _ in range(5000)]
+    new = [min(n, rng.choice([0, 0, 0, 1])) for n in lengths]
+    store, table, le, starts = world(23, lengths, new, 2, 64, 64, 16, torch.float16)
+    q = rows(24, sum(new), 4, 64, torch.float16, False)
+    want, bound = R.attend_l2(q, store, table, le, starts, 0.125)
+    for hints in ({}, dict(max_new=1, max_length=30)):
+        assert R.within_l2(S.paged_attention(q, store, table, le, starts, 0.125, **hints), want, bound)
+
+
+def test_requests_that_share_pages():
+    """Two requests over the same first pages, as after a fork of a prompt."""
+    store, table, le, starts = world(25, [64, 90], [1, 1], 2, 64, 64, 16, torch.float16)
+    table[0, :3], le = table[1, :3], ints([48, 90])
+    q = rows(26, 2, 4, 64, torch.float16, False)
+    out = S.paged_attention(q, store, table, le, starts, 0.125)
+    assert R.within_l2(out, *R.attend_l2(q, store, table, le, starts, 0.125))
