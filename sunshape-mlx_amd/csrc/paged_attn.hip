@@ -22,12 +22,18 @@ constexpr int kStages = 4;         // tiles of a wave in LDS, one computed while
 constexpr int kNt = 2;
 // Requests of more than kPromptRows query rows a KV head are the prompt
 // kernel's, where this one would have more than kPromptUnits units a compute
-// unit (twice that at 64 dims).  At 8192 tokens and 64 (request, head) columns
-// 64 rows take 88 us here and 113 us there, 96 rows 131 and 114 us.  Smaller
-// calls, here and there: a prompt of 128 tokens and 32 heads 8.8 and 21 us,
-// 512 tokens (16 units) 32 and 39, 640 tokens (25) 52 and 43; 24 tokens at
-// 8192 (12) 31 and 49 us; at 64 dims, 1024 tokens of 16 heads (32) 21 and 36.
-constexpr int kPromptRows = 64, kPromptUnits = 16;
+// unit (at 128 dims; half as much work each at 64) than that one: a column
+// costs kColumnUnits beside its units (queries, tables, the join), and a unit of
+// a tile of 256 rows there kTileUnits of those here.  Fitted to 888 shapes (1 to
+// 32 requests of 17 to 1024 new tokens at up to 8192, 1 to 8 rows a token, all
+// groups): the kernel that is taken is 1.5 % behind the better one in the mean
+// (work alone, without columns and tiles: 8.6 %).  Here and there: 64 rows of 64
+// (request, head) columns at 8192 tokens 88 and 113 us, 96 rows 131 and 114; a
+// prompt of 128 tokens and 32 heads 8.8 and 21 us, 512 tokens 32 and 39, 640
+// tokens 52 and 43; 32 prompts of 64 tokens 72 and 22; 24 tokens of 8 requests at
+// 2048 39 and 49, at 8192 tokens of one 30 and 51.  Below kPromptRows 256-row tiles
+// are mostly empty.
+constexpr int kPromptRows = 64, kPromptUnits = 32, kColumnUnits = 6, kTileUnits = 3;
 // Columns of at most kWhole units are not cut, twice that if there are enough
 // of them to give every second compute unit one: a cut adds a launch and a
 // pass over the parts.  1 request of 8 heads, 640 tokens: 9.8 us whole, 11.7
@@ -645,7 +651,7 @@ struct PagedPlan {
 // unit), or as the hints' units need.
 static PagedPlan paged_plan(const ss_paged_store *s, int64_t n_tokens, int64_t n_requests, int n_q_heads,
                             int64_t max_new, int64_t max_length) {
-    PagedPlan p;
+    PagedPlan p{};
     const int rep = n_q_heads / s->n_kv_heads, rs = 16 / (s->head_dim / s->group_size);
     int64_t rows = max_new * rep;
     p.sets = rows > rs ? 2 : 1;
@@ -656,8 +662,15 @@ static PagedPlan paged_plan(const ss_paged_store *s, int64_t n_tokens, int64_t n
         return s->n_kv_heads * min((double)n_requests * ((rows + p.rows - 1) / p.rows),
                                    (double)(n_tokens * rep / p.rows) + (double)n_requests);
     };
-    p.prompts = rows > kPromptRows && columns_of(rows) * units * s->head_dim >
-                                           128. * kPromptUnits * device_cu_count();
+    if (rows > kPromptRows) {
+        // what is more than a token a request, in as few requests as it fits
+        const double more = (double)max(n_tokens - n_requests, (int64_t)0) * rep;
+        const double longs = min((double)n_requests, ceil(more / rows));
+        const double columns = s->n_kv_heads * (more / p.rows + longs);
+        const double tiles = s->n_kv_heads * longs * (double)((rows + kPromptTile - 1) / kPromptTile);
+        p.prompts = kColumnUnits * columns + (columns - kTileUnits * tiles) * units * s->head_dim / 128. >
+                    (double)kPromptUnits * device_cu_count();
+    }
     if (p.prompts) rows = kPromptRows;
     const double columns = columns_of(rows);
     p.cut = units > (2 * columns < device_cu_count() ? kWhole : 2 * kWhole);

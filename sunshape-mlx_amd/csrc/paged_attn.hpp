@@ -207,6 +207,8 @@ __device__ __forceinline__ float column_max(const float (&x)[N]) {
     return m;
 }
 
+constexpr int kPromptTile = 256;  // query rows of a workgroup of the prompt kernel
+
 // The requests with more than most_rows query rows a KV head (paged_prompt.hip),
 // with `workspace` of paged_prompt_bytes for n_tokens * rep rows in all (with
 // less no column is cut).

@@ -33,6 +33,7 @@ typedef __bf16 bf8_t __attribute__((ext_vector_type(8)));
 
 constexpr int kPWaves = 8;
 constexpr int kRows = 32 * kPWaves;  // query rows of a workgroup
+static_assert(kRows == kPromptTile, "the rows that launches are planned for");
 constexpr int kTokens = 64;          // of a tile
 constexpr int kSlots = 3;            // tiles in LDS as they come: one being prepared, two on their way
 // Fewest tiles of a part, where a workgroup's column is cut (1024 tokens, 32
