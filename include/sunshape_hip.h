@@ -1074,7 +1074,8 @@ int ss_block_tables(const int32_t *lengths, const int32_t *new_lengths, int64_t 
  * elements, rounded to the store's dtype first).  Per group: zero = the
  * smallest value, scale = (largest - smallest)/15 rounded to the store's
  * dtype, code = the nearest of 0 .. 15 to (x - zero)/scale, ties to even (0
- * where the scale is 0).  A group with an infinity or NaN is stored as NaN.
+ * where the scale is 0).  A group with an infinity or NaN, or whose range
+ * passes float32, is stored as NaN.
  * Tokens whose slot is negative or outside the pool are not stored.  Slots
  * must be distinct: the content of one that is given twice is undefined.
  * n_tokens (in whole blocks of 8) * n_kv_heads is at most 2^29 - 32.

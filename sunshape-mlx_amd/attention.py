@@ -532,7 +532,8 @@ def sunshape_sdpa(queries: torch.Tensor,
     Returns (B, n_q_heads, T_q, D) in the query dtype, as the reference does
     (attention.py:292, 304), or in ``out_dtype`` when given (an extension:
     float32 keeps the kernels' fp32 accumulation in the result).  A
-    ``PagedKVCache`` takes None and ``"causal"``, in the query dtype."""
+    ``PagedKVCache`` takes None and ``"causal"`` and float16 or bfloat16 queries,
+    in whose dtype it returns."""
     if isinstance(cache, PagedKVCache):
         if out_dtype not in (None, queries.dtype):
             raise ValueError(f"a paged cache's output has the query dtype, not {out_dtype}")

@@ -134,8 +134,8 @@ __device__ __forceinline__ float groups_sum(float v) {
 // 16/G query rows share the stream.
 //
 // Long caches are bound by HBM and, nearly as much, by the vector ALUs (65 % of
-// the cycles): 8 requests of up to 32768 tokens, 8 heads, 195 MB, take 41 us,
-// 4.7 TB/s.  One such request, 38 MB, takes 17 us: tables, queries, four tiles
+// the cycles): 8 requests of up to 32768 tokens, 8 heads, 195 MB, take 42 us,
+// 4.6 TB/s.  One such request, 38 MB, takes 17 us: tables, queries, four tiles
 // a wave and the join follow each other.
 template <int D, int G, bool BF, int NS>
 __global__ void __launch_bounds__(256, 2) paged_attn_kernel(const PagedAttn a) {
@@ -342,7 +342,8 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(const PagedAttn a) {
         if (a.causal) all_see = max(0, min(rq.len, rq.len - rq.n_all + rb * ROWS / a.rep + 1));
 
         // Probabilities are kept times 2^kProb, so that a sum of bfloat16's largest
-        // values stays finite; p * scale enters the products times 2^(kScaled -
+        // values stays finite (up to 2^20 tokens) and values down to 2^-102 keep
+        // their bits; p * scale enters the products times 2^(kScaled -
         // vexp): vexp is above every value scale (as a power of two) that the
         // column's group has met, so it stays within fp16 whatever the scales.
         // top is in units of S.

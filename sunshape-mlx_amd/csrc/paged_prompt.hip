@@ -22,8 +22,8 @@
 // scale and sum, 32 exponentials), so what does not depend on the row is done
 // once a workgroup.  32 rows a wave and 64 tokens are what the 256 registers of
 // two waves a SIMD hold.  A prompt of 4093 tokens, 32 heads, 137 GFLOP, takes
-// 262 us back to back under the profiler, 220 us between other calls: 0.5 to
-// 0.6 PFLOP/s, vector ALUs 48 % of the cycles, matrix cores 28 %.
+// 266 us back to back under the profiler, 230 us between other calls: 0.5 to
+// 0.6 PFLOP/s, vector ALUs 49 % of the cycles, matrix cores 27 %.
 #include "paged_attn.hpp"
 
 namespace ss {

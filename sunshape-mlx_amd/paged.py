@@ -17,7 +17,7 @@ A row of ``head_dim`` values is held in groups of ``group_size``: zero = the
 group's smallest value, scale = (largest - smallest) / 15 in the cache's
 16-bit type, and a 4-bit code per value, the nearest of 0 .. 15 to
 (x - zero) / scale; the held value is zero + code * scale.  A group with an
-infinity or NaN is held as NaN.
+infinity or NaN, or whose range passes float32, is held as NaN.
 """
 
 from __future__ import annotations
