@@ -397,6 +397,7 @@ class PagedKVCache:
         self.free_pages = torch.arange(n_pages, dtype=torch.int32, device=dev)
         self.n_free = torch.full((1,), n_pages, dtype=torch.int32, device=dev)
         self.plan: BlockPlan | None = None  # of the last step
+        self._kept: list[BlockPlan] = []    # of steps that graphs go on reading
         self._version = 0                   # bumped by every change of the stored tokens
         # what the host knows of the lengths: all of them (steps given as
         # lists), or a bound
@@ -419,7 +420,10 @@ class PagedKVCache:
         is added (``max_new``, the most one adds, sizes later launches).  It is
         held to what a row of the block table takes, ``max_tokens`` rounded up
         to whole pages; whether it was possible is seen by ``check``, as with a
-        list whose lengths only the GPU knows."""
+        list whose lengths only the GPU knows.  Captured, it goes into the graph
+        with its append and attend, and the plan holds what the last replay
+        made of it; a graph with append or attend alone goes on with the slots
+        and starts of the step that they were captured after."""
         host, bound, row = None, self._bound, self.block_table.shape[1] * self.page_size
         if isinstance(new_lengths, torch.Tensor):
             if n_tokens is None:
@@ -466,20 +470,24 @@ class PagedKVCache:
         if self.plan is not None:
             check_plan(self.plan)
 
+    def _last_plan(self, name: str) -> BlockPlan:
+        if self.plan is None:
+            raise RuntimeError(f"{name} needs a step first")
+        if _capturing(self.lengths) and (not self._kept or self._kept[-1] is not self.plan):
+            # the graph reads it after the next step has replaced it here
+            self._kept.append(self.plan)
+        return self.plan
+
     def append(self, keys: torch.Tensor, values: torch.Tensor) -> None:
         """Store the keys and values (N, H, D) of the last step's tokens."""
-        if self.plan is None:
-            raise RuntimeError("append needs a step first")
-        append_paged(self.store, keys, values, self.plan.slots)
+        append_paged(self.store, keys, values, self._last_plan("append").slots)
         self._version += 1
 
     def attend(self, queries: torch.Tensor, scale: float, *, causal: bool = True,
                out: torch.Tensor | None = None) -> torch.Tensor:
         """Attention of the last step's tokens' queries (N, Hq, D)."""
-        if self.plan is None:
-            raise RuntimeError("attend needs a step first")
         return paged_attention(queries, self.store, self.block_table, self.lengths,
-                               self.plan.token_starts, scale, causal=causal,
+                               self._last_plan("attend").token_starts, scale, causal=causal,
                                max_new=self._max_new, max_length=max(1, self._bound), out=out)
 
     def release(self, requests) -> None:

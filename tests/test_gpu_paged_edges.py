@@ -303,3 +303,29 @@ def test_starts_that_descend_name_no_rows(max_new):
 
 def test_large_attention_of_starts_that_descend(wide):
     test_starts_that_descend_name_no_rows(64)
+
+
+def test_attention_captured_without_its_step():
+    """append and attend of an eager step in a graph: replays give the same
+    after other steps have come and their plans gone."""
+    hq, hkv, d = 8, 2, 64
+    c = S.PagedKVCache(n_requests=2, n_kv_heads=hkv, head_dim=d, max_tokens=900, page_size=16)
+    c.step([300, 500])
+    c.append(rows(111, 800, hkv, d, torch.float16), rows(112, 800, hkv, d, torch.float16, False))
+    c.step([1, 3])
+    k, v, q = (rows(113 + i, 4, h, d, torch.float16) for i, h in enumerate((hkv, hkv, hq)))
+    c.append(k, v)
+    want = c.attend(q, 0.125)
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        c.append(k, v)
+        out = c.attend(q, 0.125)
+    for _ in range(4):
+        c.step([2, 1])  # other plans, and back again
+        c.step([-2, -1])
+        junk = [torch.full((n,), -1, dtype=torch.int32, device=DEV) for n in (13, 15, 17, 19)]
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+        del junk

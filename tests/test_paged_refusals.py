@@ -472,3 +472,29 @@ def test_the_bound_follows_what_tensor_steps_may_add(on_cpu, monkeypatch):
     monkeypatch.setattr(paged, "_capturing", lambda t: False)
     with pytest.raises(ValueError, match="within 0 .. 100"):
         small_cache().step([101, 0])
+
+
+def test_a_plan_that_a_graph_reads_stays(on_cpu, monkeypatch):
+    """append and attend captured after an eager step read its plan at every
+    replay: its memory is not given back when the next step replaces it."""
+    import weakref
+
+    monkeypatch.setattr(paged, "_launch", lambda *a: None)
+    c = small_cache()
+    z, q = torch.zeros(2, 2, 128), torch.zeros(2, 4, 128, dtype=torch.float16)
+
+    def slots_after(captured):
+        c.step([1, 1])
+        monkeypatch.setattr(paged, "_capturing", lambda t: captured)
+        c.append(z, z)
+        c.attend(q, 0.1)
+        c.attend(q, 0.1)
+        monkeypatch.setattr(paged, "_capturing", lambda t: False)
+        slots = weakref.ref(c.plan.slots)
+        c.step([1, 1])
+        return slots()
+
+    assert slots_after(False) is None
+    assert slots_after(True) is not None and len(c._kept) == 1
+    with pytest.raises(RuntimeError, match="attend needs a step"):
+        small_cache().attend(q, 0.1)
