@@ -1085,6 +1085,42 @@ int ss_append_paged(const ss_paged_store *store, const void *keys, const void *v
                     int64_t v_sh, const int32_t *slots, void *stream);
 
 /*
+ * The same append with the layer's norms and rotation on the way: queries and
+ * keys are normalised head by head (where there is a weight) and rotated by
+ * their positions, keys and values quantised into their slots as
+ * ss_append_paged does.  Element d of token t and head h is at
+ * queries[t*q_st + h*q_sh + d] (keys: k_st, k_sh; values: v_st, v_sh).
+ *   y = (x r) w with r = 1/sqrt(mean(x^2) + eps), mean and root in 64 bits and
+ *   rounded to float32 once; a pair (a, b) becomes (a c - b s, b c + a s).
+ * Every operation is rounded to float32 by itself.  Pairs are dims (i,
+ * i + rotary_dim/2), or (2i, 2i + 1) with `neighbours`; dims from rotary_dim on
+ * stay as they are.  table: float32 [n_positions][rotary_dim/2][2], cosine and
+ * sine of each position and pair.  A position past its end makes the turned
+ * dims NaN.
+ *   out  [n_tokens][n_q_heads][head_dim]: the queries, rounded once to in_dtype
+ *        (float32 ones to the store's dtype); may be `queries` itself where
+ *        that is laid out alike.  Rows of tokens whose position is negative
+ *        are zeroed if zero_rest, else left; their keys and values are not
+ *        stored, whatever their slots.
+ * rotary_dim a multiple of 16 up to head_dim; table and out 16-byte aligned;
+ * weights [head_dim] of weight_dtype.  Tokens in whole blocks of 8, times query
+ * and KV heads together, are at most 2^29 - 32.
+ */
+typedef struct {
+    const void *table;
+    int64_t n_positions;
+    int rotary_dim, neighbours;
+    const void *q_weight, *k_weight; /* NULL: no norm */
+    double eps;
+    int weight_dtype;
+} ss_rotation;
+int ss_append_rotated_paged(const ss_paged_store *store, const void *queries, const void *keys,
+                            const void *values, int in_dtype, int64_t n_tokens, int n_q_heads,
+                            int64_t q_st, int64_t q_sh, int64_t k_st, int64_t k_sh, int64_t v_st,
+                            int64_t v_sh, const int32_t *slots, const int32_t *positions,
+                            const ss_rotation *rotation, void *out, int zero_rest, void *stream);
+
+/*
  * What the slots hold: keys and values [n_tokens][n_kv_heads][head_dim] in
  * the store's dtype (zeros for a slot outside the pool).  n_tokens *
  * n_kv_heads is at most 2^28 - 16 (head_dim 128) or 2^29 - 32 (64).

@@ -62,10 +62,12 @@ from .paged import (  # noqa: E402
     PagedKVCache,
     PagedKVStore,
     append_paged,
+    append_rotated_paged,
     build_block_tables,
     check_plan,
     paged_attention,
     read_paged,
+    rotary_table,
 )
 from .serialize import load_cache, load_codec, save_cache, save_codec  # noqa: E402
 
@@ -79,5 +81,5 @@ __all__ = [
     "reset_kernel_stats", "apply_permutation", "invert_permutation", "generate_rotation_matrix",
     "covariance_block_permutation", "save_codec", "load_codec", "save_cache", "load_cache",
     "PagedKVCache", "PagedKVStore", "BlockPlan", "build_block_tables", "check_plan", "append_paged", "read_paged",
-    "paged_attention",
+    "paged_attention", "append_rotated_paged", "rotary_table",
 ]

@@ -8,6 +8,8 @@ step runs without the host knowing any length:
 ``build_block_tables``  pages, slots and positions of a step from the
                         requests' lengths, on the GPU
 ``append_paged``        quantise the new tokens into their slots
+``append_rotated_paged``  the same with the norms and the rotation of queries
+                        and keys on the way (``rotary_table``)
 ``read_paged``          what slots hold
 ``paged_attention``     the new tokens' queries over their requests
 ``PagedKVCache``        the four tied together; ``sunshape_sdpa`` and the SDPA
@@ -44,6 +46,15 @@ class _Store(ctypes.Structure):
                 ("n_pages", ctypes.c_int64), ("n_kv_heads", ctypes.c_int),
                 ("head_dim", ctypes.c_int), ("group_size", ctypes.c_int),
                 ("page_size", ctypes.c_int), ("dtype", ctypes.c_int)]
+
+
+class _Rotation(ctypes.Structure):
+    """``ss_rotation``."""
+
+    _fields_ = [("table", ctypes.c_void_p), ("n_positions", ctypes.c_int64),
+                ("rotary_dim", ctypes.c_int), ("neighbours", ctypes.c_int),
+                ("q_weight", ctypes.c_void_p), ("k_weight", ctypes.c_void_p),
+                ("eps", ctypes.c_double), ("weight_dtype", ctypes.c_int)]
 
 
 class PagedKVStore(NamedTuple):
@@ -145,8 +156,8 @@ def _struct(store: PagedKVStore) -> _Store:
 
 
 # names of the dispatch counters (get_kernel_stats)
-_STATS = {f"ss_{n}": f"{n}_hip" for n in ("block_tables", "append_paged", "read_paged",
-                                          "paged_attn")}
+_STATS = {f"ss_{n}": f"{n}_hip" for n in ("block_tables", "append_paged", "append_rotated_paged",
+                                          "read_paged", "paged_attn")}
 _CODE = {torch.float32: _hip.SS_F32, torch.float16: _hip.SS_F16, torch.bfloat16: _hip.SS_BF16}
 
 
@@ -268,6 +279,111 @@ def append_paged(store: PagedKVStore, keys: torch.Tensor, values: torch.Tensor,
             k.stride(0), k.stride(1), v.stride(0), v.stride(1), at_slots)
 
 
+def rotary_table(n_positions: int, rotary_dim: int, base: float = 10000.0, *,
+                 frequencies: torch.Tensor | None = None, device=None) -> torch.Tensor:
+    """Cosines and sines of ``append_rotated_paged``, (n_positions,
+    rotary_dim / 2, 2) float32: pair i of position p turns by p *
+    frequencies[i] (by default base^(-2i / rotary_dim)), an angle in 64 bits."""
+    if n_positions < 1 or rotary_dim < 16 or rotary_dim % 16:
+        raise ValueError(f"n_positions must be positive and rotary_dim a multiple of 16 (got "
+                         f"{n_positions}, {rotary_dim})")
+    dev = torch.device("cuda") if device is None else torch.device(device)
+    half = rotary_dim // 2
+    if frequencies is None:
+        if not 0.0 < base < float("inf"):
+            raise ValueError(f"base must be positive, got {base}")
+        freq = float(base) ** (-torch.arange(half, dtype=torch.float64, device=dev) / half)
+    else:
+        freq = torch.as_tensor(frequencies, dtype=torch.float64, device=dev)
+        if freq.shape != (half,):
+            raise ValueError(f"{half} frequencies expected, got {tuple(freq.shape)}")
+    angle = torch.arange(n_positions, dtype=torch.float64, device=dev)[:, None] * freq
+    return torch.stack((angle.cos(), angle.sin()), -1).float()
+
+
+def _no_derivative(name: str, *tensors) -> None:
+    """Refuse tensors through which something is differentiated."""
+    for t in tensors:
+        if t is None:
+            continue
+        if t.requires_grad and torch.is_grad_enabled():
+            raise ValueError(f"{name} has no backward pass: call it under torch.no_grad()")
+        if _forward_ad._current_level >= 0 and _forward_ad.unpack_dual(t).tangent is not None:
+            raise ValueError(f"{name} has no forward-mode derivative: unpack its dual tensors")
+
+
+def append_rotated_paged(store: PagedKVStore, queries: torch.Tensor, keys: torch.Tensor,
+                         values: torch.Tensor, slots: torch.Tensor, positions: torch.Tensor,
+                         rotary: torch.Tensor, *, q_weight: torch.Tensor | None = None,
+                         k_weight: torch.Tensor | None = None, eps: float = 1e-6,
+                         neighbours: bool = False,
+                         out: torch.Tensor | None = None) -> torch.Tensor:
+    """``append_paged`` of keys that are normalised and rotated on the way;
+    returns the ``queries`` (N, Hq, D), normalised and rotated too, in their
+    type (float32 ones in the store's).  All of one type, float16, bfloat16 or
+    float32; keys and values (N, H, D).
+
+    ``q_weight``, ``k_weight`` (D,): y = x / sqrt(mean(x^2) + eps) * weight, head
+    by head (no norm without one).  ``rotary`` (n_positions, R/2, 2) float32:
+    cosine and sine of each position (``rotary_table``); the first R dims turn,
+    pairs are (i, i + R/2) or, with ``neighbours``, (2i, 2i + 1).  Each operation
+    is rounded to float32 by itself, the result once.  ``positions`` (N,) int32,
+    as ``build_block_tables`` gives them: a token with a negative one is not
+    stored, and its query is zero, or, with ``out``, left as it was (``out`` may
+    be contiguous ``queries``).  A position past the table makes the turned dims
+    NaN.  Queries or weights under autograd are refused; keys and values are
+    stored without a derivative."""
+    st = _struct(store)
+    dev, device = store[0].get_device(), store[0].device
+    d = st.head_dim
+    if queries.dim() != 3 or queries.shape[1] < 1 or slots.dim() != 1:
+        raise ValueError("queries (N, Hq, D) and slots (N,) expected")
+    n, hq, _ = queries.shape
+    if queries.dtype is not keys.dtype:
+        raise TypeError("queries, keys and values must share a dtype")
+    _no_derivative("append_rotated_paged", queries, q_weight, k_weight)
+    at_slots = _index("slots", slots, (n,), dev)
+    at_positions = _index("positions", positions, (n,), dev)
+    k, v, code = _new_rows(keys, values, (n, st.n_kv_heads, d), dev)
+    q = _rows("queries", queries, (n, hq, d), dev)
+    if not rotary.is_cuda:
+        _hip.require_gpu(rotary)
+    if rotary.dtype is not torch.float32:
+        raise TypeError(f"rotary must be float32, not {rotary.dtype}")
+    if rotary.dim() != 3 or rotary.shape[2] != 2 or not rotary.is_contiguous() or \
+            rotary.get_device() != dev:
+        raise ValueError(f"rotary must be contiguous (n_positions, R/2, 2) on cuda:{dev}, got "
+                         f"{tuple(rotary.shape)} on {rotary.device}")
+    w_type, w_at = 0, []
+    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
+        if w is None:
+            w_at.append(None)
+            continue
+        if not w.is_cuda:
+            _hip.require_gpu(w)
+        if w.shape != (d,) or not w.is_contiguous() or w.get_device() != dev:
+            raise ValueError(f"{name} must be contiguous ({d},) on cuda:{dev}, got "
+                             f"{tuple(w.shape)} on {w.device}")
+        if w_at and w_at[0] is not None and w.dtype is not q_weight.dtype:
+            raise TypeError("q_weight and k_weight must share a dtype")
+        w_type = _hip.dtype_code(w.dtype)
+        w_at.append(w.data_ptr())
+    dtype = store[2].dtype if queries.dtype is torch.float32 else queries.dtype
+    zero_rest = out is None
+    if zero_rest:
+        out = torch.empty((n, hq, d), dtype=dtype, device=device)
+    elif out.shape != (n, hq, d) or out.dtype is not dtype or out.device != device or \
+            not out.is_contiguous():
+        raise ValueError(f"out must be contiguous {dtype} {(n, hq, d)} on {device}")
+    ro = _Rotation(rotary.data_ptr(), rotary.shape[0], 2 * rotary.shape[1], neighbours, *w_at, eps,
+                   w_type)
+    _launch("ss_append_rotated_paged", dev, ctypes.addressof(st), q.data_ptr(), k.data_ptr(),
+            v.data_ptr(), code, n, hq, q.stride(0), q.stride(1), k.stride(0), k.stride(1),
+            v.stride(0), v.stride(1), at_slots, at_positions, ctypes.addressof(ro), out.data_ptr(),
+            zero_rest)
+    return out
+
+
 def read_paged(store: PagedKVStore, slots: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """(keys, values) that ``slots`` (N,) hold, (N, H, D) in the store's type
     (zeros for a slot outside the pool)."""
@@ -321,10 +437,7 @@ def paged_attention(queries: torch.Tensor, store: PagedKVStore, block_table: tor
     dtype = queries.dtype
     if dtype not in _HALF:
         raise TypeError(f"queries must be float16 or bfloat16, not {dtype}")
-    if queries.requires_grad and torch.is_grad_enabled():
-        raise ValueError("paged_attention has no backward pass: call it under torch.no_grad()")
-    if _forward_ad._current_level >= 0 and _forward_ad.unpack_dual(queries).tangent is not None:
-        raise ValueError("paged_attention has no forward-mode derivative: unpack its dual queries")
+    _no_derivative("paged_attention", queries)
     if hq < 1 or hq % st.n_kv_heads:
         raise ValueError(f"{hq} query heads do not share {st.n_kv_heads} KV heads")
     shape = (n, hq, st.head_dim)
@@ -482,6 +595,20 @@ class PagedKVCache:
         """Store the keys and values (N, H, D) of the last step's tokens."""
         append_paged(self.store, keys, values, self._last_plan("append").slots)
         self._version += 1
+
+    def append_rotated(self, queries: torch.Tensor, keys: torch.Tensor, values: torch.Tensor,
+                       rotary: torch.Tensor, *, q_weight: torch.Tensor | None = None,
+                       k_weight: torch.Tensor | None = None, eps: float = 1e-6,
+                       neighbours: bool = False, out: torch.Tensor | None = None) -> torch.Tensor:
+        """``append`` with the norms and the rotation of the last step's tokens
+        on the way (``append_rotated_paged``); returns their queries for
+        ``attend``."""
+        plan = self._last_plan("append_rotated")
+        out = append_rotated_paged(self.store, queries, keys, values, plan.slots, plan.positions,
+                                   rotary, q_weight=q_weight, k_weight=k_weight, eps=eps,
+                                   neighbours=neighbours, out=out)
+        self._version += 1
+        return out
 
     def attend(self, queries: torch.Tensor, scale: float, *, causal: bool = True,
                out: torch.Tensor | None = None) -> torch.Tensor:
