@@ -1161,6 +1161,61 @@ int ss_paged_attn(const ss_paged_store *store, const void *q, int q_dtype, int64
                   int64_t max_length, void *out, int zero_rest, void *workspace,
                   size_t workspace_bytes, void *stream);
 
+/*
+ * The same with other scores and masks, and with requests that continue
+ * others.  Score s = scale q.k of a row at position p with token t becomes
+ *   softcap tanh(s / softcap)      (softcap > 0)
+ *   s - slopes[hq] |p - t|         (slopes: float32 [n_q_heads])
+ * and the row sees the tokens t > p - window (window > 0), of those the ones up
+ * to p, or, causal or not, any below prefix_lengths[r] of its request's.
+ * (Tokens at or behind a row's own that no mask hides count |p - t| too.)
+ * group_starts, group_rows, parents: a plan of ss_shared_plan for these
+ * token_starts; rows of request r with parents[r] >= 0 then see all
+ * lengths[parents[r]] tokens of that request before their own, whose positions
+ * follow them.  Every parent's tokens are read once for all rows that see them.
+ * n_groups and max_shared (how many parents, and their longest length) size the
+ * launch, as max_new and max_length (of own tokens) do.  Not together with a
+ * window or prefix_lengths.
+ * A capped score is off by up to 2^-21 of the largest around it more than others.
+ */
+typedef struct {
+    float softcap;                 /* 0: none */
+    const float *slopes;           /* NULL: none */
+    int64_t window;                /* 0: none */
+    const int32_t *prefix_lengths; /* [n_requests]; NULL: none */
+    const int32_t *group_starts, *group_rows, *parents; /* all three or NULL */
+    int64_t n_groups, max_shared;
+} ss_paged_scores;
+size_t ss_paged_attn_scored_workspace_bytes(const ss_paged_store *store, int64_t n_tokens,
+                                            int64_t n_requests, int n_q_heads, int64_t max_new,
+                                            int64_t max_length, const ss_paged_scores *scores);
+int ss_paged_attn_scored(const ss_paged_store *store, const void *q, int q_dtype, int64_t n_tokens,
+                         int64_t q_st, int64_t q_sh, int n_q_heads, const int32_t *block_table,
+                         int64_t table_width, const int32_t *lengths, const int32_t *token_starts,
+                         int64_t n_requests, float scale, int causal, int64_t max_new,
+                         int64_t max_length, void *out, int zero_rest,
+                         const ss_paged_scores *scores, void *workspace, size_t workspace_bytes,
+                         void *stream);
+
+/*
+ * Which rows continue which request: request r continues parents[r] where that
+ * is another request (0 .. n_requests - 1), else none; a parent's own parent is
+ * not followed.  Rows are the packed new tokens, token_starts as
+ * ss_block_tables gives them.
+ *   group_starts [n_requests + 1], group_rows [n_tokens][2]: the rows that see
+ *     parent p's tokens are entries group_starts[p] .. group_starts[p+1], each a
+ *     token and its position among its request's own tokens
+ *   parents_out [n_requests]: the parents, -1 for none
+ *   offsets [n_requests]: the entry of each such request's first row
+ *   positions [n_tokens] (may be NULL): the tokens' positions behind their
+ *     parents' tokens, -1 behind the last row
+ * token_starts that descend name no rows.  At most 4096 requests.
+ */
+int ss_shared_plan(const int32_t *parents, const int32_t *lengths, const int32_t *token_starts,
+                   int64_t n_requests, int64_t n_tokens, int32_t *group_starts,
+                   int32_t *group_rows, int32_t *parents_out, int32_t *offsets, int32_t *positions,
+                   void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -61,9 +61,11 @@ from .paged import (  # noqa: E402
     BlockPlan,
     PagedKVCache,
     PagedKVStore,
+    SharedPlan,
     append_paged,
     append_rotated_paged,
     build_block_tables,
+    build_shared_plan,
     check_plan,
     paged_attention,
     read_paged,
@@ -82,4 +84,5 @@ __all__ = [
     "covariance_block_permutation", "save_codec", "load_codec", "save_cache", "load_cache",
     "PagedKVCache", "PagedKVStore", "BlockPlan", "build_block_tables", "check_plan", "append_paged", "read_paged",
     "paged_attention", "append_rotated_paged", "rotary_table",
+    "SharedPlan", "build_shared_plan",
 ]

@@ -220,6 +220,8 @@ _SIGNATURES = {
                                _c_void_p, _c_void_p, _c_void_p]),
     "ss_append_paged": (_int, [_c_void_p, _c_void_p, _c_void_p, _int, _i64, _i64, _i64, _i64,
                                _i64, _c_void_p, _c_void_p]),
+    "ss_shared_plan": (_int, [_c_void_p, _c_void_p, _c_void_p, _i64, _i64, _c_void_p, _c_void_p,
+                              _c_void_p, _c_void_p, _c_void_p, _c_void_p]),
     "ss_append_rotated_paged": (_int, [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _int, _i64, _int,
                                        _i64, _i64, _i64, _i64, _i64, _i64, _c_void_p, _c_void_p,
                                        _c_void_p, _c_void_p, _int, _c_void_p]),
@@ -228,6 +230,11 @@ _SIGNATURES = {
     "ss_paged_attn": (_int, [_c_void_p, _c_void_p, _int, _i64, _i64, _i64, _int, _c_void_p, _i64,
                              _c_void_p, _c_void_p, _i64, _f32, _int, _i64, _i64, _c_void_p, _int,
                              _c_void_p, _size, _c_void_p]),
+    "ss_paged_attn_scored_workspace_bytes": (_size, [_c_void_p, _i64, _i64, _int, _i64, _i64,
+                                                     _c_void_p]),
+    "ss_paged_attn_scored": (_int, [_c_void_p, _c_void_p, _int, _i64, _i64, _i64, _int, _c_void_p,
+                                    _i64, _c_void_p, _c_void_p, _i64, _f32, _int, _i64, _i64,
+                                    _c_void_p, _int, _c_void_p, _c_void_p, _size, _c_void_p]),
 }
 # the masked decodes: a mask descriptor before the stream
 _MASKED = {"ss_decode_attn_il8_hybrid": "ss_decode_attn_il8_masked",

@@ -215,6 +215,126 @@ __global__ void __launch_bounds__(256)
     if (t < n_tok) write_slot(t, starts, n_req, ends, table, width, log_page, slots, positions);
 }
 
+// ------------------------------------------------------------- shared plan
+
+// Row of token `tok` in the group of its request's parent, and its position.
+__device__ __forceinline__ void write_shared(int64_t tok, const int32_t *starts, int n_req, const int32_t *lengths,
+                                             const int32_t *parents, const int32_t *offsets, int2 *rows,
+                                             int32_t *positions) {
+    int64_t pos = -1;
+    if (tok >= starts[0] && tok < starts[n_req]) {
+        const int r = request_of(starts, n_req, (int)tok), p = parents[r];
+        const int own = lengths[r] - (starts[r + 1] - (int)tok);
+        if (p >= 0) rows[offsets[r] + (int)tok - starts[r]] = make_int2((int)tok, own);
+        pos = max((int64_t)own + (p >= 0 ? max(lengths[p], 0) : 0), (int64_t)-1);
+    }
+    if (positions) positions[tok] = (int32_t)min(pos, (int64_t)INT32_MAX);
+}
+
+// One workgroup sorts the requests by their parents, in the requests' order:
+// each wave ranks 64 of them among themselves, then the 64s follow each other.
+// Latency bounds it, as the block tables.
+__global__ void __launch_bounds__(kTableThreads)
+    shared_plan_kernel(const int32_t *parents, const int32_t *lengths, const int32_t *token_starts, int n_req,
+                       int64_t n_tok, int32_t *group_starts, int2 *rows, int32_t *parents_out, int32_t *offsets,
+                       int32_t *positions, int inline_rows) {
+    __shared__ int32_t starts[kMaxRequests + 1];
+    __shared__ int32_t parent[kMaxRequests];
+    __shared__ int32_t offset[kMaxRequests];     // of a request's rows among its parent's
+    __shared__ int32_t count[kMaxRequests + 1];  // rows of a parent: so far, then all, then before it
+    __shared__ int32_t sums[kTableThreads / kWave];
+    __shared__ int bad;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    if (tid == 0) bad = 0;
+    for (int r = tid; r <= n_req; r += kTableThreads) starts[r] = token_starts[r], count[r] = 0;
+    __syncthreads();
+    for (int r = tid; r < n_req; r += kTableThreads)
+        if (starts[r + 1] < starts[r]) bad = 1;
+    __syncthreads();
+    const bool failed = bad;
+    auto rows_of = [&](int r) {  // of those that exist
+        return r >= n_req || failed || starts[r] < 0 ? 0 : (int)max(min((int64_t)starts[r + 1], n_tok) - starts[r], (int64_t)0);
+    };
+    for (int r0 = wave * kWave; r0 < n_req; r0 += kTableThreads) {
+        const int r = r0 + lane, n = rows_of(r);
+        int p = r < n_req && !failed && starts[r] >= 0 ? parents[r] : -1;
+        if ((uint32_t)p >= (uint32_t)n_req || p == r) p = -1;
+        int before = 0;
+        for (int k = 0; k < kWave - 1; ++k) {
+            const int pk = __builtin_amdgcn_readlane(p, k), nk = __builtin_amdgcn_readlane(n, k);
+            if (k < lane && pk == p) before += nk;
+        }
+        if (r < n_req) parent[r] = p, offset[r] = before;
+    }
+    __syncthreads();
+    for (int r0 = 0; r0 < n_req; r0 += kWave) {
+        if (wave == 0) {
+            const int r = r0 + lane, p = r < n_req ? parent[r] : -1;
+            if (p >= 0) offset[r] += count[p];
+            wave_lds_sync();
+            if (p >= 0) atomicAdd(&count[p], rows_of(r));
+            wave_lds_sync();
+        }
+    }
+    __syncthreads();
+    // where each parent's rows start
+    const int per = (n_req + kTableThreads - 1) / kTableThreads;
+    const int p0 = min(tid * per, n_req), p1 = min(p0 + per, n_req);
+    int s = 0;
+    for (int p = p0; p < p1; ++p) s += count[p];
+    int scan = s;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int y = __shfl_up(scan, o);
+        if (lane >= o) scan += y;
+    }
+    if (lane == 63) sums[wave] = scan;
+    __syncthreads();
+    int from = scan - s;
+    for (int w = 0; w < wave; ++w) from += sums[w];
+    for (int p = p0; p < p1; ++p) {
+        const int n = count[p];
+        count[p] = from, group_starts[p] = from;
+        from += n;
+    }
+    if (p1 == n_req && p0 < p1) group_starts[n_req] = from;
+    __syncthreads();
+    for (int r = tid; r < n_req; r += kTableThreads) {
+        const int p = parent[r];
+        if (p >= 0) offset[r] += count[p];
+        parents_out[r] = p, offsets[r] = offset[r];
+    }
+    if (!inline_rows) return;
+    __syncthreads();
+    if (failed) {
+        if (positions)
+            for (int64_t t = tid; t < n_tok; t += kTableThreads) positions[t] = -1;
+        return;
+    }
+    for (int64_t t = tid; t < n_tok; t += kTableThreads)
+        write_shared(t, starts, n_req, lengths, parent, offset, rows, positions);
+}
+
+__global__ void __launch_bounds__(256)
+    shared_rows_kernel(const int32_t *token_starts, int n_req, int64_t n_tok, const int32_t *lengths,
+                       const int32_t *parents, const int32_t *offsets, int2 *rows, int32_t *positions) {
+    __shared__ int32_t starts[kMaxRequests + 1];
+    __shared__ int bad;
+    if (threadIdx.x == 0) bad = 0;
+    for (int r = threadIdx.x; r <= n_req; r += 256) starts[r] = token_starts[r];
+    __syncthreads();
+    for (int r = threadIdx.x; r < n_req; r += 256)
+        if (starts[r + 1] < starts[r]) bad = 1;
+    __syncthreads();
+    const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (t >= n_tok) return;
+    if (bad) {
+        if (positions) positions[t] = -1;
+        return;
+    }
+    write_shared(t, starts, n_req, lengths, parents, offsets, rows, positions);
+}
+
 // ------------------------------------------------------------------ append
 
 // A wave takes 8 consecutive new tokens of one KV head, 8 values a lane.
@@ -397,6 +517,30 @@ extern "C" int ss_block_tables(const int32_t *lengths, const int32_t *new_length
                            (int)n_requests, lengths_out, block_table, table_width, log_page, n_tokens, slots,
                            positions);
         SS_LAUNCH_CHECK("slots_kernel launch");
+    }
+    return SS_OK;
+}
+
+extern "C" int ss_shared_plan(const int32_t *parents, const int32_t *lengths, const int32_t *token_starts,
+                              int64_t n_requests, int64_t n_tokens, int32_t *group_starts, int32_t *group_rows,
+                              int32_t *parents_out, int32_t *offsets, int32_t *positions, void *stream) {
+    SS_REQUIRE(n_requests >= 1 && n_tokens >= 0, "bad sizes");
+    SS_REQUIRE(parents && lengths && token_starts && group_starts && parents_out && offsets &&
+                   (group_rows || n_tokens == 0),
+               "null pointer argument");
+    SS_REQUIRE(((uintptr_t)group_rows & 7) == 0, "group_rows must be 8-byte aligned");
+    SS_UNSUPPORTED(n_requests <= kMaxRequests, "%lld requests (at most %d)", (long long)n_requests, kMaxRequests);
+    SS_UNSUPPORTED(n_tokens <= INT32_MAX, "too many tokens for one launch");
+    const int in_one = n_tokens <= kSlotsInline;
+    hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+    int2 *const rows = reinterpret_cast<int2 *>(group_rows);
+    hipLaunchKernelGGL(shared_plan_kernel, dim3(1), dim3(kTableThreads), 0, st, parents, lengths, token_starts,
+                       (int)n_requests, n_tokens, group_starts, rows, parents_out, offsets, positions, in_one);
+    SS_LAUNCH_CHECK("shared_plan_kernel launch");
+    if (!in_one) {
+        hipLaunchKernelGGL(shared_rows_kernel, dim3((unsigned)((n_tokens + 255) / 256)), dim3(256), 0, st,
+                           token_starts, (int)n_requests, n_tokens, lengths, parents_out, offsets, rows, positions);
+        SS_LAUNCH_CHECK("shared_rows_kernel launch");
     }
     return SS_OK;
 }

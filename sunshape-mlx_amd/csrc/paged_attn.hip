@@ -20,6 +20,7 @@ constexpr int kStages = 4;         // tiles of a wave in LDS, one computed while
 // Cache policy of the stream: non-temporal (8 requests of 32768 tokens: 66 us;
 // cached: 75 us.  1 request: 20.6 and 21.1 us).
 constexpr int kNt = 2;
+constexpr int kProb = -24;         // probabilities are kept times 2^kProb
 // Requests of more than kPromptRows query rows a KV head are the prompt
 // kernel's, where this one would have more than kPromptUnits units a compute
 // unit (at 128 dims; half as much work each at 64) than that one: a column
@@ -49,7 +50,15 @@ constexpr int kMinRun = 4;
 __device__ __forceinline__ int blocks_of(const PagedAttn &a, const Request &q, int rows) {
     return q.rows > a.most_rows ? 0 : (q.rows + rows - 1) / rows;
 }
-__device__ __forceinline__ int units_of(const Request &q) { return max(1, (q.len + kUnit - 1) / kUnit); }
+// (from the first that one of its rows sees)
+template <int MODE>
+__device__ __forceinline__ int first_unit_of(const PagedAttn &a, const Request &q) {
+    return first_seen<MODE>(a, q, 0) / kUnit;
+}
+template <int MODE>
+__device__ __forceinline__ int units_of(const PagedAttn &a, const Request &q) {
+    return max(1, (q.len + kUnit - 1) / kUnit - first_unit_of<MODE>(a, q));
+}
 
 // Parts of a column of `units` units at `share` units a part.
 __device__ __forceinline__ int parts_of(int units, int share) {
@@ -137,7 +146,7 @@ __device__ __forceinline__ float groups_sum(float v) {
 // the cycles): 8 requests of up to 32768 tokens, 8 heads, 195 MB, take 42 us,
 // 4.6 TB/s.  One such request, 38 MB, takes 17 us: tables, queries, four tiles
 // a wave and the join follow each other.
-template <int D, int G, bool BF, int NS>
+template <int D, int G, bool BF, int NS, int MODE>
 __global__ void __launch_bounds__(256, 2) paged_attn_kernel(const PagedAttn a) {
     constexpr int RS = 16 / G;       // rows of a column set
     constexpr int ROWS = RS * NS;    // rows of a workgroup
@@ -173,10 +182,10 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(const PagedAttn a) {
     int units = 0, columns = 0;  // of the lane's requests
     bool down = false;
     for (int i = r0; i < r1; ++i) {
-        const Request q = request(a, i);
+        const Request q = request<MODE>(a, i);
         down |= descends(a, i);
         const int n = blocks_of(a, q, ROWS) * heads;
-        units += units_of(q) * n, columns += n;
+        units += units_of<MODE>(a, q) * n, columns += n;
     }
     if (__any(down)) {
         units = columns = 0, r1 = r0;
@@ -199,8 +208,8 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(const PagedAttn a) {
         auto items = [&](int share) {
             int n = 0;
             for (int i = r0; i < r1; ++i) {
-                const Request q = request(a, i);
-                n += blocks_of(a, q, ROWS) * heads * parts_of(units_of(q), share);
+                const Request q = request<MODE>(a, i);
+                n += blocks_of(a, q, ROWS) * heads * parts_of(units_of<MODE>(a, q), share);
             }
             return n;
         };
@@ -219,8 +228,8 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(const PagedAttn a) {
             base = holder ? __builtin_amdgcn_readlane(units_scan, holder - 1) : 0;
             list = holder ? __builtin_amdgcn_readlane(columns_scan, holder - 1) : 0;
             for (r = holder * per;; ++r) {
-                const Request q = request(a, r);
-                const int n = blocks_of(a, q, ROWS) * heads, n_units = units_of(q);
+                const Request q = request<MODE>(a, r);
+                const int n = blocks_of(a, q, ROWS) * heads, n_units = units_of<MODE>(a, q);
                 parts = __builtin_amdgcn_readfirstlane(parts_of(n_units, share));
                 if (left < n * parts) {
                     const int column = uniform_div(left, parts), part = left - column * parts;
@@ -250,8 +259,8 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(const PagedAttn a) {
     const int first_unit = u;
 
     while (u < stop) {
-        const Request rq = request(a, r);
-        const int row_blocks = blocks_of(a, rq, ROWS), n_units = units_of(rq), in_request = row_blocks * heads * n_units;
+        const Request rq = request<MODE>(a, r);
+        const int row_blocks = blocks_of(a, rq, ROWS), n_units = units_of<MODE>(a, rq), in_request = row_blocks * heads * n_units;
         if (u >= base + in_request) {
             base += in_request, ++r;
             continue;
@@ -263,9 +272,10 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(const PagedAttn a) {
             continue;
         }
         const int h = uniform_div(column, row_blocks), rb = column - h * row_blocks;
-        const int begin = (u - c0) * kUnit;
+        const int skipped = first_unit_of<MODE>(a, rq) * kUnit;
+        const int begin = (u - c0) * kUnit + skipped;
         const int part_end = a.cut ? min(stop, c1) : c1;
-        const int end = min((part_end - c0) * kUnit, rq.len);
+        const int end = min((part_end - c0) * kUnit + skipped, rq.len);
         const bool whole = c0 >= first_unit && (!a.cut || c1 <= stop);
         const int place = c0 < first_unit ? 0 : 1;  // of this part, if it is one
         if (!few && !whole && place == 1)
@@ -279,7 +289,9 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(const PagedAttn a) {
         auto in_pool = [&](int p) { return (uint32_t)p < (uint32_t)a.st.n_pages ? p : -1; };
         auto page_at = [&](int token) { return table_read(row_table, min(token >> log_page, last_page)); };
         // queries first: what is loaded later would hold them back
-        int limit[NS];  // tokens that the column's row sees
+        int limit[NS], low[NS];  // the tokens that the column's row sees: [low, limit)
+        int position[NS];        // and its own
+        float slope[NS];         // of the row's head
         uint4 raw[NS][KS];
         bool live[NS];
 #pragma unroll
@@ -287,9 +299,15 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(const PagedAttn a) {
             const int row = rb * ROWS + s * RS + col / G;
             live[s] = row < rq.rows;
             const int i = live[s] ? row / a.rep : 0, hd = live[s] ? row % a.rep : 0;
-            limit[s] = live[s] && a.causal ? max(0, min(rq.len, rq.len - rq.n_all + i + 1)) : rq.len;
+            limit[s] = live[s] ? last_seen<MODE>(a, rq, i) : rq.len;
+            low[s] = live[s] ? first_seen<MODE>(a, rq, i) : 0;
+            const int2 token = token_at<MODE>(a, rq, i);
+            if (MODE == kScores) {
+                position[s] = token.y;
+                slope[s] = a.slopes ? a.slopes[h * a.rep + hd] * kLog2e : 0.f;
+            }
             const uint16_t *q =
-                static_cast<const uint16_t *>(a.q) + (rq.t0 + i) * a.q_st + (h * a.rep + hd) * a.q_sh + quad * (D / 4);
+                static_cast<const uint16_t *>(a.q) + token.x * a.q_st + (h * a.rep + hd) * a.q_sh + quad * (D / 4);
 #pragma unroll
             for (int k = 0; k < KS; ++k) raw[s][k] = load_query8(q + 8 * k, a.vec);
         }
@@ -336,10 +354,16 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(const PagedAttn a) {
                 }
             qz[s] = lanes4_sum(sum);
             factor[s] = by.factor;
-            lag[s] = kLag / factor[s];
+            lag[s] = MODE == kScores ? kLag : kLag / factor[s];
         }
-        // (limits grow with the row: the first row's is the smallest)
-        if (a.causal) all_see = max(0, min(rq.len, rq.len - rq.n_all + rb * ROWS / a.rep + 1));
+        // (both ends grow with the row: all rows see from the last row's first
+        // token to the first row's last)
+        if (a.causal) all_see = last_seen<MODE>(a, rq, rb * ROWS / a.rep);
+        int all_from = 0, any_from = 0;
+        if (MODE != kPlain) {
+            any_from = first_seen<MODE>(a, rq, rb * ROWS / a.rep);
+            all_from = first_seen<MODE>(a, rq, (min(rb * ROWS + ROWS, rq.rows) - 1) / a.rep);
+        }
 
         // Probabilities are kept times 2^kProb, so that a sum of bfloat16's largest
         // values stays finite (up to 2^20 tokens) and values down to 2^-102 keep
@@ -347,9 +371,9 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(const PagedAttn a) {
         // vexp): vexp is above every value scale (as a power of two) that the
         // column's group has met, so it stays within fp16 whatever the scales.
         // top is in units of S.
-        constexpr int kProb = -24, kScaled = 10 - kProb;
+        constexpr int kScaled = 10 - kProb;
         float top[NS], l[NS], z[NS];
-        float back[NS];  // added to each group's sum: minus the row's reference / G
+        float back[NS];  // added to each group's sum: minus the row's reference / G (kScores: the reference)
         float4_t o[NS][VT], ones[NS];
 #pragma unroll
         for (int s = 0; s < NS; ++s) {
@@ -362,7 +386,9 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(const PagedAttn a) {
         int vexp = -92;  // (2^(kScaled - vexp) is a float)
         float up = exp2i(kScaled - vexp);
         float offset[NS];  // of the exponents: kProb less the maximum's
-        auto set_offset = [&](int s) { offset[s] = kProb - (top[s] == -INFINITY ? 0.f : top[s] * factor[s]); };
+        // (scores are in log2 units by then)
+        auto unit = [&](int s) { return MODE == kScores ? 1.f : factor[s]; };
+        auto set_offset = [&](int s) { offset[s] = kProb - (top[s] == -INFINITY ? 0.f : top[s] * unit(s)); };
 #pragma unroll
         for (int s = 0; s < NS; ++s) set_offset(s);
         const CodeBits code_bits;
@@ -399,12 +425,17 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(const PagedAttn a) {
             if (mask) {  // (behind the request's tokens a page may hold anything, NaN too)
 #pragma unroll
                 for (int j = 0; j < 8; ++j)
-                    if (!ok || first + j >= rq.len) vm[j] = 0;
+                    if (!ok || first + j >= rq.len || (MODE != kPlain && first + j < any_from)) vm[j] = 0;
             }
             float vs[8];
 #pragma unroll
             for (int j = 0; j < 8; ++j) vs[j] = low16<BF>(vm[j]);
-            const float vtop = column_max(vs);
+            float vtop = column_max(vs);
+            if (MODE != kPlain && mask) {  // (an infinite one that some row does not see costs that row nothing)
+                vtop = 0.f;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) vtop = vs[j] < INFINITY ? fmaxf(vtop, vs[j]) : vtop;
+            }
             if (__any(vtop > exp2i(vexp))) {
                 const float c = lanes4_max(vtop);
                 const int e = (int)((__float_as_uint(c) >> 23) & 0xffu) - 126;  // c < 2^e
@@ -432,9 +463,14 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(const PagedAttn a) {
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const uint32_t m = km[4 * y + i];
-                        xs[s][4 * y + i] = groups_sum<G>(fmaf(low16<BF>(m), d[s][i], fmaf(high16<BF>(m), qz[s] / 64.f, back[s])));
+                        xs[s][4 * y + i] = groups_sum<G>(
+                            fmaf(low16<BF>(m), d[s][i], fmaf(high16<BF>(m), qz[s] / 64.f, MODE == kScores ? 0.f : back[s])));
                     }
             }
+            if constexpr (MODE == kScores)
+#pragma unroll
+                for (int s = 0; s < NS; ++s)
+                    apply_scores<8>(a, slope[s], factor[s], back[s], (float)(position[s] - first), xs[s]);
             half8_t p16[NS];
 #pragma unroll
             for (int s = 0; s < NS; ++s) {
@@ -446,18 +482,19 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(const PagedAttn a) {
                     const int see = ok ? limit[s] : 0;
 #pragma unroll
                     for (int j = 0; j < 8; ++j)
-                        if (first + j >= see) x[j] = -INFINITY, v[j] = mid[j] = 0.f;
+                        if (first + j >= see || (MODE != kPlain && first + j < low[s]))
+                            x[j] = -INFINITY, v[j] = mid[j] = 0.f;
                 }
                 const float m = column_max(x);
                 if (__any(m > top[s] + lag[s])) {
                     const float now = fmaxf(top[s], lanes4_max(m));
-                    const float f = now == top[s] ? 1.f : fast_exp2((top[s] - now) * factor[s]);
+                    const float f = now == top[s] ? 1.f : fast_exp2((top[s] - now) * unit(s));
                     l[s] *= f, z[s] *= f;
                     rescale(s, f);
                     top[s] = now;
-                    if (__any(is_far(now, factor[s]))) {
-                        const float move = is_far(now, factor[s]) ? now : 0.f;
-                        back[s] -= move / G, top[s] -= move;
+                    if (__any(is_far(now, unit(s)))) {
+                        const float move = is_far(now, unit(s)) ? now : 0.f;
+                        back[s] += MODE == kScores ? move : -move / G, top[s] -= move;
 #pragma unroll
                         for (int j = 0; j < 8; ++j) x[j] -= move;
                     }
@@ -466,7 +503,7 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(const PagedAttn a) {
                 float w[8];
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
-                    const float p = fast_exp2(fmaf(x[j], factor[s], offset[s]));
+                    const float p = fast_exp2(fmaf(x[j], unit(s), offset[s]));
                     // the value's middle, zero + 7.5 scale, in float32: what is
                     // left for the product, (code - 7.5) scale, is small
                     l[s] += p;
@@ -501,7 +538,7 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(const PagedAttn a) {
                 wait_loads<0>();
             }
             const bool ok = (quad < 2 ? p0 : p1) >= 0;
-            compute(slot, tb, ok, tb + kTile > all_see || p0 < 0 || p1 < 0);
+            compute(slot, tb, ok, tb + kTile > all_see || (MODE != kPlain && tb < all_from) || p0 < 0 || p1 < 0);
         };
         int slot = 0;
         for (int tb = begin + kTile * wave; tb < end; tb += kUnit) {
@@ -523,7 +560,10 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(const PagedAttn a) {
         for (int s = 0; s < NS; ++s) {
             const float lsum = lanes4_sum(l[s]), zsum = lanes4_sum(z[s]);
             const int row = s * RS + col / G;
-            if (g == 0 && quad == 0) stats[wave][row][0] = (top[s] - G * back[s]) * factor[s], stats[wave][row][1] = lsum;
+            if (g == 0 && quad == 0) {
+                stats[wave][row][0] = MODE == kScores ? top[s] + back[s] : (top[s] - G * back[s]) * factor[s];
+                stats[wave][row][1] = lsum;
+            }
             if (in_group) {
                 // tile j, element i: dim (4 * quad + i) * D/16 + j
 #pragma unroll
@@ -549,9 +589,8 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(const PagedAttn a) {
                 for (int k = 0; k < 4; ++k) x[k] += f * part[w][row][c + k];
             }
             if (whole) {
-                const float inv = l == 0.f ? 0.f : 1.f / l;
-                const int64_t at = ((int64_t)(rq.t0 + n / a.rep) * a.hq + h * a.rep + n % a.rep) * D + c;
-                store_out4(a, at, x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
+                finish_row<MODE, D, kProb>(a, r, token_at<MODE>(a, rq, n / a.rep).x, h * a.rep + n % a.rep, c, m, l, x[0],
+                                           x[1], x[2], x[3]);
             } else {
                 const int64_t at = ((int64_t)blockIdx.x * 2 + place) * ROWS + row;
                 *reinterpret_cast<float4 *>(a.acc + at * D + c) = make_float4(x[0], x[1], x[2], x[3]);
@@ -573,7 +612,7 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(const PagedAttn a) {
 // no more workgroups than that: 4.4 us for 8 columns of 64 parts, of which the
 // launch and four reads in a row are nearly all (a workgroup for each of 512
 // possible parts: 4.9 us).
-template <int D>
+template <int D, int MODE>
 __global__ void __launch_bounds__(256) paged_merge_kernel(const PagedAttn a, int rows_per_block,
                                                           int groups) {
     constexpr int CH = D / 4, PARTS = 256 / CH, PER = 8, STEP = PARTS * PER;
@@ -585,7 +624,7 @@ __global__ void __launch_bounds__(256) paged_merge_kernel(const PagedAttn a, int
         const int4 cut = k == (int)blockIdx.y ? begin : a.cut[k];
         const int parts = cut.x, row = blockIdx.x;
         if (parts == 0) continue;
-        const Request rq = request(a, cut.y);
+        const Request rq = request<MODE>(a, cut.y);
         const int row_blocks = blocks_of(a, rq, rows_per_block);
         const int h = uniform_div(cut.w, row_blocks), n = (cut.w - h * row_blocks) * rows_per_block + row;
         if (n >= rq.rows) continue;
@@ -630,9 +669,8 @@ __global__ void __launch_bounds__(256) paged_merge_kernel(const PagedAttn a, int
 #pragma unroll
                 for (int k = 0; k < 4; ++k) y[k] += red[i][c + k];
             }
-            const float inv = t == 0.f ? 0.f : 1.f / t;
-            const int64_t o = ((int64_t)(rq.t0 + n / a.rep) * a.hq + h * a.rep + n % a.rep) * D + c;
-            store_out4(a, o, y[0] * inv, y[1] * inv, y[2] * inv, y[3] * inv);
+            finish_row<MODE, D, kProb>(a, cut.y, token_at<MODE>(a, rq, n / a.rep).x, h * a.rep + n % a.rep, c, m, t, y[0],
+                                       y[1], y[2], y[3]);
         }
         __syncthreads();  // (the next column's sums)
     }
@@ -707,39 +745,125 @@ static int check_hints(const ss_paged_store *s, int64_t n_requests, int n_q_head
     return SS_OK;
 }
 
-template <int D, int G, bool BF>
+template <int D, int G, bool BF, int MODE>
 static void launch_paged(const PagedAttn &a, const PagedPlan &p, hipStream_t st) {
     if (p.sets == 1)
-        hipLaunchKernelGGL((paged_attn_kernel<D, G, BF, 1>), dim3(p.groups), dim3(256), 0, st, a);
+        hipLaunchKernelGGL((paged_attn_kernel<D, G, BF, 1, MODE>), dim3(p.groups), dim3(256), 0, st, a);
     else
-        hipLaunchKernelGGL((paged_attn_kernel<D, G, BF, 2>), dim3(p.groups), dim3(256), 0, st, a);
+        hipLaunchKernelGGL((paged_attn_kernel<D, G, BF, 2, MODE>), dim3(p.groups), dim3(256), 0, st, a);
     if (p.cut)
-        hipLaunchKernelGGL(paged_merge_kernel<D>, dim3(p.rows, p.columns), dim3(256), 0, st, a, p.rows, p.groups);
+        hipLaunchKernelGGL((paged_merge_kernel<D, MODE>), dim3(p.rows, p.columns), dim3(256), 0, st, a, p.rows, p.groups);
 }
 
-}  // namespace ss
+template <int MODE>
+static void launch_paged_store(const PagedAttn &a, const ss_paged_store *s, const PagedPlan &p, hipStream_t st) {
+    const bool bf = s->dtype == SS_BF16;
+    const int key = s->head_dim * 1000 + s->group_size;
+    if (key == 128032) bf ? launch_paged<128, 4, true, MODE>(a, p, st) : launch_paged<128, 4, false, MODE>(a, p, st);
+    else if (key == 128064) bf ? launch_paged<128, 2, true, MODE>(a, p, st) : launch_paged<128, 2, false, MODE>(a, p, st);
+    else if (key == 128128) bf ? launch_paged<128, 1, true, MODE>(a, p, st) : launch_paged<128, 1, false, MODE>(a, p, st);
+    else if (key == 64032) bf ? launch_paged<64, 2, true, MODE>(a, p, st) : launch_paged<64, 2, false, MODE>(a, p, st);
+    else bf ? launch_paged<64, 1, true, MODE>(a, p, st) : launch_paged<64, 1, false, MODE>(a, p, st);
+}
 
-using namespace ss;
+// One pass: the requests whose rows are few, then (p.prompts) the others.
+static int launch_pass(PagedAttn &a, const ss_paged_store *s, const PagedPlan &p, int mode, void *workspace,
+                       size_t workspace_bytes, hipStream_t st) {
+    a.most_rows = p.prompts ? kPromptRows : INT32_MAX;
+    a.cut = p.cut ? static_cast<int4 *>(workspace) : nullptr;
+    a.acc = reinterpret_cast<float *>(a.cut + p.groups + 1);
+    a.ml = a.acc + (size_t)p.groups * 2 * p.rows * s->head_dim;
+    if (mode == kPlain) launch_paged_store<kPlain>(a, s, p, st);
+    else if (mode == kRanges) launch_paged_store<kRanges>(a, s, p, st);
+    else launch_paged_store<kScores>(a, s, p, st);
+    SS_LAUNCH_CHECK("paged_attn_kernel launch");
+    return p.prompts ? launch_paged_prompt(a, s, mode, workspace, workspace_bytes, st) : SS_OK;
+}
 
-extern "C" size_t ss_paged_attn_workspace_bytes(const ss_paged_store *store, int64_t n_tokens, int64_t n_requests,
-                                                int n_q_heads, int64_t max_new, int64_t max_length) {
+// What ss_paged_scores asks for.
+struct Asked {
+    int mode;
+    bool shared;
+    int64_t window;  // INT32_MAX: none
+};
+
+static int check_scores(const ss_paged_store *s, const ss_paged_scores *sc, Asked *asked) {
+    *asked = {kPlain, false, INT32_MAX};
+    if (!sc) return SS_OK;
+    SS_REQUIRE(sc->softcap == 0.f || (sc->softcap >= 0x1p-60f && sc->softcap <= 0x1p60f),
+               "softcap must be 0 or from 2^-60 to 2^60");
+    SS_REQUIRE(sc->window >= 0, "window must not be negative");
+    asked->shared = sc->group_starts || sc->group_rows || sc->parents;
+    if (sc->window > 0 && sc->window < INT32_MAX) asked->window = sc->window;
+    const bool ranges = asked->window != INT32_MAX || sc->prefix_lengths;
+    asked->mode = sc->softcap > 0.f || sc->slopes ? kScores : ranges || asked->shared ? kRanges : kPlain;
+    if (!asked->shared) return SS_OK;
+    SS_REQUIRE(sc->group_starts && sc->group_rows && sc->parents, "null pointer in a shared plan");
+    SS_REQUIRE(((uintptr_t)sc->group_rows & 7) == 0, "group_rows must be 8-byte aligned");
+    SS_UNSUPPORTED(!ranges, "a window or prefix lengths with shared tokens");
+    SS_REQUIRE(sc->max_shared >= 1 && sc->max_shared <= INT32_MAX && sc->n_groups >= 1 && sc->n_groups <= 65535,
+               "max_shared and n_groups must be positive");
+    return SS_OK;
+}
+
+// The launch shapes of a call: of the pass over shared tokens, if there is one,
+// and of the pass over the requests' own.
+struct PagedPasses {
+    PagedPlan shared, own;
+    size_t part, bytes;  // sums of the first pass; the whole workspace
+};
+
+static PagedPasses paged_passes(const ss_paged_store *s, int64_t n_tokens, int64_t n_requests, int n_q_heads,
+                                int64_t max_new, int64_t max_length, const ss_paged_scores *sc, const Asked &asked) {
+    PagedPasses p{};
+    // (a window is seen through whole units)
+    if (asked.window != INT32_MAX) max_length = min(max_length, asked.window + max_new + kUnit);
+    p.own = paged_plan(s, n_tokens, n_requests, n_q_heads, max_new, max_length);
+    p.bytes = p.own.bytes;
+    if (asked.shared) {
+        const int64_t groups = min(sc->n_groups, n_requests);
+        p.shared = paged_plan(s, n_tokens, groups, n_q_heads, max((int64_t)1, n_tokens / groups), sc->max_shared);
+        p.part = ((size_t)n_tokens * n_q_heads * (s->head_dim + 2) * 4 + 15) & ~(size_t)15;
+        p.bytes = p.part + max(p.shared.bytes, p.own.bytes);
+    }
+    return p;
+}
+
+// Takes the prompt kernel where the decode kernel's units would pass 32 bits
+// (hints that are too low for the tables), and refuses where they still would.
+static int check_units(const ss_paged_store *s, PagedPlan &p, int64_t n_tokens, int64_t n_requests, int rep,
+                       int64_t table_width) {
+    p.prompts |= most_units(s, p, n_tokens, n_requests, rep, table_width) >= kCounted;
+    SS_UNSUPPORTED(most_units(s, p, n_tokens, n_requests, rep, table_width) < kCounted,
+                   "%lld requests, %lld tokens and %lld pages a table row: more blocks of query rows and of %d tokens "
+                   "than 32 bits count",
+                   (long long)n_requests, (long long)n_tokens, (long long)table_width, kUnit);
+    return SS_OK;
+}
+
+static size_t workspace_bytes_of(const ss_paged_store *store, int64_t n_tokens, int64_t n_requests, int n_q_heads,
+                                 int64_t max_new, int64_t max_length, const ss_paged_scores *sc) {
     PagedStore ps;
     int log_page;
+    Asked asked;
     if (check_paged_store(store, &ps, &log_page) || check_hints(store, n_requests, n_q_heads, max_new, max_length) ||
-        n_tokens < 0 || n_tokens > INT32_MAX / n_q_heads)
+        check_scores(store, sc, &asked) || n_tokens < 0 || n_tokens > INT32_MAX / n_q_heads)
         return 0;
-    return paged_plan(store, n_tokens, n_requests, n_q_heads, max_new, max_length).bytes;
+    return paged_passes(store, n_tokens, n_requests, n_q_heads, max_new, max_length, sc, asked).bytes;
 }
 
-extern "C" int ss_paged_attn(const ss_paged_store *store, const void *q, int q_dtype, int64_t n_tokens,
-                             int64_t q_st, int64_t q_sh, int n_q_heads, const int32_t *block_table,
-                             int64_t table_width, const int32_t *lengths, const int32_t *token_starts,
-                             int64_t n_requests, float scale, int causal, int64_t max_new, int64_t max_length,
-                             void *out, int zero_rest, void *workspace, size_t workspace_bytes, void *stream) {
-    PagedAttn a;
+static int paged_attn(const ss_paged_store *store, const void *q, int q_dtype, int64_t n_tokens,
+                      int64_t q_st, int64_t q_sh, int n_q_heads, const int32_t *block_table,
+                      int64_t table_width, const int32_t *lengths, const int32_t *token_starts,
+                      int64_t n_requests, float scale, int causal, int64_t max_new, int64_t max_length,
+                      void *out, int zero_rest, const ss_paged_scores *sc, void *workspace, size_t workspace_bytes,
+                      void *stream) {
+    PagedAttn a{};
     int log_page;
+    Asked asked;
     if (int rc = check_paged_store(store, &a.st, &log_page)) return rc;
     if (int rc = check_hints(store, n_requests, n_q_heads, max_new, max_length)) return rc;
+    if (int rc = check_scores(store, sc, &asked)) return rc;
     SS_UNSUPPORTED(q_dtype == SS_F16 || q_dtype == SS_BF16, "queries must be float16 or bfloat16");
     SS_REQUIRE(n_tokens >= 0, "bad token count");
     if (n_tokens == 0) return SS_OK;
@@ -748,14 +872,11 @@ extern "C" int ss_paged_attn(const ss_paged_store *store, const void *q, int q_d
     SS_REQUIRE(((uintptr_t)out & 7) == 0, "out must be 8-byte aligned");
     SS_REQUIRE(table_width >= 1, "bad block table width");
     SS_UNSUPPORTED(table_width <= (1 << 30) / store->page_size, "a table row of more than 2^30 tokens");
-    PagedPlan p = paged_plan(store, n_tokens, n_requests, n_q_heads, max_new, max_length);
-    // (hints that are too low for the tables)
     const int rep = n_q_heads / store->n_kv_heads;
-    p.prompts |= most_units(store, p, n_tokens, n_requests, rep, table_width) >= kCounted;
-    SS_UNSUPPORTED(most_units(store, p, n_tokens, n_requests, rep, table_width) < kCounted,
-                   "%lld requests, %lld tokens and %lld pages a table row: more blocks of query rows and of %d tokens "
-                   "than 32 bits count",
-                   (long long)n_requests, (long long)n_tokens, (long long)table_width, kUnit);
+    PagedPasses p = paged_passes(store, n_tokens, n_requests, n_q_heads, max_new, max_length, sc, asked);
+    if (int rc = check_units(store, p.own, n_tokens, n_requests, rep, table_width)) return rc;
+    if (asked.shared)
+        if (int rc = check_units(store, p.shared, n_tokens, n_requests, rep, table_width)) return rc;
     if (p.bytes > workspace_bytes || (p.bytes && !workspace)) {
         set_error("workspace of %zu bytes, %zu needed", workspace_bytes, p.bytes);
         return SS_ERR_WORKSPACE;
@@ -767,18 +888,54 @@ extern "C" int ss_paged_attn(const ss_paged_store *store, const void *q, int q_d
     a.hq = n_q_heads, a.rep = rep;
     a.q_dtype = q_dtype, a.causal = causal, a.zero_rest = zero_rest, a.scale = scale;
     a.vec = ((uintptr_t)q & 15) == 0 && q_st % 8 == 0 && q_sh % 8 == 0;
-    a.most_rows = p.prompts ? kPromptRows : INT32_MAX;
-    a.cut = p.cut ? static_cast<int4 *>(workspace) : nullptr;
-    a.acc = reinterpret_cast<float *>(a.cut + p.groups + 1);
-    a.ml = a.acc + (size_t)p.groups * 2 * p.rows * store->head_dim;
+    a.window = (int)asked.window;
+    if (sc) a.open = sc->prefix_lengths, a.cap = sc->softcap, a.slopes = sc->slopes;
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-    const bool bf = store->dtype == SS_BF16;
-    const int key = store->head_dim * 1000 + store->group_size;
-    if (key == 128032) bf ? launch_paged<128, 4, true>(a, p, st) : launch_paged<128, 4, false>(a, p, st);
-    else if (key == 128064) bf ? launch_paged<128, 2, true>(a, p, st) : launch_paged<128, 2, false>(a, p, st);
-    else if (key == 128128) bf ? launch_paged<128, 1, true>(a, p, st) : launch_paged<128, 1, false>(a, p, st);
-    else if (key == 64032) bf ? launch_paged<64, 2, true>(a, p, st) : launch_paged<64, 2, false>(a, p, st);
-    else bf ? launch_paged<64, 1, true>(a, p, st) : launch_paged<64, 1, false>(a, p, st);
-    SS_LAUNCH_CHECK("paged_attn_kernel launch");
-    return p.prompts ? launch_paged_prompt(a, store, workspace, workspace_bytes, st) : SS_OK;
+    char *const scratch = static_cast<char *>(workspace) + p.part;
+    const size_t left = workspace_bytes - p.part;
+    if (asked.shared) {
+        a.part = static_cast<float *>(workspace);
+        PagedAttn first = a;
+        first.starts = sc->group_starts, first.rows_of = reinterpret_cast<const int2 *>(sc->group_rows);
+        first.causal = first.zero_rest = 0;
+        if (int rc = launch_pass(first, store, p.shared, asked.mode, scratch, left, st)) return rc;
+        a.parents = sc->parents;
+    }
+    return launch_pass(a, store, p.own, asked.mode, scratch, left, st);
+}
+
+}  // namespace ss
+
+using namespace ss;
+
+extern "C" size_t ss_paged_attn_workspace_bytes(const ss_paged_store *store, int64_t n_tokens, int64_t n_requests,
+                                                int n_q_heads, int64_t max_new, int64_t max_length) {
+    return workspace_bytes_of(store, n_tokens, n_requests, n_q_heads, max_new, max_length, nullptr);
+}
+
+extern "C" size_t ss_paged_attn_scored_workspace_bytes(const ss_paged_store *store, int64_t n_tokens,
+                                                       int64_t n_requests, int n_q_heads, int64_t max_new,
+                                                       int64_t max_length, const ss_paged_scores *scores) {
+    return workspace_bytes_of(store, n_tokens, n_requests, n_q_heads, max_new, max_length, scores);
+}
+
+extern "C" int ss_paged_attn(const ss_paged_store *store, const void *q, int q_dtype, int64_t n_tokens,
+                             int64_t q_st, int64_t q_sh, int n_q_heads, const int32_t *block_table,
+                             int64_t table_width, const int32_t *lengths, const int32_t *token_starts,
+                             int64_t n_requests, float scale, int causal, int64_t max_new, int64_t max_length,
+                             void *out, int zero_rest, void *workspace, size_t workspace_bytes, void *stream) {
+    return paged_attn(store, q, q_dtype, n_tokens, q_st, q_sh, n_q_heads, block_table, table_width, lengths,
+                      token_starts, n_requests, scale, causal, max_new, max_length, out, zero_rest, nullptr, workspace,
+                      workspace_bytes, stream);
+}
+
+extern "C" int ss_paged_attn_scored(const ss_paged_store *store, const void *q, int q_dtype, int64_t n_tokens,
+                                    int64_t q_st, int64_t q_sh, int n_q_heads, const int32_t *block_table,
+                                    int64_t table_width, const int32_t *lengths, const int32_t *token_starts,
+                                    int64_t n_requests, float scale, int causal, int64_t max_new, int64_t max_length,
+                                    void *out, int zero_rest, const ss_paged_scores *scores, void *workspace,
+                                    size_t workspace_bytes, void *stream) {
+    return paged_attn(store, q, q_dtype, n_tokens, q_st, q_sh, n_q_heads, block_table, table_width, lengths,
+                      token_starts, n_requests, scale, causal, max_new, max_length, out, zero_rest, scores, workspace,
+                      workspace_bytes, stream);
 }

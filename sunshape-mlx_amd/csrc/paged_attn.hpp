@@ -37,6 +37,11 @@ __device__ __forceinline__ bool is_far(float top, float factor) {
     return fabsf(top * factor) > kFar && top > -INFINITY;
 }
 
+// What a kernel is built for: causal or no mask alone; rows that see an interval
+// of their own and requests that continue others; and scores that are capped
+// or get a bias too (in a kernel of its own, as its scores take operations more).
+enum { kPlain = 0, kRanges = 1, kScores = 2 };
+
 struct PagedAttn {
     PagedStore st;
     const void *q;
@@ -51,6 +56,18 @@ struct PagedAttn {
     int4 *cut;          // columns to be joined (each kernel's merge says what it lists)
     float *acc;         // [workgroups][2][rows of a workgroup][D]
     float *ml;          // [workgroups][2][rows of a workgroup][2]
+    // kRanges:
+    const int32_t *open;     // tokens of its beginning that all rows of a request see, or null
+    int window;              // tokens up to its own that a row sees; INT32_MAX: all
+    // A pass over shared tokens: row i of request r is that of token rows[starts[r]
+    // + i].x, at .y behind the r's tokens; its sums go to `part`, for the pass over
+    // the own tokens of a request that continues parents[r] >= 0.
+    const int2 *rows_of;
+    const int32_t *parents;
+    float *part;             // [n_tokens][hq][D], then [n_tokens][hq][2] (maximum, sum)
+    // kScores:
+    float cap;               // of the scores; 0: none
+    const float *slopes;     // [hq], or null
 };
 
 // Tables do not change while the kernel runs: through the constant address
@@ -71,8 +88,10 @@ __device__ __forceinline__ uint4 load_query8(const uint16_t *p, int vec) {
 // number (n_all, of which n rows exist), its length, its query rows a KV head.
 struct Request {
     int t0, n, n_all, len, rows;
+    int open;  // (kRanges) tokens that all rows see
 };
 
+template <int MODE = kPlain>
 __device__ __forceinline__ Request request(const PagedAttn &a, int r) {
     Request q;
     q.t0 = table_read(a.starts, r);
@@ -80,7 +99,34 @@ __device__ __forceinline__ Request request(const PagedAttn &a, int r) {
     q.n = q.t0 < 0 ? 0 : (int)max((int64_t)0, min((int64_t)q.n_all, a.n_tokens - q.t0));
     q.len = (int)max((int64_t)0, min((int64_t)table_read(a.lengths, r), a.width << a.st.log_page));
     q.rows = q.n * a.rep;
+    q.open = 0;
+    if (MODE != kPlain && a.open) q.open = max(0, min(table_read(a.open, r), q.len));
     return q;
+}
+
+// The tokens [first_seen, last_seen) that the request's new token i sees; both
+// grow with i.
+template <int MODE>
+__device__ __forceinline__ int last_seen(const PagedAttn &a, const Request &q, int i) {
+    if (!a.causal) return q.len;
+    const int own = max(0, min(q.len, q.len - q.n_all + i + 1));
+    return MODE == kPlain ? own : max(own, q.open);
+}
+template <int MODE>
+__device__ __forceinline__ int first_seen(const PagedAttn &a, const Request &q, int i) {
+    if (MODE == kPlain) return 0;
+    return max(0, min(q.len, max(0, q.len - q.n_all + i + 1)) - a.window);
+}
+
+// The token whose query is row i of the request, and its position among the
+// request's tokens.
+template <int MODE>
+__device__ __forceinline__ int2 token_at(const PagedAttn &a, const Request &q, int i) {
+    if (MODE != kPlain && a.rows_of) {
+        const int2 t = a.rows_of[q.t0 + i];
+        return make_int2(max(0, min(t.x, (int)a.n_tokens - 1)), q.len + t.y);
+    }
+    return make_int2(q.t0 + i, q.len - q.n_all + i);
 }
 
 // Whether request r ends before it begins.  Starts that descend name no rows at
@@ -98,6 +144,80 @@ __device__ __forceinline__ void store_out4(const PagedAttn &a, int64_t i, float 
     const bool f16 = a.q_dtype == SS_F16;
     *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(a.out) + i) =
         make_uint2(f16 ? __builtin_bit_cast(uint32_t, h0) : b0, f16 ? __builtin_bit_cast(uint32_t, h1) : b1);
+}
+
+// Row (token t, query head `head`) is done: of its dims c .. c+3 the sums of
+// values x, of probabilities l, and what 2^m stands for in both.  SHIFT: sums
+// are times 2^SHIFT (of partial ones, kPart).
+constexpr int kPart = -24;
+template <int MODE, int D, int SHIFT>
+__device__ __forceinline__ void finish_row(const PagedAttn &a, int r, int64_t t, int head, int c, float m, float l,
+                                           float x0, float x1, float x2, float x3) {
+    const int64_t at = t * a.hq + head;
+    if constexpr (MODE != kPlain) {
+        float *const ml = a.part + a.n_tokens * a.hq * D + at * 2;
+        float4 *const part = reinterpret_cast<float4 *>(a.part + at * D + c);
+        if (a.rows_of || (a.part && table_read(a.parents, r) >= 0)) {
+            if (SHIFT != kPart) {
+                constexpr float f = 1.f / (1ull << (SHIFT - kPart));
+                l *= f, x0 *= f, x1 *= f, x2 *= f, x3 *= f;
+            }
+            if (a.rows_of) {
+                *part = make_float4(x0, x1, x2, x3);
+                if (c == 0) *reinterpret_cast<float2 *>(ml) = make_float2(m, l);
+                return;
+            }
+            const float2 e = *reinterpret_cast<const float2 *>(ml);
+            const float4 v = *part;
+            const float top = fmaxf(m, e.x);
+            const float f = m == top ? 1.f : fast_exp2(m - top), g = e.x == top ? 1.f : fast_exp2(e.x - top);
+            l = f * l + g * e.y;
+            x0 = f * x0 + g * v.x, x1 = f * x1 + g * v.y, x2 = f * x2 + g * v.z, x3 = f * x3 + g * v.w;
+        }
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    store_out4(a, at * D + c, x0 * inv, x1 * inv, x2 * inv, x3 * inv);
+}
+
+// A row's products x with tokens 16 (i / 8) + i % 8 become scores in log2 units,
+// capped and biased, less the row's reference `ref`.  slope: the head's, in
+// log2 units a token; far: how many tokens the row is behind token 0.
+// A cap's tanh(u) is u times a polynomial of u^2 (least largest error below
+// |u| = 5/8, 2^-23 of it) where a wave's scores are all that small, which most
+// are and which takes 8 operations each; else 1 - 2 / (1 + exp(2 u)), 11
+// operations' time, off by 2^-22 and more exactly so where u is small.  Either
+// way a score is off by 2^-21 of the largest in the tile.
+template <int N, typename X>
+__device__ __forceinline__ void apply_scores(const PagedAttn &a, float slope, float factor, float ref, float far,
+                                             X &x) {
+    if (a.cap > 0.f) {
+        const float cap = a.cap * kLog2e, by = factor / cap;
+        float most = 0.f;
+#pragma unroll
+        for (int i = 0; i < N; ++i) x[i] *= by, most = fmaxf(most, fabsf(x[i]));
+        if (__any(most > 0.625f)) {
+            const float less = cap - ref;
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+                x[i] = fmaf(-2.f * cap, __builtin_amdgcn_rcpf(1.f + fast_exp2(x[i] * (2.f * kLog2e))), less);
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const float v = x[i] * x[i];
+                float p = fmaf(v, 0.0150509445f, -0.0518218674f);
+                p = fmaf(v, p, 0.133045261f);
+                p = fmaf(v, p, -0.333319543f);
+                p = fmaf(v, p, 0.999999893f);
+                x[i] = fmaf(x[i] * p, cap, -ref);
+            }
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) x[i] = fmaf(x[i], factor, -ref);
+    }
+    if (a.slopes)
+#pragma unroll
+        for (int i = 0; i < N; ++i) x[i] = fmaf(-slope, fabsf(far - (float)(16 * (i / 8) + i % 8)), x[i]);
 }
 
 // How a query row whose largest magnitude is `top` enters the products: times
@@ -213,7 +333,7 @@ constexpr int kPromptTile = 256;  // query rows of a workgroup of the prompt ker
 // with `workspace` of paged_prompt_bytes for n_tokens * rep rows in all (with
 // less no column is cut).
 size_t paged_prompt_bytes(const ss_paged_store *s, int64_t n_requests, int64_t rows, int most_rows);
-int launch_paged_prompt(PagedAttn a, const ss_paged_store *s, void *workspace, size_t workspace_bytes,
+int launch_paged_prompt(PagedAttn a, const ss_paged_store *s, int mode, void *workspace, size_t workspace_bytes,
                         hipStream_t st);
 
 }  // namespace ss

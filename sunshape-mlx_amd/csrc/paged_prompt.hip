@@ -39,6 +39,7 @@ constexpr int kSlots = 3;            // tiles in LDS as they come: one being pre
 // Fewest tiles of a part, where a workgroup's column is cut (1024 tokens, 32
 // heads: 54 us for 2 to 8, 62 us for 16).
 constexpr int kMinTiles = 8;
+constexpr int kProb = 10;  // probabilities are kept times 2^kProb
 
 template <int D, int G>
 struct PromptTile {
@@ -105,9 +106,19 @@ __device__ __forceinline__ int tiles_of(const PagedAttn &a, const Request &q) {
     return q.rows > a.most_rows ? (q.rows + kRows - 1) / kRows : 0;
 }
 
+// Tiles of a request's longest column: with a window no row tile sees more than
+// that before its own tokens.
+template <int MODE>
+__device__ __forceinline__ int column_tiles(const PagedAttn &a, const Request &q) {
+    int64_t most = q.len;
+    if (MODE != kPlain && q.open == 0) most = min(most, (int64_t)a.window + kRows / a.rep + kTokens);
+    return (int)((most + kTokens - 1) / kTokens);
+}
+
 // Parts of a request's columns at `share` tiles a part.
-__device__ __forceinline__ int parts_of_tiles(const Request &q, int share) {
-    return max(1, (int)(((int64_t)(q.len + kTokens - 1) / kTokens + share - 1) / share));
+template <int MODE>
+__device__ __forceinline__ int parts_of_tiles(const PagedAttn &a, const Request &q, int share) {
+    return max(1, (int)(((int64_t)column_tiles<MODE>(a, q) + share - 1) / share));
 }
 
 // The bits of the 16-bit float 2^k, k >= -126 (positive ones compare as
@@ -154,7 +165,7 @@ __device__ __forceinline__ void lds_barrier() {
 
 __device__ __forceinline__ float half_max(float v) { return fmaxf(v, __shfl_xor(v, 32)); }
 
-template <int D, int G, bool BF>
+template <int D, int G, bool BF, int MODE>
 __global__ void __launch_bounds__(64 * kPWaves, 2) paged_prompt_kernel(const PagedAttn a) {
     using PT = PromptTile<D, G>;
     constexpr int GW = D / 8 / G, HW = GW / 2;  // words of a group, and of a lane's half of it
@@ -173,10 +184,10 @@ __global__ void __launch_bounds__(64 * kPWaves, 2) paged_prompt_kernel(const Pag
     bool down = false;
     uint32_t all_tiles = 0;  // (up to 128 columns of 2^24; of more it is not used)
     for (int i = r0; i < r1; ++i) {
-        const Request q = request(a, i);
+        const Request q = request<MODE>(a, i);
         const int n = tiles_of(a, q) * heads;
         down |= descends(a, i);
-        columns += n, all_tiles += (uint32_t)n * ((q.len + kTokens - 1) / kTokens);
+        columns += n, all_tiles += (uint32_t)n * column_tiles<MODE>(a, q);
     }
     if (__any(down)) columns = 0, all_tiles = 0, r1 = r0;
     int scan = wave_scan(columns);
@@ -191,8 +202,8 @@ __global__ void __launch_bounds__(64 * kPWaves, 2) paged_prompt_kernel(const Pag
             share = max(uniform_div((int)(total + free_groups - 1), free_groups), kMinTiles);
             columns = 0;
             for (int i = r0; i < r1; ++i) {
-                const Request q = request(a, i);
-                columns += tiles_of(a, q) * heads * parts_of_tiles(q, share);
+                const Request q = request<MODE>(a, i);
+                columns += tiles_of(a, q) * heads * parts_of_tiles<MODE>(a, q, share);
             }
             scan = wave_scan(columns);
             if (spare == n_columns || __builtin_amdgcn_readlane(scan, 63) <= a.target) break;
@@ -207,9 +218,9 @@ __global__ void __launch_bounds__(64 * kPWaves, 2) paged_prompt_kernel(const Pag
         int r = holder * per, parts, row_tile;
         Request rq;
         for (;; ++r) {
-            rq = request(a, r);
+            rq = request<MODE>(a, r);
             const int n = tiles_of(a, rq);
-            parts = __builtin_amdgcn_readfirstlane(parts_of_tiles(rq, share));
+            parts = __builtin_amdgcn_readfirstlane(parts_of_tiles<MODE>(a, rq, share));
             if (left < n * heads * parts) {
                 // the longest row tiles first; heads side by side, so that a head's
                 // tiles tend to meet in one L2
@@ -227,26 +238,37 @@ __global__ void __launch_bounds__(64 * kPWaves, 2) paged_prompt_kernel(const Pag
             const int p = table_read(row_table, min((int64_t)(token >> log_page), a.width - 1));
             return (uint32_t)p < (uint32_t)a.st.n_pages ? p : -1;
         };
-        auto sees = [&](int row) {  // tokens that a row sees
-            return a.causal ? max(0, min(rq.len, rq.len - rq.n_all + row / a.rep + 1)) : rq.len;
-        };
+        // the tokens that a row sees: [from(row), sees(row))
+        auto sees = [&](int row) { return last_seen<MODE>(a, rq, row / a.rep); };
+        auto from = [&](int row) { return first_seen<MODE>(a, rq, row / a.rep); };
         const int last_row = min(row_tile * kRows + kRows, rq.rows) - 1;
+        const int unseen = __builtin_amdgcn_readfirstlane(from(row_tile * kRows)) / kTokens;  // tiles, by the workgroup
         const int seen_tiles =
-            (__builtin_amdgcn_readfirstlane(sees(last_row)) + kTokens - 1) / kTokens;  // by the workgroup
-        const int first_tile = part_begin(part, seen_tiles, parts);
-        const int n_tiles = part_begin(part + 1, seen_tiles, parts);
+            max((__builtin_amdgcn_readfirstlane(sees(last_row)) + kTokens - 1) / kTokens - unseen, 0);
+        const int first_tile = unseen + part_begin(part, seen_tiles, parts);
+        const int n_tiles = unseen + part_begin(part + 1, seen_tiles, parts);
         const int wave_last = min(row0 + 31, rq.rows - 1);
         const int wave_end = row0 < rq.rows ? __builtin_amdgcn_readfirstlane(sees(wave_last)) : 0;
         const int all_see = row0 < rq.rows ? __builtin_amdgcn_readfirstlane(sees(row0)) : 0;
+        const int wave_from = row0 < rq.rows ? __builtin_amdgcn_readfirstlane(from(row0)) : 0;
+        const int all_from = row0 < rq.rows ? __builtin_amdgcn_readfirstlane(from(wave_last)) : 0;
         const int row = row0 + col;
         const bool live = row < rq.rows;
         const int limit = live ? sees(row) : rq.len;
+        const int low = live ? from(row) : 0;
 
         // queries: B operand of step s of group g: dims of word g*GW + half*HW + s
         uint4 rawq[G][HW];
+        int position = 0;    // (kScores: the row's, and its head's slope)
+        float slope = 0.f;
         {
             const int i = live ? row / a.rep : 0, hd = live ? row % a.rep : 0;
-            const uint16_t *q = static_cast<const uint16_t *>(a.q) + (rq.t0 + i) * a.q_st + (h * a.rep + hd) * a.q_sh;
+            const int2 token = token_at<MODE>(a, rq, i);
+            if (MODE == kScores) {
+                position = token.y;
+                slope = a.slopes ? a.slopes[h * a.rep + hd] * kLog2e : 0.f;
+            }
+            const uint16_t *q = static_cast<const uint16_t *>(a.q) + token.x * a.q_st + (h * a.rep + hd) * a.q_sh;
 #pragma unroll
             for (int g = 0; g < G; ++g)
 #pragma unroll
@@ -298,7 +320,7 @@ __global__ void __launch_bounds__(64 * kPWaves, 2) paged_prompt_kernel(const Pag
                 }
             const QueryScale by(half_max(top), a.scale);
             factor = by.factor;
-            lag = kLag / factor;
+            lag = MODE == kScores ? kLag : kLag / factor;
             float sums[(G + 1) / 2];  // of group 2y + half
 #pragma unroll
             for (int y = 0; y < (G + 1) / 2; ++y) sums[y] = 0.f;
@@ -492,7 +514,8 @@ __global__ void __launch_bounds__(64 * kPWaves, 2) paged_prompt_kernel(const Pag
                             if (group_of(i) == g) o[j][i] *= f;
                 }
             __builtin_amdgcn_s_setprio(0);
-            if (tb < wave_end) {
+            if (tb < wave_end && (MODE == kPlain || tb + kTokens > wave_from)) {
+                const float unit = MODE == kScores ? 1.f : factor;  // (of scores: in log2 units by then)
 #pragma unroll
                 for (int y = 0; y < 2; ++y) {
                     float16_t x = float16_t{}, d[G];
@@ -524,11 +547,15 @@ __global__ void __launch_bounds__(64 * kPWaves, 2) paged_prompt_kernel(const Pag
                             for (int e = 0; e < 8; ++e)
                                 x[i + e] = fmaf((e & 1) ? high16<BF>(m[e / 2]) : low16<BF>(m[e / 2]), d[g][i + e], x[i + e]);
                         }
-                    if (tb + 32 * y + 32 > all_see || ok[0] != 15) {
+                    if constexpr (MODE == kScores)
+                        apply_scores<16>(a, slope, factor, ref, (float)(position - (tb + 32 * y + 8 * half)), x);
+                    if (tb + 32 * y + 32 > all_see || (MODE != kPlain && tb + 32 * y < all_from) || ok[0] != 15) {
 #pragma unroll
                         for (int i = 0; i < 16; ++i) {
                             const int t = 32 * y + 16 * (i / 8) + 8 * half + i % 8;
-                            if (tb + t >= limit || !((ok[0] >> (2 * y + i / 8)) & 1)) x[i] = -INFINITY;
+                            if (tb + t >= limit || (MODE != kPlain && tb + t < low) ||
+                                !((ok[0] >> (2 * y + i / 8)) & 1))
+                                x[i] = -INFINITY;
                         }
                     }
                     float m = x[0];
@@ -536,15 +563,15 @@ __global__ void __launch_bounds__(64 * kPWaves, 2) paged_prompt_kernel(const Pag
                     for (int i = 1; i < 16; ++i) m = fmaxf(m, x[i]);
                     if (__any(m > top + lag)) {
                         const float now = fmaxf(top, half_max(m));
-                        const float f = now == top ? 1.f : fast_exp2((top - now) * factor);
+                        const float f = now == top ? 1.f : fast_exp2((top - now) * unit);
                         top = now;
-                        if (__any(is_far(now, factor))) {
-                            const float move = is_far(now, factor) ? now : 0.f;
+                        if (__any(is_far(now, unit))) {
+                            const float move = is_far(now, unit) ? now : 0.f;
                             ref += move, top -= move;
 #pragma unroll
                             for (int i = 0; i < 16; ++i) x[i] -= move;
                             // minus the reference as three bf16 parts, in the zeros' product
-                            float part[3], rest = -ref;
+                            float part[3], rest = MODE == kScores ? 0.f : -ref;
 #pragma unroll
                             for (int k = 0; k < 3; ++k) {
                                 part[k] = __bfloat162float(__float2bfloat16(rest));
@@ -558,14 +585,14 @@ __global__ void __launch_bounds__(64 * kPWaves, 2) paged_prompt_kernel(const Pag
                         for (int j = 0; j < NT; ++j) o[j] *= f;
                     }
                     // (times 2^10: a probability below 2^-24 of the largest is one fp16 step)
-                    const float off = 10.f - (top == -INFINITY ? 0.f : top * factor);
+                    const float off = kProb - (top == -INFINITY ? 0.f : top * unit);
 #pragma unroll
                     for (int b = 0; b < 2; ++b) {
                         half8_t p16;
 #pragma unroll
                         for (int i = 0; i < 8; i += 2) {
-                            const float p0 = fast_exp2(fmaf(x[8 * b + i], factor, off));
-                            const float p1 = fast_exp2(fmaf(x[8 * b + i + 1], factor, off));
+                            const float p0 = fast_exp2(fmaf(x[8 * b + i], unit, off));
+                            const float p1 = fast_exp2(fmaf(x[8 * b + i + 1], unit, off));
                             l += p0 + p1;
                             const half2_t hh = __builtin_convertvector(float2_t{p0, p1}, half2_t);
                             p16[i] = hh[0], p16[i + 1] = hh[1];
@@ -581,8 +608,9 @@ __global__ void __launch_bounds__(64 * kPWaves, 2) paged_prompt_kernel(const Pag
 #pragma unroll
                 for (int g = 0; g < G; ++g)
                     if (bad[g]) {
-                        const int see = min(limit - tb, kTokens);
-                        const uint64_t seen = see <= 0 ? 0 : see == 64 ? ~0ull : (1ull << see) - 1;
+                        // the first `n` of the tile's tokens
+                        auto first = [](int n) { return n <= 0 ? 0 : n >= kTokens ? ~0ull : (1ull << n) - 1; };
+                        const uint64_t seen = first(limit - tb) & (MODE == kPlain ? ~0ull : ~first(low - tb));
                         if (bad[g] & seen)
 #pragma unroll
                             for (int j = 0; j < NT; ++j)
@@ -622,7 +650,20 @@ __global__ void __launch_bounds__(64 * kPWaves, 2) paged_prompt_kernel(const Pag
         const float sum = l + __shfl_xor(l, 32);
         if (parts == 1) {
             const float inv = sum == 0.f ? 0.f : 1.f / sum;
-            if (live) {
+            if (MODE != kPlain && live && (a.rows_of || (a.part && table_read(a.parents, r) >= 0))) {
+                const int t = token_at<MODE>(a, rq, row / a.rep).x, head = h * a.rep + row % a.rep;
+                const float m = MODE == kScores ? top + ref : (ref + top) * factor;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const int c = NT * (8 * (i / 4) + 4 * half + i % 4), e = vexp[group_of(i)] - 15;
+                    if constexpr (NT == 4)
+                        finish_row<MODE, D, kProb>(a, r, t, head, c, m, sum, ldexpf(o[0][i], e), ldexpf(o[1][i], e),
+                                                   ldexpf(o[2][i], e), ldexpf(o[3][i], e));
+                    else if (i % 2 == 0)
+                        finish_row<MODE, D, kProb>(a, r, t, head, c, m, sum, ldexpf(o[0][i], e), ldexpf(o[1][i], e),
+                                                   ldexpf(o[0][i + 1], e), ldexpf(o[1][i + 1], e));
+                }
+            } else if (live) {
                 const int64_t at = ((int64_t)(rq.t0 + row / a.rep) * a.hq + h * a.rep + row % a.rep) * D;
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
@@ -641,7 +682,7 @@ __global__ void __launch_bounds__(64 * kPWaves, 2) paged_prompt_kernel(const Pag
             // a part: the sums as they are (times 2^10), for prompt_merge_kernel
             if (part == 0) cut = make_int4(parts, r, h, row_tile);
             const int64_t at = (int64_t)item * kRows + wave * 32 + col;
-            if (half == 0) *reinterpret_cast<float2 *>(a.ml + at * 2) = make_float2((ref + top) * factor, sum);
+            if (half == 0) *reinterpret_cast<float2 *>(a.ml + at * 2) = make_float2(MODE == kScores ? top + ref : (ref + top) * factor, sum);
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
                 const int m = 8 * (i / 4) + 4 * half + i % 4;
@@ -658,13 +699,13 @@ __global__ void __launch_bounds__(64 * kPWaves, 2) paged_prompt_kernel(const Pag
 // Joins the parts of the column that cut[blockIdx.y] names: part i is at item
 // blockIdx.y + i * heads.  A thread takes four dims of a row.  The parts' sums
 // bound it: 256 of 256 rows, 34 MB, 9 us.
-template <int D>
+template <int D, int MODE>
 __global__ void __launch_bounds__(256) prompt_merge_kernel(const PagedAttn a) {
     constexpr int CH = D / 4, AT_ONCE = 256 / CH;
     const int4 cut = a.cut[blockIdx.y];
     const int parts = cut.x, r = cut.y, h = cut.z, c = threadIdx.x % CH * 4;
     if (parts == 0) return;
-    const Request rq = request(a, r);
+    const Request rq = request<MODE>(a, r);
     for (int row = blockIdx.x * AT_ONCE + threadIdx.x / CH; row < kRows; row += gridDim.x * AT_ONCE) {
         const int n = cut.w * kRows + row;
         if (n >= rq.rows) return;
@@ -679,20 +720,30 @@ __global__ void __launch_bounds__(256) prompt_merge_kernel(const PagedAttn a) {
             l += f * e.y;
             x[0] += f * v.x, x[1] += f * v.y, x[2] += f * v.z, x[3] += f * v.w;
         }
-        const float inv = l == 0.f ? 0.f : 1.f / l;
-        const int64_t o = ((int64_t)(rq.t0 + n / a.rep) * a.hq + h * a.rep + n % a.rep) * D + c;
-        store_out4(a, o, x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
+        finish_row<MODE, D, kProb>(a, r, token_at<MODE>(a, rq, n / a.rep).x, h * a.rep + n % a.rep, c, m, l, x[0], x[1],
+                                   x[2], x[3]);
     }
 }
 
-template <int D, int G>
+template <int D, int G, int MODE>
 static void launch_prompt(const PagedAttn &a, bool bf, unsigned groups, hipStream_t st) {
     const dim3 block(64 * kPWaves);
     if (bf)
-        hipLaunchKernelGGL((paged_prompt_kernel<D, G, true>), dim3(groups), block, 0, st, a);
+        hipLaunchKernelGGL((paged_prompt_kernel<D, G, true, MODE>), dim3(groups), block, 0, st, a);
     else
-        hipLaunchKernelGGL((paged_prompt_kernel<D, G, false>), dim3(groups), block, 0, st, a);
-    if (a.target) hipLaunchKernelGGL(prompt_merge_kernel<D>, dim3(16, a.target), dim3(256), 0, st, a);
+        hipLaunchKernelGGL((paged_prompt_kernel<D, G, false, MODE>), dim3(groups), block, 0, st, a);
+    if (a.target) hipLaunchKernelGGL((prompt_merge_kernel<D, MODE>), dim3(16, a.target), dim3(256), 0, st, a);
+}
+
+template <int MODE>
+static void launch_prompt_store(const PagedAttn &a, const ss_paged_store *s, unsigned groups, hipStream_t st) {
+    const bool bf = s->dtype == SS_BF16;
+    const int key = s->head_dim * 1000 + s->group_size;
+    if (key == 128032) launch_prompt<128, 4, MODE>(a, bf, groups, st);
+    else if (key == 128064) launch_prompt<128, 2, MODE>(a, bf, groups, st);
+    else if (key == 128128) launch_prompt<128, 1, MODE>(a, bf, groups, st);
+    else if (key == 64032) launch_prompt<64, 2, MODE>(a, bf, groups, st);
+    else launch_prompt<64, 1, MODE>(a, bf, groups, st);
 }
 
 // Workgroups that fill the device (one a compute unit) if the columns alone
@@ -706,7 +757,7 @@ size_t paged_prompt_bytes(const ss_paged_store *s, int64_t n_requests, int64_t r
     return (size_t)cut_target(n_requests, s->n_kv_heads, rows, most_rows) * (16 + kRows * (s->head_dim + 2) * 4);
 }
 
-int launch_paged_prompt(PagedAttn a, const ss_paged_store *s, void *workspace, size_t workspace_bytes,
+int launch_paged_prompt(PagedAttn a, const ss_paged_store *s, int mode, void *workspace, size_t workspace_bytes,
                         hipStream_t st) {
     // at most this many row tiles: whole ones, and one a request of more than most_rows rows
     const int64_t rows = a.n_tokens * a.rep;
@@ -718,13 +769,9 @@ int launch_paged_prompt(PagedAttn a, const ss_paged_store *s, void *workspace, s
     a.acc = reinterpret_cast<float *>(a.cut + a.target);
     a.ml = a.acc + (size_t)a.target * kRows * s->head_dim;
     const unsigned groups = (unsigned)max(min(tiles * a.st.heads, (int64_t)1 << 20), (int64_t)a.target);
-    const bool bf = s->dtype == SS_BF16;
-    const int key = s->head_dim * 1000 + s->group_size;
-    if (key == 128032) launch_prompt<128, 4>(a, bf, groups, st);
-    else if (key == 128064) launch_prompt<128, 2>(a, bf, groups, st);
-    else if (key == 128128) launch_prompt<128, 1>(a, bf, groups, st);
-    else if (key == 64032) launch_prompt<64, 2>(a, bf, groups, st);
-    else launch_prompt<64, 1>(a, bf, groups, st);
+    if (mode == kPlain) launch_prompt_store<kPlain>(a, s, groups, st);
+    else if (mode == kRanges) launch_prompt_store<kRanges>(a, s, groups, st);
+    else launch_prompt_store<kScores>(a, s, groups, st);
     SS_LAUNCH_CHECK("paged_prompt_kernel launch");
     return SS_OK;
 }

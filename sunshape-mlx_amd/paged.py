@@ -57,6 +57,16 @@ class _Rotation(ctypes.Structure):
                 ("eps", ctypes.c_double), ("weight_dtype", ctypes.c_int)]
 
 
+class _Scores(ctypes.Structure):
+    """``ss_paged_scores``."""
+
+    _fields_ = [("softcap", ctypes.c_float), ("slopes", ctypes.c_void_p),
+                ("window", ctypes.c_int64), ("prefix_lengths", ctypes.c_void_p),
+                ("group_starts", ctypes.c_void_p), ("group_rows", ctypes.c_void_p),
+                ("parents", ctypes.c_void_p), ("n_groups", ctypes.c_int64),
+                ("max_shared", ctypes.c_int64)]
+
+
 class PagedKVStore(NamedTuple):
     """The pool's pages:
 
@@ -127,6 +137,21 @@ class BlockPlan(NamedTuple):
     status: torch.Tensor
 
 
+class SharedPlan(NamedTuple):
+    """What ``build_shared_plan`` gives: the rows that see the tokens of request
+    p, ``rows[group_starts[p]:group_starts[p + 1]]`` (token, position among its
+    request's own tokens); each request's parent or -1; the packed tokens'
+    positions, which follow their parents' tokens (-1 behind the last); and
+    what the caller knows of the sizes."""
+
+    group_starts: torch.Tensor
+    rows: torch.Tensor
+    parents: torch.Tensor
+    positions: torch.Tensor
+    n_groups: int = 1
+    max_shared: int | None = None
+
+
 def _struct(store: PagedKVStore) -> _Store:
     """The store's C form, its tensors checked (every call: they may have been
     given other memory in place)."""
@@ -157,7 +182,8 @@ def _struct(store: PagedKVStore) -> _Store:
 
 # names of the dispatch counters (get_kernel_stats)
 _STATS = {f"ss_{n}": f"{n}_hip" for n in ("block_tables", "append_paged", "append_rotated_paged",
-                                          "read_paged", "paged_attn")}
+                                          "read_paged", "paged_attn", "paged_attn_scored",
+                                          "shared_plan")}
 _CODE = {torch.float32: _hip.SS_F32, torch.float16: _hip.SS_F16, torch.bfloat16: _hip.SS_BF16}
 
 
@@ -244,6 +270,36 @@ def check_plan(plan: BlockPlan) -> None:
     status = int(plan.status.item())
     if status:
         raise RuntimeError("block tables: " + ", ".join(t for b, t in _STATUS if status & b))
+
+
+def build_shared_plan(parents: torch.Tensor, lengths: torch.Tensor, token_starts: torch.Tensor,
+                      n_tokens: int, *, n_groups: int = 1,
+                      max_shared: int | None = None) -> SharedPlan:
+    """Which of the packed tokens continue which request.  Request r continues
+    ``parents[r]`` where that is another request, else (-1, say) none: its
+    tokens follow all of the parent's, which the cache holds once for all that
+    continue it.  A parent's own parent is not followed.  ``lengths`` and
+    ``token_starts`` are the step's (``build_block_tables``); all int32 on one
+    device.  ``n_groups`` (how many parents) and ``max_shared`` (their longest
+    length) size later launches: wrong ones cost time and change roundings
+    only.  One plan serves every layer of the step."""
+    if parents.dim() != 1:
+        raise ValueError("parents (R,) expected")
+    if n_tokens < 0 or n_groups < 1 or (max_shared is not None and max_shared < 0):
+        raise ValueError("n_tokens and max_shared must not be negative, n_groups positive")
+    if not parents.is_cuda:
+        _hip.require_gpu(parents)
+    dev, r = parents.get_device(), parents.shape[0]
+    args = (_index("parents", parents, (r,), dev), _index("lengths", lengths, (r,), dev),
+            _index("token_starts", token_starts, (r + 1,), dev), r, n_tokens)
+    # one allocation for everything that is new
+    buf = torch.empty(3 * n_tokens + 3 * r + 1, dtype=torch.int32, device=parents.device)
+    rows, starts, of, _, positions = buf.split_with_sizes((2 * n_tokens, r + 1, r, r, n_tokens))
+    at = buf.data_ptr()
+    at_starts = at + 8 * n_tokens
+    at_of = at_starts + 4 * (r + 1)
+    _launch("ss_shared_plan", dev, *args, at_starts, at, at_of, at_of + 4 * r, at_of + 8 * r)
+    return SharedPlan(starts, rows.view(n_tokens, 2), of, positions, n_groups, max_shared)
 
 
 def _rows(name: str, t: torch.Tensor, shape, dev: int) -> torch.Tensor:
@@ -409,11 +465,62 @@ def _workspace_bytes(dev: int, shape: tuple, n: int, r: int, hq: int, max_new: i
             ctypes.addressof(like), n, r, hq, max_new, max_length)
 
 
+@lru_cache(maxsize=4096)
+def _scored_workspace_bytes(dev: int, shape: tuple, n: int, r: int, hq: int, max_new: int,
+                            max_length: int, window: int, n_groups: int, max_shared: int) -> int:
+    """Workspace of a scored call of these sizes on device ``dev`` (n_groups 0:
+    without shared tokens)."""
+    like = _Store(1 << 20, 1 << 20, 1 << 20, 1 << 20, *shape)
+    at = (1 << 20) if n_groups else None
+    sc = _Scores(0.0, None, window, None, at, at, at, n_groups, max_shared)
+    with torch.cuda.device(dev):
+        return _hip.load_library().ss_paged_attn_scored_workspace_bytes(
+            ctypes.addressof(like), n, r, hq, max_new, max_length, ctypes.addressof(sc))
+
+
+def _scores(softcap, slopes, window, prefix_lengths, shared, n: int, r: int, hq: int, most: int,
+            dev: int) -> _Scores:
+    """The options of a scored call, checked."""
+    sc = _Scores()
+    if softcap is not None:
+        if not 2.0 ** -60 <= softcap <= 2.0 ** 60:
+            raise ValueError(f"softcap must be from 2^-60 to 2^60, got {softcap}")
+        sc.softcap = softcap
+    if slopes is not None:
+        _no_derivative("paged_attention", slopes)
+        if not slopes.is_cuda:
+            _hip.require_gpu(slopes)
+        if slopes.dtype is not torch.float32:
+            raise TypeError(f"slopes must be float32, not {slopes.dtype}")
+        if slopes.shape != (hq,) or not slopes.is_contiguous() or slopes.get_device() != dev:
+            raise ValueError(f"slopes must be contiguous ({hq},) on cuda:{dev}, got "
+                             f"{tuple(slopes.shape)} on {slopes.device}")
+        sc.slopes = slopes.data_ptr()
+    if window is not None:
+        if window < 1:
+            raise ValueError(f"window must be positive, got {window}")
+        sc.window = min(window, 2 ** 31 - 1)
+    if prefix_lengths is not None:
+        sc.prefix_lengths = _index("prefix_lengths", prefix_lengths, (r,), dev)
+    if shared is not None:
+        if window is not None or prefix_lengths is not None:
+            raise ValueError("shared tokens are not combined with window or prefix_lengths")
+        sc.group_starts = _index("shared.group_starts", shared.group_starts, (r + 1,), dev)
+        sc.group_rows = _index("shared.rows", shared.rows, (n, 2), dev)
+        sc.parents = _index("shared.parents", shared.parents, (r,), dev)
+        sc.n_groups = max(1, min(r, shared.n_groups))
+        longest = most if shared.max_shared is None else shared.max_shared
+        sc.max_shared = max(1, min(most, longest))
+    return sc
+
+
 def paged_attention(queries: torch.Tensor, store: PagedKVStore, block_table: torch.Tensor,
                     lengths: torch.Tensor, token_starts: torch.Tensor, scale: float, *,
                     causal: bool = True, max_new: int | None = None,
-                    max_length: int | None = None,
-                    out: torch.Tensor | None = None) -> torch.Tensor:
+                    max_length: int | None = None, out: torch.Tensor | None = None,
+                    softcap: float | None = None, slopes: torch.Tensor | None = None,
+                    window: int | None = None, prefix_lengths: torch.Tensor | None = None,
+                    shared: SharedPlan | None = None) -> torch.Tensor:
     """Attention of packed ``queries`` (N, Hq, D), float16 or bfloat16, over
     the pages of their requests.  Rows ``token_starts[r]`` to
     ``token_starts[r + 1]`` are the last of the ``lengths[r]`` tokens of
@@ -426,6 +533,17 @@ def paged_attention(queries: torch.Tensor, store: PagedKVStore, block_table: tor
     if the caller knows them, size the launch (by default every request adds
     a token and a table row is full); wrong ones cost time and change roundings
     only.
+
+    Other scores: with ``softcap`` c, a score s becomes c tanh(s / c); with
+    ``slopes`` (Hq,) float32, a head's slope times the distance of the two
+    tokens is taken off.  Other masks: with ``window`` w, a row sees none before
+    the last w tokens up to its own; with ``prefix_lengths`` (R,) int32, all rows
+    of request r see its first ``prefix_lengths[r]`` tokens (that the window
+    leaves).  ``shared`` (``build_shared_plan`` for these starts and lengths): the
+    rows of a request that continues another see all of that one's tokens
+    first, which are read once for all of them; distances count them.  Not
+    together with ``window`` or ``prefix_lengths``; ``max_length`` is then that
+    of the tokens that requests hold themselves.
     Queries under autograd, forward mode too, are refused: there is no
     derivative."""
     st = _struct(store)
@@ -458,8 +576,19 @@ def paged_attention(queries: torch.Tensor, store: PagedKVStore, block_table: tor
     most = width * st.page_size
     max_new = max(1, min(n, n - r + 1 if max_new is None else max_new))
     max_length = max(1, min(most, most if max_length is None else max_length))
-    need = _workspace_bytes(dev, (st.n_pages, st.n_kv_heads, st.head_dim, st.group_size,
-                                  st.page_size, st.dtype), n, r, hq, max_new, max_length)
+    shape = (st.n_pages, st.n_kv_heads, st.head_dim, st.group_size, st.page_size, st.dtype)
+    if softcap is not None or slopes is not None or window is not None or \
+            prefix_lengths is not None or shared is not None:
+        sc = _scores(softcap, slopes, window, prefix_lengths, shared, n, r, hq, most, dev)
+        need = _scored_workspace_bytes(dev, shape, n, r, hq, max_new, max_length, sc.window,
+                                       sc.n_groups, sc.max_shared)
+        ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+        _launch("ss_paged_attn_scored", dev, ctypes.addressof(st), q.data_ptr(), _CODE[dtype], n,
+                q.stride(0), q.stride(1), hq, at_table, width, at_lengths, at_starts, r, scale,
+                causal, max_new, max_length, out.data_ptr(), zero_rest, ctypes.addressof(sc),
+                _hip.ptr(ws), need)
+        return out
+    need = _workspace_bytes(dev, shape, n, r, hq, max_new, max_length)
     # of this call alone: calls on other streams and captured graphs have their own
     ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
     _launch("ss_paged_attn", dev, ctypes.addressof(st), q.data_ptr(), _CODE[dtype], n, q.stride(0),
@@ -611,11 +740,16 @@ class PagedKVCache:
         return out
 
     def attend(self, queries: torch.Tensor, scale: float, *, causal: bool = True,
-               out: torch.Tensor | None = None) -> torch.Tensor:
-        """Attention of the last step's tokens' queries (N, Hq, D)."""
+               out: torch.Tensor | None = None, softcap: float | None = None,
+               slopes: torch.Tensor | None = None, window: int | None = None,
+               prefix_lengths: torch.Tensor | None = None) -> torch.Tensor:
+        """Attention of the last step's tokens' queries (N, Hq, D); scores and
+        masks other than the causal ones as in ``paged_attention``."""
         return paged_attention(queries, self.store, self.block_table, self.lengths,
                                self._last_plan("attend").token_starts, scale, causal=causal,
-                               max_new=self._max_new, max_length=max(1, self._bound), out=out)
+                               max_new=self._max_new, max_length=max(1, self._bound), out=out,
+                               softcap=softcap, slopes=slopes, window=window,
+                               prefix_lengths=prefix_lengths)
 
     def release(self, requests) -> None:
         """End these requests: their pages go back to the pool."""
