@@ -12,6 +12,7 @@ step runs without the host knowing any length:
                         and keys on the way (``rotary_table``)
 ``read_paged``          what slots hold
 ``paged_attention``     the new tokens' queries over their requests
+``build_shared_plan``   which requests continue others, for ``paged_attention``
 ``PagedKVCache``        the four tied together; ``sunshape_sdpa`` and the SDPA
                         router take it as they take the other caches
 
@@ -610,7 +611,8 @@ class PagedKVCache:
 
     Lengths, tables and the stack of free pages live on the GPU and are
     stepped there in place, so a step needs no synchronisation and can be
-    captured in a graph.  A batch whose sequences all add the same number of
+    captured in a graph.  ``share`` lets requests continue another, whose tokens are
+    held and read once for all.  A batch whose sequences all add the same number of
     tokens may use ``update_and_fetch`` and ``sunshape_sdpa`` (or the SDPA
     router) instead, as with the other caches."""
 
@@ -639,7 +641,10 @@ class PagedKVCache:
         self.free_pages = torch.arange(n_pages, dtype=torch.int32, device=dev)
         self.n_free = torch.full((1,), n_pages, dtype=torch.int32, device=dev)
         self.plan: BlockPlan | None = None  # of the last step
-        self._kept: list[BlockPlan] = []    # of steps that graphs go on reading
+        self.shared: SharedPlan | None = None  # of it, where a request continues another
+        self._kept: list[tuple] = []        # of steps that graphs go on reading
+        self.parents: torch.Tensor | None = None  # on the GPU, once a request has one
+        self._parent = [-1] * n_requests
         self._version = 0                   # bumped by every change of the stored tokens
         # what the host knows of the lengths: all of them (steps given as
         # lists), or a bound
@@ -703,6 +708,13 @@ class PagedKVCache:
                                   lengths_out=self.lengths, n_free_out=self.n_free)
         # (only now: a step that was refused has changed nothing here either)
         self._host, self._bound = host, bound
+        self.shared = None
+        of = {p for p in self._parent if p >= 0}
+        if of:
+            longest = bound if host is None else max(host[p] for p in of)
+            self.shared = build_shared_plan(self.parents, self.lengths, plan.token_starts, n_tokens,
+                                            n_groups=len(of), max_shared=longest)
+            plan = plan._replace(positions=self.shared.positions)
         self.plan, self._max_new = plan, max(1, most)
         self._version += 1
         return plan
@@ -715,10 +727,46 @@ class PagedKVCache:
     def _last_plan(self, name: str) -> BlockPlan:
         if self.plan is None:
             raise RuntimeError(f"{name} needs a step first")
-        if _capturing(self.lengths) and (not self._kept or self._kept[-1] is not self.plan):
+        if _capturing(self.lengths) and (not self._kept or self._kept[-1][0] is not self.plan):
             # the graph reads it after the next step has replaced it here
-            self._kept.append(self.plan)
+            self._kept.append((self.plan, self.shared))
         return self.plan
+
+    def share(self, requests, parent: int | None) -> None:
+        """From the next step on these requests continue ``parent``: their tokens
+        follow all of its tokens, which the cache holds once; ``attend`` reads
+        those once for all of them, and positions (``append_rotated``) count them.
+        They hold no tokens yet; a request continues only one that continues none.
+        ``parent`` None: they continue nothing.  Graphs follow, but for those of a
+        step that was captured while no request continued another."""
+        at = [int(r) for r in requests]
+        every = range(self.n_requests)
+        if any(r not in every for r in at) or (parent is not None and parent not in every):
+            raise ValueError(f"requests must be within 0 .. {self.n_requests - 1}")
+        if _capturing(self.lengths):
+            raise RuntimeError("share cannot be captured: the host keeps the parents")
+        p = -1 if parent is None else int(parent)
+        if p >= 0:
+            if p in at or self._parent[p] >= 0:
+                raise ValueError(f"request {p} continues another or itself")
+            if any(x in at for x in self._parent):
+                raise ValueError("a request that others continue cannot continue another")
+            if self._host is not None and any(self._host[r] for r in at):
+                raise ValueError("requests hold tokens already: share before their first step")
+        new = list(self._parent)
+        for r in at:
+            new[r] = p
+        self._set_parents(new)
+
+    def _set_parents(self, new: list) -> None:
+        if new == self._parent:
+            return
+        on_gpu = torch.tensor(new, dtype=torch.int32)
+        if self.parents is None:
+            self.parents = on_gpu.to(self.lengths.device)
+        else:
+            self.parents.copy_(on_gpu)
+        self._parent = new
 
     def append(self, keys: torch.Tensor, values: torch.Tensor) -> None:
         """Store the keys and values (N, H, D) of the last step's tokens."""
@@ -745,40 +793,59 @@ class PagedKVCache:
                prefix_lengths: torch.Tensor | None = None) -> torch.Tensor:
         """Attention of the last step's tokens' queries (N, Hq, D); scores and
         masks other than the causal ones as in ``paged_attention``."""
-        return paged_attention(queries, self.store, self.block_table, self.lengths,
-                               self._last_plan("attend").token_starts, scale, causal=causal,
-                               max_new=self._max_new, max_length=max(1, self._bound), out=out,
+        starts = self._last_plan("attend").token_starts
+        longest = self._bound
+        if self.shared is not None and self._host is not None:  # (of those with tokens of their own)
+            longest = max(n for r, n in enumerate(self._host) if r not in self._parent)
+        return paged_attention(queries, self.store, self.block_table, self.lengths, starts, scale,
+                               causal=causal, max_new=self._max_new, max_length=max(1, longest), out=out,
                                softcap=softcap, slopes=slopes, window=window,
-                               prefix_lengths=prefix_lengths)
+                               prefix_lengths=prefix_lengths, shared=self.shared)
 
     def release(self, requests) -> None:
-        """End these requests: their pages go back to the pool."""
+        """End these requests: their pages go back to the pool, and they continue
+        nothing any more.  One that others continue ends with them or after."""
         at = torch.as_tensor(list(requests), dtype=torch.int64)
         if at.numel() and (int(at.min()) < 0 or int(at.max()) >= self.n_requests):
             raise ValueError(f"requests must be within 0 .. {self.n_requests - 1}")
+        gone = set(at.tolist())
+        if any(p in gone and r not in gone for r, p in enumerate(self._parent)):
+            raise ValueError("a request that others continue ends with them or after them")
         if self._host is not None:
-            gone = set(at.tolist())
             self.step([-n if r in gone else 0 for r, n in enumerate(self._host)])
-            return
-        new = torch.zeros_like(self.lengths)
-        at = at.to(new.device)
-        new[at] = -self.lengths[at]
-        self.step(new, 0)
+        else:
+            new = torch.zeros_like(self.lengths)
+            at = at.to(new.device)
+            new[at] = -self.lengths[at]
+            self.step(new, 0)
+        if any(self._parent[r] >= 0 for r in gone):
+            self._set_parents([-1 if r in gone else p for r, p in enumerate(self._parent)])
 
     def trim(self, n: int) -> None:
-        """Give the last ``n`` tokens of every request back."""
+        """Give the last ``n`` tokens of every request back (of those that others
+        continue none)."""
         n = max(0, n)
+        keep = set(self._parent)
         if self._host is not None:
-            self.step([-min(n, have) for have in self._host])
+            self.step([0 if r in keep else -min(n, have) for r, have in enumerate(self._host)])
         else:
-            self.step(-self.lengths.clamp(max=n), 0)
+            new = -self.lengths.clamp(max=n)
+            for r in keep - {-1}:
+                new[r] = 0
+            self.step(new, 0)
 
     # ------------------------------------------- batches of equal steps
+    def _none_shared(self, name: str) -> None:
+        if max(self._parent) >= 0:
+            raise RuntimeError(f"{name} steps all requests alike: where some continue others, use "
+                               f"step, append and attend")
+
     def update_and_fetch(self, keys: torch.Tensor, values: torch.Tensor):
         """Append ``keys`` and ``values`` (B, H, T, D), T tokens to each of the
         cache's B requests.  Returns them as held, (B, H, offset, D) in the
         cache's type (read when used, with ``lazy_fetch``), where all requests
         have one length, else (None, None)."""
+        self._none_shared("update_and_fetch")
         b_, h_, t_, d = keys.shape
         if (b_, h_, d) != (self.n_requests, self.n_kv_heads, self.head_dim) or \
                 values.shape != keys.shape:
@@ -816,6 +883,7 @@ class PagedKVCache:
         if mask is not None and not (isinstance(mask, str) and mask in ("causal", "none")):
             raise ValueError("a paged cache takes no mask array: its requests have lengths of "
                              "their own (mask None or 'causal')")
+        self._none_shared("sdpa")
         b_, hq, t_, d = queries.shape
         if b_ != self.n_requests:
             raise ValueError(f"queries of {b_} sequences, {self.n_requests} requests")
