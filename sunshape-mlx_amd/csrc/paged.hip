@@ -233,61 +233,62 @@ __device__ __forceinline__ void write_shared(int64_t tok, const int32_t *starts,
 
 // One workgroup sorts the requests by their parents, in the requests' order:
 // each wave ranks 64 of them among themselves, then the 64s follow each other.
-// Latency bounds it, as the block tables.
-__global__ void __launch_bounds__(kTableThreads)
+// Latency bounds it, as the block tables: everything is read first, and few
+// requests take a workgroup of four waves, whose barriers are cheaper.
+template <int THREADS>
+__global__ void __launch_bounds__(THREADS)
     shared_plan_kernel(const int32_t *parents, const int32_t *lengths, const int32_t *token_starts, int n_req,
                        int64_t n_tok, int32_t *group_starts, int2 *rows, int32_t *parents_out, int32_t *offsets,
                        int32_t *positions, int inline_rows) {
-    __shared__ int32_t starts[kMaxRequests + 1];
-    __shared__ int32_t parent[kMaxRequests];
-    __shared__ int32_t offset[kMaxRequests];     // of a request's rows among its parent's
-    __shared__ int32_t count[kMaxRequests + 1];  // rows of a parent: so far, then all, then before it
-    __shared__ int32_t sums[kTableThreads / kWave];
-    __shared__ int bad;
+    constexpr int MOST = THREADS == kTableThreads ? kMaxRequests : THREADS;
+    __shared__ int32_t starts[MOST + 1];
+    __shared__ int32_t parent[MOST];
+    __shared__ int32_t length[MOST];
+    __shared__ int32_t offset[MOST];     // of a request's rows among its parent's
+    __shared__ int32_t count[MOST + 1];  // rows of a parent: so far, then all, then before it
+    __shared__ int32_t sums[THREADS / kWave];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    if (tid == 0) bad = 0;
-    for (int r = tid; r <= n_req; r += kTableThreads) starts[r] = token_starts[r], count[r] = 0;
-    __syncthreads();
-    for (int r = tid; r < n_req; r += kTableThreads)
-        if (starts[r + 1] < starts[r]) bad = 1;
-    __syncthreads();
-    const bool failed = bad;
+    int down = 0;
+    for (int r = tid; r <= n_req; r += THREADS) {
+        const int32_t from = token_starts[r];
+        if (r < n_req) {
+            const int32_t to = token_starts[r + 1], p = parents[r], n = lengths[r];
+            down |= to < from;
+            parent[r] = (uint32_t)p < (uint32_t)n_req && p != r && from >= 0 ? p : -1;
+            length[r] = n;
+        }
+        starts[r] = from, count[r] = 0;
+    }
+    const bool failed = __syncthreads_or(down);
     auto rows_of = [&](int r) {  // of those that exist
         return r >= n_req || failed || starts[r] < 0 ? 0 : (int)max(min((int64_t)starts[r + 1], n_tok) - starts[r], (int64_t)0);
     };
-    for (int r0 = wave * kWave; r0 < n_req; r0 += kTableThreads) {
-        const int r = r0 + lane, n = rows_of(r);
-        int p = r < n_req && !failed && starts[r] >= 0 ? parents[r] : -1;
-        if ((uint32_t)p >= (uint32_t)n_req || p == r) p = -1;
+    for (int r0 = wave * kWave; r0 < n_req; r0 += THREADS) {
+        const int r = r0 + lane, n = rows_of(r), p = r < n_req && !failed ? parent[r] : -1;
+        const int m = min(n_req - r0, kWave) - 1;
         int before = 0;
-        for (int k = 0; k < kWave - 1; ++k) {
+        for (int k = 0; k < m; ++k) {
             const int pk = __builtin_amdgcn_readlane(p, k), nk = __builtin_amdgcn_readlane(n, k);
             if (k < lane && pk == p) before += nk;
         }
         if (r < n_req) parent[r] = p, offset[r] = before;
     }
     __syncthreads();
-    for (int r0 = 0; r0 < n_req; r0 += kWave) {
-        if (wave == 0) {
+    if (wave == 0)
+        for (int r0 = 0; r0 < n_req; r0 += kWave) {
             const int r = r0 + lane, p = r < n_req ? parent[r] : -1;
             if (p >= 0) offset[r] += count[p];
             wave_lds_sync();
             if (p >= 0) atomicAdd(&count[p], rows_of(r));
             wave_lds_sync();
         }
-    }
     __syncthreads();
     // where each parent's rows start
-    const int per = (n_req + kTableThreads - 1) / kTableThreads;
+    const int per = (n_req + THREADS - 1) / THREADS;
     const int p0 = min(tid * per, n_req), p1 = min(p0 + per, n_req);
     int s = 0;
     for (int p = p0; p < p1; ++p) s += count[p];
-    int scan = s;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const int y = __shfl_up(scan, o);
-        if (lane >= o) scan += y;
-    }
+    int scan = wave_scan(s);
     if (lane == 63) sums[wave] = scan;
     __syncthreads();
     int from = scan - s;
@@ -299,7 +300,7 @@ __global__ void __launch_bounds__(kTableThreads)
     }
     if (p1 == n_req && p0 < p1) group_starts[n_req] = from;
     __syncthreads();
-    for (int r = tid; r < n_req; r += kTableThreads) {
+    for (int r = tid; r < n_req; r += THREADS) {
         const int p = parent[r];
         if (p >= 0) offset[r] += count[p];
         parents_out[r] = p, offsets[r] = offset[r];
@@ -308,11 +309,10 @@ __global__ void __launch_bounds__(kTableThreads)
     __syncthreads();
     if (failed) {
         if (positions)
-            for (int64_t t = tid; t < n_tok; t += kTableThreads) positions[t] = -1;
+            for (int64_t t = tid; t < n_tok; t += THREADS) positions[t] = -1;
         return;
     }
-    for (int64_t t = tid; t < n_tok; t += kTableThreads)
-        write_shared(t, starts, n_req, lengths, parent, offset, rows, positions);
+    for (int64_t t = tid; t < n_tok; t += THREADS) write_shared(t, starts, n_req, length, parent, offset, rows, positions);
 }
 
 __global__ void __launch_bounds__(256)
@@ -534,8 +534,12 @@ extern "C" int ss_shared_plan(const int32_t *parents, const int32_t *lengths, co
     const int in_one = n_tokens <= kSlotsInline;
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
     int2 *const rows = reinterpret_cast<int2 *>(group_rows);
-    hipLaunchKernelGGL(shared_plan_kernel, dim3(1), dim3(kTableThreads), 0, st, parents, lengths, token_starts,
-                       (int)n_requests, n_tokens, group_starts, rows, parents_out, offsets, positions, in_one);
+    auto launch = [&](auto kernel, int threads) {
+        hipLaunchKernelGGL(kernel, dim3(1), dim3(threads), 0, st, parents, lengths, token_starts, (int)n_requests,
+                           n_tokens, group_starts, rows, parents_out, offsets, positions, in_one);
+    };
+    if (n_requests <= 256 && n_tokens <= 1024) launch(shared_plan_kernel<256>, 256);
+    else launch(shared_plan_kernel<kTableThreads>, kTableThreads);
     SS_LAUNCH_CHECK("shared_plan_kernel launch");
     if (!in_one) {
         hipLaunchKernelGGL(shared_rows_kernel, dim3((unsigned)((n_tokens + 255) / 256)), dim3(256), 0, st,

@@ -198,7 +198,10 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(const PagedAttn a) {
     int u, stop, base, r, share, parts = 0;
     // Columns to be joined are listed for the merge, (parts, request, first
     // workgroup, column of the request) at `list`: by column where they are few.
-    const bool few = a.cut && all_columns <= groups / 2;
+    // (Of ranges also where no column is cut and each can have a workgroup of its
+    // own: the own tokens of 64 requests behind a shared prefix, up to 512 each, XX us
+    // instead of 24.)
+    const bool few = a.cut ? all_columns <= groups / 2 : MODE != kPlain && all_columns <= groups;
     int list = blockIdx.x;
     int4 cut = make_int4(0, 0, 0, 0);
     if (few) {
@@ -213,7 +216,9 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(const PagedAttn a) {
             }
             return n;
         };
-        share = max(uniform_div(total + groups - all_columns / 2 - 1, groups - all_columns / 2), 1);
+        share = INT32_MAX;
+        if (MODE == kPlain || a.cut)
+            share = max(uniform_div(total + groups - all_columns / 2 - 1, groups - all_columns / 2), 1);
         int scan = wave_scan(items(share));
         if (__builtin_amdgcn_readlane(scan, 63) > groups) {
             share = uniform_div(total + groups - all_columns - 1, groups - all_columns);
@@ -237,7 +242,7 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(const PagedAttn a) {
                     stop = u + part_begin(part + 1, n_units, parts);
                     u += part_begin(part, n_units, parts);
                     list += column;
-                    if (part == 0 && threadIdx.x == 0)
+                    if (part == 0 && threadIdx.x == 0 && (MODE == kPlain || a.cut))
                         a.cut[list] = make_int4(parts > 1 ? parts : 0, r, blockIdx.x, column);
                     break;
                 }
@@ -388,18 +393,18 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(const PagedAttn a) {
         float offset[NS];  // of the exponents: kProb less the maximum's
         // (scores are in log2 units by then)
         auto unit = [&](int s) { return MODE == kScores ? 1.f : factor[s]; };
-        auto set_offset = [&](int s) { offset[s] = kProb - (top[s] == -INFINITY ? 0.f : top[s] * unit(s)); };
+        auto set_offset = [&](int s) __attribute__((always_inline)) { offset[s] = kProb - (top[s] == -INFINITY ? 0.f : top[s] * unit(s)); };
 #pragma unroll
         for (int s = 0; s < NS; ++s) set_offset(s);
         const CodeBits code_bits;
-        auto rescale = [&](int s, float f) {  // (what is times up)
+        auto rescale = [&](int s, float f) __attribute__((always_inline)) {  // (what is times up)
             ones[s] *= f;
 #pragma unroll
             for (int j = 0; j < VT; ++j) o[s][j] *= f;
         };
 
         // mask: some row does not see some token of the tile
-        auto compute = [&](const char *slot, int tb, bool ok, bool mask) {
+        auto compute = [&](const char *slot, int tb, bool ok, bool mask) __attribute__((always_inline)) {
             uint32_t kw[2][KS], vw[VT], km[8], vm[8];
 #pragma unroll
             for (int y = 0; y < 2; ++y) {
@@ -530,7 +535,7 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(const PagedAttn a) {
 
         // one tile: the next to fetch goes into `into`, the oldest is at `slot`
         auto step = [&](char *__restrict into, const char *__restrict slot, int tb, int p0, int p1, int next0,
-                        int next1) {
+                        int next1) __attribute__((always_inline)) {
             if (tb + (kStages - 1) * kUnit < end) {
                 TL::fetch(a.st, h, lane, into, tb + (kStages - 1) * kUnit, next0, next1);
                 wait_loads<(kStages - 1) * TL::kLoads>();
@@ -769,7 +774,10 @@ static void launch_paged_store(const PagedAttn &a, const ss_paged_store *s, cons
 // One pass: the requests whose rows are few, then (p.prompts) the others.
 static int launch_pass(PagedAttn &a, const ss_paged_store *s, const PagedPlan &p, int mode, void *workspace,
                        size_t workspace_bytes, hipStream_t st) {
-    a.most_rows = p.prompts ? kPromptRows : INT32_MAX;
+    // Shared tokens are one kernel's: of one prefix all rows come together, and a
+    // launch that finds none costs 5 us, its merge 5 more.
+    a.most_rows = !p.prompts ? INT32_MAX : a.rows_of ? 0 : kPromptRows;
+    if (a.most_rows == 0) return launch_paged_prompt(a, s, mode, workspace, workspace_bytes, st);
     a.cut = p.cut ? static_cast<int4 *>(workspace) : nullptr;
     a.acc = reinterpret_cast<float *>(a.cut + p.groups + 1);
     a.ml = a.acc + (size_t)p.groups * 2 * p.rows * s->head_dim;
@@ -823,6 +831,8 @@ static PagedPasses paged_passes(const ss_paged_store *s, int64_t n_tokens, int64
     if (asked.shared) {
         const int64_t groups = min(sc->n_groups, n_requests);
         p.shared = paged_plan(s, n_tokens, groups, n_q_heads, max((int64_t)1, n_tokens / groups), sc->max_shared);
+        if (p.shared.prompts)  // (of any number of rows)
+            p.shared.bytes = paged_prompt_bytes(s, n_requests, n_tokens * (n_q_heads / s->n_kv_heads), 0);
         p.part = ((size_t)n_tokens * n_q_heads * (s->head_dim + 2) * 4 + 15) & ~(size_t)15;
         p.bytes = p.part + max(p.shared.bytes, p.own.bytes);
     }

@@ -38,6 +38,17 @@ __device__ __forceinline__ uint32_t to_bits16(float x) {
     return __half_as_ushort(__float2half(x));
 }
 
+// Inclusive sum over the lanes before (lane moves, no LDS).
+__device__ __forceinline__ int wave_scan(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);  // row_shr:1
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // row_bcast:15 -> rows 1, 3
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // row_bcast:31 -> rows 2, 3
+    return v;
+}
+
 // Two nearest 16-bit floats (one instruction), `a` in the low half.
 template <bool BF>
 __device__ __forceinline__ uint32_t pack16(float a, float b) {

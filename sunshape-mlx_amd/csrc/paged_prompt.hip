@@ -374,11 +374,13 @@ __global__ void __launch_bounds__(64 * kPWaves, 2) paged_prompt_kernel(const Pag
         // Element i of a product's 16: its value's group, as NT dims a row of
         // the A operand make neighbours (row m of tile j is dim NT*m + j).
         auto group_of = [](int i) { return i / 4 * G / 4; };
+        // (Inlined by force, as all that reaches LDS here: out of line it would do so
+        // through generic pointers, which end where LDS passes 64 KB.)
         // The tile's prepared form, its values times a power of two that holds
         // them (a lane looks at one token's pairs); bit t of bad_next[g]: token
         // t's group g is not finite.
         uint64_t bad_next[G];
-        auto prepare = [&](const char *__restrict slot, char *__restrict out, int tb, int ok) {
+        auto prepare = [&](const char *__restrict slot, char *__restrict out, int tb, int ok) __attribute__((always_inline)) {
             const CodeBits code_bits;
             constexpr uint32_t kInf = BF ? 0x7f80u : 0x7c00u;
             constexpr int KW = D / 64, VW = NT / 2;  // words of keys and values that a lane takes
@@ -489,7 +491,7 @@ __global__ void __launch_bounds__(64 * kPWaves, 2) paged_prompt_kernel(const Pag
         // `out`; the copy of a later one started into `into`.  (The pointers
         // differ: no read here waits for that copy.)
         auto step = [&](char *__restrict into, const char *__restrict next, const char *__restrict cur,
-                        char *__restrict out, int tile) {
+                        char *__restrict out, int tile) __attribute__((always_inline)) {
             const int tb = tile * kTokens;
             if (tile + kSlots < n_tiles)
                 PT::fetch(a.st, h, lane, into + seg * PT::kSeg, own(pages), offset(tile + kSlots), wave >> 2);
@@ -732,7 +734,10 @@ static void launch_prompt(const PagedAttn &a, bool bf, unsigned groups, hipStrea
         hipLaunchKernelGGL((paged_prompt_kernel<D, G, true, MODE>), dim3(groups), block, 0, st, a);
     else
         hipLaunchKernelGGL((paged_prompt_kernel<D, G, false, MODE>), dim3(groups), block, 0, st, a);
-    if (a.target) hipLaunchKernelGGL((prompt_merge_kernel<D, MODE>), dim3(16, a.target), dim3(256), 0, st, a);
+    // (of ranges, where a few columns of many parts are the rule, more workgroups a
+    // column: 8 columns of 31 parts XX us instead of 11.3)
+    if (a.target)
+        hipLaunchKernelGGL((prompt_merge_kernel<D, MODE>), dim3(MODE == kPlain ? 16 : 32, a.target), dim3(256), 0, st, a);
 }
 
 template <int MODE>
