@@ -274,6 +274,11 @@ __global__ void __launch_bounds__(64 * kPWaves, 2) paged_prompt_kernel(const Pag
 #pragma unroll
                 for (int s = 0; s < HW; ++s) rawq[g][s] = load_query8(q + (g * GW + half * HW + s) * 8, a.vec);
         }
+        // With a bias of distance the last tile comes first (as in the decode kernel).
+        // The tile in place i of the order:
+        auto tile_at = [&](int i) __attribute__((always_inline)) {
+            return MODE == kScores && a.slopes ? max(first_tile + n_tiles - 1 - i, 0) : i;
+        };
         // A tile's four pages, of 16 tokens each; bit w of the mask: it is in the pool.
         auto pages_of = [&](int tile, int (&p)[4]) {
 #pragma unroll
@@ -292,13 +297,13 @@ __global__ void __launch_bounds__(64 * kPWaves, 2) paged_prompt_kernel(const Pag
         wait_loads<0>();  // the queries, before tiles are waited for with them
 #pragma unroll
         for (int i = 0; i < kSlots; ++i) {
-            pages_of(first_tile + i, pages);
+            pages_of(tile_at(first_tile + i), pages);
             ok[i] = mask_of(pages);
             if (first_tile + i < n_tiles)
-                PT::fetch(a.st, h, lane, raw + i * PT::kBytes + seg * PT::kSeg, own(pages), offset(first_tile + i),
+                PT::fetch(a.st, h, lane, raw + i * PT::kBytes + seg * PT::kSeg, own(pages), offset(tile_at(first_tile + i)),
                           wave >> 2);
         }
-        pages_of(first_tile + kSlots, pages);
+        pages_of(tile_at(first_tile + kSlots), pages);
 
         half8_t qf[G][HW];
         bf8_t qz[(G + 1) / 2];
@@ -492,9 +497,9 @@ __global__ void __launch_bounds__(64 * kPWaves, 2) paged_prompt_kernel(const Pag
         // differ: no read here waits for that copy.)
         auto step = [&](char *__restrict into, const char *__restrict next, const char *__restrict cur,
                         char *__restrict out, int tile) __attribute__((always_inline)) {
-            const int tb = tile * kTokens;
+            const int tb = tile_at(tile) * kTokens, tb_next = tile_at(tile + 1) * kTokens;
             if (tile + kSlots < n_tiles)
-                PT::fetch(a.st, h, lane, into + seg * PT::kSeg, own(pages), offset(tile + kSlots), wave >> 2);
+                PT::fetch(a.st, h, lane, into + seg * PT::kSeg, own(pages), offset(tile_at(tile + kSlots)), wave >> 2);
             // Of the two waves of a SIMD, w and w + 4, one prepares first and one
             // last, so that one's products meet the other's softmax.  The wave that
             // prepares goes first: the other has matrix products on their way (4093
@@ -504,7 +509,7 @@ __global__ void __launch_bounds__(64 * kPWaves, 2) paged_prompt_kernel(const Pag
 #pragma unroll
             for (int g = 0; g < G; ++g) bad[g] = bad_next[g], move[g] = vexp[g] - vnext[g], vexp[g] = vnext[g];
             __builtin_amdgcn_s_setprio(1);
-            if (tile + 1 < n_tiles && wave >= 4) prepare(next, out, tb + kTokens, ok[1]);
+            if (tile + 1 < n_tiles && wave >= 4) prepare(next, out, tb_next, ok[1]);
 #pragma unroll
             for (int g = 0; g < G; ++g)
                 if (move[g]) {
@@ -622,12 +627,12 @@ __global__ void __launch_bounds__(64 * kPWaves, 2) paged_prompt_kernel(const Pag
                     }
             }
             __builtin_amdgcn_s_setprio(1);
-            if (tile + 1 < n_tiles && wave < 4) prepare(next, out, tb + kTokens, ok[1]);
+            if (tile + 1 < n_tiles && wave < 4) prepare(next, out, tb_next, ok[1]);
         };
 
         wait_loads<0>();
         __syncthreads();
-        if (first_tile < n_tiles) prepare(raw, prepared, first_tile * kTokens, ok[0]);
+        if (first_tile < n_tiles) prepare(raw, prepared, tile_at(first_tile) * kTokens, ok[0]);
         int slot = 0, into = 1;  // raw slot and prepared form of the tile computed
         for (int i = first_tile; i < n_tiles; ++i) {
             // the wave's copies of the next tile (of the one after it, two loads or
@@ -646,7 +651,7 @@ __global__ void __launch_bounds__(64 * kPWaves, 2) paged_prompt_kernel(const Pag
 #pragma unroll
             for (int k = 0; k < kSlots; ++k) ok[k] = ok[k + 1];
             ok[kSlots - 1] = mask_of(pages);
-            pages_of(i + kSlots + 1, pages);
+            pages_of(tile_at(i + kSlots + 1), pages);
         }
 
         const float sum = l + __shfl_xor(l, 32);
