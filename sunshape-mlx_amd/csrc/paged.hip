@@ -265,11 +265,12 @@ __global__ void __launch_bounds__(THREADS)
     };
     for (int r0 = wave * kWave; r0 < n_req; r0 += THREADS) {
         const int r = r0 + lane, n = rows_of(r), p = r < n_req && !failed ? parent[r] : -1;
-        const int m = min(n_req - r0, kWave) - 1;
         int before = 0;
-        for (int k = 0; k < m; ++k) {
-            const int pk = __builtin_amdgcn_readlane(p, k), nk = __builtin_amdgcn_readlane(n, k);
-            if (k < lane && pk == p) before += nk;
+        for (uint64_t left = __ballot(p >= 0); left;) {  // (one parent after the other)
+            const bool mine = p == __builtin_amdgcn_readlane(p, __ffsll((unsigned long long)left) - 1);
+            const int rows = mine ? n : 0, sum = wave_scan(rows);
+            if (mine) before = sum - rows;
+            left &= ~__ballot(mine);
         }
         if (r < n_req) parent[r] = p, offset[r] = before;
     }
