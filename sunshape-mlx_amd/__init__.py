@@ -5,7 +5,8 @@ gauravsaini/sunshape-mlx behind that package's Python API: block-VQ key
 encoding, the per-step query x centroid table, fused split-T gather-attention
 decode over uint8 key indices with fp16 or grouped 2/3/4-bit values, KV-cache
 append and value packing; and a paged cache of 4-bit keys and values for many
-requests (``PagedKVCache``).  Compute runs in ``libsunshape_hip.so`` (C ABI in
+requests (``PagedKVCache``), with a layer's norms, rotation, score rules and
+shared prefixes around it.  Compute runs in ``libsunshape_hip.so`` (C ABI in
 ``include/sunshape_hip.h``); torch supplies device memory and streams.
 
 The source directory is ``sunshape-mlx_amd/``; it is imported under the name

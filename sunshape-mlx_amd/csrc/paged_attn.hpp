@@ -182,11 +182,10 @@ __device__ __forceinline__ void finish_row(const PagedAttn &a, int r, int64_t t,
 // A row's products x with tokens 16 (i / 8) + i % 8 become scores in log2 units,
 // capped and biased, less the row's reference `ref`.  slope: the head's, in
 // log2 units a token; far: how many tokens the row is behind token 0.
-// A cap's tanh(u) is u times a polynomial of u^2 (least largest error below
-// |u| = 5/8, 2^-23 of it) where a wave's scores are all that small, which most
-// are and which takes 8 operations each; else 1 - 2 / (1 + exp(2 u)), 11
-// operations' time, off by 2^-22 and more exactly so where u is small.  Either
-// way a score is off by 2^-21 of the largest in the tile.
+// A cap's tanh(u) is u times a polynomial of u^2 (of the least largest error below
+// |u| = 5/8: 2^-23 of it) where a wave's scores are all that small, as most are
+// (9 operations each); else 1 - 2 / (1 + exp(2 u)), off by 2^-22 (12 operations'
+// time).  Either way a score is off by 2^-21 of the largest in the tile.
 template <int N, typename X>
 __device__ __forceinline__ void apply_scores(const PagedAttn &a, float slope, float factor, float ref, float far,
                                              X &x) {

@@ -8,13 +8,23 @@
 // and once to float32), so that the keys' 16-bit roundings, and with them the
 // codes, are the same wherever this is computed: a fused multiply-add would
 // move one code in some 10^5.
+//
+// A prompt of 8192 tokens, 32 query and 8 KV heads of 128 dims, with norms, takes
+// 48 us (181 MB, 3.8 TB/s; 36 us at the rate of a large copy): vector issue (70 %
+// of the cycles: a key or value costs 20 operations, most of them its quantising, a
+// query's element 7) beside HBM.  256 tokens take 7.7 us, one 4.3: the chain
+// from a position over the table's row to the codes.
 #include "paged_append.hpp"
 
 namespace ss {
 
-constexpr int kMostRun = 2;  // query heads of a wave
-constexpr int kStripe = 8;   // workgroups in a row of one kind, queries or keys
-constexpr int kMix = 16;     // stripes that the two share
+// Query heads of a wave (1: 58 us, 2: 48 us, 4: 53 us for the prompt above).
+constexpr int kMostRun = 2;
+// Workgroups in a row of one kind, queries or keys and values, and such stripes
+// that the two share in proportion: one kind after the other takes 62 us where
+// stripes of 8 take 52, of 2 to 32 about as much (in an earlier form).
+constexpr int kStripe = 8;
+constexpr int kMix = 16;
 
 struct RotatedAppend {
     PagedStore st;
