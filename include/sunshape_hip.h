@@ -1166,9 +1166,8 @@ int ss_paged_attn(const ss_paged_store *store, const void *q, int q_dtype, int64
  * others.  Score s = scale q.k of a row at position p with token t becomes
  *   softcap tanh(s / softcap)      (softcap > 0)
  *   s - slopes[hq] |p - t|         (slopes: float32 [n_q_heads])
- * and the row sees the tokens t > p - window (window > 0), of those the ones up
- * to p, or, causal or not, any below prefix_lengths[r] of its request's.
- * (Tokens at or behind a row's own that no mask hides count |p - t| too.)
+ * and of the request's tokens t > p - window (window > 0; else all) the row sees
+ * those up to p (causal; else all) and those below prefix_lengths[r].
  * group_starts, group_rows, parents: a plan of ss_shared_plan for these
  * token_starts; rows of request r with parents[r] >= 0 then see all
  * lengths[parents[r]] tokens of that request before their own, whose positions

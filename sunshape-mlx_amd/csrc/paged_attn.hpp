@@ -186,19 +186,22 @@ __device__ __forceinline__ void finish_row(const PagedAttn &a, int r, int64_t t,
 // |u| = 5/8: 2^-23 of it) where a wave's scores are all that small, as most are
 // (9 operations each); else 1 - 2 / (1 + exp(2 u)), off by 2^-22 (12 operations'
 // time).  Either way a score is off by 2^-21 of the largest in the tile.
-template <int N, typename X>
-__device__ __forceinline__ void apply_scores(const PagedAttn &a, float slope, float factor, float ref, float far,
-                                             X &x) {
+// (A bias meets the reference first: both may be large, what is left of them is
+// rounded once.)
+template <int N, bool BIAS, typename X>
+__device__ __forceinline__ void apply_rule(const PagedAttn &a, float slope, float factor, float ref, float far, X &x) {
+    auto rest = [&](int i) __attribute__((always_inline)) {
+        return BIAS ? fmaf(-slope, fabsf(far - (float)(16 * (i / 8) + i % 8)), -ref) : -ref;
+    };
     if (a.cap > 0.f) {
         const float cap = a.cap * kLog2e, by = factor / cap;
         float most = 0.f;
 #pragma unroll
         for (int i = 0; i < N; ++i) x[i] *= by, most = fmaxf(most, fabsf(x[i]));
         if (__any(most > 0.625f)) {
-            const float less = cap - ref;
 #pragma unroll
             for (int i = 0; i < N; ++i)
-                x[i] = fmaf(-2.f * cap, __builtin_amdgcn_rcpf(1.f + fast_exp2(x[i] * (2.f * kLog2e))), less);
+                x[i] = fmaf(-2.f * cap, __builtin_amdgcn_rcpf(1.f + fast_exp2(x[i] * (2.f * kLog2e))), cap + rest(i));
         } else {
 #pragma unroll
             for (int i = 0; i < N; ++i) {
@@ -207,16 +210,21 @@ __device__ __forceinline__ void apply_scores(const PagedAttn &a, float slope, fl
                 p = fmaf(v, p, 0.133045261f);
                 p = fmaf(v, p, -0.333319543f);
                 p = fmaf(v, p, 0.999999893f);
-                x[i] = fmaf(x[i] * p, cap, -ref);
+                x[i] = fmaf(x[i] * p, cap, rest(i));
             }
         }
     } else {
 #pragma unroll
-        for (int i = 0; i < N; ++i) x[i] = fmaf(x[i], factor, -ref);
+        for (int i = 0; i < N; ++i) x[i] = fmaf(x[i], factor, rest(i));
     }
+}
+template <int N, typename X>
+__device__ __forceinline__ void apply_scores(const PagedAttn &a, float slope, float factor, float ref, float far,
+                                             X &x) {
     if (a.slopes)
-#pragma unroll
-        for (int i = 0; i < N; ++i) x[i] = fmaf(-slope, fabsf(far - (float)(16 * (i / 8) + i % 8)), x[i]);
+        apply_rule<N, true>(a, slope, factor, ref, far, x);
+    else
+        apply_rule<N, false>(a, slope, factor, ref, far, x);
 }
 
 // How a query row whose largest magnitude is `top` enters the products: times

@@ -254,7 +254,8 @@ __global__ void __launch_bounds__(64 * kPWaves, 2) paged_prompt_kernel(const Pag
         auto sees = [&](int row) { return last_seen<MODE>(a, rq, row / a.rep); };
         auto from = [&](int row) { return first_seen<MODE>(a, rq, row / a.rep); };
         const int last_row = min(row_tile * kRows + kRows, rq.rows) - 1;
-        const int unseen = __builtin_amdgcn_readfirstlane(from(row_tile * kRows)) / kTokens;  // tiles, by the workgroup
+        const int any_from = __builtin_amdgcn_readfirstlane(from(row_tile * kRows));  // by the workgroup
+        const int unseen = any_from / kTokens;
         const int seen_tiles =
             max((__builtin_amdgcn_readfirstlane(sees(last_row)) + kTokens - 1) / kTokens - unseen, 0);
         const int first_tile = unseen + part_begin(part, seen_tiles, parts);
@@ -444,8 +445,8 @@ __global__ void __launch_bounds__(64 * kPWaves, 2) paged_prompt_kernel(const Pag
                     reinterpret_cast<uint16_t *>(out + 2 * PT::kOperands + PT::kZeros)[wave * kTokens + lane] = (uint16_t)km;
             }
 
-            const bool real = tb + lane < rq.len && (ok >> (lane >> 4) & 1);
-            bool odd_ones = tb + kTokens > rq.len || ok != 15;
+            const bool real = tb + lane < rq.len && (MODE == kPlain || tb + lane >= any_from) && (ok >> (lane >> 4) & 1);
+            bool odd_ones = tb + kTokens > rq.len || (MODE != kPlain && tb < any_from) || ok != 15;
             bool more = false;
 #pragma unroll
             for (int g = 0; g < G; ++g) {
@@ -481,7 +482,8 @@ __global__ void __launch_bounds__(64 * kPWaves, 2) paged_prompt_kernel(const Pag
                 for (int g = 0; g < G; ++g) keep = vg == g ? ~bad_next[g] : keep;
 #pragma unroll
                 for (int i = 0; i < 8; ++i)
-                    if (tb + 8 * wave + i >= rq.len || !((ok >> (wave >> 1)) & 1) || !((keep >> (8 * wave + i)) & 1))
+                    if (tb + 8 * wave + i >= rq.len || (MODE != kPlain && tb + 8 * wave + i < any_from) ||
+                        !((ok >> (wave >> 1)) & 1) || !((keep >> (8 * wave + i)) & 1))
                         vm[i] = 0;
             }
             // (read as scalars: as elements the compiler would index an array in memory)

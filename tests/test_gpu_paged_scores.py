@@ -194,6 +194,40 @@ def test_what_a_window_hides_may_hold_anything(kw, many):
 
 
 @pytest.mark.parametrize("many", [False, True])
+def test_large_values_before_a_window_cost_nothing(many):
+    """Finite ones too: the row's values keep their bits."""
+    lengths, new = ([400, 1000], [200, 300]) if many else ([400, 1000], [1, 3])
+    store, table = pool(29, lengths, 2, 128, 64, 16, BF16, width=1 << 12 if many else None)
+    for r, n in enumerate(lengths):
+        for t in range(max(0, n - new[r] + 1 - 75)):
+            store.v_meta[int(table[r, t // 16]), :, :, t % 16] = 1e37
+    q = queries(30, sum(new), 8, 128, BF16)
+    starts = ints([0, new[0], sum(new)])
+    for kw in (dict(window=75), dict(window=75, softcap=4.0)):
+        got = S.paged_attention(q, store, table, ints(lengths), starts, 0.1, **kw)
+        error = R.check(got, R.attend(q, store, table, ints(lengths), starts, 0.1, **kw))
+        assert not error, error
+
+
+@pytest.mark.parametrize("many", [False, True])
+def test_a_steep_bias_keeps_the_scores_of_near_tokens(many):
+    """Biases of 10^5 and more beside scores of a few units, with a cap and
+    without."""
+    lengths, new = ([9000, 800], [150, 90]) if many else ([9000, 800], [1, 5])
+    store, table = pool(31, lengths, 2, 128, 64, 64, F16, width=1 << 12 if many else None)
+    # nothing is held near the rows: their largest scores are far below 0
+    table[0, 130:] = -1
+    q = queries(32, sum(new), 8, 128, F16)
+    starts, slopes = ints([0, new[0], sum(new)]), torch.full((8,), 0.0, device=DEV)
+    slopes[:] = torch.tensor([300.0, 40.0, 7.0, 1.0, 0.3, 0.01, 150.0, 2.0])
+    for kw in (dict(slopes=slopes), dict(slopes=slopes, softcap=5.0)):
+        got = S.paged_attention(q, store, table, ints(lengths), starts, 0.1, **kw)
+        want = R.attend(q, store, table, ints(lengths), starts, 0.1, **kw)
+        error = R.check(got, want, False)
+        assert not error, error
+
+
+@pytest.mark.parametrize("many", [False, True])
 def test_pages_outside_the_pool(many):
     lengths, new = ([300, 500], [100, 90]) if many else ([300, 500], [1, 2])
     store, table = pool(12, lengths, 2, 64, 32, 16, BF16, width=1 << 12 if many else None)
@@ -259,6 +293,27 @@ def test_wrong_hints_change_roundings_only():
             got = S.paged_attention(q, store, table, ints(lengths), starts, 0.1, **hints, **call)
             error = R.check(got, want)
             assert not error, (hints, error)
+
+
+@pytest.mark.parametrize("new", [0, 1, 5, 40, 300])
+@pytest.mark.parametrize("kw", [dict(softcap=9.0), dict(window=100), dict(prefix_lengths=None)])
+def test_one_request_with_hints_of_many_rows(kw, new):
+    """One request's rows are one kernel's, whichever the hints name; rows in
+    front of it and behind it are zeroed there too."""
+    store, table = pool(27, [700], 2, 128, 64, 16, F16, width=1 << 13)
+    q, starts = queries(28, new + 5, 8, 128, F16), ints([2, 2 + new])
+    call = dict(kw)
+    if "prefix_lengths" in kw:
+        call, kw = dict(prefix_lengths=ints([600])), dict(prefix=[600])
+    for hints in (dict(max_new=10 ** 5, max_length=10 ** 6), dict(max_new=1, max_length=700), dict()):
+        got = S.paged_attention(q, store, table, ints([700]), starts, 0.1, **hints, **call)
+        error = R.check(got, R.attend(q, store, table, ints([700]), starts, 0.1, **kw))
+        assert not error, (hints, error)
+        assert not bool(got[:2].any() | got[2 + new:].any())
+        out = torch.full_like(q, 7.0)
+        S.paged_attention(q, store, table, ints([700]), starts, 0.1, out=out, **hints, **call)
+        assert torch.equal(out[2:2 + new], got[2:2 + new])
+        assert bool((out[:2] == 7.0).all()) and bool((out[2 + new:] == 7.0).all())
 
 
 def test_strided_and_unaligned_queries():
