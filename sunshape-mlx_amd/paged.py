@@ -653,6 +653,7 @@ class PagedKVCache:
         self._kept: list[tuple] = []        # of steps that graphs go on reading
         self.parents: torch.Tensor | None = None  # on the GPU, once a request has one
         self._parent = [-1] * n_requests
+        self._prefixes: frozenset[int] = frozenset()  # the requests that others continue
         self._version = 0                   # bumped by every change of the stored tokens
         # what the host knows of the lengths: all of them (steps given as
         # lists), or a bound
@@ -717,11 +718,10 @@ class PagedKVCache:
         # (only now: a step that was refused has changed nothing here either)
         self._host, self._bound = host, bound
         self.shared = None
-        of = {p for p in self._parent if p >= 0}
-        if of:
-            longest = bound if host is None else max(host[p] for p in of)
+        if self._prefixes:
+            longest = bound if host is None else max(host[p] for p in self._prefixes)
             self.shared = build_shared_plan(self.parents, self.lengths, plan.token_starts, n_tokens,
-                                            n_groups=len(of), max_shared=longest)
+                                            n_groups=len(self._prefixes), max_shared=longest)
             plan = plan._replace(positions=self.shared.positions)
         self.plan, self._max_new = plan, max(1, most)
         self._version += 1
@@ -757,7 +757,7 @@ class PagedKVCache:
         if p >= 0:
             if p in at or self._parent[p] >= 0:
                 raise ValueError(f"request {p} continues another or itself")
-            if any(x in at for x in self._parent):
+            if not self._prefixes.isdisjoint(at):
                 raise ValueError("a request that others continue cannot continue another")
             if self._host is not None and any(self._host[r] for r in at):
                 raise ValueError("requests hold tokens already: share before their first step")
@@ -774,7 +774,7 @@ class PagedKVCache:
             self.parents = on_gpu.to(self.lengths.device)
         else:
             self.parents.copy_(on_gpu)
-        self._parent = new
+        self._parent, self._prefixes = new, frozenset(new) - {-1}
 
     def append(self, keys: torch.Tensor, values: torch.Tensor) -> None:
         """Store the keys and values (N, H, D) of the last step's tokens."""
@@ -804,7 +804,7 @@ class PagedKVCache:
         starts = self._last_plan("attend").token_starts
         longest = self._bound
         if self.shared is not None and self._host is not None:  # (of those with tokens of their own)
-            longest = max(n for r, n in enumerate(self._host) if r not in self._parent)
+            longest = max((n for r, n in enumerate(self._host) if r not in self._prefixes), default=1)
         return paged_attention(queries, self.store, self.block_table, self.lengths, starts, scale,
                                causal=causal, max_new=self._max_new, max_length=max(1, longest), out=out,
                                softcap=softcap, slopes=slopes, window=window,
@@ -817,7 +817,8 @@ class PagedKVCache:
         if at.numel() and (int(at.min()) < 0 or int(at.max()) >= self.n_requests):
             raise ValueError(f"requests must be within 0 .. {self.n_requests - 1}")
         gone = set(at.tolist())
-        if any(p in gone and r not in gone for r, p in enumerate(self._parent)):
+        if not self._prefixes.isdisjoint(gone) and \
+                any(p in gone and r not in gone for r, p in enumerate(self._parent)):
             raise ValueError("a request that others continue ends with them or after them")
         if self._host is not None:
             self.step([-n if r in gone else 0 for r, n in enumerate(self._host)])
@@ -826,25 +827,25 @@ class PagedKVCache:
             at = at.to(new.device)
             new[at] = -self.lengths[at]
             self.step(new, 0)
-        if any(self._parent[r] >= 0 for r in gone):
+        if self._prefixes and any(self._parent[r] >= 0 for r in gone):
             self._set_parents([-1 if r in gone else p for r, p in enumerate(self._parent)])
 
     def trim(self, n: int) -> None:
         """Give the last ``n`` tokens of every request back (of those that others
         continue none)."""
         n = max(0, n)
-        keep = set(self._parent)
+        keep = self._prefixes
         if self._host is not None:
             self.step([0 if r in keep else -min(n, have) for r, have in enumerate(self._host)])
         else:
             new = -self.lengths.clamp(max=n)
-            for r in keep - {-1}:
+            for r in keep:
                 new[r] = 0
             self.step(new, 0)
 
     # ------------------------------------------- batches of equal steps
     def _none_shared(self, name: str) -> None:
-        if max(self._parent) >= 0:
+        if self._prefixes:
             raise RuntimeError(f"{name} steps all requests alike: where some continue others, use "
                                f"step, append and attend")
 
