@@ -294,7 +294,7 @@ def build_shared_plan(parents: torch.Tensor, lengths: torch.Tensor, token_starts
     args = (_index("parents", parents, (r,), dev), _index("lengths", lengths, (r,), dev),
             _index("token_starts", token_starts, (r + 1,), dev), r, n_tokens)
     # one allocation for everything that is new
-    buf = torch.empty(3 * n_tokens + 3 * r + 1, dtype=torch.int32, device=parents.device)
+    buf = parents.new_empty(3 * n_tokens + 3 * r + 1)
     rows, starts, of, _, positions = buf.split_with_sizes((2 * n_tokens, r + 1, r, r, n_tokens))
     at = buf.data_ptr()
     at_starts = at + 8 * n_tokens
@@ -457,9 +457,8 @@ def read_paged(store: PagedKVStore, slots: torch.Tensor) -> tuple[torch.Tensor, 
     dev = store[0].get_device()
     at_slots = _index("slots", slots, (n,), dev)
     shape = (n, st.n_kv_heads, st.head_dim)
-    dtype, device = store[2].dtype, store[0].device
-    k = torch.empty(shape, dtype=dtype, device=device)
-    v = torch.empty(shape, dtype=dtype, device=device)
+    k = store[2].new_empty(shape)
+    v = torch.empty_like(k)
     _launch("ss_read_paged", dev, ctypes.addressof(st), at_slots, n, k.data_ptr(), v.data_ptr())
     return k, v
 
