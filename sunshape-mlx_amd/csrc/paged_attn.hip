@@ -732,7 +732,7 @@ static PagedPlan paged_plan(const ss_paged_store *s, int64_t n_tokens, int64_t n
     p.columns = (int)min(columns, (double)p.groups);
     p.bytes = p.cut ? 16 + (size_t)p.groups * (16 + 2 * p.rows * (s->head_dim + 2) * 4) : 0;
     if (p.prompts)  // (one after the other: they share it)
-        p.bytes = max(p.bytes, paged_prompt_bytes(s, n_requests, n_tokens * rep, kPromptRows));
+        p.bytes = max(p.bytes, paged_prompt_bytes(s, n_requests, n_tokens * rep, kPromptRows, false));
     return p;
 }
 
@@ -781,12 +781,12 @@ static void launch_paged_store(const PagedAttn &a, const ss_paged_store *s, cons
 }
 
 // One pass: the requests whose rows are few, then (p.prompts) the others.
-static int launch_pass(PagedAttn &a, const ss_paged_store *s, const PagedPlan &p, int mode, void *workspace,
+static int launch_pass(PagedAttn &a, const ss_paged_store *s, const PagedPlan &p, int mode, int64_t n_groups, void *workspace,
                        size_t workspace_bytes, hipStream_t st) {
     // One prefix's rows, or one request's, come together and are one kernel's: a
     // launch that finds none costs 5 us, its merge 5 more.
     a.most_rows = !p.prompts ? INT32_MAX : mode != kPlain && (a.rows_of || a.n_req == 1) ? 0 : kPromptRows;
-    if (a.most_rows == 0) return launch_paged_prompt(a, s, mode, workspace, workspace_bytes, st);
+    if (a.most_rows == 0) return launch_paged_prompt(a, s, mode, n_groups, workspace, workspace_bytes, st);
     a.cut = p.cut ? static_cast<int4 *>(workspace) : nullptr;
     a.acc = reinterpret_cast<float *>(a.cut + p.groups + 1);
     a.ml = a.acc + (size_t)p.groups * 2 * p.rows * s->head_dim;
@@ -794,7 +794,7 @@ static int launch_pass(PagedAttn &a, const ss_paged_store *s, const PagedPlan &p
     else if (mode == kRanges) launch_paged_store<kRanges>(a, s, p, st);
     else launch_paged_store<kScores>(a, s, p, st);
     SS_LAUNCH_CHECK("paged_attn_kernel launch");
-    return p.prompts ? launch_paged_prompt(a, s, mode, workspace, workspace_bytes, st) : SS_OK;
+    return p.prompts ? launch_paged_prompt(a, s, mode, n_groups, workspace, workspace_bytes, st) : SS_OK;
 }
 
 // What ss_paged_scores asks for.
@@ -836,12 +836,14 @@ static PagedPasses paged_passes(const ss_paged_store *s, int64_t n_tokens, int64
     // (a window is seen through whole units)
     if (asked.window != INT32_MAX) max_length = min(max_length, asked.window + max_new + kUnit);
     p.own = paged_plan(s, n_tokens, n_requests, n_q_heads, max_new, max_length);
+    if (sc && p.own.prompts && n_requests == 1 && asked.window == INT32_MAX)
+        p.own.bytes = max(p.own.bytes, paged_prompt_bytes(s, n_requests, n_tokens * (n_q_heads / s->n_kv_heads), kPromptRows, true));
     p.bytes = p.own.bytes;
     if (asked.shared) {
         const int64_t groups = min(sc->n_groups, n_requests);
         p.shared = paged_plan(s, n_tokens, groups, n_q_heads, max((int64_t)1, n_tokens / groups), sc->max_shared);
         if (p.shared.prompts)  // (of any number of rows)
-            p.shared.bytes = paged_prompt_bytes(s, n_requests, n_tokens * (n_q_heads / s->n_kv_heads), 0);
+            p.shared.bytes = paged_prompt_bytes(s, n_requests, n_tokens * (n_q_heads / s->n_kv_heads), 0, false);
         p.part = ((size_t)n_tokens * n_q_heads * (s->head_dim + 2) * 4 + 15) & ~(size_t)15;
         p.bytes = p.part + max(p.shared.bytes, p.own.bytes);
     }
@@ -917,10 +919,10 @@ static int paged_attn(const ss_paged_store *store, const void *q, int q_dtype, i
         PagedAttn first = a;
         first.starts = sc->group_starts, first.rows_of = reinterpret_cast<const int2 *>(sc->group_rows);
         first.causal = first.zero_rest = 0;
-        if (int rc = launch_pass(first, store, p.shared, asked.mode, scratch, left, st)) return rc;
+        if (int rc = launch_pass(first, store, p.shared, asked.mode, sc->n_groups, scratch, left, st)) return rc;
         a.parents = sc->parents;
     }
-    return launch_pass(a, store, p.own, asked.mode, scratch, left, st);
+    return launch_pass(a, store, p.own, asked.mode, n_requests, scratch, left, st);
 }
 
 }  // namespace ss

@@ -57,6 +57,9 @@ struct PagedAttn {
     float *acc;         // [workgroups][2][rows of a workgroup][D]
     float *ml;          // [workgroups][2][rows of a workgroup][2]
     // kRanges:
+    // of the prompt kernel: workgroups that may leave parts; up to how many columns
+    // the longer ones are halved
+    int slots, halved;
     const int32_t *open;     // tokens of its beginning that all rows of a request see, or null
     int window;              // tokens up to its own that a row sees; INT32_MAX: all
     // A pass over shared tokens: row i of request r is that of token rows[starts[r]
@@ -327,9 +330,10 @@ constexpr int kPromptTile = 256;  // query rows of a workgroup of the prompt ker
 
 // The requests with more than most_rows query rows a KV head (paged_prompt.hip),
 // with `workspace` of paged_prompt_bytes for n_tokens * rep rows in all (with
-// less no column is cut).
-size_t paged_prompt_bytes(const ss_paged_store *s, int64_t n_requests, int64_t rows, int most_rows);
-int launch_paged_prompt(PagedAttn a, const ss_paged_store *s, int mode, void *workspace, size_t workspace_bytes,
+// less no column is cut; `uneven`: of calls with options, whose rows see what
+// is before them).
+size_t paged_prompt_bytes(const ss_paged_store *s, int64_t n_requests, int64_t rows, int most_rows, bool uneven);
+int launch_paged_prompt(PagedAttn a, const ss_paged_store *s, int mode, int64_t n_groups, void *workspace, size_t workspace_bytes,
                         hipStream_t st);
 
 }  // namespace ss

@@ -123,6 +123,13 @@ __device__ __forceinline__ int parts_of_tiles(const PagedAttn &a, const Request 
     return max(1, (int)(((int64_t)column_tiles<MODE>(a, q) + share - 1) / share));
 }
 
+// A request's row tiles of which the last sees twice what the first does, or
+// more, in fours: the longest two of each are halved (halved_tile).
+template <int MODE>
+__device__ __forceinline__ int halved_fours(const PagedAttn &a, const Request &q) {
+    return 2 * (int64_t)last_seen<MODE>(a, q, (kRows - 1) / a.rep) <= q.len ? tiles_of(a, q) / 4 : 0;
+}
+
 // The bits of the 16-bit float 2^k, k >= -126 (positive ones compare as
 // integers); above the finite ones those of infinity, below all of them 1.
 template <bool BF>
@@ -166,6 +173,15 @@ __device__ __forceinline__ void lds_barrier() {
 }
 
 __device__ __forceinline__ float half_max(float v) { return fmaxf(v, __shfl_xor(v, 32)); }
+
+// Where the four dims from c on of a part's row lie among its sums: lane after
+// lane as paged_prompt_kernel holds them (other than plain).
+template <int D>
+__device__ __forceinline__ int part_place(int row, int c) {
+    constexpr int NT = D / 32;
+    const int m = c / NT, i = m / 8 * 4 + m % 4, half = m / 4 % 2;
+    return ((row / 32 * (D / 8) + i * NT / 4) * 64 + half * 32 + row % 32) * 4;
+}
 
 template <int D, int G, bool BF, int MODE>
 __global__ void __launch_bounds__(64 * kPWaves, 2) paged_prompt_kernel(const PagedAttn a) {
@@ -221,17 +237,42 @@ __global__ void __launch_bounds__(64 * kPWaves, 2) paged_prompt_kernel(const Pag
             if (spare == n_columns || __builtin_amdgcn_readlane(scan, 63) <= a.target) break;
         }
     }
+    // Where they would fill the device about once, the longest of what prompts see
+    // takes twice the average: the longer half of a request's row tiles is cut in
+    // two each, every four halves followed by the shorter half's longest.
+    const bool halve = MODE != kPlain && share == INT32_MAX && a.slots && n_columns <= a.halved;
+    if (halve) {
+        columns = 0;
+        for (int i = r0; i < r1; ++i) {
+            const Request q = request<MODE>(a, i);
+            columns += (tiles_of(a, q) + 2 * halved_fours<MODE>(a, q)) * heads;
+        }
+        scan = wave_scan(columns);
+    }
     const int n_items = __builtin_amdgcn_readlane(scan, 63);
     int4 cut = make_int4(0, 0, 0, 0);
 
     for (int item = blockIdx.x; item < n_items; item += gridDim.x) {
         const int holder = __ffsll((unsigned long long)__ballot(item < scan)) - 1;
         int left = item - (holder ? __builtin_amdgcn_readlane(scan, holder - 1) : 0);
-        int r = holder * per, parts, row_tile;
+        int r = holder * per, parts, row_tile, part, h;
         Request rq;
         for (;; ++r) {
             rq = request<MODE>(a, r);
             const int n = tiles_of(a, rq);
+            if (MODE != kPlain && halve) {
+                const int fours = __builtin_amdgcn_readfirstlane(halved_fours<MODE>(a, rq));
+                const int items = (n + 2 * fours) * heads;
+                if (left < items) {
+                    const int i = uniform_div(left, heads), four = i / 5, k = i - 5 * four;
+                    const bool in_two = four < fours && k < 4;
+                    row_tile = n - 1 - (in_two ? 2 * four + k / 2 : four < fours ? 2 * fours + four : i - 2 * fours);
+                    parts = in_two ? 2 : 1, part = in_two ? k % 2 : 0, h = left - i * heads;
+                    break;
+                }
+                left -= items;
+                continue;
+            }
             parts = __builtin_amdgcn_readfirstlane(parts_of_tiles<MODE>(a, rq, share));
             if (left < n * heads * parts) {
                 // the longest row tiles first; heads side by side, so that a head's
@@ -239,11 +280,11 @@ __global__ void __launch_bounds__(64 * kPWaves, 2) paged_prompt_kernel(const Pag
                 const int t = uniform_div(left, heads * parts);
                 left -= t * heads * parts;
                 row_tile = n - 1 - t;
+                part = uniform_div(left, heads), h = left - part * heads;
                 break;
             }
             left -= n * heads * parts;
         }
-        const int part = uniform_div(left, heads), h = left - part * heads;
         const int row0 = row_tile * kRows + wave * 32;  // the wave's first row
         const int32_t *row_table = a.table + (int64_t)r * a.width;
         auto page_at = [&](int token) {
@@ -712,13 +753,21 @@ __global__ void __launch_bounds__(64 * kPWaves, 2) paged_prompt_kernel(const Pag
             for (int i = 0; i < 16; ++i) {
                 const int m = 8 * (i / 4) + 4 * half + i % 4;
                 const int e = vexp[group_of(i)] - 15;
+                if constexpr (MODE == kPlain) {
 #pragma unroll
-                for (int j = 0; j < NT; ++j) a.acc[at * D + NT * m + j] = ldexpf(o[j][i], e);
+                    for (int j = 0; j < NT; ++j) a.acc[at * D + NT * m + j] = ldexpf(o[j][i], e);
+                } else if (NT == 4 || i % 2 == 0) {
+                    // (1 KB in a row of a wave's store: row by row, 16 bytes each, 256
+                    // workgroups' parts took 6 us longer)
+                    *reinterpret_cast<float4 *>(a.acc + (int64_t)item * kRows * D + ((wave * (D / 8) + i * NT / 4) * 64 + lane) * 4) =
+                        make_float4(ldexpf(o[0][i], e), ldexpf(o[1][i], e), ldexpf(o[NT == 4 ? 2 : 0][NT == 4 ? i : i + 1], e),
+                                    ldexpf(o[NT == 4 ? 3 : 1][NT == 4 ? i : i + 1], e));
+                }
             }
         }
         __syncthreads();  // (the next item's copies)
     }
-    if (a.cut && (int)blockIdx.x < a.target && threadIdx.x == 0) a.cut[blockIdx.x] = cut;
+    if (a.cut && (int)blockIdx.x < (MODE == kPlain ? a.target : a.slots) && threadIdx.x == 0) a.cut[blockIdx.x] = cut;
 }
 
 // Joins the parts of the column that cut[blockIdx.y] names: part i is at item
@@ -726,39 +775,68 @@ __global__ void __launch_bounds__(64 * kPWaves, 2) paged_prompt_kernel(const Pag
 // bound it: 256 of 256 rows, 34 MB, 9 us.
 template <int D, int MODE>
 __global__ void __launch_bounds__(256) prompt_merge_kernel(const PagedAttn a) {
-    constexpr int CH = D / 4, AT_ONCE = 256 / CH;
+    constexpr int CH = D / 4, AT_ONCE = 256 / CH, EIGHTS = 2;
     const int4 cut = a.cut[blockIdx.y];
-    const int parts = cut.x, r = cut.y, h = cut.z, c = threadIdx.x % CH * 4;
+    const int parts = cut.x, r = cut.y, h = cut.z;
     if (parts == 0) return;
     const Request rq = request<MODE>(a, r);
-    for (int row = blockIdx.x * AT_ONCE + threadIdx.x / CH; row < kRows; row += gridDim.x * AT_ONCE) {
+    // a wave takes the dims of one row after the other; other than plain, 32 dims
+    // of each of 8 rows, 128 bytes in a row of every load
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int c = MODE == kPlain ? threadIdx.x % CH * 4 : (wave % (CH / 8) * 8 + lane / 8) * 4;
+    const int row0 = MODE == kPlain ? threadIdx.x / CH : wave / (CH / 8) * 8 + lane % 8;
+    for (int row = blockIdx.x * AT_ONCE + row0; row < kRows; row += gridDim.x * AT_ONCE) {
         const int n = cut.w * kRows + row;
-        if (n >= rq.rows) return;
+        if (MODE == kPlain && n >= rq.rows) return;
         auto at = [&](int i) { return ((int64_t)blockIdx.y + (int64_t)i * a.st.heads) * kRows + row; };
         float m = -INFINITY, l = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
         if constexpr (MODE != kPlain) {
-            // the row's threads look at a part's statistics each
-            const int lane = threadIdx.x % CH;
-            for (int i = lane; i < parts; i += CH) m = fmaxf(m, a.ml[at(i) * 2]);
+            // 8 * EIGHTS parts at a time, all on their way before the first is looked at; the
+            // row's 8 threads look at a part's statistics each (EIGHTS 1, 2, 4: 8 columns of 31
+            // parts 13.3, 8.5, 11.4 us; 64 of 4, where registers count, 8.7, 10.4, 17)
+            const int mine = lane / 8, place = part_place<D>(row, c);
+            const int t = n < rq.rows ? token_at<MODE>(a, rq, n / a.rep).x : 0;
+            for (int from = 0; from < parts; from += 8 * EIGHTS) {
+                float2 e[EIGHTS];
+                float4 v[EIGHTS][8];
 #pragma unroll
-            for (int o = CH / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
-            for (int from = 0; from < parts; from += CH) {
-                const int mine = min(from + lane, parts - 1);
-                const float2 e = *reinterpret_cast<const float2 *>(a.ml + at(mine) * 2);
-                const float f = from + lane >= parts ? 0.f : e.x == m ? 1.f : fast_exp2(e.x - m);
-                l += f * e.y;
-                const int n_here = min(parts - from, CH);
-#pragma unroll 8
-                for (int i = 0; i < n_here; ++i) {
-                    const float4 v = *reinterpret_cast<const float4 *>(a.acc + at(from + i) * D + c);
-                    const float fi = __shfl(f, i, CH);
-                    x[0] += fi * v.x, x[1] += fi * v.y, x[2] += fi * v.z, x[3] += fi * v.w;
+                for (int k = 0; k < EIGHTS; ++k) {
+                    e[k] = make_float2(-INFINITY, 0.f);
+                    if (from + 8 * k < parts) {
+                        const int part = from + 8 * k + mine;
+                        const float2 read = *reinterpret_cast<const float2 *>(a.ml + at(min(part, parts - 1)) * 2);
+                        if (part < parts) e[k] = read;
+#pragma unroll
+                        for (int i = 0; i < 8; ++i)
+                            v[k][i] = *reinterpret_cast<const float4 *>(
+                                a.acc + ((int64_t)blockIdx.y + (int64_t)min(from + 8 * k + i, parts - 1) * a.st.heads) * kRows * D + place);
+                    }
+                }
+                float now = m;
+#pragma unroll
+                for (int k = 0; k < EIGHTS; ++k) now = fmaxf(now, e[k].x);
+#pragma unroll
+                for (int o = 8; o < 64; o *= 2) now = fmaxf(now, __shfl_xor(now, o));
+                const float by = m == now ? 1.f : fast_exp2(m - now);
+                m = now, l *= by;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) x[i] *= by;
+#pragma unroll
+                for (int k = 0; k < EIGHTS; ++k) {
+                    const float f = e[k].x == m ? 1.f : fast_exp2(e[k].x - m);
+                    l += f * e[k].y;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        if (from + 8 * k + i >= parts) break;
+                        const float fi = __shfl(f, i * 8 + lane % 8);
+                        x[0] += fi * v[k][i].x, x[1] += fi * v[k][i].y, x[2] += fi * v[k][i].z, x[3] += fi * v[k][i].w;
+                    }
                 }
             }
 #pragma unroll
-            for (int o = CH / 2; o > 0; o >>= 1) l += __shfl_xor(l, o);
-            finish_row<MODE, D, kProb>(a, r, token_at<MODE>(a, rq, n / a.rep).x, h * a.rep + n % a.rep, c, m, l, x[0],
-                                       x[1], x[2], x[3]);
+            for (int o = 8; o < 64; o *= 2) l += __shfl_xor(l, o);
+            if (n >= rq.rows) return;
+            finish_row<MODE, D, kProb>(a, r, t, h * a.rep + n % a.rep, c, m, l, x[0], x[1], x[2], x[3]);
             continue;
         }
         for (int i = 0; i < parts; ++i) m = fmaxf(m, a.ml[at(i) * 2]);
@@ -782,11 +860,9 @@ static void launch_prompt(const PagedAttn &a, bool bf, unsigned groups, hipStrea
         hipLaunchKernelGGL((paged_prompt_kernel<D, G, true, MODE>), dim3(groups), block, 0, st, a);
     else
         hipLaunchKernelGGL((paged_prompt_kernel<D, G, false, MODE>), dim3(groups), block, 0, st, a);
-    // (of ranges, where a few columns of many parts are the rule, more workgroups a
-    // column: 8 columns of 31 parts 11.6 us, 16.2 with 16 and a thread's own look at
-    // every part's statistics)
-    if (a.target)
-        hipLaunchKernelGGL((prompt_merge_kernel<D, MODE>), dim3(MODE == kPlain ? 16 : 32, a.target), dim3(256), 0, st, a);
+    // (of ranges, where a few columns of many parts are the rule, more workgroups a column)
+    if (a.slots)
+        hipLaunchKernelGGL((prompt_merge_kernel<D, MODE>), dim3(MODE == kPlain ? 16 : 32, a.slots), dim3(256), 0, st, a);
 }
 
 template <int MODE>
@@ -807,22 +883,45 @@ static int cut_target(int64_t n_requests, int heads, int64_t rows, int most_rows
     return 2 * least <= device_cu_count() ? device_cu_count() : 0;
 }
 
-size_t paged_prompt_bytes(const ss_paged_store *s, int64_t n_requests, int64_t rows, int most_rows) {
-    return (size_t)cut_target(n_requests, s->n_kv_heads, rows, most_rows) * (16 + kRows * (s->head_dim + 2) * 4);
+// Up to how many columns the longer ones of a call's one request are halved (a
+// capped prompt of 1100 tokens 84 -> 68 us, of 1364 102 -> 79, of 2041 148 -> 135,
+// of 2800 198 -> 189; 4 KV heads, 4093 tokens 213 -> 170).  Of more columns each
+// compute unit takes long and short ones, and of several requests, which come one
+// after the other, the last one's halves start late (2 of 1500 tokens 109 -> 147).
+static int halved_columns() { return device_cu_count() * 3 / 2; }
+
+// Workgroups that may leave parts: `target`, and of uneven columns three for
+// every two that there can be.
+static int part_slots(int64_t n_requests, int heads, int64_t rows, int most_rows, bool uneven) {
+    const int target = cut_target(n_requests, heads, rows, most_rows);
+    const int64_t least = max((int64_t)0, rows - n_requests * most_rows) / kRows * heads;
+    if (!uneven || least > halved_columns()) return target;
+    const int64_t most = min((rows / kRows + min(n_requests, rows / (most_rows + 1))) * heads, (int64_t)halved_columns());
+    return max(target, (int)(most * 3 / 2));
 }
 
-int launch_paged_prompt(PagedAttn a, const ss_paged_store *s, int mode, void *workspace, size_t workspace_bytes,
+size_t paged_prompt_bytes(const ss_paged_store *s, int64_t n_requests, int64_t rows, int most_rows, bool uneven) {
+    return (size_t)part_slots(n_requests, s->n_kv_heads, rows, most_rows, uneven) * (16 + kRows * (s->head_dim + 2) * 4);
+}
+
+int launch_paged_prompt(PagedAttn a, const ss_paged_store *s, int mode, int64_t n_groups, void *workspace, size_t workspace_bytes,
                         hipStream_t st) {
-    // at most this many row tiles: whole ones, and one a request of more than most_rows rows
+    // at most this many row tiles: whole ones, and one a request of more than most_rows
+    // rows (of shared tokens, one a prefix that the hints name: a workgroup without a
+    // column waits for a compute unit all the same)
     const int64_t rows = a.n_tokens * a.rep;
-    const int64_t tiles = rows / kRows + min((int64_t)a.n_req, rows / (a.most_rows + 1));
+    const int64_t tiles = rows / kRows + min(a.rows_of ? n_groups : (int64_t)a.n_req, rows / (a.most_rows + 1));
     if (tiles == 0) return SS_OK;
+    bool uneven = mode != kPlain && a.n_req == 1 && a.causal && a.window == INT32_MAX && !a.rows_of;
+    uneven = uneven && paged_prompt_bytes(s, a.n_req, rows, a.most_rows, true) <= workspace_bytes;
     a.target = cut_target(a.n_req, a.st.heads, rows, a.most_rows);
-    if (paged_prompt_bytes(s, a.n_req, rows, a.most_rows) > workspace_bytes) a.target = 0;
-    a.cut = a.target ? static_cast<int4 *>(workspace) : nullptr;
-    a.acc = reinterpret_cast<float *>(a.cut + a.target);
-    a.ml = a.acc + (size_t)a.target * kRows * s->head_dim;
-    const unsigned groups = (unsigned)max(min(tiles * a.st.heads, (int64_t)1 << 20), (int64_t)a.target);
+    a.slots = part_slots(a.n_req, a.st.heads, rows, a.most_rows, uneven);
+    if (paged_prompt_bytes(s, a.n_req, rows, a.most_rows, uneven) > workspace_bytes) a.target = a.slots = 0;
+    a.halved = uneven ? halved_columns() : 0;
+    a.cut = a.slots ? static_cast<int4 *>(workspace) : nullptr;
+    a.acc = reinterpret_cast<float *>(a.cut + a.slots);
+    a.ml = a.acc + (size_t)a.slots * kRows * s->head_dim;
+    const unsigned groups = (unsigned)max(min(tiles * a.st.heads, (int64_t)1 << 20), (int64_t)a.slots);
     if (mode == kPlain) launch_prompt_store<kPlain>(a, s, groups, st);
     else if (mode == kRanges) launch_prompt_store<kRanges>(a, s, groups, st);
     else launch_prompt_store<kScores>(a, s, groups, st);

@@ -295,6 +295,22 @@ def test_wrong_hints_change_roundings_only():
             assert not error, (hints, error)
 
 
+@pytest.mark.parametrize("held", [0, 1, 700])
+@pytest.mark.parametrize("new,hkv,d", [(1100, 8, 128), (1090, 8, 64), (2041, 4, 128), (2300, 8, 64)])
+def test_one_prompt_whose_columns_fill_the_device_once(new, hkv, d, held):
+    """The longer ones are halved, where rows see little beside their own."""
+    store, table = pool(37, [held + new], hkv, d, 64, 64, F16)
+    q, starts = queries(38, new + 3, 4 * hkv, d, F16), ints([0, new])
+    for call, kw in ((dict(softcap=8.0), dict(softcap=8.0)),
+                     (dict(prefix_lengths=ints([300])), dict(prefix=[300])),
+                     (dict(prefix_lengths=ints([900])), dict(prefix=[900])),
+                     (dict(slopes=slopes_of(4 * hkv)), dict(slopes=slopes_of(4 * hkv)))):
+        got = S.paged_attention(q, store, table, ints([held + new]), starts, 0.1, **call)
+        error = R.check(got, R.attend(q, store, table, ints([held + new]), starts, 0.1, **kw))
+        assert not error, (kw, error)
+        assert not bool(got[new:].any())
+
+
 @pytest.mark.parametrize("new", [0, 1, 5, 40, 300])
 @pytest.mark.parametrize("kw", [dict(softcap=9.0), dict(window=100), dict(prefix_lengths=None)])
 def test_one_request_with_hints_of_many_rows(kw, new):

@@ -210,6 +210,28 @@ def test_wrong_hints_change_roundings_only():
             assert not error, (groups, most, hints, error)
 
 
+@pytest.mark.parametrize("d,group", [(128, 64), (64, 32)])
+def test_many_prefixes_where_one_is_expected(d, group):
+    """More columns than workgroups, which then take several one after the other."""
+    rng = random.Random(d)
+    lengths = [2500] + [rng.randint(1, 300) for _ in range(63)] + [rng.randint(8, 40) for _ in range(64)]
+    new, parents = [0] * 64 + [8] * 64, [-1] * 64 + rng.sample(range(64), 64)
+    store, table = pool(33, lengths, 8, d, group, 16, F16, width=1 << 12)
+    starts = ints([sum(new[:i]) for i in range(129)])
+    q, le = queries(34, 512, 32, d, F16), ints(lengths)
+    plan = S.build_shared_plan(ints(parents), le, starts, 512, n_groups=1)
+    got = S.paged_attention(q, store, table, le, starts, 0.1, shared=plan, max_new=8, max_length=40)
+    error = R.check(got, R.attend(q, store, table, le, starts, 0.1, parents=parents))
+    assert not error, error
+
+
+@pytest.mark.parametrize("prefix", [33 * 64 * 8, 40000])
+def test_a_prefix_in_more_parts_than_are_joined_at_once(prefix):
+    lengths = [prefix] + [5 + i % 7 for i in range(64)]
+    for d, group, dtype, kw in ((128, 64, BF16, {}), (64, 64, F16, dict(softcap=7.0))):
+        run(35, lengths, [0] + [1] * 64, [-1] + [0] * 64, hq=4, hkv=1, d=d, group=group, page=128, dtype=dtype, **kw)
+
+
 def test_graphs_follow_the_plan():
     """The plan and the attention captured, replayed with other parents and
     lengths and eager work between."""
