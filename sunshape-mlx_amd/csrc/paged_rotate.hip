@@ -11,9 +11,9 @@
 //
 // A prompt of 8192 tokens, 32 query and 8 KV heads of 128 dims, with norms, takes
 // 48 us (181 MB, 3.8 TB/s; 36 us at the rate of a large copy): vector issue (70 %
-// of the cycles: a key or value costs 20 operations, most of them its quantising, a
-// query's element 7) beside HBM.  256 tokens take 7.7 us, one 4.3: the chain
-// from a position over the table's row to the codes.
+// of the cycles: a key's element costs some 30 operations, a value's 20, most of
+// them the quantising, a query's 10) beside HBM.  256 tokens take 7.9 us, one
+// 4.4: the chain from a position over the table's row to the codes.
 #include "paged_append.hpp"
 
 namespace ss {

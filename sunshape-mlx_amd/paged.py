@@ -742,7 +742,9 @@ class PagedKVCache:
     def share(self, requests, parent: int | None) -> None:
         """From the next step on these requests continue ``parent``: their tokens
         follow all of its tokens, which the cache holds once; ``attend`` reads
-        those once for all of them, and positions (``append_rotated``) count them.
+        those once for all of them, and positions (``append_rotated``) count them
+        (a parent that grows later moves them: keys rotated before that stay as
+        they are).
         They hold no tokens yet; a request continues only one that continues none.
         ``parent`` None: they continue nothing.  Graphs follow, but for those of a
         step that was captured while no request continued another."""
