@@ -221,7 +221,7 @@ __global__ void __launch_bounds__(64 * kPWaves, 2) paged_prompt_kernel(const Pag
     int scan = wave_scan(columns);
     const int n_columns = __builtin_amdgcn_readlane(scan, 63);
     int share = INT32_MAX;
-    if (a.cut && 2 * n_columns <= a.target) {
+    if (a.cut && 2 * n_columns <= a.target && (MODE == kPlain || a.target)) {
         // sum of ceil(n / share) is at most total / share + columns, and about
         // total / share + columns / 2
         const uint32_t total = __builtin_amdgcn_readlane(wave_scan((int)all_tiles), 63);

@@ -311,6 +311,23 @@ def test_one_prompt_whose_columns_fill_the_device_once(new, hkv, d, held):
         assert not bool(got[new:].any())
 
 
+@pytest.mark.parametrize("real", [0, 1, 300, 1100, 1500])
+def test_one_prompt_that_fills_its_batch_in_part(real):
+    """A step sized for 1500 tokens of which fewer come (a captured one, say)."""
+    n, hkv = 1500, 8
+    store, table = pool(39, [max(real, 1)], hkv, 128, 64, 64, F16, width=40)
+    q = queries(40, n, 4 * hkv, 128, F16)
+    for starts in ([0, real], [n - real, n]) if real else ([0, 0], [7, 7], [9, 5]):
+        st, le = ints(starts), ints([real])
+        got = S.paged_attention(q, store, table, le, st, 0.1, softcap=8.0, max_new=n, max_length=n)
+        at = slice(starts[0], starts[0] + real)
+        if real:
+            want = R.attend(q, store, table, le, st, 0.1, softcap=8.0)
+            error = R.check(got[at], [x[at] for x in want])
+            assert not error, error
+        assert not bool(got[:at.start].any() | got[at.stop:].any())
+
+
 @pytest.mark.parametrize("new", [0, 1, 5, 40, 300])
 @pytest.mark.parametrize("kw", [dict(softcap=9.0), dict(window=100), dict(prefix_lengths=None)])
 def test_one_request_with_hints_of_many_rows(kw, new):
