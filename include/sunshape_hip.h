@@ -1175,7 +1175,7 @@ int ss_paged_attn(const ss_paged_store *store, const void *q, int q_dtype, int64
  * n_groups and max_shared (how many parents, and their longest length) size the
  * launch, as max_new and max_length (of own tokens) do.  Not together with a
  * window or prefix_lengths.
- * A capped score is off by up to 2^-21 of the largest around it more than others.
+ * A capped score is off by up to 2^-21 of itself more than others.
  */
 typedef struct {
     float softcap;                 /* 0: none */
