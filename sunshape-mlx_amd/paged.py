@@ -669,7 +669,9 @@ class PagedKVCache:
 
         A list of ints raises here when the step is impossible, as long as the
         host knows the lengths: until a first step given as a tensor.  It
-        cannot be captured.
+        cannot be captured.  A request that others continue gives tokens back only
+        where all of these end in the same step; one that ends continues nothing
+        any more.
 
         An int32 tensor on the GPU needs ``n_tokens``, at least the sum of what
         is added (``max_new``, the most one adds, sizes later launches).  It is
@@ -678,7 +680,14 @@ class PagedKVCache:
         list whose lengths only the GPU knows.  Captured, it goes into the graph
         with its append and attend, and the plan holds what the last replay
         made of it; a graph with append or attend alone goes on with the slots
-        and starts of the step that they were captured after."""
+        and starts of the step that they were captured after.  The host does not see
+        what such steps end: requests that share have to end through ``release``."""
+        return self._step(new_lengths, n_tokens, max_new)
+
+    def _step(self, new_lengths, n_tokens: int | None = None, max_new: int | None = None,
+              ended: set | None = None) -> BlockPlan:
+        """``step``; ``ended``: the requests that end, whatever they add (by
+        default those of a list that give back all they hold)."""
         host, bound, row = None, self._bound, self.block_table.shape[1] * self.page_size
         if isinstance(new_lengths, torch.Tensor):
             if n_tokens is None:
@@ -708,8 +717,14 @@ class PagedKVCache:
                 if pages > self.free_pages.shape[0]:
                     raise RuntimeError(f"{pages} pages needed, {self.free_pages.shape[0]} there")
                 bound = max(host)
+                if ended is None:
+                    ended = {r for r, x in enumerate(adds) if x < 0 and not host[r]}
             else:
                 bound = min(row, bound + max(0, most))
+            for p in self._prefixes:
+                if adds[p] < 0 and any(q == p and r not in (ended or ()) for r, q in enumerate(self._parent)):
+                    raise ValueError(f"request {p}, which others continue, gives tokens back only where these "
+                                     f"end too (see release)")
             new = torch.tensor(adds, dtype=torch.int32).to(self.lengths.device)
         plan = build_block_tables(self.lengths, new, self.block_table, self.free_pages,
                                   self.n_free, self.page_size, n_tokens,
@@ -724,6 +739,8 @@ class PagedKVCache:
             plan = plan._replace(positions=self.shared.positions)
         self.plan, self._max_new = plan, max(1, most)
         self._version += 1
+        if ended and self._prefixes:
+            self._set_parents([-1 if r in ended else p for r, p in enumerate(self._parent)])
         return plan
 
     def check(self) -> None:
@@ -746,7 +763,9 @@ class PagedKVCache:
         (a parent that grows later moves them: keys rotated before that stay as
         they are).
         They hold no tokens yet; a request continues only one that continues none.
-        ``parent`` None: they continue nothing.  Graphs follow, but for those of a
+        ``parent`` None: they continue nothing; not while they hold tokens behind
+        one.  (Where only the GPU knows the lengths, after a step given as a tensor,
+        both are the caller's to see to.)  Graphs follow, but for those of a
         step that was captured while no request continued another."""
         at = [int(r) for r in requests]
         every = range(self.n_requests)
@@ -762,6 +781,8 @@ class PagedKVCache:
                 raise ValueError("a request that others continue cannot continue another")
             if self._host is not None and any(self._host[r] for r in at):
                 raise ValueError("requests hold tokens already: share before their first step")
+        elif self._host is not None and any(self._host[r] and self._parent[r] >= 0 for r in at):
+            raise ValueError("requests hold tokens behind those of another: release ends them")
         new = list(self._parent)
         for r in at:
             new[r] = p
@@ -822,22 +843,21 @@ class PagedKVCache:
                 any(p in gone and r not in gone for r, p in enumerate(self._parent)):
             raise ValueError("a request that others continue ends with them or after them")
         if self._host is not None:
-            self.step([-n if r in gone else 0 for r, n in enumerate(self._host)])
+            self._step([-n if r in gone else 0 for r, n in enumerate(self._host)], ended=gone)
         else:
             new = torch.zeros_like(self.lengths)
             at = at.to(new.device)
             new[at] = -self.lengths[at]
-            self.step(new, 0)
-        if self._prefixes and any(self._parent[r] >= 0 for r in gone):
-            self._set_parents([-1 if r in gone else p for r, p in enumerate(self._parent)])
+            self._step(new, 0, ended=gone)
 
     def trim(self, n: int) -> None:
         """Give the last ``n`` tokens of every request back (of those that others
-        continue none)."""
+        continue none).  A request of which none are left goes on where it was: it
+        continues what it continued."""
         n = max(0, n)
         keep = self._prefixes
         if self._host is not None:
-            self.step([0 if r in keep else -min(n, have) for r, have in enumerate(self._host)])
+            self._step([0 if r in keep else -min(n, have) for r, have in enumerate(self._host)], ended=set())
         else:
             new = -self.lengths.clamp(max=n)
             for r in keep:
