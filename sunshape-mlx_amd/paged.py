@@ -658,7 +658,7 @@ class PagedKVCache:
         # lists), or a bound
         self._host: list[int] | None = [0] * n_requests
         self._bound = 0
-        self._max_new = 1
+        self._max_new = self._longest = 1   # of the last step, for its attends' launches
         self._starts: tuple[int, torch.Tensor] | None = None
 
     # -------------------------------------------------------------- serving
@@ -731,8 +731,10 @@ class PagedKVCache:
                                   lengths_out=self.lengths, n_free_out=self.n_free)
         # (only now: a step that was refused has changed nothing here either)
         self._host, self._bound = host, bound
-        self.shared = None
+        self.shared, self._longest = None, max(1, bound)
         if self._prefixes:
+            if host is not None:  # (rows are of those that add tokens: others' lengths do not matter)
+                self._longest = max((n for n, x in zip(host, adds) if x > 0), default=1)
             longest = bound if host is None else max(host[p] for p in self._prefixes)
             self.shared = build_shared_plan(self.parents, self.lengths, plan.token_starts, n_tokens,
                                             n_groups=len(self._prefixes), max_shared=longest)
@@ -824,11 +826,8 @@ class PagedKVCache:
         """Attention of the last step's tokens' queries (N, Hq, D); scores and
         masks other than the causal ones as in ``paged_attention``."""
         starts = self._last_plan("attend").token_starts
-        longest = self._bound
-        if self.shared is not None and self._host is not None:  # (of those with tokens of their own)
-            longest = max((n for r, n in enumerate(self._host) if r not in self._prefixes), default=1)
         return paged_attention(queries, self.store, self.block_table, self.lengths, starts, scale,
-                               causal=causal, max_new=self._max_new, max_length=max(1, longest), out=out,
+                               causal=causal, max_new=self._max_new, max_length=self._longest, out=out,
                                softcap=softcap, slopes=slopes, window=window,
                                prefix_lengths=prefix_lengths, shared=self.shared)
 

@@ -145,3 +145,43 @@ def test_a_step_that_fails_ends_nobody(monkeypatch):
         with pytest.raises(RuntimeError, match="no launch"):
             call()
         assert known(c) == before
+
+
+# ------------------------------------------------- what attend is told
+
+
+class Once(list):
+    """A list that is not gone through again."""
+
+    def __iter__(self):
+        raise AssertionError("every attend goes through all requests")
+
+
+@pytest.mark.parametrize("adds,longest", [([0, 1, 1, 1], 7), ([512, 1, 0, 0], 532), ([9, 0, 0, 0], 29),
+                                          ([0, 0, 0, 200], 205), ([0, 0, 0, 0], 1)])
+def test_attend_is_sized_for_the_requests_that_add_tokens(monkeypatch, adds, longest):
+    """A prefix that goes on among them; no attend goes through the requests, of which there
+    may be thousands."""
+    c = S.PagedKVCache(n_requests=4, n_kv_heads=2, max_tokens=1000, device="cpu")
+    c.step([20, 0, 0, 4])
+    c.share([1, 2], 0)
+    c.step([0, 6, 3, 1])
+    plan = c.step(adds)
+    told = []
+    monkeypatch.setattr(paged, "_scored_workspace_bytes", lambda *a: told.append(a[6]) or 0)
+    c._host = Once(c._host)
+    n = sum(adds)
+    c.attend(torch.zeros((n, 4, 128), dtype=torch.float16), 0.1)
+    assert c.shared is not None and plan.slots.shape[0] == n
+    assert told == ([longest] if n else [])
+
+
+def test_attend_without_sharing_is_sized_for_the_longest(monkeypatch):
+    c = S.PagedKVCache(n_requests=3, n_kv_heads=2, max_tokens=1000, device="cpu")
+    told = []
+    monkeypatch.setattr(paged, "_workspace_bytes", lambda *a: told.append(a[6]) or 0)
+    q = torch.zeros((1, 4, 128), dtype=torch.float16)
+    for adds in ([300, 2, 0], [0, 1, 0], ints(1, 0, 0)):
+        c.step(adds, 400)
+        c.attend(q.expand(400, 4, 128), 0.1)
+    assert told == [300, 300, 700]
