@@ -20,7 +20,7 @@ constexpr int kStages = 4;         // tiles of a wave in LDS, one computed while
 // Cache policy of the stream: non-temporal (8 requests of 32768 tokens: 66 us;
 // cached: 75 us.  1 request: 20.6 and 21.1 us).
 constexpr int kNt = 2;
-constexpr int kProb = -24;         // probabilities are kept times 2^kProb
+constexpr int kProb = kPart;       // probabilities are kept times 2^kProb
 // Requests of more than kPromptRows query rows a KV head are the prompt
 // kernel's, where this one would have more than kPromptUnits units a compute
 // unit (at 128 dims; half as much work each at 64) than that one: a column
@@ -603,8 +603,8 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(const PagedAttn a) {
                 for (int k = 0; k < 4; ++k) x[k] += f * part[w][row][c + k];
             }
             if (whole) {
-                finish_row<MODE, D, kProb>(a, r, token_at<MODE>(a, rq, n / a.rep).x, h * a.rep + n % a.rep, c, m, l, x[0],
-                                           x[1], x[2], x[3]);
+                finish_row<MODE, D>(a, r, token_at<MODE>(a, rq, n / a.rep).x, h * a.rep + n % a.rep, c, m, l, x[0], x[1],
+                                    x[2], x[3]);
             } else {
                 const int64_t at = ((int64_t)blockIdx.x * 2 + place) * ROWS + row;
                 *reinterpret_cast<float4 *>(a.acc + at * D + c) = make_float4(x[0], x[1], x[2], x[3]);
@@ -683,8 +683,8 @@ __global__ void __launch_bounds__(256) paged_merge_kernel(const PagedAttn a, int
 #pragma unroll
                 for (int k = 0; k < 4; ++k) y[k] += red[i][c + k];
             }
-            finish_row<MODE, D, kProb>(a, cut.y, token_at<MODE>(a, rq, n / a.rep).x, h * a.rep + n % a.rep, c, m, t, y[0],
-                                       y[1], y[2], y[3]);
+            finish_row<MODE, D>(a, cut.y, token_at<MODE>(a, rq, n / a.rep).x, h * a.rep + n % a.rep, c, m, t, y[0], y[1],
+                                y[2], y[3]);
         }
         __syncthreads();  // (the next column's sums)
     }

@@ -150,10 +150,11 @@ __device__ __forceinline__ void store_out4(const PagedAttn &a, int64_t i, float 
 }
 
 // Row (token t, query head `head`) is done: of its dims c .. c+3 the sums of
-// values x, of probabilities l, and what 2^m stands for in both.  SHIFT: sums
-// are times 2^SHIFT (of partial ones, kPart).
+// values x, of probabilities l, both times 2^(kPart - m).  Every sum that leaves a
+// kernel, or joins another's, is so: bfloat16's largest values stay finite (up to
+// 2^20 tokens), and values down to 2^-102 keep their bits.
 constexpr int kPart = -24;
-template <int MODE, int D, int SHIFT>
+template <int MODE, int D>
 __device__ __forceinline__ void finish_row(const PagedAttn &a, int r, int64_t t, int head, int c, float m, float l,
                                            float x0, float x1, float x2, float x3) {
     const int64_t at = t * a.hq + head;
@@ -161,10 +162,6 @@ __device__ __forceinline__ void finish_row(const PagedAttn &a, int r, int64_t t,
         float *const ml = a.part + a.n_tokens * a.hq * D + at * 2;
         float4 *const part = reinterpret_cast<float4 *>(a.part + at * D + c);
         if (a.rows_of || (a.part && table_read(a.parents, r) >= 0)) {
-            if (SHIFT != kPart) {
-                constexpr float f = 1.f / (1ull << (SHIFT - kPart));
-                l *= f, x0 *= f, x1 *= f, x2 *= f, x3 *= f;
-            }
             if (a.rows_of) {
                 *part = make_float4(x0, x1, x2, x3);
                 if (c == 0) *reinterpret_cast<float2 *>(ml) = make_float2(m, l);

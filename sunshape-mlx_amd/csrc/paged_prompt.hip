@@ -42,6 +42,7 @@ constexpr int kSlots = 3;            // tiles in LDS as they come: one being pre
 // heads: 54 us for 2 to 8, 62 us for 16).
 constexpr int kMinTiles = 8;
 constexpr int kProb = 10;  // probabilities are kept times 2^kProb
+constexpr int kLeave = kPart - kProb;  // and sums that leave the kernel times 2^kLeave more
 
 template <int D, int G>
 struct PromptTile {
@@ -713,23 +714,23 @@ __global__ void __launch_bounds__(64 * kPWaves, 2) paged_prompt_kernel(const Pag
             pages_of(tile_at(i + kSlots + 1), pages);
         }
 
-        const float sum = l + __shfl_xor(l, 32);
+        const float sum = l + __shfl_xor(l, 32), all = ldexpf(sum, kLeave);
         if (parts == 1) {
-            const float inv = sum == 0.f ? 0.f : 1.f / sum;
             if (MODE != kPlain && live && (a.rows_of || (a.part && table_read(a.parents, r) >= 0))) {
                 const int t = token_at<MODE>(a, rq, row / a.rep).x, head = h * a.rep + row % a.rep;
                 const float m = MODE == kScores ? top + ref : (ref + top) * factor;
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    const int c = NT * (8 * (i / 4) + 4 * half + i % 4), e = vexp[group_of(i)] - 15;
+                    const int c = NT * (8 * (i / 4) + 4 * half + i % 4), e = vexp[group_of(i)] - 15 + kLeave;
                     if constexpr (NT == 4)
-                        finish_row<MODE, D, kProb>(a, r, t, head, c, m, sum, ldexpf(o[0][i], e), ldexpf(o[1][i], e),
-                                                   ldexpf(o[2][i], e), ldexpf(o[3][i], e));
+                        finish_row<MODE, D>(a, r, t, head, c, m, all, ldexpf(o[0][i], e), ldexpf(o[1][i], e),
+                                            ldexpf(o[2][i], e), ldexpf(o[3][i], e));
                     else if (i % 2 == 0)
-                        finish_row<MODE, D, kProb>(a, r, t, head, c, m, sum, ldexpf(o[0][i], e), ldexpf(o[1][i], e),
-                                                   ldexpf(o[0][i + 1], e), ldexpf(o[1][i + 1], e));
+                        finish_row<MODE, D>(a, r, t, head, c, m, all, ldexpf(o[0][i], e), ldexpf(o[1][i], e),
+                                            ldexpf(o[0][i + 1], e), ldexpf(o[1][i + 1], e));
                 }
             } else if (live) {
+                const float inv = sum == 0.f ? 0.f : 1.f / sum;
                 const int64_t at = ((int64_t)(rq.t0 + row / a.rep) * a.hq + h * a.rep + row % a.rep) * D;
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
@@ -745,14 +746,14 @@ __global__ void __launch_bounds__(64 * kPWaves, 2) paged_prompt_kernel(const Pag
                 }
             }
         } else {
-            // a part: the sums as they are (times 2^10), for prompt_merge_kernel
+            // a part: the sums as they are, for prompt_merge_kernel
             if (part == 0) cut = make_int4(parts, r, h, row_tile);
             const int64_t at = (int64_t)item * kRows + wave * 32 + col;
-            if (half == 0) *reinterpret_cast<float2 *>(a.ml + at * 2) = make_float2(MODE == kScores ? top + ref : (ref + top) * factor, sum);
+            if (half == 0) *reinterpret_cast<float2 *>(a.ml + at * 2) = make_float2(MODE == kScores ? top + ref : (ref + top) * factor, all);
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
                 const int m = 8 * (i / 4) + 4 * half + i % 4;
-                const int e = vexp[group_of(i)] - 15;
+                const int e = vexp[group_of(i)] - 15 + kLeave;
                 if constexpr (MODE == kPlain) {
 #pragma unroll
                     for (int j = 0; j < NT; ++j) a.acc[at * D + NT * m + j] = ldexpf(o[j][i], e);
@@ -836,7 +837,7 @@ __global__ void __launch_bounds__(256) prompt_merge_kernel(const PagedAttn a) {
 #pragma unroll
             for (int o = 8; o < 64; o *= 2) l += __shfl_xor(l, o);
             if (n >= rq.rows) return;
-            finish_row<MODE, D, kProb>(a, r, t, h * a.rep + n % a.rep, c, m, l, x[0], x[1], x[2], x[3]);
+            finish_row<MODE, D>(a, r, t, h * a.rep + n % a.rep, c, m, l, x[0], x[1], x[2], x[3]);
             continue;
         }
         for (int i = 0; i < parts; ++i) m = fmaxf(m, a.ml[at(i) * 2]);
@@ -848,8 +849,8 @@ __global__ void __launch_bounds__(256) prompt_merge_kernel(const PagedAttn a) {
             l += f * e.y;
             x[0] += f * v.x, x[1] += f * v.y, x[2] += f * v.z, x[3] += f * v.w;
         }
-        finish_row<MODE, D, kProb>(a, r, token_at<MODE>(a, rq, n / a.rep).x, h * a.rep + n % a.rep, c, m, l, x[0], x[1],
-                                   x[2], x[3]);
+        finish_row<MODE, D>(a, r, token_at<MODE>(a, rq, n / a.rep).x, h * a.rep + n % a.rep, c, m, l, x[0], x[1], x[2],
+                            x[3]);
     }
 }
 
