@@ -483,7 +483,7 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(const PagedAttn a) {
             if constexpr (MODE == kScores)
 #pragma unroll
                 for (int s = 0; s < NS; ++s)
-                    apply_scores<8>(a, slope[s], factor[s], back[s], (float)(position[s] - first), xs[s]);
+                    apply_scores<8>(a, slope[s], ScoreScale(a, factor[s]), back[s], (float)(position[s] - first), xs[s]);
             half8_t p16[NS];
 #pragma unroll
             for (int s = 0; s < NS; ++s) {

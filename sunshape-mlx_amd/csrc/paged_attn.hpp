@@ -181,7 +181,8 @@ __device__ __forceinline__ void finish_row(const PagedAttn &a, int r, int64_t t,
 
 // A row's products x with tokens 16 (i / 8) + i % 8 become scores in log2 units,
 // capped and biased, less the row's reference `ref`.  slope: the head's, in
-// log2 units a token; far: how many tokens the row is behind token 0.
+// log2 units a token; far: how many tokens the row is behind token 0; by: what a
+// row's products are multiplied with, and the cap in log2 units.
 // A cap's tanh(u) is u times a polynomial of u^2 (of the least largest error below
 // |u| = 5/8: 2^-23 of it; 9 operations each), above that 1 - 2 / (1 + exp(2 u)), off
 // by 2^-22 (12 operations' time), which is computed where one of the wave's scores is
@@ -192,16 +193,27 @@ __device__ __forceinline__ void finish_row(const PagedAttn &a, int r, int64_t t,
 // 302, but small scores were off by 2^-22 of the cap beside a large one.)
 // (A bias meets the reference first: both may be large, what is left of them is
 // rounded once.)
+struct ScoreScale {
+    float gain, cap;
+    // (The gain is a normal number, whatever the cap: more would make products of 0
+    // NaN; for less the cap is lowered to what products below 2^125 do not reach.)
+    __device__ ScoreScale(const PagedAttn &a, float factor) : gain(factor), cap(a.cap * kLog2e) {
+        if (cap > 0.f) {
+            cap = fminf(cap, factor * 0x1p126f);
+            gain = fminf(factor / cap, 0x1.fffffep127f);
+        }
+    }
+};
 template <int N, bool BIAS, typename X>
-__device__ __forceinline__ void apply_rule(const PagedAttn &a, float slope, float factor, float ref, float far, X &x) {
+__device__ __forceinline__ void apply_rule(const PagedAttn &a, float slope, const ScoreScale &by, float ref, float far, X &x) {
     auto rest = [&](int i) __attribute__((always_inline)) {
         return BIAS ? fmaf(-slope, fabsf(far - (float)(16 * (i / 8) + i % 8)), -ref) : -ref;
     };
     if (a.cap > 0.f) {
-        const float cap = a.cap * kLog2e, by = factor / cap;
+        const float cap = by.cap;
         float most = 0.f;
 #pragma unroll
-        for (int i = 0; i < N; ++i) x[i] *= by, most = fmaxf(most, fabsf(x[i]));
+        for (int i = 0; i < N; ++i) x[i] *= by.gain, most = fmaxf(most, fabsf(x[i]));
         auto small = [&](float u, int i) __attribute__((always_inline)) {
             const float v = u * u;
             float p = fmaf(v, 0.0150509445f, -0.0518218674f);
@@ -222,16 +234,16 @@ __device__ __forceinline__ void apply_rule(const PagedAttn &a, float slope, floa
         }
     } else {
 #pragma unroll
-        for (int i = 0; i < N; ++i) x[i] = fmaf(x[i], factor, rest(i));
+        for (int i = 0; i < N; ++i) x[i] = fmaf(x[i], by.gain, rest(i));
     }
 }
 template <int N, typename X>
-__device__ __forceinline__ void apply_scores(const PagedAttn &a, float slope, float factor, float ref, float far,
-                                             X &x) {
+__device__ __forceinline__ void apply_scores(const PagedAttn &a, float slope, const ScoreScale &by, float ref,
+                                             float far, X &x) {
     if (a.slopes)
-        apply_rule<N, true>(a, slope, factor, ref, far, x);
+        apply_rule<N, true>(a, slope, by, ref, far, x);
     else
-        apply_rule<N, false>(a, slope, factor, ref, far, x);
+        apply_rule<N, false>(a, slope, by, ref, far, x);
 }
 
 // How a query row whose largest magnitude is `top` enters the products: times

@@ -611,7 +611,7 @@ __global__ void __launch_bounds__(64 * kPWaves, 2) paged_prompt_kernel(const Pag
                                 x[i + e] = fmaf((e & 1) ? high16<BF>(m[e / 2]) : low16<BF>(m[e / 2]), d[g][i + e], x[i + e]);
                         }
                     if constexpr (MODE == kScores)
-                        apply_scores<16>(a, slope, factor, ref, (float)(position - (tb + 32 * y + 8 * half)), x);
+                        apply_scores<16>(a, slope, ScoreScale(a, factor), ref, (float)(position - (tb + 32 * y + 8 * half)), x);
                     if (tb + 32 * y + 32 > all_see || (MODE != kPlain && tb + 32 * y < all_from) || ok[0] != 15) {
 #pragma unroll
                         for (int i = 0; i < 16; ++i) {

@@ -86,3 +86,25 @@ def test_a_prefix_of_many_rows_beside_a_row_of_large_scores():
     rest = [i for i in range(n) if i != 7]
     error = strict.check(got[rest], [x[rest] for x in want])
     assert not error, error
+
+
+@pytest.mark.parametrize("many", [False, True])
+@pytest.mark.parametrize("q_size,k_size,scale,cap", [
+    (1e24, 1.0, 1.0, 2.0 ** -60), (1e30, 1e-30, 1.0, 2.0 ** -60), (1e30, 1e-30, 1.0, 0.5), (1e20, 1e10, 1.0, 2.0 ** 60),
+    (2.0 ** -60, 2.0 ** 97, 2.0 ** -40, 2.0 ** 60), (2.0 ** -100, 2.0 ** 100, 0.5, 2.0 ** 40),
+    (1.0, 1.0, 1.0, 2.0 ** -60), (1.0, 1.0, 1.0, 2.0 ** 60)])
+def test_caps_of_any_size(q_size, k_size, scale, cap, many):
+    """The factor of a product over the cap may pass float32 either way; half of the
+    tokens' keys are 0, and score 0."""
+    lengths, new = ([399, 1001], [200, 300]) if many else ([399, 1001], [1, 3])
+    store, table = pool(47, lengths, 2, 128, 64, 16, BF16, width=1 << 12 if many else None)
+    n = store[0].shape[0] * 16
+    g = torch.Generator(device="cuda").manual_seed(48)
+    k, v = (torch.randn((n, 2, 128), generator=g, device="cuda").to(BF16) for _ in range(2))
+    k[::2] = 0
+    S.append_paged(store, k * k_size, v, torch.arange(n, dtype=torch.int32, device="cuda"))
+    q, starts = queries(49, sum(new), 8, 128, BF16) * q_size, ints([0, new[0], sum(new)])
+    got = S.paged_attention(q, store, table, ints(lengths), starts, scale, softcap=cap)
+    want = R.attend(q, store, table, ints(lengths), starts, scale, softcap=cap)
+    error = strict.check(got, want, False)
+    assert not error, error
