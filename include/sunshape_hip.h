@@ -1104,7 +1104,8 @@ int ss_append_paged(const ss_paged_store *store, const void *keys, const void *v
  *        stored, whatever their slots.
  * rotary_dim a multiple of 16 up to head_dim; table and out 16-byte aligned;
  * weights [head_dim] of weight_dtype.  Tokens in whole blocks of 8, times query
- * and KV heads together, are at most 2^29 - 32.
+ * and KV heads together, may be 2^27; for most mixes of heads more are taken,
+ * for none more than 2^31.
  */
 typedef struct {
     const void *table;

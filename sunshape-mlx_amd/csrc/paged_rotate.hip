@@ -363,8 +363,6 @@ extern "C" int ss_append_rotated_paged(const ss_paged_store *store, const void *
     SS_REQUIRE(ro.eps >= 0., "eps must not be negative");
     SS_REQUIRE(n_q_heads >= 1 && n_tokens >= 0, "bad sizes");
     if (n_tokens == 0) return SS_OK;
-    SS_REQUIRE(queries && keys && values && slots && positions && out, "null pointer argument");
-    SS_REQUIRE(((uintptr_t)out & 15) == 0, "out must be 16-byte aligned");
     SS_UNSUPPORTED(n_tokens <= INT32_MAX, "too many tokens for one launch");
     // as many heads a wave of queries as leave two waves for every SIMD
     const int per_wave = 1024 / store->head_dim;  // tokens
@@ -376,6 +374,8 @@ extern "C" int ss_append_rotated_paged(const ss_paged_store *store, const void *
     const int64_t groups = max(mixes_of(kv_items, a.kv_share), mixes_of(q_items, kMix - a.kv_share)) * kMix * kStripe;
     SS_UNSUPPORTED(groups <= kMostGroups, "%lld tokens of %d and %d heads: too many for one launch",
                    (long long)n_tokens, n_q_heads, a.st.heads);
+    SS_REQUIRE(queries && keys && values && slots && positions && out, "null pointer argument");
+    SS_REQUIRE(((uintptr_t)out & 15) == 0, "out must be 16-byte aligned");
     a.q = queries, a.k = keys, a.v = values;
     a.q_st = q_st, a.q_sh = q_sh, a.k_st = k_st, a.k_sh = k_sh, a.v_st = v_st, a.v_sh = v_sh;
     a.slots = slots, a.positions = positions, a.table = static_cast<const float *>(ro.table);
