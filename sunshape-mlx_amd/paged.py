@@ -395,8 +395,8 @@ def append_rotated_paged(store: PagedKVStore, queries: torch.Tensor, keys: torch
     as ``build_block_tables`` gives them: a token with a negative one is not
     stored, and its query is zero, or, with ``out``, left as it was (``out`` may
     be contiguous ``queries``).  A position past the table makes the turned dims
-    NaN.  Queries or weights under autograd are refused; keys and values are
-    stored without a derivative."""
+    NaN.  Queries, weights or a table under autograd are refused; keys and values
+    are stored without a derivative."""
     st = _struct(store)
     dev, d = store[0].get_device(), st.head_dim
     shape = queries.shape
@@ -405,7 +405,7 @@ def append_rotated_paged(store: PagedKVStore, queries: torch.Tensor, keys: torch
     n, hq, _ = shape
     if queries.dtype is not keys.dtype:
         raise TypeError("queries, keys and values must share a dtype")
-    _no_derivative("append_rotated_paged", queries, q_weight, k_weight)
+    _no_derivative("append_rotated_paged", queries, q_weight, k_weight, rotary)
     at_slots = _index("slots", slots, (n,), dev)
     at_positions = _index("positions", positions, (n,), dev)
     k, v, code = _new_rows(keys, values, (n, st.n_kv_heads, d), dev)

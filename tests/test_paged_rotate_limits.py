@@ -1,10 +1,14 @@
 """How many tokens the rotated append takes, on the CPU: sizes are checked before
-pointers, and these are null, so nothing is launched on either side."""
+pointers, and these are null, so nothing is launched on either side.  And what of
+autograd it refuses."""
 
 import ctypes
 
 import pytest
+import torch
+from torch.autograd import forward_ad
 
+import sunshape_mlx_amd as S
 from sunshape_mlx_amd import _hip, paged
 
 FAKE = 1 << 20  # an address that nothing reads
@@ -28,3 +32,36 @@ def test_the_stated_size_is_taken_with_any_heads(hq, d):
             assert status(n, hq, hkv, d) == -1, (n, hkv)  # (null pointers)
         assert status((1 << 31) // (hq + hkv) + 8, hq, hkv, d) == -2, hkv
         assert b"too many" in _hip.load_library().ss_last_error()
+
+
+# ------------------------------------------------- a table under autograd
+
+
+class Launched(Exception):
+    pass
+
+
+def append(rotary):
+    store = S.PagedKVStore.zeros(4, 2, 128, page_size=16, device="cpu")
+    q, k = (torch.zeros((3, h, 128), dtype=torch.float16) for h in (4, 2))
+    at = torch.zeros(3, dtype=torch.int32)
+    return S.append_rotated_paged(store, q, k, k, at, at, rotary)
+
+
+def test_a_table_under_autograd_is_refused(monkeypatch):
+    """Of learned frequencies, say: their gradient would be dropped."""
+    def launch(name, dev, *args):
+        raise Launched(name)
+
+    monkeypatch.setattr(_hip, "require_gpu", lambda *t: None)
+    monkeypatch.setattr(paged, "_launch", launch)
+    learned = S.rotary_table(9, 128, frequencies=torch.ones(64, requires_grad=True), device="cpu")
+    with pytest.raises(ValueError, match="no backward"):
+        append(learned)
+    for rotary in (learned.detach(), S.rotary_table(9, 128, device="cpu")):
+        with pytest.raises(Launched):
+            append(rotary)
+    with torch.no_grad(), pytest.raises(Launched):
+        append(learned)
+    with forward_ad.dual_level(), pytest.raises(ValueError, match="forward-mode"):
+        append(forward_ad.make_dual(learned.detach(), torch.ones_like(learned)))
