@@ -405,7 +405,7 @@ def append_rotated_paged(store: PagedKVStore, queries: torch.Tensor, keys: torch
     n, hq, _ = shape
     if queries.dtype is not keys.dtype:
         raise TypeError("queries, keys and values must share a dtype")
-    _no_derivative("append_rotated_paged", queries, q_weight, k_weight, rotary)
+    _no_derivative("append_rotated_paged", queries, q_weight, k_weight, rotary, out)
     at_slots = _index("slots", slots, (n,), dev)
     at_positions = _index("positions", positions, (n,), dev)
     k, v, code = _new_rows(keys, values, (n, st.n_kv_heads, d), dev)
@@ -446,6 +446,8 @@ def append_rotated_paged(store: PagedKVStore, queries: torch.Tensor, keys: torch
     _launch("ss_append_rotated_paged", dev, ctypes.addressof(st), q.data_ptr(), k.data_ptr(),
             v.data_ptr(), code, n, hq, q_st, q_sh, k_st, k_sh, v_st, v_sh, at_slots, at_positions,
             ctypes.addressof(ro), out.data_ptr(), zero_rest)
+    if not zero_rest:  # (graphs that saved it refuse their backward pass)
+        torch.autograd.graph.increment_version(out)
     return out
 
 
@@ -563,7 +565,7 @@ def paged_attention(queries: torch.Tensor, store: PagedKVStore, block_table: tor
     dtype = queries.dtype
     if dtype not in _HALF:
         raise TypeError(f"queries must be float16 or bfloat16, not {dtype}")
-    _no_derivative("paged_attention", queries)
+    _no_derivative("paged_attention", queries, out)
     if hq < 1 or hq % st.n_kv_heads:
         raise ValueError(f"{hq} query heads do not share {st.n_kv_heads} KV heads")
     shape = (n, hq, st.head_dim)
@@ -595,13 +597,15 @@ def paged_attention(queries: torch.Tensor, store: PagedKVStore, block_table: tor
                 q.stride(0), q.stride(1), hq, at_table, width, at_lengths, at_starts, r, scale,
                 causal, max_new, max_length, out.data_ptr(), zero_rest, ctypes.addressof(sc),
                 _hip.ptr(ws), need)
-        return out
-    need = _workspace_bytes(dev, shape, n, r, hq, max_new, max_length)
-    # of this call alone: calls on other streams and captured graphs have their own
-    ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
-    _launch("ss_paged_attn", dev, ctypes.addressof(st), q.data_ptr(), _CODE[dtype], n, q.stride(0),
-            q.stride(1), hq, at_table, width, at_lengths, at_starts, r, scale, causal, max_new,
-            max_length, out.data_ptr(), zero_rest, _hip.ptr(ws), need)
+    else:
+        need = _workspace_bytes(dev, shape, n, r, hq, max_new, max_length)
+        # of this call alone: calls on other streams and captured graphs have their own
+        ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+        _launch("ss_paged_attn", dev, ctypes.addressof(st), q.data_ptr(), _CODE[dtype], n, q.stride(0),
+                q.stride(1), hq, at_table, width, at_lengths, at_starts, r, scale, causal, max_new,
+                max_length, out.data_ptr(), zero_rest, _hip.ptr(ws), need)
+    if not zero_rest:  # (graphs that saved it refuse their backward pass)
+        torch.autograd.graph.increment_version(out)
     return out
 
 
