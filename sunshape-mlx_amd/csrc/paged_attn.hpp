@@ -189,7 +189,7 @@ __device__ __forceinline__ void finish_row(const PagedAttn &a, int r, int64_t t,
 // that large, hidden ones among them, and taken for those that are.  So a score is
 // off by 2^-21 of itself, and its bits are its own, whatever other rows' scores or the
 // tokens are that no row sees.  (A prompt of 4093 tokens capped at 50, which few scores
-// come near, 302 us; at 15 331, at 3 383.  One form for all of a wave's scores: 299 to
+// come near, 303 us; at 15 330, at 3 383.  One form for all of a wave's scores: 299 to
 // 302, but small scores were off by 2^-22 of the cap beside a large one.)
 // (A bias meets the reference first: both may be large, what is left of them is
 // rounded once.)

@@ -24,8 +24,9 @@
 // two waves a SIMD hold.  A prompt of 4093 tokens, 32 heads, 137 GFLOP, takes
 // 266 us back to back under the profiler, 230 us between other calls: 0.5 to
 // 0.6 PFLOP/s, vector ALUs 49 % of the cycles, matrix cores 27 %.  With capped
-// scores 302 us (vector ALUs 58 %).  256 rows of 64 requests over 32768 shared
-// tokens, 33 GFLOP: 84 us (43 %), of which some 7 write the 256 parts' sums.
+// scores 298 us between other calls (vector ALUs 58 %).  256 rows of 64 requests over
+// 32768 shared tokens, 33 GFLOP: 76 us under the profiler (48 %), of which some 7
+// write the 256 parts' sums.
 #include "paged_attn.hpp"
 
 namespace ss {
@@ -885,8 +886,8 @@ static int cut_target(int64_t n_requests, int heads, int64_t rows, int most_rows
 }
 
 // Up to how many columns the longer ones of a call's one request are halved (a
-// capped prompt of 1100 tokens 84 -> 68 us, of 1364 102 -> 79, of 2041 148 -> 135,
-// of 2800 198 -> 189; 4 KV heads, 4093 tokens 213 -> 170).  Of more columns each
+// capped prompt of 1100 tokens 82 -> 67 us, of 1364 98 -> 76, of 2041 142 -> 124,
+// of 2800 190 -> 175; 16 query and 4 KV heads, 4093 tokens 269 -> 203).  Of more columns each
 // compute unit takes long and short ones, and of several requests, which come one
 // after the other, the last one's halves start late (2 of 1500 tokens 109 -> 147).
 static int halved_columns() { return device_cu_count() * 3 / 2; }

@@ -553,7 +553,12 @@ def paged_attention(queries: torch.Tensor, store: PagedKVStore, block_table: tor
     rows of a request that continues another see all of that one's tokens
     first, which are read once for all of them; distances count them.  Not
     together with ``window`` or ``prefix_lengths``; ``max_length`` is then that
-    of the tokens that requests hold themselves.
+    that of the tokens that requests hold themselves.
+
+    Scores, softmax statistics and sums are float32.  Probabilities, in prompts and
+    over shared tokens values too, enter the products rounded to fp16 (2^-11; values
+    below 2^-29 of a request's largest by 2^-40 of it); of bfloat16 queries the bits
+    down to 2^-29 of a row's largest count; a capped score is off by 2^-21 of itself.
     Queries under autograd, forward mode too, are refused: there is no
     derivative."""
     st = _struct(store)
