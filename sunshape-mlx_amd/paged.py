@@ -689,8 +689,9 @@ class PagedKVCache:
         list whose lengths only the GPU knows.  Captured, it goes into the graph
         with its append and attend, and the plan holds what the last replay
         made of it; a graph with append or attend alone goes on with the slots
-        and starts of the step that they were captured after.  The host does not see
-        what such steps end: requests that share have to end through ``release``."""
+        and starts of the step that they were captured after.  The host sees neither
+        what such a step ends nor, after one, what a list ends: requests that share
+        have to end through ``release`` there."""
         return self._step(new_lengths, n_tokens, max_new)
 
     def _step(self, new_lengths, n_tokens: int | None = None, max_new: int | None = None,
